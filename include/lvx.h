@@ -326,6 +326,36 @@ int lvx_bwd_block_gathered(const lvx_shape* s, const void* q, const void* d_o, c
                            float* dk_acc, float* dv_acc, int accumulate_dkdv, const lvx_block_wait* wait, void* stream);
 int lvx_p2p_wait(const uint32_t* my_flags, int world, int slot, uint32_t epoch, void* stream);
 
+/* A strided [B, heads, S, 128] tensor: element (b, h, s, d) at data[b*stride_b + h*stride_h + s*stride_s + d], strides in
+ * elements. Rows (128 elements) are contiguous; 16-byte aligned, with strides that keep them so (8 bytes suffice for
+ * lvx_head_norm_rope on 16-bit types). */
+typedef struct lvx_view {
+  void* data;
+  int64_t stride_b, stride_h, stride_s;
+} lvx_view;
+
+/* RMSNorm of every query and key head and the rotary embedding in one pass: x -> x rsqrt(mean(x^2) + eps) w, then
+ * (y_d cos_d - y_{d+64} sin_d, y_{d+64} cos_{d+64} + y_d sin_{d+64}) for d < 64, in fp32 and rounded once. The outputs are
+ * dense [B, H, S, 128]. The reference runs MllamaTextRMSNorm and apply_rotary_pos_emb as torch modules on transposed copies
+ * (test_llama3.py:294-312, :394-419). */
+typedef struct lvx_head_norm {
+  int32_t dtype;              /* enum lvx_dtype, of inputs, outputs and gradients */
+  int32_t B, S, Hq, Hkv;
+  int32_t weight_fp32;        /* the weights are fp32, else `dtype` */
+  int32_t table_fp32;         /* cos and sin are fp32, else `dtype` */
+  float eps;
+  const void *wq, *wk;        /* [128]; NULL: no norm (of the queries, of the keys) */
+  const void *cos, *sin;      /* element (b, s, d) at [b*table_stride_b + s*table_stride_s + d]; both NULL: no rotation */
+  int64_t table_stride_b, table_stride_s;
+} lvx_head_norm;
+/* q or k (with its output) may be NULL. */
+int lvx_head_norm_rope(const lvx_head_norm* c, const lvx_view* q, const lvx_view* k, void* q_out, void* k_out, void* stream);
+/* Its backward: dq, dk dense [B, S, H, 128] from the outputs' gradients gq, gk, and dwq, dwk [128] in the weights' type, summed
+ * in a fixed order. Of dq, dk, dwq, dwk those that are NULL are not made; without dwq and dwk no scratch is needed. */
+#define LVX_HEAD_NORM_SCRATCH 606208
+int lvx_head_norm_rope_bwd(const lvx_head_norm* c, const lvx_view* q, const lvx_view* k, const lvx_view* gq, const lvx_view* gk,
+                           void* dq, void* dk, void* dwq, void* dwk, void* scratch, size_t scratch_bytes, void* stream);
+
 /* Self-test of the tensor-core building blocks (TMA tile load, shared-memory and TMEM operand
  * descriptors, TMEM load/store): runs one 128 x N x K product in the operand arrangement `mode`
  * and writes D (fp32 [128,N]) to `d_out`. a/b are device buffers in the arrangement the mode

@@ -32,3 +32,4 @@ from .hf_patch import (  # noqa: F401,E402
 )
 from .host_io import HostStreamedAttention  # noqa: F401,E402
 from .peer_memory import check_device_status  # noqa: F401,E402
+from .rotary import head_norm_rope  # noqa: F401,E402

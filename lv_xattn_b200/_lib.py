@@ -26,9 +26,11 @@ SYMBOLS = [
     "lvx_fwd_block_static", "lvx_fwd_merge_parts", "lvx_sum_cast",
     "lvx_p2p_signal", "lvx_p2p_gather", "lvx_p2p_fwd_merge", "lvx_p2p_sum_cast", "lvx_p2p_push", "lvx_p2p_wait",
     "lvx_p2p_push_dma",
+    "lvx_head_norm_rope", "lvx_head_norm_rope_bwd",
 ]
 MAX_PEERS = 16      # LVX_MAX_PEERS
 P2P_SLOTS = 8       # LVX_P2P_SLOTS
+HEAD_NORM_SCRATCH = 606208      # LVX_HEAD_NORM_SCRATCH
 
 
 class LvxShape(ctypes.Structure):
@@ -43,6 +45,16 @@ class LvxPeers(ctypes.Structure):
 class LvxBias(ctypes.Structure):
     _fields_ = [("bias", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in
                                                ("stride_block", "stride_b", "stride_h", "stride_q", "stride_kv")]
+
+
+class LvxView(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("stride_b", "stride_h", "stride_s")]
+
+
+class LvxHeadNorm(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "B", "S", "Hq", "Hkv", "weight_fp32", "table_fp32")] \
+        + [("eps", ctypes.c_float)] + [(n, ctypes.c_void_p) for n in ("wq", "wk", "cos", "sin")] \
+        + [(n, ctypes.c_int64) for n in ("table_stride_b", "table_stride_s")]
 
 
 class LvxBlockWait(ctypes.Structure):
@@ -106,6 +118,9 @@ def load():
     lib.lvx_attn_backward.argtypes = [sp, vp, vp, vp, vp, vp, fp, i32p, bp, ctypes.c_float, vp, ctypes.c_size_t, vp, vp, vp, vp]
     lib.lvx_local_valid.argtypes = [vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int, i32p, vp]
     lib.lvx_device_status_host.argtypes = [vp, ctypes.POINTER(ctypes.c_void_p)]
+    hp, viewp = ctypes.POINTER(LvxHeadNorm), ctypes.POINTER(LvxView)
+    lib.lvx_head_norm_rope.argtypes = [hp, viewp, viewp, vp, vp, vp]
+    lib.lvx_head_norm_rope_bwd.argtypes = [hp, viewp, viewp, viewp, viewp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
     for name in SYMBOLS:
         getattr(lib, name)  # AttributeError here means header and library disagree
         if name != "lvx_last_error":

@@ -523,6 +523,81 @@ int lvx_add_cast(const float* a, const float* b, void* out, int out_dtype, size_
   return launch_add_cast(a, b, out, out_dtype, n, static_cast<cudaStream_t>(stream));
 }
 
+static int check_view(const lvx_view* v, int elt, int align, const char* who, const char* name) {
+  if (!v) return LVX_OK;
+  if (!v->data) return fail(LVX_ERR_NULL, "%s: %s is NULL", who, name);
+  if ((reinterpret_cast<uintptr_t>(v->data) & (align - 1)) ||
+      ((v->stride_b | v->stride_h | v->stride_s) * elt) & (align - 1))
+    return fail(LVX_ERR_ALIGN, "%s: rows of %s are not %d-byte aligned", who, name, align);
+  return LVX_OK;
+}
+
+static int64_t head_norm_rows(const lvx_head_norm* c, const lvx_view* q, const lvx_view* k) {
+  return int64_t(c->B) * c->S * ((q ? c->Hq : 0) + (k ? c->Hkv : 0));
+}
+
+static int check_head_norm(const lvx_head_norm* c, const lvx_view* q, const lvx_view* k, const char* who) {
+  if (!c) return fail(LVX_ERR_NULL, "%s: the description is NULL", who);
+  if (c->dtype != LVX_BF16 && c->dtype != LVX_FP16 && c->dtype != LVX_FP32) return fail(LVX_ERR_DTYPE, "%s: dtype %d unsupported", who, c->dtype);
+  if (c->B < 0 || c->S < 0 || c->Hq < 0 || c->Hkv < 0) return fail(LVX_ERR_SHAPE, "%s: negative dimension", who);
+  if (!q && !k) return fail(LVX_ERR_NULL, "%s: neither q nor k is given", who);
+  if (!(c->eps >= 0.f)) return fail(LVX_ERR_SHAPE, "%s: eps must be non-negative", who);
+  if ((c->cos == nullptr) != (c->sin == nullptr)) return fail(LVX_ERR_NULL, "%s: cos and sin go together", who);
+  const int es = elt_size(c->dtype), align = es * 4;
+  if (head_norm_rows(c, q, k) == 0) return LVX_OK;      // nothing is read, and nothing need be there
+  int rc = check_view(q, es, align, who, "q");
+  if (!rc) rc = check_view(k, es, align, who, "k");
+  if (rc) return rc;
+  const int ws = c->weight_fp32 ? 4 : es, ts = c->table_fp32 ? 4 : es;
+  if ((reinterpret_cast<uintptr_t>(c->wq) | reinterpret_cast<uintptr_t>(c->wk)) & (ws * 4 - 1))
+    return fail(LVX_ERR_ALIGN, "%s: a weight is not %d-byte aligned", who, ws * 4);
+  if ((reinterpret_cast<uintptr_t>(c->cos) | reinterpret_cast<uintptr_t>(c->sin) |
+       (c->cos ? uintptr_t(c->table_stride_b | c->table_stride_s) * ts : 0)) & (ts * 4 - 1))
+    return fail(LVX_ERR_ALIGN, "%s: rows of cos and sin are not %d-byte aligned", who, ts * 4);
+  return validate_arch();
+}
+
+int lvx_head_norm_rope(const lvx_head_norm* c, const lvx_view* q, const lvx_view* k, void* q_out, void* k_out, void* stream) {
+  const char* who = "lvx_head_norm_rope";
+  const int rc = check_head_norm(c, q, k, who);
+  if (rc) return rc;
+  if (head_norm_rows(c, q, k) == 0) return LVX_OK;
+  if (q) LVX_REQUIRE_PTR(q_out, who);
+  if (k) LVX_REQUIRE_PTR(k_out, who);
+  return launch_head_norm(*c, q, k, q_out, k_out, static_cast<cudaStream_t>(stream));
+}
+
+int lvx_head_norm_rope_bwd(const lvx_head_norm* c, const lvx_view* q, const lvx_view* k, const lvx_view* gq, const lvx_view* gk,
+                           void* dq, void* dk, void* dwq, void* dwk, void* scratch, size_t scratch_bytes, void* stream) {
+  const char* who = "lvx_head_norm_rope_bwd";
+  int rc = check_head_norm(c, q, k, who);
+  if (rc) return rc;
+  if ((q == nullptr) != (gq == nullptr) || (k == nullptr) != (gk == nullptr))
+    return fail(LVX_ERR_NULL, "%s: q and gq, k and gk go together", who);
+  const int es = elt_size(c->dtype), align = es * 4;
+  const bool rows = head_norm_rows(c, q, k) > 0;
+  if (rows && ((rc = check_view(gq, es, align, who, "gq")) || (rc = check_view(gk, es, align, who, "gk")))) return rc;
+  if ((dwq && !(q && c->wq)) || (dwk && !(k && c->wk))) return fail(LVX_ERR_NULL, "%s: a gradient of a weight that is not there", who);
+  if ((dq && !q) || (dk && !k)) return fail(LVX_ERR_NULL, "%s: a gradient of an input that is not there", who);
+  if (dq && rows) LVX_REQUIRE_PTR(dq, who);
+  if (dk && rows) LVX_REQUIRE_PTR(dk, who);
+  if (!dq && !dk && !dwq && !dwk) return LVX_OK;
+  if (dwq || dwk) {
+    LVX_REQUIRE_PTR(scratch, who);
+    if (scratch_bytes < LVX_HEAD_NORM_SCRATCH)
+      return fail(LVX_ERR_WORKSPACE, "%s: scratch has %zu bytes, %d needed", who, scratch_bytes, LVX_HEAD_NORM_SCRATCH);
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!rows) {      // no rows: the sums are empty
+    const size_t n = 128 * (c->weight_fp32 ? 4 : es);
+    cudaError_t e = cudaSuccess;
+    if (dwq) e = cudaMemsetAsync(dwq, 0, n, st);
+    if (e == cudaSuccess && dwk) e = cudaMemsetAsync(dwk, 0, n, st);
+    return e == cudaSuccess ? LVX_OK : cuda_fail(e, "cudaMemsetAsync(dw)");
+  }
+  return launch_head_norm_bwd(*c, q, k, gq, gk, dq, dk, static_cast<float*>(scratch), dwq, dwk, st);
+}
+
 int lvx_selftest_mma(int mode, const void* a, const void* b, float* d_out, void* stream) {
   const char* who = "lvx_selftest_mma";
   int rc = check_arch();

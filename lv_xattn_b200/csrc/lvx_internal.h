@@ -96,6 +96,10 @@ int launch_knorm_bwd(int dtype, const void* k, const void* dk, const float* rstd
                      float* dw, long rows, cudaStream_t st);
 int launch_kvproj_grad_rows(int dtype, const void* k, const void* dk, const void* dv, const float* rstd, const void* norm_w,
                             void* dk_rows, void* dv_rows, float* dw, int batch, int hkv, int s, cudaStream_t st);
+// Head norms and rotary embedding (head_norm.cu).
+int launch_head_norm(const lvx_head_norm& c, const lvx_view* q, const lvx_view* k, void* q_out, void* k_out, cudaStream_t st);
+int launch_head_norm_bwd(const lvx_head_norm& c, const lvx_view* q, const lvx_view* k, const lvx_view* gq, const lvx_view* gk,
+                         void* dq, void* dk, float* scratch, void* dwq, void* dwk, cudaStream_t st);
 int launch_fwd_merge_parts(const lvx_shape& s, const float* o_parts, const float* lse_parts, int count,
                            size_t stride_o, size_t stride_lse, void* o_out, float* lse_out, cudaStream_t st);
 int launch_sum_cast(const float* parts, int count, size_t stride, void* out, int out_dtype, size_t n, cudaStream_t st);

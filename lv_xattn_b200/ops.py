@@ -546,3 +546,59 @@ def selftest_mma(mode: int, a, b, n_cols: int):
     _lib.check(lib.lvx_selftest_mma(mode, _lib.ptr(a), _lib.ptr(b), _lib.ptr(d), _lib.stream_ptr()),
                "lvx_selftest_mma")
     return d
+
+
+# ---- head norms and rotary embedding (see rotary.py for the entry point) -------------------------------------
+def rows_view(t, align_elements: int):
+    """(lvx_view, tensor kept alive) of a [B, H, S, 128] tensor with any strides that keep its rows contiguous and aligned
+    to `align_elements` elements; other tensors are copied first."""
+    sb, sh, ss, sd = t.stride()
+    if sd != 1 or (sb | sh | ss) % align_elements or t.data_ptr() % (align_elements * t.element_size()):
+        t = t.contiguous() if not t.is_contiguous() else t.clone()
+        sb, sh, ss, _ = t.stride()
+    return _lib.LvxView(t.data_ptr(), sb, sh, ss), t
+
+
+def _head_norm(q, k, q_weight, k_weight, cos, sin, eps):
+    like = q if q is not None else k
+    B, S = like.shape[:2]
+    weight = q_weight if q_weight is not None else k_weight
+    c = _lib.LvxHeadNorm(_lib.dtype_code(like.dtype), B, S, 0 if q is None else q.shape[2], 0 if k is None else k.shape[2],
+                         int(weight is not None and weight.dtype == torch.float32),
+                         int(cos is not None and cos.dtype == torch.float32), eps,
+                         None if q is None or q_weight is None else q_weight.data_ptr(),
+                         None if k is None or k_weight is None else k_weight.data_ptr(),
+                         None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
+                         0 if cos is None or cos.shape[0] == 1 else cos.stride(0), 0 if cos is None else cos.stride(1))
+    return c, [None if t is None else rows_view(t.transpose(1, 2), 4) for t in (q, k)]
+
+
+def _ref(view):
+    return None if view is None else ctypes.byref(view[0])
+
+
+def head_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float):
+    """(q_out, k_out) [B, H, S, 128] of q, k [B, S, H, 128] (either may be None); cos and sin [1 or B, S, 128]. The caller
+    has checked types and shapes; weights and tables are contiguous where a row is."""
+    c, (qv, kv) = _head_norm(q, k, q_weight, k_weight, cos, sin, eps)
+    out = [None if t is None else t.new_empty(c.B, t.shape[2], c.S, 128) for t in (q, k)]
+    _lib.check(_lib.load().lvx_head_norm_rope(ctypes.byref(c), _ref(qv), _ref(kv), *(None if t is None else t.data_ptr() for t in out),
+                                              _lib.stream_int()), "lvx_head_norm_rope")
+    _count()
+    return out
+
+
+def head_norm_rope_bwd(q, k, q_weight, k_weight, cos, sin, eps: float, gq, gk, want):
+    """Gradients (dq, dk [B, S, H, 128], dwq, dwk [128]) from the outputs' gradients; `want` says which are made."""
+    c, (qv, kv) = _head_norm(q, k, q_weight, k_weight, cos, sin, eps)
+    gv = [None if t is None else rows_view(t, 4) for t in (gq, gk)]
+    dx = [t.new_empty(t.shape) if w else None for t, w in zip((q, k), want[:2])]
+    dw = [torch.empty_like(t) if w else None for t, w in zip((q_weight, k_weight), want[2:])]
+    with_dw = dw[0] is not None or dw[1] is not None
+    scratch = (q if q is not None else k).new_empty(_lib.HEAD_NORM_SCRATCH // 4, dtype=torch.float32) if with_dw else None
+    _lib.check(_lib.load().lvx_head_norm_rope_bwd(
+        ctypes.byref(c), _ref(qv), _ref(kv), _ref(gv[0]), _ref(gv[1]),
+        *(None if t is None else t.data_ptr() for t in (*dx, *dw, scratch)), _lib.HEAD_NORM_SCRATCH if with_dw else 0,
+        _lib.stream_int()), "lvx_head_norm_rope_bwd")
+    _count(2 if with_dw else 1)
+    return (*dx, *dw)

@@ -1,0 +1,117 @@
+"""Head norms and the rotary embedding of a text layer's queries and keys, in one pass over them.
+
+The reference's text layers run the norm, the rotation and the transposition into [B, H, S, D] as separate torch modules
+(test_llama3.py:294-312 for the self-attention, :394-419 for the norms); here they are one kernel, which reads the
+projections' output where it is and writes the layout that the attention kernels read.
+"""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _lib, ops
+
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def on_device(t):
+    """Makes t's device current for the duration of a call (kernels launch on the current device)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def watch_status(t):
+    """Start of a call: raises if a kernel of an earlier call gave up on a bounded wait (see peer_memory.StatusWatch)."""
+    from .peer_memory import status_watch
+    status_watch.watch(t.device.index)
+
+
+def _check(q, k, q_weight, k_weight, cos, sin, eps):
+    like = q if q is not None else k
+    if like is None:
+        raise ValueError("head_norm_rope: q or k must be given")
+    for name, t in (("q", q), ("k", k)):
+        if t is not None and (t.dim() != 4 or t.shape[-1] != 128):
+            raise ValueError(f"head_norm_rope: {name} must be [batch, tokens, heads, 128], got {tuple(t.shape)}")
+    if like.dtype not in _TYPES:
+        raise ValueError(f"head_norm_rope: dtype {like.dtype} unsupported; expected bfloat16, float16 or float32")
+    if q is not None and k is not None and (q.dtype != k.dtype or q.shape[:2] != k.shape[:2]):
+        raise ValueError("head_norm_rope: q and k must agree on dtype, batch and tokens")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    if (q is None and q_weight is not None) or (k is None and k_weight is not None):
+        raise ValueError("head_norm_rope: a weight without the tensor that it scales")
+    for w in weights:
+        if w.shape != (128,) or w.dtype not in (like.dtype, torch.float32) or w.dtype != weights[0].dtype:
+            raise ValueError("head_norm_rope: weights must be [128], both fp32 or both in the dtype of q and k")
+    if (cos is None) != (sin is None):
+        raise ValueError("head_norm_rope: cos and sin go together")
+    if cos is None and not weights:
+        raise ValueError("head_norm_rope: neither a weight nor cos and sin: nothing to do")
+    if cos is not None:
+        B, S = like.shape[:2]
+        if cos.shape != sin.shape or tuple(cos.shape) not in ((S, 128), (1, S, 128), (B, S, 128)):
+            raise ValueError(f"head_norm_rope: cos and sin must be [{S}, 128] or [1 or {B}, {S}, 128], got {tuple(cos.shape)} and {tuple(sin.shape)}")
+        if cos.dtype != sin.dtype or cos.dtype not in (like.dtype, torch.float32):
+            raise ValueError("head_norm_rope: cos and sin must be fp32 or in the dtype of q and k")
+    if not eps >= 0:
+        raise ValueError("head_norm_rope: eps must be non-negative")
+    for t in (q, k, cos, sin, *weights):
+        if t is not None:
+            if not t.is_cuda:
+                raise _lib.LvxError("lv_xattn_b200 runs on CUDA tensors only; there is no CPU path")
+            if t.device != like.device:
+                raise ValueError("head_norm_rope: all tensors must be on one device")
+
+
+def _rows(t):
+    """A table or a weight as the kernel reads it: contiguous, 16-byte aligned rows (a copy where it is not so)."""
+    if t is None:
+        return None
+    if t.dim() == 2:
+        t = t[None]
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.contiguous().clone()
+
+
+class HeadNormRopeFunc(torch.autograd.Function):
+    """(q, k, q_weight, k_weight, cos, sin, eps) -> (q_out, k_out). Keeps its inputs for the backward, nothing else."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps):
+        with on_device(q if q is not None else k):
+            out = ops.head_norm_rope(q, k, q_weight, k_weight, cos, sin, eps)
+        # without a norm the gradient does not depend on the input
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return tuple(out)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        q, k, q_weight, k_weight, cos, sin = ctx.saved_tensors
+        want = list(ctx.needs_input_grad[:4])
+        # an output that nothing used has no gradient, and neither have what it was made of
+        if gq is None:
+            q = q_weight = None
+            want[0] = want[2] = False
+        if gk is None:
+            k = k_weight = None
+            want[1] = want[3] = False
+        if not any(want):
+            return (None,) * 7
+        with on_device(q if q is not None else k):
+            grads = ops.head_norm_rope_bwd(q, k, q_weight, k_weight, cos, sin, ctx.eps, gq, gk, want)
+        return (*grads, None, None, None)
+
+
+def head_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-6):
+    """Per-head RMSNorm and rotary embedding of queries and keys in one pass: (q_out, k_out), dense [B, H, S, 128].
+
+    q [B, S, Hq, 128] and k [B, S, Hkv, 128] are the projections' outputs seen by head (any strides; either may be None),
+    bf16, fp16 or fp32. q_weight and k_weight [128] scale the normalised heads (None: that tensor is not normalised). cos and
+    sin [S, 128] or [1 or B, S, 128] are the rotary tables as Hugging Face models hand them to their layers, both halves of
+    the 128 columns filled (None: no rotation). Computed in fp32 and rounded once. Gradients flow into q, k and the weights;
+    the weights' are summed in a fixed order."""
+    _check(q, k, q_weight, k_weight, cos, sin, eps)
+    q_weight, k_weight, cos, sin = (_rows(t) for t in (q_weight, k_weight, cos, sin))
+    watch_status(q if q is not None else k)
+    return HeadNormRopeFunc.apply(q, k, q_weight, k_weight, cos, sin, float(eps))
