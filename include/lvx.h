@@ -356,6 +356,27 @@ int lvx_head_norm_rope(const lvx_head_norm* c, const lvx_view* q, const lvx_view
 int lvx_head_norm_rope_bwd(const lvx_head_norm* c, const lvx_view* q, const lvx_view* k, const lvx_view* gq, const lvx_view* gk,
                            void* dq, void* dk, void* dwq, void* dwk, void* scratch, size_t scratch_bytes, void* stream);
 
+/* Causal attention with a sliding window and sinks: query i of batch entry b sits at position p = first_b + i and sees key j
+ * iff j < n_b, j <= p and (j > p - window or j < sinks), n_b = kv_valid_len[b] (Skv where kv_valid_len is NULL).
+ * The reference's text layers apply a causal mask through torch's scaled_dot_product_attention (test_llama3.py:313-340); its
+ * kernels' own causal mask uses rank-local indices (lv_xattn/attn.py:229). */
+typedef struct lvx_window {
+  int32_t window;        /* keys that a query sees, its own position included; 0 = all behind it */
+  int32_t sinks;         /* leading keys that stay visible */
+  int32_t query_start;   /* first_b for every batch entry; -1: first_b = n_b - Sq */
+} lvx_window;
+/* Scratch of lvx_window_forward and lvx_window_backward for these sizes. */
+int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_bytes, size_t* bwd_bytes);
+/* o dense [B, Hq, Sq, 128] in shape.dtype, lse fp32 [B*Hq, Sq] (a row without keys: zeros and -inf). q, k, v may have any
+ * strides for 16-bit types, and are dense for fp32. Keys from n_b on are never looked at, whatever they hold. */
+int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* q, const lvx_view* k, const lvx_view* v,
+                       const int32_t* kv_valid_len, float sm_scale, void* workspace, size_t workspace_bytes, void* o, float* lse,
+                       void* stream);
+/* dq, dk, dv dense, in shape.dtype; o, d_o dense. */
+int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o, const lvx_view* q, const lvx_view* k,
+                        const lvx_view* v, const void* o, const float* lse, const int32_t* kv_valid_len, float sm_scale,
+                        void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream);
+
 /* Self-test of the tensor-core building blocks (TMA tile load, shared-memory and TMEM operand
  * descriptors, TMEM load/store): runs one 128 x N x K product in the operand arrangement `mode`
  * and writes D (fp32 [128,N]) to `d_out`. a/b are device buffers in the arrangement the mode

@@ -26,7 +26,7 @@ SYMBOLS = [
     "lvx_fwd_block_static", "lvx_fwd_merge_parts", "lvx_sum_cast",
     "lvx_p2p_signal", "lvx_p2p_gather", "lvx_p2p_fwd_merge", "lvx_p2p_sum_cast", "lvx_p2p_push", "lvx_p2p_wait",
     "lvx_p2p_push_dma",
-    "lvx_head_norm_rope", "lvx_head_norm_rope_bwd",
+    "lvx_head_norm_rope", "lvx_head_norm_rope_bwd", "lvx_window_workspace", "lvx_window_forward", "lvx_window_backward",
 ]
 MAX_PEERS = 16      # LVX_MAX_PEERS
 P2P_SLOTS = 8       # LVX_P2P_SLOTS
@@ -55,6 +55,10 @@ class LvxHeadNorm(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "B", "S", "Hq", "Hkv", "weight_fp32", "table_fp32")] \
         + [("eps", ctypes.c_float)] + [(n, ctypes.c_void_p) for n in ("wq", "wk", "cos", "sin")] \
         + [(n, ctypes.c_int64) for n in ("table_stride_b", "table_stride_s")]
+
+
+class LvxWindow(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("window", "sinks", "query_start")]
 
 
 class LvxBlockWait(ctypes.Structure):
@@ -121,6 +125,11 @@ def load():
     hp, viewp = ctypes.POINTER(LvxHeadNorm), ctypes.POINTER(LvxView)
     lib.lvx_head_norm_rope.argtypes = [hp, viewp, viewp, vp, vp, vp]
     lib.lvx_head_norm_rope_bwd.argtypes = [hp, viewp, viewp, viewp, viewp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    winp, szp = ctypes.POINTER(LvxWindow), ctypes.POINTER(ctypes.c_size_t)
+    lib.lvx_window_workspace.argtypes = [sp, winp, szp, szp]
+    lib.lvx_window_forward.argtypes = [sp, winp, viewp, viewp, viewp, vp, ctypes.c_float, vp, ctypes.c_size_t, vp, vp, vp]
+    lib.lvx_window_backward.argtypes = [sp, winp, vp, viewp, viewp, viewp, vp, vp, vp, ctypes.c_float, vp, ctypes.c_size_t, vp, vp,
+                                        vp, vp]
     for name in SYMBOLS:
         getattr(lib, name)  # AttributeError here means header and library disagree
         if name != "lvx_last_error":

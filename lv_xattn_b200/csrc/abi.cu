@@ -1,6 +1,7 @@
 // extern "C" surface of liblvx.so (see include/lvx.h): argument validation, error text,
 // tensor-map encoding through the driver entry point, and the device status word.
 #include "lvx_internal.h"
+#include "window.cuh"
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -107,6 +108,26 @@ int make_tmap_3d(CUtensorMap* out, int dtype, const void* base, uint64_t dim0, u
   if (r != CUDA_SUCCESS)
     return fail(LVX_ERR_SHAPE, "cuTensorMapEncodeTiled failed with CUresult %d (dims %llu,%llu,%llu box %u,%u)",
                 int(r), (unsigned long long)dim0, (unsigned long long)dim1, (unsigned long long)dim2, box0, box1);
+  return LVX_OK;
+}
+
+int make_tmap_nd(CUtensorMap* out, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                 const uint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(LVX_ERR_DRIVER, "cuTensorMapEncodeTiled could not be resolved");
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  CUresult r = fn(out, dtype == LVX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                  const_cast<void*>(base), d, st, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(LVX_ERR_SHAPE, "cuTensorMapEncodeTiled failed with CUresult %d (rank %d, dims %llu,%llu,%llu)", int(r), rank,
+                (unsigned long long)dims[0], (unsigned long long)dims[1], (unsigned long long)dims[2]);
   return LVX_OK;
 }
 
@@ -596,6 +617,130 @@ int lvx_head_norm_rope_bwd(const lvx_head_norm* c, const lvx_view* q, const lvx_
     return e == cudaSuccess ? LVX_OK : cuda_fail(e, "cudaMemsetAsync(dw)");
   }
   return launch_head_norm_bwd(*c, q, k, gq, gk, dq, dk, static_cast<float*>(scratch), dwq, dwk, st);
+}
+
+static lvx_view dense_view(const void* data, int heads, int rows) {
+  return lvx_view{const_cast<void*>(data), int64_t(heads) * rows * 128, int64_t(rows) * 128, 128};
+}
+
+static int check_window(const lvx_shape* s, const lvx_window* w, const char* who) {
+  const int rc = check_shape(s, who);
+  if (rc) return rc;
+  if (!w) return fail(LVX_ERR_NULL, "%s: the window is NULL", who);
+  if (s->q_blocks > 1) return fail(LVX_ERR_SHAPE, "%s: one query block only", who);
+  if (w->window < 0 || w->sinks < 0 || w->query_start < -1)
+    return fail(LVX_ERR_SHAPE, "%s: window %d, sinks %d, query_start %d: negative", who, w->window, w->sinks, w->query_start);
+  if (s->Sq >= kWindowMaxLen || s->Skv >= kWindowMaxLen || w->query_start >= kWindowMaxLen)
+    return fail(LVX_ERR_SHAPE, "%s: lengths and positions must be below %d", who, kWindowMaxLen);
+  // the grid's second axis
+  if (s->dtype != LVX_FP32 && make_q_tiles(s->Hq / s->Hkv, s->Sq).count > 2 * 65535)
+    return fail(LVX_ERR_LIMIT, "%s: %d query rows per KV head are more than 2 x 65,535 tiles", who, s->Hq / s->Hkv * s->Sq);
+  return LVX_OK;
+}
+
+// q, k, v of a windowed call: rows that start on 16 bytes, and dense tensors for the fp32 kernels
+static int check_qkv_views(const lvx_shape* s, const lvx_view* q, const lvx_view* k, const lvx_view* v, const char* who) {
+  if (!q || !k || !v) return fail(LVX_ERR_NULL, "%s: q, k or v is NULL", who);
+  const int es = elt_size(s->dtype);
+  int rc = check_view(q, es, 16, who, "q");
+  if (!rc && s->Skv > 0) rc = check_view(k, es, 16, who, "k");
+  if (!rc && s->Skv > 0) rc = check_view(v, es, 16, who, "v");
+  if (rc || s->dtype != LVX_FP32) return rc;
+  auto dense = [](const lvx_view* t, int b, int h, int n) {
+    return (n < 2 || t->stride_s == 128) && (h < 2 || t->stride_h == int64_t(n) * 128) && (b < 2 || t->stride_b == int64_t(h) * n * 128);
+  };
+  if (!dense(q, s->B, s->Hq, s->Sq) || (s->Skv > 0 && (!dense(k, s->B, s->Hkv, s->Skv) || !dense(v, s->B, s->Hkv, s->Skv))))
+    return fail(LVX_ERR_SHAPE, "%s: fp32 tensors must be dense", who);
+  return LVX_OK;
+}
+
+int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_bytes, size_t* bwd_bytes) {
+  const int rc = check_window(s, w, "lvx_window_workspace");
+  if (rc) return rc;
+  bool few;
+  const FwdPlan p = plan_window(*s, *w, &few);
+  const bool direct = !few && p.nsplit == 1 && s->dtype != LVX_FP32;
+  if (fwd_bytes) *fwd_bytes = direct ? 0 : p.o_part_bytes + p.ml_part_bytes;
+  const size_t delta = ((size_t(s->B) * s->Hq * s->Sq * 4 + 255) & ~size_t(255));
+  if (bwd_bytes) *bwd_bytes = delta + (s->dtype == LVX_FP32 ? 0 : window_dq_floats(*s) * 4);
+  return LVX_OK;
+}
+
+// The partials of a windowed forward, or where they are not needed (and o is given) its results.
+static int window_forward(const lvx_shape* s, const lvx_window* w, const FwdPlan& p, bool few, const lvx_view* q, const lvx_view* k,
+                          const lvx_view* v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
+                          float* lse, int* sp, cudaStream_t st) {
+  if (s->dtype == LVX_FP32)
+    return launch_fwd_block_general(*s, p, q->data, k->data, v->data, kv_valid_len, nullptr, sm_scale, o_part, ml_part, st, w);
+  if (few) return launch_window_rows(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, sp, st);
+  return launch_window_fwd(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, lse, sp, st);
+}
+
+int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* q, const lvx_view* k, const lvx_view* v,
+                       const int32_t* kv_valid_len, float sm_scale, void* workspace, size_t workspace_bytes, void* o, float* lse,
+                       void* stream) {
+  const char* who = "lvx_window_forward";
+  int rc = check_window(s, w, who);
+  if (!rc) rc = check_qkv_views(s, q, k, v, who);
+  if (!rc) rc = check_arch();
+  if (rc) return rc;
+  if (!(sm_scale > 0.f)) return fail(LVX_ERR_SHAPE, "%s: sm_scale must be positive", who);
+  LVX_REQUIRE_PTR(o, who);
+  LVX_REQUIRE_PTR(lse, who);
+  size_t need = 0;
+  if ((rc = lvx_window_workspace(s, w, &need, nullptr))) return rc;
+  if (need) LVX_REQUIRE_PTR(workspace, who);
+  if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
+  int* sp = status_ptr();
+  if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
+  bool few;
+  const FwdPlan p = plan_window(*s, *w, &few);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (need == 0) return window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, nullptr, nullptr, o, lse, sp, st);
+  float* o_part = static_cast<float*>(workspace);
+  float* ml_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_part_bytes);
+  rc = window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, o_part, ml_part, nullptr, nullptr, sp, st);
+  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st);
+}
+
+int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o, const lvx_view* q, const lvx_view* k,
+                        const lvx_view* v, const void* o, const float* lse, const int32_t* kv_valid_len, float sm_scale,
+                        void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream) {
+  const char* who = "lvx_window_backward";
+  int rc = check_window(s, w, who);
+  if (!rc) rc = check_qkv_views(s, q, k, v, who);
+  if (!rc) rc = check_arch();
+  if (rc) return rc;
+  if (!(sm_scale > 0.f)) return fail(LVX_ERR_SHAPE, "%s: sm_scale must be positive", who);
+  LVX_REQUIRE_PTR(d_o, who);
+  LVX_REQUIRE_PTR(o, who);
+  LVX_REQUIRE_PTR(lse, who);
+  LVX_REQUIRE_PTR(dq, who);
+  LVX_REQUIRE_PTR(workspace, who);
+  if (s->Skv > 0) {
+    LVX_REQUIRE_PTR(dk, who);
+    LVX_REQUIRE_PTR(dv, who);
+  }
+  size_t need = 0;
+  if ((rc = lvx_window_workspace(s, w, nullptr, &need))) return rc;
+  if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
+  int* sp = status_ptr();
+  if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool direct = s->dtype == LVX_FP32;      // dQ is accumulated where it is wanted
+  const size_t rows = size_t(s->B) * s->Hq * s->Sq;
+  float* delta = static_cast<float*>(workspace);
+  float* dq_acc = direct ? static_cast<float*>(dq) : reinterpret_cast<float*>(static_cast<char*>(workspace) + ((rows * 4 + 255) & ~size_t(255)));
+  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
+  const cudaError_t e = cudaMemsetAsync(dq_acc, 0, direct ? rows * 512 : window_dq_floats(*s) * 4, st);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dq)");
+  if (s->Skv > 0) {
+    const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
+    rc = direct ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, dq_acc,
+                                           dk, dv, 2, st, w)
+                : launch_window_bwd(*s, *w, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, dq_acc, dk, dv, sp, st);
+  }
+  return rc || direct ? rc : launch_window_dq(*s, dq_acc, dq, sp, st);
 }
 
 int lvx_selftest_mma(int mode, const void* a, const void* b, float* d_out, void* stream) {

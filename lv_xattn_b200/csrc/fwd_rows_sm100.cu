@@ -19,8 +19,15 @@
 // Up to 32 rows the call runs at the rate of its bytes; with 64 the mma work of a tile takes longer than they do, and where
 // the grid is large both kernels are even. More rows would be slower here than there.
 // The partials have the layout of that kernel, so the combine kernel does not care which of the two ran.
+//
+// WIN: the same for causal attention with a sliding window and sinks (window.cuh says which keys a query sees), on q, k
+// and v of any strides. The CTAs of a slab share out the key tiles that its queries turn out to see. What lies behind
+// the last valid key may hold anything: its scores are replaced and its rows of V cleared in shared memory (each warp its
+// own keys' rows). Where keys that only some rows see hold an infinity or a NaN, the others' outputs are made again as
+// plain sums (rows_plain_values), as in window_fwd_sm100.cu.
 #include "lvx_internal.h"
 #include "sm100_prims.cuh"
+#include "window.cuh"
 #include <math.h>
 #include <type_traits>
 
@@ -45,7 +52,25 @@ struct RowsParams {
   float scale_log2;
   float *o_part, *ml_part;
   int* status;
+  // WIN
+  WindowMask mask;
+  int sq, g;
+  const void *k, *v;
+  long long q_b, q_h, q_s, k_b, k_h, k_s, v_b, v_h, v_s;
 };
+
+// four columns of one row's O over keys [key0, key1), as plain fp32 sums
+template <bool IS_BF16>
+__device__ __noinline__ float4 rows_plain_values(float4 o, const uint16_t* q, const uint16_t* k, const uint16_t* v, long long ks,
+                                                 long long vs, int key0, int key1, float c, float m) {
+  for (int key = key0; key < key1; ++key) {
+    const float w = ex2f(dot128<IS_BF16>(q, k + key * ks) * c - m);
+    const uint2 x = *reinterpret_cast<const uint2*>(v + key * vs);
+    const float2 a = unpack16x2<IS_BF16>(x.x), b = unpack16x2<IS_BF16>(x.y);
+    o = make_float4(fmaf(w, a.x, o.x), fmaf(w, a.y, o.y), fmaf(w, b.x, o.z), fmaf(w, b.y, o.w));
+  }
+  return o;
+}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -68,7 +93,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 }
 
 // RG: groups of 16 query rows (1, 2 or 4); the other 8 / RG warps of a group split the keys of a tile.
-template <bool IS_BF16, int RG>
+template <bool IS_BF16, int RG, bool WIN>
 __global__ void __launch_bounds__(FR_THREADS, 1)
 fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const RowsParams p) {
   constexpr int KG = FR_WARPS / RG;          // warps that share a row group
@@ -88,8 +113,21 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   int valid = p.skv;
   if (p.kv_valid_len) valid = min(valid, max(0, p.kv_valid_len[slab / p.hkv]));
   const int valid_tiles = (valid + 127) >> 7;
-  const int tile0 = split * p.tiles_per_split;
-  const int n = max(0, min(tile0 + p.tiles_per_split, valid_tiles) - tile0);
+  int tile0 = split * p.tiles_per_split;
+  int n = max(0, min(tile0 + p.tiles_per_split, valid_tiles) - tile0);
+  // WIN: positions of the first and the last query, and the slab's key tiles, of which the CTA takes n from tile0 on
+  int pos0 = 0, pos1 = 0;
+  KeyTiles kt = {};
+  if constexpr (WIN) {
+    pos0 = p.mask.start >= 0 ? p.mask.start : valid - p.sq;
+    pos1 = pos0 + p.sq - 1;
+    kt = key_tiles(p.mask, valid, pos0, pos1, 7);
+    const int per = (kt.n + p.nsplit - 1) / p.nsplit;
+    tile0 = min(kt.n, split * per);
+    n = min(kt.n, tile0 + per) - tile0;
+  }
+  auto tile_at = [&](int j) { return WIN ? kt.tile(tile0 + j) : tile0 + j; };
+  const int batch = slab / p.hkv, kvh = slab % p.hkv;
   if (tid == 0) {
     for (int s = 0; s < FR_STAGES; ++s) {
       mbar_init(&bars[FR_K_FULL + s], 1);
@@ -116,17 +154,21 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       tma_prefetch_desc(&tmV);
       int issued = 0;
       for (int j = 0; j < n; ++j) {
-        const int s = j % FR_STAGES, y = (tile0 + j) * 128;
+        const int s = j % FR_STAGES, y = tile_at(j) * 128;
         if (!mbar_wait(&bars[FR_EMPTY + s], ((j / FR_STAGES) & 1) ^ 1, abort_flag, p.status, FR_CODE(2, FR_EMPTY),
                        LVX_SPIN_LIMIT_CYCLES))
           break;
         uint8_t* dst = smem + s * FR_STAGE;
+        auto load = [&](uint8_t* to, const CUtensorMap* map, uint64_t* bar, int x) {
+          if constexpr (WIN) tma_load_4d(to, map, bar, x, y, kvh, batch);
+          else tma_load_3d(to, map, bar, x, y, slab);
+        };
         mbar_arrive_expect_tx(&bars[FR_K_FULL + s], 2 * FR_HALF);
-        tma_load_3d(dst, &tmK, &bars[FR_K_FULL + s], 0, y, slab);
-        tma_load_3d(dst + FR_HALF, &tmK, &bars[FR_K_FULL + s], 64, y, slab);
+        load(dst, &tmK, &bars[FR_K_FULL + s], 0);
+        load(dst + FR_HALF, &tmK, &bars[FR_K_FULL + s], 64);
         mbar_arrive_expect_tx(&bars[FR_V_FULL + s], 2 * FR_HALF);
-        tma_load_3d(dst + 2 * FR_HALF, &tmV, &bars[FR_V_FULL + s], 0, y, slab);
-        tma_load_3d(dst + 3 * FR_HALF, &tmV, &bars[FR_V_FULL + s], 64, y, slab);
+        load(dst + 2 * FR_HALF, &tmV, &bars[FR_V_FULL + s], 0);
+        load(dst + 3 * FR_HALF, &tmV, &bars[FR_V_FULL + s], 64);
         issued = j + 1;
       }
       if (*abort_flag) {   // a CTA that is giving up must not leave while a copy into its shared memory is in flight
@@ -144,7 +186,30 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   const int rg = warp % RG, kg = warp / RG;
   const int r0 = rg * 16 + (lane >> 2), cq = (lane & 3) * 2;   // fragment rows r0, r0 + 8; column pair cq
   uint32_t qf[8][4];
-  {
+  // WIN: keys that this thread's rows see: [0, sink_end) and [lo, hi] (rows that do not exist: none)
+  int hi[2] = {-1, -1}, lo[2] = {0, 0}, sink_end[2] = {0, 0};
+  auto q_row = [&](int r) {
+    return static_cast<const uint16_t*>(p.q) + batch * p.q_b + (kvh * p.g + r / p.sq) * p.q_h + (r % p.sq) * p.q_s;
+  };
+  if constexpr (WIN) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = r0 + 8 * i;
+      if (r < p.rows) {
+        const int pos = pos0 + r % p.sq;
+        hi[i] = min(pos, valid - 1);
+        lo[i] = max(0, pos - p.mask.window + 1);
+        sink_end[i] = min(p.mask.sinks, hi[i] + 1);
+      }
+      const uint32_t* row = reinterpret_cast<const uint32_t*>(q_row(min(r, p.rows - 1)));
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const int c = (kk * 16 + cq) >> 1;
+        qf[kk][i] = r < p.rows ? row[c] : 0u;
+        qf[kk][2 + i] = r < p.rows ? row[c + 4] : 0u;
+      }
+    }
+  } else {
     const uint32_t* qs = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + size_t(slab) * p.rows * 128);
     const bool ok0 = r0 < p.rows, ok1 = r0 + 8 < p.rows;
 #pragma unroll
@@ -177,6 +242,10 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     alive = __all_sync(0xffffffffu, alive);
     if (!alive) break;
     const int left = valid - (tile0 + j) * 128 - kg * KPW;   // valid keys from this warp's first key on
+    const int key0 = tile_at(j) * 128;
+    // WIN: the tile's keys that every query sees need no mask; those that none sees must not reach the second product
+    const bool full = WIN && key0 + 127 <= min(pos0, valid - 1) &&
+                      (key0 > pos1 - p.mask.window || key0 + 128 <= min(p.mask.sinks, pos0 + 1));
 #pragma unroll
     for (int c0 = 0; c0 < KPW; c0 += CH) {
       float sc[CH / 8][4];
@@ -193,7 +262,17 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
           mma_16816<IS_BF16>(sc[2 * g], qf[kk], b[0], b[1]);
           mma_16816<IS_BF16>(sc[2 * g + 1], qf[kk], b[2], b[3]);
         }
-      if (left < c0 + CH) {
+      if constexpr (WIN) {
+        if (!full) {
+#pragma unroll
+          for (int t = 0; t < CH / 8; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = key0 + kg * KPW + c0 + t * 8 + cq + (e & 1), i = e >> 1;
+              if (key > hi[i] || (key < lo[i] && key >= sink_end[i])) sc[t][e] = -INFINITY;
+            }
+        }
+      } else if (left < c0 + CH) {
 #pragma unroll
         for (int t = 0; t < CH / 8; ++t)
 #pragma unroll
@@ -245,6 +324,18 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         alive = mbar_wait(&bars[FR_V_FULL + s], ph, abort_flag, p.status, FR_CODE(0, FR_V_FULL), LVX_SPIN_LIMIT_CYCLES);
         alive = __all_sync(0xffffffffu, alive);
         if (!alive) break;
+        if (WIN && !full) {
+          const int last = min(pos1, valid - 1), first = pos0 - p.mask.window + 1;      // what some query sees
+#pragma unroll 1
+          for (int at = lane; at < KPW * 16; at += 32) {
+            const int row = kg * KPW + (at >> 4), key = key0 + row;
+            if (key > last || (key < first && key >= p.mask.sinks))
+              *reinterpret_cast<uint4*>(smem + s * FR_STAGE + 2 * FR_HALF + ((at >> 3) & 1) * FR_HALF + row * 128 + (at & 7) * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();      // the stage's next copy comes after these
+          __syncwarp();
+        }
       }
 #pragma unroll
       for (int g = 0; g < CH / 16; ++g)
@@ -307,6 +398,20 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       acc.z = fmaf(v.z, w, acc.z);
       acc.w = fmaf(v.w, w, acc.w);
     }
+    if constexpr (WIN) {
+      if (isnan(acc.x + acc.y + acc.z + acc.w) && ls < INFINITY) {
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int pos = pos0 + row % p.sq, last = min(pos, valid - 1), first = max(0, pos - p.mask.window + 1);
+        const uint16_t* kb = static_cast<const uint16_t*>(p.k) + batch * p.k_b + kvh * p.k_h;
+        const uint16_t* vb = static_cast<const uint16_t*>(p.v) + batch * p.v_b + kvh * p.v_h + c4 * 4;
+        for (int j = 0; j < n; ++j) {      // the sinks, then what of the window lies behind them
+          const int key0 = tile_at(j) * 128, cut = min(key0 + 128, min(p.mask.sinks, last + 1));
+          acc = rows_plain_values<IS_BF16>(acc, q_row(row), kb, vb, p.k_s, p.v_s, key0, cut, c, moff);
+          acc = rows_plain_values<IS_BF16>(acc, q_row(row), kb, vb, p.k_s, p.v_s, max(max(key0, cut), first),
+                                           min(key0 + 128, last + 1), c, moff);
+        }
+      }
+    }
     reinterpret_cast<float4*>(o_dst)[row * 32 + c4] = acc;
     if (c4 == 0) *reinterpret_cast<float2*>(ml_dst + row * 2) = make_float2(mm, ls);
   }
@@ -342,9 +447,9 @@ int launch_fwd_rows(const lvx_shape& s, const FwdPlan& pl, const void* q, const 
   };
   auto pick = [&](auto bf16) {
     constexpr bool B16 = decltype(bf16)::value;
-    if (pl.rows <= 16) go(fwd_rows_kernel<B16, 1>);
-    else if (pl.rows <= 32) go(fwd_rows_kernel<B16, 2>);
-    else go(fwd_rows_kernel<B16, 4>);
+    if (pl.rows <= 16) go(fwd_rows_kernel<B16, 1, false>);
+    else if (pl.rows <= 32) go(fwd_rows_kernel<B16, 2, false>);
+    else go(fwd_rows_kernel<B16, 4, false>);
   };
   if (s.dtype == LVX_BF16) pick(std::true_type{});
   else pick(std::false_type{});
@@ -352,6 +457,51 @@ int launch_fwd_rows(const lvx_shape& s, const FwdPlan& pl, const void* q, const 
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "fwd_rows_kernel launch");
   return LVX_OK;
+}
+
+int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl, const lvx_view& q, const lvx_view& k,
+                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
+                       cudaStream_t st) {
+  CUtensorMap tmK, tmV;
+  int rc = make_kv_map(&tmK, s, k, q);
+  if (!rc) rc = make_kv_map(&tmV, s, v, q);
+  if (rc) return rc;
+  RowsParams p{};
+  p.q = q.data;
+  p.rows = pl.rows;
+  p.skv = s.Skv;
+  p.hkv = s.Hkv;
+  p.nsplit = pl.nsplit;
+  p.kv_valid_len = kv_valid_len;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.o_part = o_part;
+  p.ml_part = ml_part;
+  p.status = status;
+  p.mask = make_window_mask(w);
+  p.sq = s.Sq;
+  p.g = s.Hq / s.Hkv;
+  p.k = k.data;
+  p.v = v.data;
+  p.q_b = q.stride_b; p.q_h = q.stride_h; p.q_s = q.stride_s;
+  p.k_b = k.stride_b; p.k_h = k.stride_h; p.k_s = k.stride_s;
+  p.v_b = v.stride_b; p.v_h = v.stride_h; p.v_s = v.stride_s;
+  dim3 grid(pl.nsplit, unsigned(s.B) * s.Hkv, 1);
+  cudaError_t e = cudaSuccess;
+  auto go = [&](auto kern) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FR_SMEM);
+    if (e == cudaSuccess) kern<<<grid, FR_THREADS, FR_SMEM, st>>>(tmK, tmV, p);
+  };
+  auto pick = [&](auto bf16) {
+    constexpr bool B16 = decltype(bf16)::value;
+    if (pl.rows <= 16) go(fwd_rows_kernel<B16, 1, true>);
+    else if (pl.rows <= 32) go(fwd_rows_kernel<B16, 2, true>);
+    else go(fwd_rows_kernel<B16, 4, true>);
+  };
+  if (s.dtype == LVX_BF16) pick(std::true_type{});
+  else pick(std::false_type{});
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(window rows)");
+  e = cudaGetLastError();
+  return e == cudaSuccess ? LVX_OK : cuda_fail(e, "window rows kernel launch");
 }
 
 }  // namespace lvx

@@ -1,6 +1,8 @@
 // The general path: forward and backward flash-attention blocks with fp32 accuracy. It serves (1) fp32 inputs, with or
 // without a dense additive bias (the reference's bias_func protocol, lv_xattn/attn.py:386-389: S = scale * q.k + bias,
-// bias [B, 1 or H, Sq, Skv] fp32), and (2) the backward of fp16 inputs with a bias.
+// bias [B, 1 or H, Sq, Skv] fp32), (2) the backward of fp16 inputs with a bias, and (3) fp32 causal attention with a sliding
+// window and sinks (WIN; window.cuh says which keys a query sees): only the 64-key tiles that some row of a CTA sees are
+// walked, and in the backward only the 64-row tiles that see some of its keys.
 //
 // Every product runs on the tensor core as three tf32 products (mma.sync.m16n8k8): an operand x is taken as hi + lo, hi =
 // x rounded to tf32's 11 bits, lo = the next 11, and a*b as hi*lo + lo*hi + hi*hi; what is dropped is 2^-22 of a
@@ -24,6 +26,7 @@
 // both ways of reading a B fragment free of bank conflicts (4g+t, and 8t+g with k = 2t).
 #include "lvx_internal.h"
 #include "sm100_prims.cuh"
+#include "window.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -187,7 +190,31 @@ struct Fp32FwdParams {
   float scale_log2;
   float *o_part, *ml_part;
   const int* status;   // device status word: non-zero => return at once
+  WindowMask mask;     // WIN
+  int sq;
 };
+
+// Positions of the first and last token among packed rows [row0, row1] (rows run through the tokens head by head)
+__device__ __forceinline__ int2 token_span(int row0, int row1, int sq) {
+  return row0 / sq == row1 / sq ? make_int2(row0 % sq, row1 % sq) : make_int2(0, sq - 1);
+}
+
+// WIN: a thread's 32 columns (8n + 0, 1 from v on) of one row's O over keys [key0, key1), as plain fp32 sums: for rows that a
+// key which others see has made NaN.
+__device__ __noinline__ void fp32_plain_values(float* o, const float* q, const float* k, const float* v, int key0, int key1,
+                                               float c, float m) {
+  for (int key = key0; key < key1; ++key) {
+    const float* kr = k + size_t(key) * 128;
+    const float* vr = v + size_t(key) * 128;
+    float s = 0.f;
+    for (int d = 0; d < 128; ++d) s = fmaf(q[d], kr[d], s);
+    const float w = exp2f(s * c - m);
+    for (int n = 0; n < 16; ++n) {
+      o[2 * n] = fmaf(w, vr[8 * n], o[2 * n]);
+      o[2 * n + 1] = fmaf(w, vr[8 * n + 1], o[2 * n + 1]);
+    }
+  }
+}
 
 // A CTA owns 128 packed rows (a warp 16 of them) and a range of keys, 64 at a time through two stages. Scores and P stay in
 // the warp that made them.
@@ -196,7 +223,7 @@ constexpr int GF_SMEM = (128 * GT_LD + 4 * GT_TILE) * sizeof(float);
 // BIAS: a thread's 32 values of a tile are all requested before the products, under which they arrive. Requested one by one
 // between the products and the softmax they took nearly as long as the products: 32 slabs of 130 rows x 1,601 keys 289 -> 188
 // us (168 without a bias), 8 slabs of 160 rows x 6,404 keys 196 -> 160. Without a bias the kernel carries none of it.
-template <bool BIAS>
+template <bool BIAS, bool WIN>
 __global__ void __launch_bounds__(256, 1)
 fp32_fwd_kernel(const Fp32FwdParams p) {
   if (p.status && *reinterpret_cast<const volatile int*>(p.status) != 0) return;
@@ -208,8 +235,8 @@ fp32_fwd_kernel(const Fp32FwdParams p) {
   const int kvs = slab % p.kv_slabs;          // several query blocks may share one K/V batch entry
   int valid = p.skv;
   if (p.kv_valid_len) valid = min(valid, max(0, p.kv_valid_len[kvs / p.hkv]));
-  const int kv_begin = min(valid, split * p.tiles_per_split * 128);
-  const int kv_end = min(valid, (split + 1) * p.tiles_per_split * 128);
+  int kv_begin = min(valid, split * p.tiles_per_split * 128);
+  int kv_end = min(valid, (split + 1) * p.tiles_per_split * 128);
   const float* ks = p.k + size_t(kvs) * p.skv * 128;
   const float* vs = p.v + size_t(kvs) * p.skv * 128;
   const int row0 = mb * 128 + warp * 16 + g;  // fragment rows row0, row0 + 8
@@ -218,6 +245,28 @@ fp32_fwd_kernel(const Fp32FwdParams p) {
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     brow[i] = BIAS ? bias_row(p.bias, slab, kvs, p.kv_slabs, p.hkv, min(row0 + 8 * i, p.rows - 1)) : nullptr;
+  // WIN: the CTA's share of the keys that its rows see, in tiles of 64: from kv_begin to kv_end, where the sinks' tiles end at
+  // jump_from and the windows' begin at jump_to; and each row's keys [0, sink_end), [lo, hi].
+  int jump_from = 0, jump_to = 0, hi[2], lo[2], sink_end[2];
+  if constexpr (WIN) {
+    const int start = p.mask.start >= 0 ? p.mask.start : valid - p.sq;
+    const int2 span = token_span(mb * 128, min(mb * 128 + 127, p.rows - 1), p.sq);
+    const KeyTiles kt = key_tiles(p.mask, valid, start + span.x, start + span.y, 6);
+    const int per = (kt.n + p.nsplit - 1) / p.nsplit, j0 = min(kt.n, split * per), j1 = min(kt.n, j0 + per);
+    kv_begin = kt.tile(j0) * 64;
+    kv_end = j0 < j1 ? kt.tile(j1 - 1) * 64 + 64 : kv_begin;
+    jump_from = kt.ns * 64;
+    jump_to = kt.w0 * 64;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int pos = start + (row0 + 8 * i) % p.sq;
+      hi[i] = min(pos, valid - 1);
+      lo[i] = max(0, pos - p.mask.window + 1);
+      sink_end[i] = min(p.mask.sinks, hi[i] + 1);
+    }
+  }
+  auto after = [&](int kv0) { return WIN && kv0 + 64 == jump_from ? jump_to : kv0 + 64; };
+  const int kv_rows = WIN ? valid : p.skv;      // rows behind the last valid key may hold anything: zeros are loaded for them
 
   float m[2], l[2], o[16][4];
   // the walk over the keys; a second one with CLAMP where NaN came out
@@ -227,17 +276,17 @@ fp32_fwd_kernel(const Fp32FwdParams p) {
     set_zero(o);
     if (kv_begin < kv_end) {
       load_rows(sQ, p.q + size_t(slab) * p.rows * 128, mb * 128, p.rows, 128, tid);
-      load_rows(sKV, ks, kv_begin, p.skv, 64, tid);
-      load_rows(sKV + GT_TILE, vs, kv_begin, p.skv, 64, tid);
+      load_rows(sKV, ks, kv_begin, kv_rows, 64, tid);
+      load_rows(sKV + GT_TILE, vs, kv_begin, kv_rows, 64, tid);
       cp_commit();
     }
     const float* qa = sQ + (warp * 16 + g) * GT_LD + t;
     int st = 0;
-    for (int kv0 = kv_begin; kv0 < kv_end; kv0 += 64, st ^= 1) {
-      if (kv0 + 64 < kv_end) {
+    for (int kv0 = kv_begin; kv0 < kv_end; kv0 = after(kv0), st ^= 1) {
+      if (after(kv0) < kv_end) {
         float* nxt = sKV + 2 * (st ^ 1) * GT_TILE;
-        load_rows(nxt, ks, kv0 + 64, p.skv, 64, tid);
-        load_rows(nxt + GT_TILE, vs, kv0 + 64, p.skv, 64, tid);
+        load_rows(nxt, ks, after(kv0), kv_rows, 64, tid);
+        load_rows(nxt + GT_TILE, vs, after(kv0), kv_rows, 64, tid);
       }
       cp_commit();                               // possibly empty: the group before it is then complete after cp_wait<1>
       cp_wait<1>();
@@ -274,7 +323,7 @@ fp32_fwd_kernel(const Fp32FwdParams p) {
         for (int e = 0; e < 4; ++e) {
           const int col = kv0 + n * 8 + 2 * t + (e & 1), i = e >> 1;
           float sc = -INFINITY;
-          if (col < kv_end) {
+          if (WIN ? col <= hi[i] && (col >= lo[i] || col < sink_end[i]) : col < kv_end) {
             sc = s[n][e] * p.scale_log2;
             if constexpr (BIAS) sc = fmaf(bv[n][e], 1.4426950408889634f, sc);              // scale*q.k + bias, base 2
           }
@@ -329,6 +378,27 @@ fp32_fwd_kernel(const Fp32FwdParams p) {
     const int row = row0 + 8 * i;
     if (row >= p.rows) continue;
     const size_t prow = (size_t(slab) * p.nsplit + split) * p.rows + row;
+    if constexpr (WIN) {
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) sum += o[n][2 * i] + o[n][2 * i + 1];
+      if (isnan(sum) && l[i] < INFINITY) {
+        float again[32];
+        for (int n = 0; n < 32; ++n) again[n] = 0.f;
+        const float* qrow = p.q + (size_t(slab) * p.rows + row) * 128;
+        const float moff = m[i] == -INFINITY ? 0.f : m[i];
+        for (int key0 = kv_begin; key0 < kv_end; key0 = after(key0)) {      // the sinks, then what of the window lies behind them
+          const int cut = min(key0 + 64, sink_end[i]);
+          fp32_plain_values(again, qrow, ks, vs + 2 * t, key0, cut, p.scale_log2, moff);
+          fp32_plain_values(again, qrow, ks, vs + 2 * t, max(max(key0, cut), lo[i]), min(key0 + 64, hi[i] + 1), p.scale_log2, moff);
+        }
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          o[n][2 * i] = again[2 * n];
+          o[n][2 * i + 1] = again[2 * n + 1];
+        }
+      }
+    }
 #pragma unroll
     for (int n = 0; n < 16; ++n)
       *reinterpret_cast<float2*>(p.o_part + prow * 128 + n * 8 + 2 * t) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
@@ -347,6 +417,8 @@ struct Fp32BwdParams {
   void *dk_acc, *dv_acc;   // fp32 for accumulate 0/1; the input dtype for accumulate 2
   int accumulate;
   const int* status;   // device status word: non-zero => return at once
+  WindowMask mask;     // WIN (one query block, dense rows)
+  int sq;
 };
 
 // A CTA owns 64 keys (K, V in shared memory, dK, dV in registers) and walks over the packed query rows 64 at a time: S and
@@ -355,7 +427,7 @@ struct Fp32BwdParams {
 // while dK and dQ are computed.
 constexpr int GB_SMEM = (5 * GT_TILE + 2 * GT_PTILE) * sizeof(float);
 
-template <typename T>
+template <typename T, bool WIN>
 __global__ void __launch_bounds__(256, 1)
 fp32_bwd_kernel(const Fp32BwdParams p) {
   constexpr bool EX = sizeof(T) == 2;          // 16-bit inputs are exact in tf32
@@ -378,9 +450,21 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
   if (p.kv_valid_len) valid = min(valid, max(0, p.kv_valid_len[slab / p.hkv]));
   const bool live = kv0 < valid;
   const int tiles_per_block = (p.rows + 63) / 64, ntot = live ? tiles_per_block * p.nblk : 0;
+  const int start = WIN ? (p.mask.start >= 0 ? p.mask.start : valid - p.sq) : 0;
+  // the first tile from `it` on with a row that sees one of the CTA's keys
+  auto walk_to = [&](int it) {
+    if constexpr (WIN) {
+      for (; it < ntot; ++it) {
+        const int2 span = token_span(it * 64, min(it * 64 + 63, p.rows - 1), p.sq);
+        if (start + span.y >= kv0 && (kv0 < p.mask.sinks || start + span.x < kv0 + 63 + p.mask.window)) break;
+      }
+    }
+    return it;
+  };
+  const int first = walk_to(0);
   auto qslab_of = [&](int it) { return slab + (it / tiles_per_block) * p.kv_slabs; };
-  auto load_q = [&](int it) {
-    load_rows(sQ + (it & 1) * GT_TILE, static_cast<const T*>(p.q) + size_t(qslab_of(it)) * p.rows * 128,
+  auto load_q = [&](int it, int stage) {
+    load_rows(sQ + stage * GT_TILE, static_cast<const T*>(p.q) + size_t(qslab_of(it)) * p.rows * 128,
               (it % tiles_per_block) * 64, p.rows, 64, tid);
   };
   auto load_do = [&](int it) {
@@ -389,9 +473,9 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
   };
 
   float dk[8][4], dv[8][4];      // keys wm*16 + g (+8), columns wn*64 + 8n + 2t (+1)
-  if (ntot > 0) {
-    load_rows(sK, static_cast<const T*>(p.k) + size_t(slab) * p.skv * 128, kv0, p.skv, 64, tid);
-    load_rows(sV, static_cast<const T*>(p.v) + size_t(slab) * p.skv * 128, kv0, p.skv, 64, tid);
+  if (first < ntot) {      // WIN: rows behind the last valid key may hold anything, and zeros are loaded for them
+    load_rows(sK, static_cast<const T*>(p.k) + size_t(slab) * p.skv * 128, kv0, WIN ? valid : p.skv, 64, tid);
+    load_rows(sV, static_cast<const T*>(p.v) + size_t(slab) * p.skv * 128, kv0, WIN ? valid : p.skv, 64, tid);
   }
   // The walk over the query rows, and a second one with CLAMP where NaN came out. dQ leaves with every tile: from the first
   // tile whose dQ holds NaN a warp adds nothing more, and the second walk adds from there.
@@ -400,12 +484,14 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
     constexpr bool CL = cl.value;
     set_zero(dk);
     set_zero(dv);
-    if (ntot > 0) {
-      load_q(0);
-      load_do(0);
+    if (first < ntot) {
+      load_q(first, 0);
+      load_do(first);
       cp_commit();
     }
-    for (int it = 0; it < ntot; ++it) {
+    int stage = 0;
+    for (int it = first, next; it < ntot; it = next, stage ^= 1) {
+      next = walk_to(it + 1);
       const int qslab = qslab_of(it), q0 = (it % tiles_per_block) * 64;
       float l2[2], dl[2];
       const float* br[2];
@@ -424,9 +510,9 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
       }
       cp_wait<0>();
       __syncthreads();                           // Q and dO are here; the previous tile is done with P, dS and its Q
-      if (it + 1 < ntot) load_q(it + 1);
+      if (next < ntot) load_q(next, stage ^ 1);
       cp_commit();
-      const float* q = sQ + (it & 1) * GT_TILE;
+      const float* q = sQ + stage * GT_TILE;
       {
         float s[4][4], dp[4][4];
         const float *qa = q + (wm * 16 + g) * GT_LD + t, *da = sDO + (wm * 16 + g) * GT_LD + t;
@@ -449,7 +535,11 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int col = kv0 + wn * 32 + n * 8 + 2 * t + e;
-              const bool ok = col < valid;
+              bool ok = col < valid;
+              if constexpr (WIN) {
+                const int pos = start + (q0 + wm * 16 + g + 8 * i) % p.sq;
+                ok = ok && col <= pos && (col > pos - p.mask.window || col < p.mask.sinks);
+              }
               float sc = s[n][2 * i + e] * p.scale_log2;
               if (ok && br[i]) sc = fmaf(br[i][col * p.bias.s_kv], 1.4426950408889634f, sc);
               pv[e] = ok ? exp2f(sc - l2[i]) : 0.f;
@@ -476,7 +566,7 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
       };
       transposed(dv, sP, sDO);
       __syncthreads();                           // dO may be loaded again
-      if (it + 1 < ntot) load_do(it + 1);
+      if (next < ntot) load_do(next);
       cp_commit();
       transposed(dk, sDS, q);
       float dq[8][4];
@@ -539,8 +629,8 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
 
 int launch_fwd_block_general(const lvx_shape& s, const FwdPlan& pl, const void* q, const void* k, const void* v,
                           const int32_t* kv_valid_len, const lvx_bias* bias, float sm_scale, float* o_part,
-                          float* ml_part, cudaStream_t st) {
-  Fp32FwdParams p;
+                          float* ml_part, cudaStream_t st, const lvx_window* win) {
+  Fp32FwdParams p{};
   p.q = static_cast<const float*>(q);
   p.k = static_cast<const float*>(k);
   p.v = static_cast<const float*>(v);
@@ -562,8 +652,15 @@ int launch_fwd_block_general(const lvx_shape& s, const FwdPlan& pl, const void* 
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GF_SMEM);
     if (e == cudaSuccess) kern<<<grid, 256, GF_SMEM, st>>>(p);
   };
-  if (bias) go(fp32_fwd_kernel<true>);
-  else go(fp32_fwd_kernel<false>);
+  if (win) {
+    p.mask = make_window_mask(*win);
+    p.sq = s.Sq;
+    go(fp32_fwd_kernel<false, true>);
+  } else if (bias) {
+    go(fp32_fwd_kernel<true, false>);
+  } else {
+    go(fp32_fwd_kernel<false, false>);
+  }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(fp32 fwd)");
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "fp32 fwd kernel launch");
@@ -573,8 +670,8 @@ int launch_fwd_block_general(const lvx_shape& s, const FwdPlan& pl, const void* 
 int launch_bwd_block_general(const lvx_shape& s, const void* q, const void* d_o, const float* lse, const float* delta,
                           const void* k, const void* v, const int32_t* kv_valid_len, const lvx_bias* bias,
                           float sm_scale, float* dq_acc, void* dk_acc, void* dv_acc, int accumulate_dkdv,
-                          cudaStream_t st) {
-  Fp32BwdParams p;
+                          cudaStream_t st, const lvx_window* win) {
+  Fp32BwdParams p{};
   p.q = q;
   p.d_o = d_o;
   p.lse = lse;
@@ -601,8 +698,15 @@ int launch_bwd_block_general(const lvx_shape& s, const void* q, const void* d_o,
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GB_SMEM);
     if (e == cudaSuccess) kern<<<grid, 256, GB_SMEM, st>>>(p);
   };
-  if (s.dtype == LVX_FP32) go(fp32_bwd_kernel<float>);
-  else go(fp32_bwd_kernel<__half>);
+  if (win) {
+    p.mask = make_window_mask(*win);
+    p.sq = s.Sq;
+    go(fp32_bwd_kernel<float, true>);
+  } else if (s.dtype == LVX_FP32) {
+    go(fp32_bwd_kernel<float, false>);
+  } else {
+    go(fp32_bwd_kernel<__half, false>);
+  }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(fp32 bwd)");
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "fp32 bwd kernel launch");

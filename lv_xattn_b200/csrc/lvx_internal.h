@@ -69,6 +69,19 @@ constexpr int kFewRows = 64;
 int launch_fwd_rows(const lvx_shape& s, const FwdPlan& p, const void* q, const void* k, const void* v,
                     const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
                     cudaStream_t st);
+// Windowed causal attention (window.cuh): few packed rows (partials), and the kernel for more (partials, or O and lse).
+int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
+                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
+                       cudaStream_t st);
+int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
+                      const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
+                      float* lse, int* status, cudaStream_t st);
+// Its backward for 16-bit types: dq_acc (window_dq_floats of them, zeroed) is in tile order, launch_window_dq rounds it.
+size_t window_dq_floats(const lvx_shape& s);
+int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q, const lvx_view& d_o, const lvx_view& k,
+                      const lvx_view& v, const float* lse, const float* delta, const int32_t* kv_valid_len, float sm_scale,
+                      float* dq_acc, void* dk, void* dv, int* status, cudaStream_t st);
+int launch_window_dq(const lvx_shape& s, const float* acc, void* dq, const int* status, cudaStream_t st);
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
                        cudaStream_t st);
@@ -83,11 +96,11 @@ long long p2p_wait_limit_cycles();
 // and fp32 or fp16 (backward), optional dense additive bias.
 int launch_fwd_block_general(const lvx_shape& s, const FwdPlan& p, const void* q, const void* k, const void* v,
                           const int32_t* kv_valid_len, const lvx_bias* bias, float sm_scale, float* o_part,
-                          float* ml_part, cudaStream_t st);
+                          float* ml_part, cudaStream_t st, const lvx_window* win = nullptr);
 int launch_bwd_block_general(const lvx_shape& s, const void* q, const void* d_o, const float* lse, const float* delta,
                           const void* k, const void* v, const int32_t* kv_valid_len, const lvx_bias* bias,
                           float sm_scale, float* dq_acc, void* dk_acc, void* dv_acc, int accumulate_dkdv,
-                          cudaStream_t st);
+                          cudaStream_t st, const lvx_window* win = nullptr);
 // K/V projection with fused per-head RMSNorm (kvproj_sm100.cu) and the backward of that norm.
 int launch_kv_project(int dtype, const void* x, const void* wk, const void* wv, const void* norm_w, float eps,
                       int batch, int s, int kd, int hkv, void* k_out, void* v_out, float* rstd, int* status,

@@ -549,12 +549,15 @@ def selftest_mma(mode: int, a, b, n_cols: int):
 
 
 # ---- head norms and rotary embedding (see rotary.py for the entry point) -------------------------------------
-def rows_view(t, align_elements: int):
+def rows_view(t, align_elements: int, repeats: bool = True):
     """(lvx_view, tensor kept alive) of a [B, H, S, 128] tensor with any strides that keep its rows contiguous and aligned
-    to `align_elements` elements; other tensors are copied first."""
-    sb, sh, ss, sd = t.stride()
-    if sd != 1 or (sb | sh | ss) % align_elements or t.data_ptr() % (align_elements * t.element_size()):
-        t = t.contiguous() if not t.is_contiguous() else t.clone()
+    to `align_elements` elements; other tensors are copied first, and unless `repeats` those that repeat rows (a stride
+    of 0, of which a tensor map does not take any)."""
+    strides = [0 if n == 1 else st for n, st in zip(t.shape, t.stride())]
+    sb, sh, ss, sd = strides
+    if (sd != 1 or (sb | sh | ss) % align_elements or t.data_ptr() % (align_elements * t.element_size())
+            or not (repeats or all(st or n < 2 for n, st in zip(t.shape, strides)))):
+        t = t.clone(memory_format=torch.contiguous_format)
         sb, sh, ss, _ = t.stride()
     return _lib.LvxView(t.data_ptr(), sb, sh, ss), t
 
@@ -602,3 +605,83 @@ def head_norm_rope_bwd(q, k, q_weight, k_weight, cos, sin, eps: float, gq, gk, w
         _lib.stream_int()), "lvx_head_norm_rope_bwd")
     _count(2 if with_dw else 1)
     return (*dx, *dw)
+
+
+# ---- causal attention of the text tokens (see text_attention.py for the entry points) -------------------------
+def device_lengths(lengths, batch: int, most: int, device):
+    """Valid lengths [batch] of any form as int32 on the device (the kernels clamp them to 0..most), or None."""
+    if lengths is None:
+        return None
+    t = torch.as_tensor(lengths)
+    if t.dtype not in (torch.int32, torch.int64) or t.shape != (batch,):
+        raise ValueError(f"valid lengths must be {batch} integers, one per batch entry")
+    if not t.is_cuda:
+        return local_valid(t.to(torch.int64).contiguous(), 0, most, device)
+    if t.device != device:
+        raise ValueError("valid lengths must be on the device of the tensors or on the host")
+    if t.dtype == torch.int64:
+        t = t.clamp(0, most).to(torch.int32)
+    # the kernels read single values: any address of an int will do
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _text_view(t):
+    # the fp32 kernels read dense tensors, the others through tensor maps
+    if t.dtype == torch.float32:
+        return rows_view(t if t.is_contiguous() else t.contiguous(), 4)
+    return rows_view(t, 8, repeats=False)
+
+
+_window_bytes: dict = {}      # a function of the sizes alone
+
+
+def _window_setup(q, k, window, sinks, query_start):
+    shp = shape_of(q, k)
+    win = _lib.LvxWindow(window, sinks, query_start)
+    key = (shp.B, shp.Hq, shp.Hkv, shp.Sq, shp.Skv, shp.dtype, window, sinks)
+    sizes = _window_bytes.get(key)
+    if sizes is None:
+        f, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        _lib.check(_lib.load().lvx_window_workspace(ctypes.byref(shp), ctypes.byref(win), ctypes.byref(f), ctypes.byref(b)),
+                   "lvx_window_workspace")
+        if len(_window_bytes) >= 4096:
+            _window_bytes.clear()
+        sizes = _window_bytes[key] = f.value, b.value
+    return shp, win, sizes
+
+
+def window_forward(q, k, v, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len):
+    """(o [B, Hq, Sq, 128], lse fp32 [B*Hq, Sq]) of causal attention (lvx_window says which keys a query sees). The caller has
+    checked the tensors."""
+    shp, win, (nbytes, _) = _window_setup(q, k, window, sinks, query_start)
+    qv, kv, vv = _text_view(q), _text_view(k), _text_view(v)
+    o = q.new_empty(q.shape)
+    lse = q.new_empty(shp.B * shp.Hq, shp.Sq, dtype=torch.float32)
+    ws = lse.new_empty(nbytes // 4) if nbytes else None
+    _lib.check(_lib.load().lvx_window_forward(ctypes.byref(shp), ctypes.byref(win), _ref(qv), _ref(kv), _ref(vv),
+                                              None if kv_valid_len is None else kv_valid_len.data_ptr(), sm_scale,
+                                              None if ws is None else ws.data_ptr(), nbytes, o.data_ptr(), lse.data_ptr(),
+                                              _lib.stream_int()), "lvx_window_forward")
+    _count(2 if nbytes else 1)
+    return o, lse
+
+
+def _dense(t):
+    """Contiguous, on 16 bytes."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def window_backward(do, q, k, v, o, lse, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len):
+    """(dq, dk, dv) of window_forward."""
+    shp, win, (_, nbytes) = _window_setup(q, k, window, sinks, query_start)
+    qv, kv, vv = _text_view(q), _text_view(k), _text_view(v)
+    do = _dense(do)
+    dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
+    ws = lse.new_empty(nbytes // 4)
+    _lib.check(_lib.load().lvx_window_backward(ctypes.byref(shp), ctypes.byref(win), do.data_ptr(), _ref(qv), _ref(kv), _ref(vv),
+                                               o.data_ptr(), lse.data_ptr(),
+                                               None if kv_valid_len is None else kv_valid_len.data_ptr(), sm_scale,
+                                               ws.data_ptr(), nbytes, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                               _lib.stream_int()), "lvx_window_backward")
+    _count(2 if q.dtype == torch.float32 else 3)
+    return dq, dk, dv

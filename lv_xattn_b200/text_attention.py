@@ -1,0 +1,104 @@
+"""Attention of the text tokens on one GPU: causal, with a sliding window and sinks.
+
+The reference's text layers gather K/V over the group and call torch's scaled_dot_product_attention with a dense causal mask
+(test_llama3.py:313-340). Here only the keys that a query sees are read and multiplied, forward, backward and for the
+single tokens of a generation. The layouts are those of `attention`: q [B, Hq, Sq, 128], k and v [B, Hkv, Skv, 128].
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib, ops
+from .rotary import on_device, watch_status
+
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_MOST = 1 << 28          # lengths and positions are below this
+
+
+def _check_attention(who, q, kv):
+    """q against every (name, k, v) of `kv`."""
+    if q.dim() != 4 or q.shape[-1] != 128:
+        raise ValueError(f"{who}: q must be [batch, heads, tokens, 128], got {tuple(q.shape)}")
+    if q.dtype not in _TYPES:
+        raise ValueError(f"{who}: dtype {q.dtype} unsupported; expected bfloat16, float16 or float32")
+    if 0 in q.shape:
+        raise ValueError(f"{who}: q is empty, {tuple(q.shape)}")
+    for name, k, v in kv:
+        if k.dim() != 4 or k.shape != v.shape or k.shape[-1] != 128:
+            raise ValueError(f"{who}: {name} must be two tensors [batch, KV heads, keys, 128] of one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise ValueError(f"{who}: q and {name} must share one dtype")
+        if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+            raise ValueError(f"{who}: {q.shape[1]} query heads are not a multiple of the {k.shape[1]} heads of {name}")
+    if max([q.shape[2]] + [k.shape[2] for _, k, _ in kv]) >= _MOST:
+        raise ValueError(f"{who}: lengths must be below {_MOST}")
+    tensors = [q] + [t for _, k, v in kv for t in (k, v)]
+    if not all(t.is_cuda for t in tensors):
+        raise _lib.LvxError("lv_xattn_b200 runs on CUDA tensors only; there is no CPU path")
+    if any(t.device != q.device for t in tensors):
+        raise ValueError(f"{who}: all tensors must be on one device")
+
+
+def _scale(who, sm_scale):
+    if sm_scale is None:
+        return 128 ** -0.5
+    if not (sm_scale > 0 and math.isfinite(sm_scale)):
+        raise ValueError(f"{who}: sm_scale must be positive and finite")
+    return float(sm_scale)
+
+
+class WindowAttentionFunc(torch.autograd.Function):
+    """(q, k, v, sm_scale, window, sinks, query_start, kv_valid_len on the device) -> (o, lse)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, sm_scale, window, sinks, query_start, kv_valid_len):
+        o, lse = ops.window_forward(q, k, v, sm_scale, window, sinks, query_start, kv_valid_len)
+        ctx.save_for_backward(q, k, v, o, lse, kv_valid_len)
+        ctx.args = sm_scale, window, sinks, query_start
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    def backward(ctx, do, _):
+        q, k, v, o, lse, kv_valid_len = ctx.saved_tensors
+        with on_device(q):
+            grads = ops.window_backward(do, q, k, v, o, lse, *ctx.args, kv_valid_len)
+        return (*(g if want else None for g, want in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
+
+
+def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=None, query_start=None, return_lse=False):
+    """Causal attention with a sliding window and sinks: o like q, dense; with `return_lse` also the log-sum-exp of every
+    row's scores, fp32 [B*Hq, Sq] (no gradient flows through it).
+
+    q [B, Hq, Sq, 128], k and v [B, Hkv, Skv, 128] in bf16, fp16 or fp32, Hq a multiple of Hkv, any strides. Query i of
+    batch entry b sits at position p = query_start + i, or, where that is None, p = n_b - Sq + i: the last query on the last
+    of the entry's n_b valid keys, as the newest tokens of a generation do. It sees key j iff j < n_b, j <= p, and j > p -
+    window or j < sinks. window None: all keys behind it. kv_valid_len: n_b, one integer per entry (a list, or a tensor on
+    the host or the device; values are taken into 0..Skv), None: Skv. Keys from n_b on are never looked at, whatever they
+    hold: a cache may be longer than what has been written. A query that sees nothing gets zeros, and -inf in the
+    log-sum-exp. In the forward a key that a query does not see has no effect on it, whatever it holds; in the backward the
+    valid keys have to be finite.
+    sm_scale scales the scores (None: 1 / sqrt(128)). Gradients flow into q, k and v."""
+    who = "window_attention"
+    sm_scale = _scale(who, sm_scale)
+    if window is not None and window < 1:
+        raise ValueError(f"{who}: window must be at least 1 (a query's own position), got {window}")
+    if sinks < 0:
+        raise ValueError(f"{who}: sinks must not be negative, got {sinks}")
+    if query_start is not None and not 0 <= query_start < _MOST:
+        raise ValueError(f"{who}: query_start must lie in 0..{_MOST - 1}, got {query_start}")
+    if k.dim() == q.dim() == 4 and k.shape[0] != q.shape[0]:
+        raise ValueError(f"{who}: q has {q.shape[0]} batch entries, k and v {k.shape[0]}")
+    _check_attention(who, q, [("k and v", k, v)])
+    watch_status(q)
+    with on_device(q):
+        lengths = ops.device_lengths(kv_valid_len, q.shape[0], k.shape[2], q.device)
+        args = (q, k, v, sm_scale, 0 if window is None or window >= _MOST else int(window), min(int(sinks), _MOST),
+                -1 if query_start is None else int(query_start), lengths)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            o, lse = WindowAttentionFunc.apply(*args)
+        else:
+            o, lse = ops.window_forward(*args)
+    return (o, lse) if return_lse else o
