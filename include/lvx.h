@@ -377,6 +377,21 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
                         const lvx_view* v, const void* o, const float* lse, const int32_t* kv_valid_len, float sm_scale,
                         void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream);
 
+/* Attention for a batch that shares long prefixes: the B requests of `s` (a multiple of `prefixes`; the first B / prefixes
+ * of them share the first prefix, and so on) see all valid keys of their prefix and their own keys (s->Skv of them, kv_valid_len
+ * valid) as in lvx_window_forward without a window and with query_start = -1; one softmax over both. s->Skv may be 0. pk, pv:
+ * [prefixes, Hkv, prefix_len, 128]; prefix_valid_len int32 [prefixes] or NULL. Keys behind the valid ones are never looked at.
+ * In the reference every sample of a batch carries visual states of its own (test_llama3.py:69-79). */
+int lvx_shared_workspace(const lvx_shape* s, int prefixes, int prefix_len, size_t* fwd_bytes, size_t* bwd_bytes);
+int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const lvx_view* q, const lvx_view* pk, const lvx_view* pv,
+                       const int32_t* prefix_valid_len, const lvx_view* k, const lvx_view* v, const int32_t* kv_valid_len,
+                       float sm_scale, void* workspace, size_t workspace_bytes, void* o, float* lse, void* stream);
+/* dpk, dpv like pk, pv and dk, dv like k, v, dense; o, d_o, dq dense. */
+int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const void* d_o, const lvx_view* q, const lvx_view* pk,
+                        const lvx_view* pv, const int32_t* prefix_valid_len, const lvx_view* k, const lvx_view* v,
+                        const int32_t* kv_valid_len, const void* o, const float* lse, float sm_scale, void* workspace,
+                        size_t workspace_bytes, void* dq, void* dpk, void* dpv, void* dk, void* dv, void* stream);
+
 /* Self-test of the tensor-core building blocks (TMA tile load, shared-memory and TMEM operand
  * descriptors, TMEM load/store): runs one 128 x N x K product in the operand arrangement `mode`
  * and writes D (fp32 [128,N]) to `d_out`. a/b are device buffers in the arrangement the mode

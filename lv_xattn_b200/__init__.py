@@ -33,4 +33,4 @@ from .hf_patch import (  # noqa: F401,E402
 from .host_io import HostStreamedAttention  # noqa: F401,E402
 from .peer_memory import check_device_status  # noqa: F401,E402
 from .rotary import head_norm_rope  # noqa: F401,E402
-from .text_attention import window_attention  # noqa: F401,E402
+from .text_attention import shared_prefix_attention, window_attention  # noqa: F401,E402

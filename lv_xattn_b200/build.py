@@ -15,7 +15,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB_PATH = os.path.join(PKG_DIR, "liblvx.so")
 SOURCES = ["abi.cu", "selftest.cu", "fwd_sm100.cu", "fwd_rows_sm100.cu", "elementwise.cu", "bwd_sm100.cu", "noalloc.cu", "general_tf32.cu", "p2p.cu", "kvproj_sm100.cu", "head_norm.cu", "window_fwd_sm100.cu",
-           "window_bwd_sm100.cu"]
+           "window_bwd_sm100.cu", "shared_prefix.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
     "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--expt-relaxed-constexpr",

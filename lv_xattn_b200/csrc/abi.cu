@@ -743,6 +743,169 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
   return rc || direct ? rc : launch_window_dq(*s, dq_acc, dq, sp, st);
 }
 
+// The pieces of a call with shared prefixes: the prefix as an attention of packed rows, and the layout of the scratch.
+struct SharedCall {
+  lvx_shape pre;            // B = prefixes, one "head" per packed row, Sq = 1
+  lvx_window pre_win, own_win;
+  FwdPlan pre_plan, own_plan;
+  bool pre_few, own_few;
+  bool packed;              // the packed order is another one than q's
+  size_t rows;              // B * Hq * Sq
+};
+static size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+static int shared_call(SharedCall* c, const lvx_shape* s, int prefixes, int prefix_len, const char* who) {
+  c->own_win = lvx_window{0, 0, -1};
+  int rc = check_window(s, &c->own_win, who);
+  if (rc) return rc;
+  if (prefixes < 1 || s->B % prefixes) return fail(LVX_ERR_SHAPE, "%s: %d requests are not a multiple of %d prefixes", who, s->B, prefixes);
+  if (prefix_len < 1 || prefix_len >= kWindowMaxLen) return fail(LVX_ERR_SHAPE, "%s: a prefix of %d keys", who, prefix_len);
+  const int64_t rows = int64_t(s->B / prefixes) * (s->Hq / s->Hkv) * s->Sq;      // of a prefix' KV head
+  if (rows * s->Hkv > (int64_t(1) << 30)) return fail(LVX_ERR_SHAPE, "%s: dimension too large", who);
+  c->pre = *s;
+  c->pre.B = prefixes;
+  c->pre.Hq = int32_t(rows * s->Hkv);
+  c->pre.Sq = 1;
+  c->pre.Skv = prefix_len;
+  c->pre_win = lvx_window{0, 0, prefix_len};      // every row stands behind all keys
+  if ((rc = check_window(&c->pre, &c->pre_win, who))) return rc;
+  c->pre_plan = plan_window(c->pre, c->pre_win, &c->pre_few);
+  c->own_plan = plan_window(*s, c->own_win, &c->own_few);
+  c->packed = s->B != prefixes && s->Hkv > 1;
+  c->rows = size_t(s->B) * s->Hq * s->Sq;
+  return LVX_OK;
+}
+
+int lvx_shared_workspace(const lvx_shape* s, int prefixes, int prefix_len, size_t* fwd_bytes, size_t* bwd_bytes) {
+  SharedCall c;
+  const int rc = shared_call(&c, s, prefixes, prefix_len, "lvx_shared_workspace");
+  if (rc) return rc;
+  const size_t es = elt_size(s->dtype), row_bytes = round256(c.rows * 128 * es), stat = round256(c.rows * 4);
+  const size_t own = s->Skv > 0 ? c.own_plan.o_part_bytes + c.own_plan.ml_part_bytes : 0;
+  if (fwd_bytes) *fwd_bytes = c.pre_plan.o_part_bytes + c.pre_plan.ml_part_bytes + own + row_bytes;
+  if (bwd_bytes) {
+    const bool f32 = s->dtype == LVX_FP32;
+    const size_t acc = f32 ? c.rows * 512 : window_dq_floats(c.pre) * 4;
+    const size_t acc_own = s->Skv == 0 ? 0 : f32 ? c.rows * 512 : window_dq_floats(*s) * 4;
+    *bwd_bytes = 3 * stat + 2 * row_bytes + round256(acc) + acc_own;
+  }
+  return LVX_OK;
+}
+
+int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const lvx_view* q, const lvx_view* pk, const lvx_view* pv,
+                       const int32_t* prefix_valid_len, const lvx_view* k, const lvx_view* v, const int32_t* kv_valid_len,
+                       float sm_scale, void* workspace, size_t workspace_bytes, void* o, float* lse, void* stream) {
+  const char* who = "lvx_shared_forward";
+  SharedCall c;
+  int rc = shared_call(&c, s, prefixes, prefix_len, who);
+  if (!rc) rc = check_qkv_views(s, q, s->Skv > 0 ? k : q, s->Skv > 0 ? v : q, who);
+  if (rc) return rc;
+  const lvx_view packed_q = dense_view(c.packed ? workspace : q->data, c.pre.Hq, 1);
+  if ((rc = check_qkv_views(&c.pre, &packed_q, pk, pv, who)) || (rc = check_arch())) return rc;
+  if (!(sm_scale > 0.f)) return fail(LVX_ERR_SHAPE, "%s: sm_scale must be positive", who);
+  LVX_REQUIRE_PTR(o, who);
+  LVX_REQUIRE_PTR(lse, who);
+  LVX_REQUIRE_PTR(workspace, who);
+  size_t need = 0;
+  if ((rc = lvx_shared_workspace(s, prefixes, prefix_len, &need, nullptr))) return rc;
+  if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
+  int* sp = status_ptr();
+  if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* at = static_cast<char*>(workspace) + round256(c.rows * 128 * elt_size(s->dtype));
+  auto take = [&](size_t n) {
+    float* p = reinterpret_cast<float*>(at);
+    at += n;
+    return p;
+  };
+  float* o_pre = take(c.pre_plan.o_part_bytes);
+  float* ml_pre = take(c.pre_plan.ml_part_bytes);
+  float *o_own = nullptr, *ml_own = nullptr;
+  // q as it lies serves where the orders agree, if it is dense
+  const bool dense = q->stride_s == 128 && q->stride_h == int64_t(s->Sq) * 128 && q->stride_b == int64_t(s->Hq) * s->Sq * 128;
+  lvx_view pq = packed_q;
+  if (c.packed || !dense) {
+    pq.data = workspace;
+    if ((rc = launch_pack_rows(*s, prefixes, *q, nullptr, nullptr, nullptr, workspace, nullptr, nullptr, nullptr, st))) return rc;
+  }
+  if (s->Skv > 0) {
+    o_own = take(c.own_plan.o_part_bytes);
+    ml_own = take(c.own_plan.ml_part_bytes);
+    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, sp, st)))
+      return rc;
+  }
+  if ((rc = window_forward(&c.pre, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre,
+                           nullptr, nullptr, sp, st)))
+    return rc;
+  return launch_shared_combine(*s, prefixes, o_pre, ml_pre, c.pre_plan.nsplit, o_own, ml_own, o_own ? c.own_plan.nsplit : 0, o, lse, st);
+}
+
+int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const void* d_o, const lvx_view* q, const lvx_view* pk,
+                        const lvx_view* pv, const int32_t* prefix_valid_len, const lvx_view* k, const lvx_view* v,
+                        const int32_t* kv_valid_len, const void* o, const float* lse, float sm_scale, void* workspace,
+                        size_t workspace_bytes, void* dq, void* dpk, void* dpv, void* dk, void* dv, void* stream) {
+  const char* who = "lvx_shared_backward";
+  SharedCall c;
+  int rc = shared_call(&c, s, prefixes, prefix_len, who);
+  if (!rc) rc = check_qkv_views(s, q, s->Skv > 0 ? k : q, s->Skv > 0 ? v : q, who);
+  if (rc) return rc;
+  const lvx_view packed_q = dense_view(c.packed ? workspace : q->data, c.pre.Hq, 1);
+  if ((rc = check_qkv_views(&c.pre, &packed_q, pk, pv, who)) || (rc = check_arch())) return rc;
+  if (!(sm_scale > 0.f)) return fail(LVX_ERR_SHAPE, "%s: sm_scale must be positive", who);
+  LVX_REQUIRE_PTR(d_o, who);
+  LVX_REQUIRE_PTR(o, who);
+  LVX_REQUIRE_PTR(lse, who);
+  LVX_REQUIRE_PTR(dq, who);
+  LVX_REQUIRE_PTR(dpk, who);
+  LVX_REQUIRE_PTR(dpv, who);
+  LVX_REQUIRE_PTR(workspace, who);
+  if (s->Skv > 0) {
+    LVX_REQUIRE_PTR(dk, who);
+    LVX_REQUIRE_PTR(dv, who);
+  }
+  size_t need = 0;
+  if ((rc = lvx_shared_workspace(s, prefixes, prefix_len, nullptr, &need))) return rc;
+  if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
+  int* sp = status_ptr();
+  if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool f32 = s->dtype == LVX_FP32;
+  const size_t row_bytes = round256(c.rows * 128 * elt_size(s->dtype)), stat = round256(c.rows * 4);
+  char* at = static_cast<char*>(workspace);
+  auto take = [&](size_t n) {
+    char* p = at;
+    at += n;
+    return p;
+  };
+  float* delta = reinterpret_cast<float*>(take(stat));
+  float* lse_p = reinterpret_cast<float*>(take(stat));
+  float* delta_p = reinterpret_cast<float*>(take(stat));
+  char* q_p = take(row_bytes);
+  char* do_p = take(row_bytes);
+  float* acc = reinterpret_cast<float*>(at);
+  const size_t acc_bytes = round256(f32 ? c.rows * 512 : window_dq_floats(c.pre) * 4);
+  float* acc_own = s->Skv > 0 ? reinterpret_cast<float*>(at + acc_bytes) : nullptr;
+  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
+  const cudaError_t e = cudaMemsetAsync(acc, 0, static_cast<char*>(workspace) + need - at, st);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dq)");
+  const bool dense = q->stride_s == 128 && q->stride_h == int64_t(s->Sq) * 128 && q->stride_b == int64_t(s->Hq) * s->Sq * 128;
+  const bool pack = c.packed || !dense;
+  if (pack && (rc = launch_pack_rows(*s, prefixes, *q, d_o, lse, delta, q_p, do_p, lse_p, delta_p, st))) return rc;
+  const lvx_view pq = dense_view(pack ? q_p : q->data, c.pre.Hq, 1), pdo = dense_view(pack ? do_p : d_o, c.pre.Hq, 1);
+  const float *pl = pack ? lse_p : lse, *pd = pack ? delta_p : delta;
+  const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
+  rc = f32 ? launch_bwd_block_general(c.pre, pq.data, pdo.data, pl, pd, pk->data, pv->data, prefix_valid_len, nullptr, sm_scale, acc,
+                                      dpk, dpv, 2, st, &c.pre_win)
+           : launch_window_bwd(c.pre, c.pre_win, pq, pdo, *pk, *pv, pl, pd, prefix_valid_len, sm_scale, acc, dpk, dpv, sp, st);
+  if (!rc && s->Skv > 0)
+    rc = f32 ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, acc_own, dk,
+                                        dv, 2, st, &c.own_win)
+             : launch_window_bwd(*s, c.own_win, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, acc_own, dk, dv, sp, st);
+  if (rc) return rc;
+  const QTiles pt = make_q_tiles(c.pre.Hq / c.pre.Hkv, 1);
+  const long pre_slab_rows = f32 ? c.pre.Hq / c.pre.Hkv : long(pt.chunks) * pt.heads;
+  return launch_shared_dq(*s, prefixes, acc, pre_slab_rows, acc_own, dq, st);
+}
+
 int lvx_selftest_mma(int mode, const void* a, const void* b, float* d_out, void* stream) {
   const char* who = "lvx_selftest_mma";
   int rc = check_arch();

@@ -82,6 +82,13 @@ int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q
                       const lvx_view& v, const float* lse, const float* delta, const int32_t* kv_valid_len, float sm_scale,
                       float* dq_acc, void* dk, void* dv, int* status, cudaStream_t st);
 int launch_window_dq(const lvx_shape& s, const float* acc, void* dq, const int* status, cudaStream_t st);
+// Around the windowed kernels for a batch that shares prefixes (shared_prefix.cu).
+int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const void* d_o, const float* lse, const float* delta,
+                     void* q_out, void* do_out, float* lse_out, float* delta_out, cudaStream_t st);
+int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
+                          const float* ml_own, int ns_own, void* o, float* lse, cudaStream_t st);
+int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, long pre_slab_rows, const float* acc_own, void* dq,
+                     cudaStream_t st);
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
                        cudaStream_t st);

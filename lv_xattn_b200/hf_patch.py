@@ -27,6 +27,8 @@ import torch.distributed as dist
 from .async_communication import get_sequence_parallel_group, get_sequence_parallel_rank, get_sequence_parallel_size
 from .attn import LVXAttnRecomputeFunc, RingAttnRecomputeFunc
 from .projection import kv_project
+from .rotary import head_norm_rope
+from .text_attention import window_attention
 
 ATTENTION_MODES = ("lv_xattn", "ring", "ring_self")      # the reference's modes (test_llama3.py:107)
 
@@ -127,7 +129,7 @@ class _AllGatherSeq(torch.autograd.Function):
         return g[:, :, r * n:(r + 1) * n].contiguous()
 
 
-def patch_self_attention_forward(attention_mode="lv_xattn"):
+def patch_self_attention_forward(attention_mode="lv_xattn", window=None, sinks=0):
     """Returns an unbound `forward` for `MllamaTextSelfAttention` (reference test_llama3.py:263-354).
 
     The text sequence is short next to the visual one (2,048 tokens in the end-to-end configuration), so the
@@ -136,8 +138,16 @@ def patch_self_attention_forward(attention_mode="lv_xattn"):
     this rank's slice of the rotary tables. The attention itself is torch's scaled_dot_product_attention: the
     self-attention layers are not the path this library accelerates. Every attention_mode gets this
     implementation: the reference's "ring_self" applies its causal mask with rank-local indices at every step
-    (ring/attn.py:280), which is not globally correct, so it is not reproduced."""
+    (ring/attn.py:280), which is not globally correct, so it is not reproduced.
+
+    With a `window` (and `sinks`) every token sees the window of tokens that ends with it, and the first `sinks` ones. The
+    layer then runs on this library's kernels: `head_norm_rope` rotates queries and keys on their way into the kernels'
+    layout, and `window_attention` reads only the keys that are seen. CUDA tensors with a head dimension of 128."""
     _check_mode(attention_mode)
+    if window is None and sinks:
+        raise ValueError("sinks stay visible beside a window: give the window")
+    if window is not None and (window < 1 or sinks < 0):
+        raise ValueError(f"window must be at least 1 and sinks not negative, got {window} and {sinks}")
 
     def forward(self, hidden_states, attention_mask=None, position_embeddings=None, output_attentions=False,
                 use_cache=False, past_key_values=None, cache_position=None, past_key_value=None, **kwargs):
@@ -148,6 +158,15 @@ def patch_self_attention_forward(attention_mode="lv_xattn"):
             raise NotImplementedError("KV caching is a decoding feature; this hook is the training path")
         bsz, q_len, _ = hidden_states.size()
         nh, nkv, hd = self.num_heads, self.num_key_value_heads, self.head_dim
+        if window is not None:
+            q, k = (proj(hidden_states).view(bsz, q_len, n, hd) for proj, n in ((self.q_proj, nh), (self.k_proj, nkv)))
+            v = self.v_proj(hidden_states).view(bsz, q_len, nkv, hd).transpose(1, 2)
+            cos, sin = position_embeddings
+            q, k = head_norm_rope(q, k, cos=cos, sin=sin)
+            if get_sequence_parallel_size() > 1:
+                k, v = _AllGatherSeq.apply(k), _AllGatherSeq.apply(v)
+            out = window_attention(q, k, v, self.scaling, window=window, sinks=sinks, query_start=get_sequence_parallel_rank() * q_len)
+            return self.o_proj(out.transpose(1, 2).reshape(bsz, q_len, nh * hd)), None
         q = self.q_proj(hidden_states).view(bsz, q_len, nh, hd).transpose(1, 2)
         k = self.k_proj(hidden_states).view(bsz, q_len, nkv, hd).transpose(1, 2)
         v = self.v_proj(hidden_states).view(bsz, q_len, nkv, hd).transpose(1, 2)
@@ -170,16 +189,20 @@ def patch_self_attention_forward(attention_mode="lv_xattn"):
 _SAVED_FORWARDS = {}
 
 
-def install_hooks(attention_mode="lv_xattn"):
+def install_hooks(attention_mode="lv_xattn", window=None, sinks=0):
     """Assigns the two hooks onto the installed transformers' Mllama text attention classes, as the reference's
     driver does (test_llama3.py:666-667). Every MllamaTextCrossAttention / MllamaTextSelfAttention of every model in
-    the process is then sequence-parallel; `uninstall_hooks()` restores the stock forwards."""
+    the process is then sequence-parallel; `uninstall_hooks()` restores the stock forwards. With a `window` (and `sinks`)
+    the self-attention layers are windowed, see patch_self_attention_forward."""
     from transformers.models.mllama import modeling_mllama as M
+    # made first: what they refuse leaves the classes as they were
+    cross_forward = patch_cross_attention_forward(attention_mode)
+    self_forward = patch_self_attention_forward(attention_mode, window, sinks)
     if not _SAVED_FORWARDS:
         _SAVED_FORWARDS["cross"] = M.MllamaTextCrossAttention.forward
         _SAVED_FORWARDS["self"] = M.MllamaTextSelfAttention.forward
-    M.MllamaTextCrossAttention.forward = patch_cross_attention_forward(attention_mode)
-    M.MllamaTextSelfAttention.forward = patch_self_attention_forward(attention_mode)
+    M.MllamaTextCrossAttention.forward = cross_forward
+    M.MllamaTextSelfAttention.forward = self_forward
 
 
 def uninstall_hooks():

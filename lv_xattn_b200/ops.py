@@ -685,3 +685,59 @@ def window_backward(do, q, k, v, o, lse, sm_scale: float, window: int, sinks: in
                                                _lib.stream_int()), "lvx_window_backward")
     _count(2 if q.dtype == torch.float32 else 3)
     return dq, dk, dv
+
+
+_shared_bytes: dict = {}
+
+
+def _shared_setup(q, pk, k):
+    shp = _lib.make_shape(q.shape[0], q.shape[1], pk.shape[1], q.shape[2], 0 if k is None else k.shape[2], 128, q.dtype)
+    P, N = pk.shape[0], pk.shape[2]
+    key = (shp.B, shp.Hq, shp.Hkv, shp.Sq, shp.Skv, shp.dtype, P, N)
+    sizes = _shared_bytes.get(key)
+    if sizes is None:
+        f, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        _lib.check(_lib.load().lvx_shared_workspace(ctypes.byref(shp), P, N, ctypes.byref(f), ctypes.byref(b)), "lvx_shared_workspace")
+        if len(_shared_bytes) >= 4096:
+            _shared_bytes.clear()
+        sizes = _shared_bytes[key] = f.value, b.value
+    return shp, P, N, sizes
+
+
+def _views(*ts):
+    return [None if t is None else _text_view(t) for t in ts]
+
+
+def _data(t):
+    return None if t is None else t.data_ptr()
+
+
+def shared_forward(q, pk, pv, k, v, sm_scale: float, prefix_valid_len, kv_valid_len):
+    """(o [B, Hq, Sq, 128], lse fp32 [B*Hq, Sq]) of attention over shared prefixes and own keys (lvx_shared_forward); k and v may
+    be None. The caller has checked the tensors."""
+    shp, P, N, (nbytes, _) = _shared_setup(q, pk, k)
+    views = _views(q, pk, pv, k, v)
+    o = q.new_empty(q.shape)
+    lse = q.new_empty(shp.B * shp.Hq, shp.Sq, dtype=torch.float32)
+    ws = lse.new_empty(nbytes // 4)
+    qv, pkv, pvv, kv, vv = (_ref(t) for t in views)
+    _lib.check(_lib.load().lvx_shared_forward(ctypes.byref(shp), P, N, qv, pkv, pvv, _data(prefix_valid_len), kv, vv,
+                                              _data(kv_valid_len), sm_scale, ws.data_ptr(), nbytes, o.data_ptr(), lse.data_ptr(),
+                                              _lib.stream_int()), "lvx_shared_forward")
+    _count(2 + (P < shp.B and shp.Hkv > 1) + (shp.Skv > 0))
+    return o, lse
+
+
+def shared_backward(do, q, pk, pv, k, v, o, lse, sm_scale: float, prefix_valid_len, kv_valid_len):
+    """(dq, dpk, dpv, dk, dv) of shared_forward."""
+    shp, P, N, (_, nbytes) = _shared_setup(q, pk, k)
+    views = _views(q, pk, pv, k, v)
+    do = _dense(do)
+    grads = [None if t is None else t.new_empty(t.shape) for t in (q, pk, pv, k, v)]
+    ws = lse.new_empty(nbytes // 4)
+    qv, pkv, pvv, kv, vv = (_ref(t) for t in views)
+    _lib.check(_lib.load().lvx_shared_backward(ctypes.byref(shp), P, N, do.data_ptr(), qv, pkv, pvv, _data(prefix_valid_len), kv, vv,
+                                               _data(kv_valid_len), o.data_ptr(), lse.data_ptr(), sm_scale, ws.data_ptr(), nbytes,
+                                               *(_data(t) for t in grads), _lib.stream_int()), "lvx_shared_backward")
+    _count(3 + (P < shp.B and shp.Hkv > 1) + (shp.Skv > 0))
+    return grads

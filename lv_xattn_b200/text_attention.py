@@ -102,3 +102,60 @@ def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=
         else:
             o, lse = ops.window_forward(*args)
     return (o, lse) if return_lse else o
+
+
+class SharedPrefixAttentionFunc(torch.autograd.Function):
+    """(q, k_prefix, v_prefix, k, v, sm_scale, prefix_valid_len, kv_valid_len, both on the device) -> (o, lse)."""
+
+    @staticmethod
+    def forward(ctx, q, pk, pv, k, v, sm_scale, prefix_valid_len, kv_valid_len):
+        o, lse = ops.shared_forward(q, pk, pv, k, v, sm_scale, prefix_valid_len, kv_valid_len)
+        ctx.save_for_backward(q, pk, pv, k, v, o, lse, prefix_valid_len, kv_valid_len)
+        ctx.sm_scale = sm_scale
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    def backward(ctx, do, _):
+        q, pk, pv, k, v, o, lse, prefix_valid_len, kv_valid_len = ctx.saved_tensors
+        with on_device(q):
+            grads = ops.shared_backward(do, q, pk, pv, k, v, o, lse, ctx.sm_scale, prefix_valid_len, kv_valid_len)
+        return (*(g if want else None for g, want in zip(grads, ctx.needs_input_grad)), None, None, None)
+
+
+def shared_prefix_attention(q, k_prefix, v_prefix, k=None, v=None, sm_scale=None, prefix_valid_len=None, kv_valid_len=None,
+                            return_lse=False):
+    """Attention of a batch of requests that share a long prefix (the tokens of a video, of a system prompt), which is read
+    once for all of them: o like q, dense; with `return_lse` also the log-sum-exp of every row's scores, fp32 [B*Hq, Sq].
+
+    q [B, Hq, Sq, 128]; k_prefix and v_prefix [P, Hkv, N, 128], B a multiple of P: the first B / P requests share the first
+    prefix, the next ones the second, and so on. k and v [B, Hkv, Skv, 128] are each request's own keys behind its prefix, or
+    None. Every query sees the whole prefix, and own key j where j < n_b and j <= n_b - Sq + i: as in `window_attention`, the
+    last query sits on the last of the n_b valid own keys. One softmax over both. bf16, fp16 or fp32, any strides.
+    prefix_valid_len (P integers) and kv_valid_len (B integers), a list or a tensor on the host or the device: how many keys
+    are valid; keys behind them are never looked at, whatever they hold. A query that sees nothing gets zeros, and -inf in
+    the log-sum-exp. Gradients flow into q and all keys and values; those of a prefix are summed over its requests."""
+    who = "shared_prefix_attention"
+    sm_scale = _scale(who, sm_scale)
+    if (k is None) != (v is None):
+        raise ValueError(f"{who}: k and v go together")
+    if k is None and kv_valid_len is not None:
+        raise ValueError(f"{who}: valid lengths of own keys that are not there")
+    if q.dim() == k_prefix.dim() == 4:
+        if k_prefix.shape[0] == 0 or q.shape[0] % k_prefix.shape[0]:
+            raise ValueError(f"{who}: {q.shape[0]} requests are not a multiple of {k_prefix.shape[0]} prefixes")
+        if k_prefix.shape[2] == 0:
+            raise ValueError(f"{who}: the prefix is empty")
+        if k is not None and k.dim() == 4 and (k.shape[0] != q.shape[0] or k.shape[1] != k_prefix.shape[1]):
+            raise ValueError(f"{who}: own keys {tuple(k.shape)} for {q.shape[0]} requests and {k_prefix.shape[1]} KV heads")
+    _check_attention(who, q, [("the prefix", k_prefix, v_prefix)] + ([] if k is None else [("k and v", k, v)]))
+    watch_status(q)
+    with on_device(q):
+        prefix_lengths = ops.device_lengths(prefix_valid_len, k_prefix.shape[0], k_prefix.shape[2], q.device)
+        lengths = ops.device_lengths(kv_valid_len, q.shape[0], 0 if k is None else k.shape[2], q.device)
+        args = (q, k_prefix, v_prefix, k, v, sm_scale, prefix_lengths, lengths)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+            o, lse = SharedPrefixAttentionFunc.apply(*args)
+        else:
+            o, lse = ops.shared_forward(*args)
+    return (o, lse) if return_lse else o

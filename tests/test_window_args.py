@@ -77,3 +77,15 @@ def test_every_seen_key_is_walked_once():
         assert len(set(walked)) == len(walked)
         seen = {j // 4 for p in range(p0, p0 + n) for j in range(min(valid, p + 1)) if j > p - window or j < sinks}
         assert seen <= set(walked) and all(4 * t < valid for t in walked)
+
+
+def test_hook_refusals():
+    from lv_xattn_b200 import hf_patch
+    mllama = pytest.importorskip("transformers.models.mllama.modeling_mllama")
+    before = mllama.MllamaTextCrossAttention.forward, mllama.MllamaTextSelfAttention.forward
+    for args in (dict(sinks=4), dict(window=0), dict(window=8, sinks=-1)):
+        with pytest.raises(ValueError):
+            hf_patch.patch_self_attention_forward("lv_xattn", **args)
+        with pytest.raises(ValueError):
+            hf_patch.install_hooks("lv_xattn", **args)
+    assert before == (mllama.MllamaTextCrossAttention.forward, mllama.MllamaTextSelfAttention.forward)
