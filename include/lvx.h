@@ -327,8 +327,7 @@ int lvx_bwd_block_gathered(const lvx_shape* s, const void* q, const void* d_o, c
 int lvx_p2p_wait(const uint32_t* my_flags, int world, int slot, uint32_t epoch, void* stream);
 
 /* A strided [B, heads, S, 128] tensor: element (b, h, s, d) at data[b*stride_b + h*stride_h + s*stride_s + d], strides in
- * elements. Rows (128 elements) are contiguous; 16-byte aligned, with strides that keep them so (8 bytes suffice for
- * lvx_head_norm_rope on 16-bit types). */
+ * elements. Rows (128 elements) are contiguous; 16-byte aligned, with strides that keep them so. */
 typedef struct lvx_view {
   void* data;
   int64_t stride_b, stride_h, stride_s;

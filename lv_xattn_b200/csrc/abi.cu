@@ -2,6 +2,7 @@
 // tensor-map encoding through the driver entry point, and the device status word.
 #include "lvx_internal.h"
 #include "window.cuh"
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -564,17 +565,20 @@ static int check_head_norm(const lvx_head_norm* c, const lvx_view* q, const lvx_
   if (!q && !k) return fail(LVX_ERR_NULL, "%s: neither q nor k is given", who);
   if (!(c->eps >= 0.f)) return fail(LVX_ERR_SHAPE, "%s: eps must be non-negative", who);
   if ((c->cos == nullptr) != (c->sin == nullptr)) return fail(LVX_ERR_NULL, "%s: cos and sin go together", who);
-  const int es = elt_size(c->dtype), align = es * 4;
+  // units (two heads of a token at least) are counted in 32 bits
+  if (int64_t(c->B) * c->S * std::max((c->Hq + 1) / 2, (c->Hkv + 1) / 2) >= (int64_t(1) << 31))
+    return fail(LVX_ERR_LIMIT, "%s: B*S*heads too large", who);
+  const int es = elt_size(c->dtype), align = 16;
   if (head_norm_rows(c, q, k) == 0) return LVX_OK;      // nothing is read, and nothing need be there
   int rc = check_view(q, es, align, who, "q");
   if (!rc) rc = check_view(k, es, align, who, "k");
   if (rc) return rc;
-  const int ws = c->weight_fp32 ? 4 : es, ts = c->table_fp32 ? 4 : es;
-  if ((reinterpret_cast<uintptr_t>(c->wq) | reinterpret_cast<uintptr_t>(c->wk)) & (ws * 4 - 1))
-    return fail(LVX_ERR_ALIGN, "%s: a weight is not %d-byte aligned", who, ws * 4);
+  const int ts = c->table_fp32 ? 4 : es;
+  if ((reinterpret_cast<uintptr_t>(c->wq) | reinterpret_cast<uintptr_t>(c->wk)) & 15u)
+    return fail(LVX_ERR_ALIGN, "%s: a weight is not 16-byte aligned", who);
   if ((reinterpret_cast<uintptr_t>(c->cos) | reinterpret_cast<uintptr_t>(c->sin) |
-       (c->cos ? uintptr_t(c->table_stride_b | c->table_stride_s) * ts : 0)) & (ts * 4 - 1))
-    return fail(LVX_ERR_ALIGN, "%s: rows of cos and sin are not %d-byte aligned", who, ts * 4);
+       (c->cos ? uintptr_t(c->table_stride_b | c->table_stride_s) * ts : 0)) & 15u)
+    return fail(LVX_ERR_ALIGN, "%s: rows of cos and sin are not 16-byte aligned", who);
   return validate_arch();
 }
 
@@ -595,7 +599,7 @@ int lvx_head_norm_rope_bwd(const lvx_head_norm* c, const lvx_view* q, const lvx_
   if (rc) return rc;
   if ((q == nullptr) != (gq == nullptr) || (k == nullptr) != (gk == nullptr))
     return fail(LVX_ERR_NULL, "%s: q and gq, k and gk go together", who);
-  const int es = elt_size(c->dtype), align = es * 4;
+  const int es = elt_size(c->dtype), align = 16;
   const bool rows = head_norm_rows(c, q, k) > 0;
   if (rows && ((rc = check_view(gq, es, align, who, "gq")) || (rc = check_view(gk, es, align, who, "gk")))) return rc;
   if ((dwq && !(q && c->wq)) || (dwk && !(k && c->wk))) return fail(LVX_ERR_NULL, "%s: a gradient of a weight that is not there", who);
@@ -662,7 +666,7 @@ int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_by
   const bool direct = !few && p.nsplit == 1 && s->dtype != LVX_FP32;
   if (fwd_bytes) *fwd_bytes = direct ? 0 : p.o_part_bytes + p.ml_part_bytes;
   const size_t delta = ((size_t(s->B) * s->Hq * s->Sq * 4 + 255) & ~size_t(255));
-  if (bwd_bytes) *bwd_bytes = delta + (s->dtype == LVX_FP32 ? 0 : window_dq_floats(*s) * 4);
+  if (bwd_bytes) *bwd_bytes = delta + (s->dtype == LVX_FP32 ? 0 : (window_dq_floats(*s) + window_sink_floats(*s, *w)) * 4);
   return LVX_OK;
 }
 
@@ -731,6 +735,7 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
   const size_t rows = size_t(s->B) * s->Hq * s->Sq;
   float* delta = static_cast<float*>(workspace);
   float* dq_acc = direct ? static_cast<float*>(dq) : reinterpret_cast<float*>(static_cast<char*>(workspace) + ((rows * 4 + 255) & ~size_t(255)));
+  float* parts = direct ? nullptr : dq_acc + window_dq_floats(*s);
   if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
   const cudaError_t e = cudaMemsetAsync(dq_acc, 0, direct ? rows * 512 : window_dq_floats(*s) * 4, st);
   if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dq)");
@@ -738,9 +743,9 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
     const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
     rc = direct ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, dq_acc,
                                            dk, dv, 2, st, w)
-                : launch_window_bwd(*s, *w, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, dq_acc, dk, dv, sp, st);
+                : launch_window_bwd(*s, *w, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, dq_acc, parts, dk, dv, sp, st);
   }
-  return rc || direct ? rc : launch_window_dq(*s, dq_acc, dq, sp, st);
+  return rc || direct ? rc : launch_window_dq(*s, *w, dq_acc, parts, dq, dk, dv, sp, st);
 }
 
 // The pieces of a call with shared prefixes: the prefix as an attention of packed rows, and the layout of the scratch.
@@ -895,11 +900,11 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
   const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
   rc = f32 ? launch_bwd_block_general(c.pre, pq.data, pdo.data, pl, pd, pk->data, pv->data, prefix_valid_len, nullptr, sm_scale, acc,
                                       dpk, dpv, 2, st, &c.pre_win)
-           : launch_window_bwd(c.pre, c.pre_win, pq, pdo, *pk, *pv, pl, pd, prefix_valid_len, sm_scale, acc, dpk, dpv, sp, st);
+           : launch_window_bwd(c.pre, c.pre_win, pq, pdo, *pk, *pv, pl, pd, prefix_valid_len, sm_scale, acc, nullptr, dpk, dpv, sp, st);
   if (!rc && s->Skv > 0)
     rc = f32 ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, acc_own, dk,
                                         dv, 2, st, &c.own_win)
-             : launch_window_bwd(*s, c.own_win, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, acc_own, dk, dv, sp, st);
+             : launch_window_bwd(*s, c.own_win, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, acc_own, nullptr, dk, dv, sp, st);
   if (rc) return rc;
   const QTiles pt = make_q_tiles(c.pre.Hq / c.pre.Hkv, 1);
   const long pre_slab_rows = f32 ? c.pre.Hq / c.pre.Hkv : long(pt.chunks) * pt.heads;

@@ -30,6 +30,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
+#include <algorithm>
 #include <type_traits>
 
 namespace lvx {
@@ -419,6 +420,7 @@ struct Fp32BwdParams {
   const int* status;   // device status word: non-zero => return at once
   WindowMask mask;     // WIN (one query block, dense rows)
   int sq;
+  int share;           // WIN: row tiles that a CTA walks at most, of those that see its keys; its share is blockIdx.z'th
 };
 
 // A CTA owns 64 keys (K, V in shared memory, dK, dV in registers) and walks over the packed query rows 64 at a time: S and
@@ -461,7 +463,11 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
     }
     return it;
   };
-  const int first = walk_to(0);
+  int first = walk_to(0);
+  if constexpr (WIN) {
+    for (int skip = blockIdx.z * p.share; skip > 0 && first < ntot; --skip) first = walk_to(first + 1);
+    if (first >= ntot && gridDim.z > 1) return;      // nothing left to add (with the whole CTA)
+  }
   auto qslab_of = [&](int it) { return slab + (it / tiles_per_block) * p.kv_slabs; };
   auto load_q = [&](int it, int stage) {
     load_rows(sQ + stage * GT_TILE, static_cast<const T*>(p.q) + size_t(qslab_of(it)) * p.rows * 128,
@@ -489,9 +495,9 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
       load_do(first);
       cp_commit();
     }
-    int stage = 0;
+    int stage = 0, left = WIN ? p.share : 0;
     for (int it = first, next; it < ntot; it = next, stage ^= 1) {
-      next = walk_to(it + 1);
+      next = WIN && --left == 0 ? ntot : walk_to(it + 1);
       const int qslab = qslab_of(it), q0 = (it % tiles_per_block) * 64;
       float l2[2], dl[2];
       const float* br[2];
@@ -614,7 +620,10 @@ fp32_bwd_kernel(const Fp32BwdParams p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float a = dk[n][2 * i + e] * p.scale, b = dv[n][2 * i + e];
-        if (p.accumulate == 2) {                          // finished gradients in the input dtype
+        if (WIN && gridDim.z > 1) {                       // several CTAs add to what the launcher has cleared
+          atomicAdd(static_cast<float*>(p.dk_acc) + off + n * 8 + e, a);
+          atomicAdd(static_cast<float*>(p.dv_acc) + off + n * 8 + e, b);
+        } else if (p.accumulate == 2) {                   // finished gradients in the input dtype
           from_f32(static_cast<T*>(p.dk_acc) + off + n * 8 + e, a);
           from_f32(static_cast<T*>(p.dv_acc) + off + n * 8 + e, b);
         } else {
@@ -701,6 +710,19 @@ int launch_bwd_block_general(const lvx_shape& s, const void* q, const void* d_o,
   if (win) {
     p.mask = make_window_mask(*win);
     p.sq = s.Sq;
+    // Keys are seen by very different numbers of rows (sinks by all of them), and small calls have fewer key tiles than the
+    // GPU has SMs, so the rows of a key tile are shared out over CTAs: about two rounds of CTAs for all of them together.
+    // 512 tokens, 32 heads, window 128: 528 us with a CTA per key tile, which waited for the sinks' 32 row tiles.
+    const long tiles = (p.rows + 63) / 64, keys = long(grid.x) * grid.y;
+    const long seen = std::min<long>(tiles, p.mask.window < kNoWindow ? (long(p.mask.window) + 126) * (p.rows / s.Sq) / 64 + 2 : tiles);
+    p.share = int(std::max<long>(2, (keys * seen + 295) / 296));
+    grid.z = unsigned((tiles + p.share - 1) / p.share);
+    if (grid.z > 1) {
+      const size_t n = size_t(s.B) * s.Hkv * s.Skv * 128 * sizeof(float);
+      e = cudaMemsetAsync(dk_acc, 0, n, st);
+      if (e == cudaSuccess) e = cudaMemsetAsync(dv_acc, 0, n, st);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dk, dv)");
+    }
     go(fp32_bwd_kernel<float, true>);
   } else if (s.dtype == LVX_FP32) {
     go(fp32_bwd_kernel<float, false>);

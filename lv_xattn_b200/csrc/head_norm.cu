@@ -7,26 +7,37 @@
 //             dx = r (w dy - xh mean_d(w dy xh)),   dw = sum over rows of dy xh
 // All of it in fp32, rounded once when it is stored. r is computed again in the backward: x is read there anyway.
 //
-// Bound by memory (a row of 128 values in and out, two in and one out in the backward). Sixteen lanes work on a row; a
-// lane holds d = 4l..4l+3 and the same of the other half, so that the rotation needs no exchange between lanes. A lane
-// group takes four heads of one token (a unit): four rows in flight, and the token's cos and sin, which are as wide as
-// two rows in fp32, are fetched once for them. The units of a block are neighbours, mostly of one token, so the tables
-// come from L1. dw is kept in registers over a walk through the units, summed per block and then by a second kernel in a
-// fixed order: atomics on its 128 addresses would cost both time and the same result twice.
+// Bound by memory (a row of 128 values in and out, two in and one out in the backward), and close behind it by the issue of
+// instructions: values go through the packed fp32 unit two at a time, the weight is multiplied into cos and sin once for all
+// heads of a unit, and index arithmetic is 32 bits wide. Sixteen lanes work on a row; a lane holds d = 4l..4l+3 and the same of
+// the other half, so that the rotation needs no exchange between lanes. A lane group takes a few heads of one token (a unit):
+// its rows are in flight together, and the token's cos and sin, which are as wide as two rows in fp32, are fetched once for
+// them. The units of a block are neighbours, mostly of one token, so the tables come from L1.
+// Measured, bf16, 2 x 4,096 tokens of 32 + 8 heads (176 and 260 MB): forward 50 -> 38 us, backward 115 -> 68 us against one
+// value an instruction and 64-bit divisions. Registers are what decides: four heads a unit and two blocks an SM in the
+// backward 68 us (three blocks, which spill: 79 with two heads, 113 with four; one block 108), eight lanes a row 82; forward
+// 38 us with four heads and four blocks (eight heads and three blocks 35, but a call of four tokens then takes 4.3 us instead of
+// 3.3, on fewer SMs; five blocks, which spill, 52). A block works on queries or on keys; dw is kept in registers over its walk through the units, summed per block and then
+// by a second kernel in a fixed order: atomics on its 128 addresses would cost time, and another result every time.
 #include "lvx_internal.h"
 #include "sm100_prims.cuh"
 #include <algorithm>
 
 namespace lvx {
 
-constexpr int HN_U = 4;             // heads of a unit
-constexpr int HN_GROUPS = 16;       // lane groups of a block
-constexpr int HN_BWD_BLOCKS = 148 * 4;
-static_assert(HN_BWD_BLOCKS * 256 * sizeof(float) == LVX_HEAD_NORM_SCRATCH, "the header names the scratch's size");
+constexpr int HN_LANES = 16;                    // lanes that work on a row
+constexpr int HN_GROUPS = 256 / HN_LANES;       // lane groups of a block
+constexpr int HN_V = 64 / HN_LANES;             // values of each half that a lane holds
+constexpr int HN_P = HN_V / 2;                  // in pairs
+constexpr int HN_BWD_BLOCKS = 148 * 8;
+static_assert(HN_BWD_BLOCKS * 128 * sizeof(float) == LVX_HEAD_NORM_SCRATCH, "the header names the scratch's size");
+constexpr int hn_unit(int t) { return t == 2 ? 2 : 4; }      // heads of a unit
 
 struct HeadNormParams {
-  int S, heads[2], chunks[2];       // [0] queries, [1] keys; chunks: units of a token
-  long units;
+  int S;
+  int blocks_q;                     // blocks that work on queries; the others on keys
+  int heads[2], chunks[2];          // [0] queries, [1] keys; chunks: units of a token
+  unsigned units[2];                // B * S * chunks
   const void* x[2];
   long long x_b[2], x_h[2], x_s[2];
   const void* w[2];                 // nullptr: no norm
@@ -37,167 +48,236 @@ struct HeadNormParams {
   void* out[2];                     // forward: [B, H, S, 128]; backward: dx [B, S, H, 128], nullptr: not wanted
   const void* g[2];                 // backward: gradient of `out`
   long long g_b[2], g_h[2], g_s[2];
-  float* dw_part;                   // backward: [blocks][2][128], nullptr: no weight wants its gradient
+  float* dw_part;                   // backward: [blocks][128], nullptr: no weight wants its gradient
   const int* status;
 };
 
-// four values of either type
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
+
+// A lane's share of half a row, of either type, as it lies in memory, and as pairs of floats.
 template <int T>      // 0 bf16, 1 fp16, 2 fp32
-__device__ __forceinline__ float4 hn_load(const void* base, long long at) {
-  if (T == 2) return *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at);
-  const float2 a = unpack16x2<T == 0>(u.x), b = unpack16x2<T == 0>(u.y);
-  return make_float4(a.x, a.y, b.x, b.y);
-}
+struct RawHalf {
+  static constexpr int WORDS = HN_V * (T == 2 ? 4 : 2) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const void* base, long long at) {
+    const char* p = static_cast<const char*>(base) + at * (T == 2 ? 4 : 2);
+    if constexpr (WORDS == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x;
+      w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = v.x;
+        w[4 * i + 1] = v.y;
+        w[4 * i + 2] = v.z;
+        w[4 * i + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void get(uint64_t (&f)[HN_P]) const {
+#pragma unroll
+    for (int i = 0; i < HN_P; ++i) {
+      if constexpr (T == 2) {
+        f[i] = f32x2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      } else {
+        const float2 t = unpack16x2<T == 0>(w[i]);
+        f[i] = f32x2(t.x, t.y);
+      }
+    }
+  }
+};
 template <int T>
-__device__ __forceinline__ float4 hn_load_either(const void* base, long long at, int fp32) {
-  return T == 2 || fp32 ? hn_load<2>(base, at) : hn_load<T>(base, at);
-}
-template <int T>
-__device__ __forceinline__ void hn_store(void* base, long long at, float4 v) {
-  if (T == 2) {
-    *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = v;
+__device__ __forceinline__ void hn_load_either(uint64_t (&f)[HN_P], const void* base, long long at, int fp32) {
+  if (T == 2 || fp32) {
+    RawHalf<2> r;
+    r.load(base, at);
+    r.get(f);
   } else {
-    const uint2 u = T == 0 ? make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w)) : make_uint2(pack_f16x2(v.x, v.y), pack_f16x2(v.z, v.w));
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) = u;
+    RawHalf<T> r;
+    r.load(base, at);
+    r.get(f);
   }
 }
-__device__ __forceinline__ float4 hn_mul(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
-__device__ __forceinline__ float4 hn_scale(float4 a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
-__device__ __forceinline__ float4 hn_fma(float4 a, float4 b, float4 c) {
-  return make_float4(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y), fmaf(a.z, b.z, c.z), fmaf(a.w, b.w, c.w));
+template <int T>
+__device__ __forceinline__ void hn_store(void* base, long long at, const uint64_t (&f)[HN_P]) {
+  constexpr int WORDS = RawHalf<T>::WORDS;
+  uint32_t w[WORDS];
+#pragma unroll
+  for (int i = 0; i < HN_P; ++i) {
+    float a, b;
+    f32x2_get(f[i], a, b);
+    if constexpr (T == 2) {
+      w[2 * i] = __float_as_uint(a);
+      w[2 * i + 1] = __float_as_uint(b);
+    } else {
+      w[i] = T == 0 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
+    }
+  }
+  char* p = static_cast<char*>(base) + at * (T == 2 ? 4 : 2);
+  if constexpr (WORDS == 2) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS / 4; ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
 }
-__device__ __forceinline__ float4 hn_neg(float4 a) { return make_float4(-a.x, -a.y, -a.z, -a.w); }
-__device__ __forceinline__ float hn_dot(float4 a, float4 b) { return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, a.w * b.w))); }
-
-struct Half2 {        // a lane's share of a row: d = 4l.. and 64 + 4l..
-  float4 a, b;
-};
-// sum over the sixteen lanes of a group, of HN_U values at a time
-__device__ __forceinline__ void hn_sum(float (&v)[HN_U]) {
+__device__ __forceinline__ float hn_add(uint64_t v) {
+  float a, b;
+  f32x2_get(v, a, b);
+  return a + b;
+}
+// sum over the lanes of a group
+__device__ __forceinline__ float hn_sum(float v) {
 #pragma unroll
-  for (int off = 8; off > 0; off >>= 1)
-#pragma unroll
-    for (int u = 0; u < HN_U; ++u) v[u] += __shfl_xor_sync(0xffffffffu, v[u], off);
+  for (int off = HN_LANES / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
 }
 
 template <int T, bool BWD>
-__global__ void __launch_bounds__(HN_GROUPS * 16)
+__global__ void __launch_bounds__(256, BWD ? 2 : 4)
 head_norm_kernel(const HeadNormParams p) {
-  __shared__ float s_dw[BWD ? HN_GROUPS : 1][128];
+  constexpr int U = hn_unit(T), PER = 32 / HN_LANES;      // lane groups of a warp
+  __shared__ float s_dw[BWD ? HN_GROUPS : 1][BWD ? 132 : 1];
   int bad = 0;
   if (p.status) bad = *reinterpret_cast<const volatile int*>(p.status);
-  const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
-  Half2 dw[2];
+  const int group = threadIdx.x / HN_LANES, d = (threadIdx.x % HN_LANES) * HN_V;
+  const int which = int(blockIdx.x) >= p.blocks_q;
+  const unsigned block = which ? blockIdx.x - p.blocks_q : blockIdx.x, blocks = which ? gridDim.x - p.blocks_q : p.blocks_q;
+  const unsigned units = p.units[which], chunks = p.chunks[which];
+  const int heads = p.heads[which];
+  const void* ww = p.w[which];
+  const bool norm = ww != nullptr, rope = p.cos != nullptr;
+  uint64_t dwa[HN_P], dwb[HN_P];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) dw[i].a = dw[i].b = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int per_token = p.chunks[0] + p.chunks[1];
-  // The two groups of a warp walk together (their sums are exchanged with the whole warp's mask): the last unit may be
-  // done twice, by a group that then stores nothing.
-  for (long u0 = long(blockIdx.x) * HN_GROUPS + (group & ~1); u0 < p.units; u0 += long(gridDim.x) * HN_GROUPS) {
-    const long unit = min(u0 + (group & 1), p.units - 1);
-    const bool mine = u0 + (group & 1) < p.units;
-    const long token = unit / per_token;
-    int chunk = int(unit - token * per_token);
-    const int which = chunk >= p.chunks[0];
-    if (which) chunk -= p.chunks[0];
-    const long b = token / p.S, s = token - b * p.S;
-    const int h0 = chunk * HN_U, heads = p.heads[which];
-    const void* xw = p.x[which];
-    const void* ww = p.w[which];
-    Half2 x[HN_U], g[BWD ? HN_U : 1];
+  for (int i = 0; i < HN_P; ++i) dwa[i] = dwb[i] = 0ull;
+  // The lane groups of a warp walk together (their sums are exchanged under the whole warp's mask): the last unit may be
+  // done more than once, by groups that then store nothing.
+  for (unsigned u0 = block * HN_GROUPS + (group & ~(PER - 1)); u0 < units; u0 += blocks * HN_GROUPS) {
+    const unsigned unit = min(u0 + (group & (PER - 1)), units - 1);
+    const bool mine = u0 + (group & (PER - 1)) < units && !bad;
+    const unsigned token = unit / chunks, b = token / unsigned(p.S);
+    const int h0 = int(unit - token * chunks) * U, s = int(token - b * unsigned(p.S));
+    RawHalf<T> xa[U], xb[U], ga[BWD ? U : 1], gb[BWD ? U : 1];
 #pragma unroll
-    for (int u = 0; u < HN_U; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int h = min(h0 + u, heads - 1);
-      const long long at = b * p.x_b[which] + h * p.x_h[which] + s * p.x_s[which] + d;
-      if (!BWD || ww != nullptr) {
-        x[u].a = hn_load<T>(xw, at);
-        x[u].b = hn_load<T>(xw, at + 64);
+      if (!BWD || norm) {
+        const long long at = b * p.x_b[which] + h * p.x_h[which] + s * p.x_s[which] + d;
+        xa[u].load(p.x[which], at);
+        xb[u].load(p.x[which], at + 64);
       }
       if constexpr (BWD) {
-        const long long ga = b * p.g_b[which] + h * p.g_h[which] + s * p.g_s[which] + d;
-        g[u].a = hn_load<T>(p.g[which], ga);
-        g[u].b = hn_load<T>(p.g[which], ga + 64);
+        const long long at = b * p.g_b[which] + h * p.g_h[which] + s * p.g_s[which] + d;
+        ga[u].load(p.g[which], at);
+        gb[u].load(p.g[which], at + 64);
       }
     }
-    Half2 c, sn, w;
-    if (p.cos != nullptr) {
+    uint64_t ca[HN_P], cb[HN_P], sa[HN_P], sb[HN_P], wa[HN_P], wb[HN_P];
+    if (rope) {
       const long long at = b * p.t_b + s * p.t_s + d;
-      c.a = hn_load_either<T>(p.cos, at, p.table_fp32);
-      c.b = hn_load_either<T>(p.cos, at + 64, p.table_fp32);
-      sn.a = hn_load_either<T>(p.sin, at, p.table_fp32);
-      sn.b = hn_load_either<T>(p.sin, at + 64, p.table_fp32);
-    }
-    // The sums are exchanged between lanes whether this group has a norm or not: the warp's other group may.
-    float r[HN_U];
-    if (ww != nullptr) {
-      w.a = hn_load_either<T>(ww, d, p.w_fp32);
-      w.b = hn_load_either<T>(ww, d + 64, p.w_fp32);
-    }
+      hn_load_either<T>(ca, p.cos, at, p.table_fp32);
+      hn_load_either<T>(cb, p.cos, at + 64, p.table_fp32);
+      hn_load_either<T>(sa, p.sin, at, p.table_fp32);
+      hn_load_either<T>(sb, p.sin, at + 64, p.table_fp32);
 #pragma unroll
-    for (int u = 0; u < HN_U; ++u) r[u] = ww != nullptr ? hn_dot(x[u].a, x[u].a) + hn_dot(x[u].b, x[u].b) : 0.f;
-    hn_sum(r);
-#pragma unroll
-    for (int u = 0; u < HN_U; ++u) r[u] = rsqrtf(r[u] * (1.f / 128.f) + p.eps);
+      for (int i = 0; i < HN_P; ++i) sa[i] = neg2(sa[i]);
+    }
+    if (norm) {
+      hn_load_either<T>(wa, ww, d, p.w_fp32);
+      hn_load_either<T>(wb, ww, d + 64, p.w_fp32);
+    }
     if constexpr (!BWD) {
+      if (norm && rope) {
 #pragma unroll
-      for (int u = 0; u < HN_U; ++u) {
-        Half2 y = x[u];
-        if (ww != nullptr) {
-          y.a = hn_mul(hn_scale(y.a, r[u]), w.a);
-          y.b = hn_mul(hn_scale(y.b, r[u]), w.b);
+        for (int i = 0; i < HN_P; ++i) {
+          ca[i] = mul2(ca[i], wa[i]);
+          sa[i] = mul2(sa[i], wb[i]);
+          cb[i] = mul2(cb[i], wb[i]);
+          sb[i] = mul2(sb[i], wa[i]);
         }
-        if (p.cos != nullptr) {
-          const Half2 z = y;
-          y.a = hn_fma(z.a, c.a, hn_neg(hn_mul(z.b, sn.a)));
-          y.b = hn_fma(z.b, c.b, hn_mul(z.a, sn.b));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint64_t a[HN_P], c[HN_P];
+        xa[u].get(a);
+        xb[u].get(c);
+        uint64_t r2 = f32x2(1.f, 1.f);
+        if (norm) {
+          uint64_t q = mul2(a[0], a[0]);
+#pragma unroll
+          for (int i = 1; i < HN_P; ++i) q = fma2(a[i], a[i], q);
+#pragma unroll
+          for (int i = 0; i < HN_P; ++i) q = fma2(c[i], c[i], q);
+          const float r = rsqrtf(hn_sum(hn_add(q)) * (1.f / 128.f) + p.eps);
+          r2 = f32x2(r, r);
         }
-        if (mine && !bad && h0 + u < heads) {
-          const long long at = ((b * heads + h0 + u) * p.S + s) * 128 + d;
-          hn_store<T>(p.out[which], at, y.a);
-          hn_store<T>(p.out[which], at + 64, y.b);
+#pragma unroll
+        for (int i = 0; i < HN_P; ++i) {
+          const uint64_t x = a[i], y = c[i];
+          if (rope) {
+            a[i] = mul2(fma2(x, ca[i], mul2(y, sa[i])), r2);
+            c[i] = mul2(fma2(y, cb[i], mul2(x, sb[i])), r2);
+          } else if (norm) {
+            a[i] = mul2(mul2(x, wa[i]), r2);
+            c[i] = mul2(mul2(y, wb[i]), r2);
+          }
+        }
+        if (mine && h0 + u < heads) {
+          const long long at = ((static_cast<long long>(b) * heads + h0 + u) * p.S + s) * 128 + d;
+          hn_store<T>(p.out[which], at, a);
+          hn_store<T>(p.out[which], at + 64, c);
         }
       }
     } else {
-      float m[HN_U];
 #pragma unroll
-      for (int u = 0; u < HN_U; ++u) {
-        if (p.cos != nullptr) {
-          const Half2 z = g[u];
-          g[u].a = hn_fma(z.a, c.a, hn_mul(z.b, sn.b));
-          g[u].b = hn_fma(z.b, c.b, hn_neg(hn_mul(z.a, sn.a)));
-        }
-        m[u] = 0.f;
-        if (ww != nullptr) {
-          x[u].a = hn_scale(x[u].a, r[u]);
-          x[u].b = hn_scale(x[u].b, r[u]);
-          if (mine && h0 + u < heads) {
-            // (selected, not indexed: an array of registers has no run-time index)
-            if (which) {
-              dw[1].a = hn_fma(g[u].a, x[u].a, dw[1].a);
-              dw[1].b = hn_fma(g[u].b, x[u].b, dw[1].b);
-            } else {
-              dw[0].a = hn_fma(g[u].a, x[u].a, dw[0].a);
-              dw[0].b = hn_fma(g[u].b, x[u].b, dw[0].b);
-            }
+      for (int u = 0; u < U; ++u) {
+        uint64_t ya[HN_P], yb[HN_P];      // dy, then dx
+        ga[u].get(ya);
+        gb[u].get(yb);
+        if (rope) {
+#pragma unroll
+          for (int i = 0; i < HN_P; ++i) {
+            const uint64_t e = ya[i], f = yb[i];
+            ya[i] = fma2(e, ca[i], mul2(f, sb[i]));
+            yb[i] = fma2(f, cb[i], mul2(e, sa[i]));
           }
-          g[u].a = hn_mul(g[u].a, w.a);
-          g[u].b = hn_mul(g[u].b, w.b);
-          m[u] = hn_dot(g[u].a, x[u].a) + hn_dot(g[u].b, x[u].b);
         }
-      }
-      hn_sum(m);
+        if (norm) {
+          uint64_t a[HN_P], c[HN_P];
+          xa[u].get(a);
+          xb[u].get(c);
+          uint64_t q = 0ull, t = 0ull;
 #pragma unroll
-      for (int u = 0; u < HN_U; ++u) {
-        if (ww != nullptr) {
-          const float mean = -m[u] * (1.f / 128.f);
-          g[u].a = hn_scale(hn_fma(x[u].a, make_float4(mean, mean, mean, mean), g[u].a), r[u]);
-          g[u].b = hn_scale(hn_fma(x[u].b, make_float4(mean, mean, mean, mean), g[u].b), r[u]);
+          for (int i = 0; i < HN_P; ++i) {
+            q = fma2(c[i], c[i], fma2(a[i], a[i], q));
+            t = fma2(c[i], mul2(yb[i], wb[i]), fma2(a[i], mul2(ya[i], wa[i]), t));
+          }
+          const float r = rsqrtf(hn_sum(hn_add(q)) * (1.f / 128.f) + p.eps);
+          const float mean = hn_sum(hn_add(t)) * r * (1.f / 128.f);
+          const uint64_t r2 = f32x2(r, r), nm = f32x2(-mean * r, -mean * r);
+          const bool add = mine && h0 + u < heads;
+#pragma unroll
+          for (int i = 0; i < HN_P; ++i) {
+            const uint64_t xha = mul2(a[i], r2), xhb = mul2(c[i], r2);
+            if (add) {
+              dwa[i] = fma2(ya[i], xha, dwa[i]);
+              dwb[i] = fma2(yb[i], xhb, dwb[i]);
+            }
+            ya[i] = fma2(xha, nm, mul2(mul2(ya[i], wa[i]), r2));
+            yb[i] = fma2(xhb, nm, mul2(mul2(yb[i], wb[i]), r2));
+          }
         }
-        if (mine && !bad && p.out[which] != nullptr && h0 + u < heads) {
-          const long long at = ((b * p.S + s) * heads + h0 + u) * 128 + d;
-          hn_store<T>(p.out[which], at, g[u].a);
-          hn_store<T>(p.out[which], at + 64, g[u].b);
+        if (mine && p.out[which] != nullptr && h0 + u < heads) {
+          const long long at = ((static_cast<long long>(b) * p.S + s) * heads + h0 + u) * 128 + d;
+          hn_store<T>(p.out[which], at, ya);
+          hn_store<T>(p.out[which], at + 64, yb);
         }
       }
     }
@@ -206,63 +286,71 @@ head_norm_kernel(const HeadNormParams p) {
   if constexpr (BWD) {
     if (p.dw_part == nullptr || __syncthreads_or(bad)) return;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      __syncthreads();
-      *reinterpret_cast<float4*>(&s_dw[group][d]) = dw[i].a;
-      *reinterpret_cast<float4*>(&s_dw[group][d + 64]) = dw[i].b;
-      __syncthreads();
-      if (threadIdx.x < 128) {
-        float a = 0.f;
+    for (int i = 0; i < HN_P; ++i) {
+      f32x2_get(dwa[i], s_dw[group][d + 2 * i], s_dw[group][d + 2 * i + 1]);
+      f32x2_get(dwb[i], s_dw[group][d + 64 + 2 * i], s_dw[group][d + 64 + 2 * i + 1]);
+    }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      float a = 0.f;
 #pragma unroll
-        for (int k = 0; k < HN_GROUPS; ++k) a += s_dw[k][threadIdx.x];
-        p.dw_part[(size_t(blockIdx.x) * 2 + i) * 128 + threadIdx.x] = a;
-      }
+      for (int k = 0; k < HN_GROUPS; ++k) a += s_dw[k][threadIdx.x];
+      p.dw_part[size_t(blockIdx.x) * 128 + threadIdx.x] = a;
     }
   }
 }
 
-// dw[i][d] = sum over blocks of dw_part[block][i][d], in a fixed order: a block of this kernel takes 32 columns with 32
-// slices of the blocks each.
+// dw[d] = sum over blocks of dw_part[block][d], in a fixed order: a block of this kernel takes 32 columns of the queries' or the
+// keys' weight, with 32 slices of the blocks each.
 template <int T>
 __global__ void __launch_bounds__(1024)
-head_norm_dw_kernel(const float* __restrict__ part, int blocks, void* dwq, void* dwk, int w_fp32, const int* status) {
-  if (status && *reinterpret_cast<const volatile int*>(status) != 0) {
+head_norm_dw_kernel(const float* __restrict__ part, int blocks_q, int blocks, void* dwq, void* dwk, int w_fp32, const int* status) {
+  if (status && __syncthreads_or(*reinterpret_cast<const volatile int*>(status) != 0)) {
     if ((threadIdx.x & 31) == 0) publish_status(status);
     return;
   }
   __shared__ float s[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, which = blockIdx.x >> 2, col0 = (blockIdx.x & 3) * 32;
+  void* dst = which ? dwk : dwq;
+  if (dst == nullptr) return;
+  const int first = which ? blocks_q : 0, end = which ? blocks : blocks_q;
   float a = 0.f;
-  for (int k = slice; k < blocks; k += 32) a += part[size_t(k) * 256 + col];
-  s[slice][threadIdx.x & 31] = a;
+  for (int k = first + slice; k < end; k += 32) a += part[size_t(k) * 128 + col0 + lane];
+  s[slice][lane] = a;
   __syncthreads();
-  a = s[threadIdx.x & 31][slice];           // lane = slice, warp = column
+  a = s[lane][slice];           // lane = slice, warp = column
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off);
-  if ((threadIdx.x & 31) == 0) {
-    const int c = blockIdx.x * 32 + slice;
-    void* dst = c < 128 ? dwq : dwk;
-    if (dst == nullptr) return;
-    if (T == 2 || w_fp32) static_cast<float*>(dst)[c & 127] = a;
-    else static_cast<uint16_t*>(dst)[c & 127] = uint16_t(T == 0 ? pack_bf16x2(a, 0.f) : pack_f16x2(a, 0.f));
+  if (lane == 0) {
+    if (T == 2 || w_fp32) static_cast<float*>(dst)[col0 + slice] = a;
+    else static_cast<uint16_t*>(dst)[col0 + slice] = uint16_t(T == 0 ? pack_bf16x2(a, 0.f) : pack_f16x2(a, 0.f));
   }
 }
 
-static HeadNormParams head_norm_params(const lvx_head_norm& c, const lvx_view* q, const lvx_view* k) {
-  HeadNormParams p{};
+// `most`: blocks at most, 0: one unit a lane group. Returns the number of blocks.
+static int head_norm_params(HeadNormParams& p, const lvx_head_norm& c, const lvx_view* q, const lvx_view* k, int unit, long most) {
   p.S = c.S;
   const lvx_view* v[2] = {q, k};
   const int heads[2] = {q ? c.Hq : 0, k ? c.Hkv : 0};
+  long blocks[2];
   for (int i = 0; i < 2; ++i) {
     p.heads[i] = heads[i];
-    p.chunks[i] = (heads[i] + HN_U - 1) / HN_U;
+    p.chunks[i] = (heads[i] + unit - 1) / unit;
+    p.units[i] = unsigned(long(c.B) * c.S * p.chunks[i]);
+    blocks[i] = (long(p.units[i]) + HN_GROUPS - 1) / HN_GROUPS;
     if (!v[i]) continue;
     p.x[i] = v[i]->data;
     p.x_b[i] = v[i]->stride_b;
     p.x_h[i] = v[i]->stride_h;
     p.x_s[i] = v[i]->stride_s;
   }
-  p.units = long(c.B) * c.S * (p.chunks[0] + p.chunks[1]);
+  if (most > 0 && blocks[0] + blocks[1] > most) {      // shared out in proportion, one at least for who has units
+    long bq = most * blocks[0] / (blocks[0] + blocks[1]);
+    bq = blocks[0] == 0 ? 0 : blocks[1] == 0 ? most : std::min(std::max(bq, 1l), most - 1);
+    blocks[1] = most - bq;
+    blocks[0] = bq;
+  }
+  p.blocks_q = int(blocks[0]);
   p.w[0] = c.wq;
   p.w[1] = c.wk;
   p.w_fp32 = c.weight_fp32;
@@ -273,24 +361,26 @@ static HeadNormParams head_norm_params(const lvx_head_norm& c, const lvx_view* q
   p.t_b = c.table_stride_b;
   p.t_s = c.table_stride_s;
   p.status = device_status_ptr();
-  return p;
+  return int(blocks[0] + blocks[1]);
 }
 
 int launch_head_norm(const lvx_head_norm& c, const lvx_view* q, const lvx_view* k, void* q_out, void* k_out, cudaStream_t st) {
-  HeadNormParams p = head_norm_params(c, q, k);
+  HeadNormParams p{};
+  const int blocks = head_norm_params(p, c, q, k, hn_unit(c.dtype), 0);
   p.out[0] = q_out;
   p.out[1] = k_out;
-  const long blocks = std::min<long>((p.units + HN_GROUPS - 1) / HN_GROUPS, 148 * 32);
-  if (c.dtype == LVX_BF16) head_norm_kernel<0, false><<<blocks, HN_GROUPS * 16, 0, st>>>(p);
-  else if (c.dtype == LVX_FP16) head_norm_kernel<1, false><<<blocks, HN_GROUPS * 16, 0, st>>>(p);
-  else head_norm_kernel<2, false><<<blocks, HN_GROUPS * 16, 0, st>>>(p);
+  if (c.dtype == LVX_BF16) head_norm_kernel<0, false><<<blocks, 256, 0, st>>>(p);
+  else if (c.dtype == LVX_FP16) head_norm_kernel<1, false><<<blocks, 256, 0, st>>>(p);
+  else head_norm_kernel<2, false><<<blocks, 256, 0, st>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "head_norm_kernel launch");
 }
 
 int launch_head_norm_bwd(const lvx_head_norm& c, const lvx_view* q, const lvx_view* k, const lvx_view* gq, const lvx_view* gk,
                          void* dq, void* dk, float* scratch, void* dwq, void* dwk, cudaStream_t st) {
-  HeadNormParams p = head_norm_params(c, q, k);
+  const bool with_dw = dwq || dwk;
+  HeadNormParams p{};
+  const int blocks = head_norm_params(p, c, q, k, hn_unit(c.dtype), with_dw ? HN_BWD_BLOCKS : 0);
   p.out[0] = dq;
   p.out[1] = dk;
   const lvx_view* g[2] = {gq, gk};
@@ -301,12 +391,10 @@ int launch_head_norm_bwd(const lvx_head_norm& c, const lvx_view* q, const lvx_vi
     p.g_h[i] = g[i]->stride_h;
     p.g_s[i] = g[i]->stride_s;
   }
-  const bool with_dw = dwq || dwk;
   p.dw_part = with_dw ? scratch : nullptr;
-  const int blocks = int(std::min<long>((p.units + HN_GROUPS - 1) / HN_GROUPS, with_dw ? HN_BWD_BLOCKS : 148 * 32));
   auto go = [&](auto kern, auto sum) {
-    kern<<<blocks, HN_GROUPS * 16, 0, st>>>(p);
-    if (with_dw) sum<<<8, 1024, 0, st>>>(scratch, blocks, dwq, dwk, c.weight_fp32, p.status);
+    kern<<<blocks, 256, 0, st>>>(p);
+    if (with_dw) sum<<<8, 1024, 0, st>>>(scratch, p.blocks_q, blocks, dwq, dwk, c.weight_fp32, p.status);
   };
   if (c.dtype == LVX_BF16) go(head_norm_kernel<0, true>, head_norm_dw_kernel<0>);
   else if (c.dtype == LVX_FP16) go(head_norm_kernel<1, true>, head_norm_dw_kernel<1>);

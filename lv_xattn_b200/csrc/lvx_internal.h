@@ -76,12 +76,15 @@ int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
                       float* lse, int* status, cudaStream_t st);
-// Its backward for 16-bit types: dq_acc (window_dq_floats of them, zeroed) is in tile order, launch_window_dq rounds it.
+// Its backward for 16-bit types: dq_acc (window_dq_floats of them, zeroed) is in tile order, launch_window_dq rounds it and
+// adds up the parts (window_sink_floats of them) of the sinks' dK and dV.
 size_t window_dq_floats(const lvx_shape& s);
+size_t window_sink_floats(const lvx_shape& s, const lvx_window& w);
 int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q, const lvx_view& d_o, const lvx_view& k,
                       const lvx_view& v, const float* lse, const float* delta, const int32_t* kv_valid_len, float sm_scale,
-                      float* dq_acc, void* dk, void* dv, int* status, cudaStream_t st);
-int launch_window_dq(const lvx_shape& s, const float* acc, void* dq, const int* status, cudaStream_t st);
+                      float* dq_acc, float* parts, void* dk, void* dv, int* status, cudaStream_t st);
+int launch_window_dq(const lvx_shape& s, const lvx_window& w, const float* acc, const float* parts, void* dq, void* dk, void* dv,
+                     const int* status, cudaStream_t st);
 // Around the windowed kernels for a batch that shares prefixes (shared_prefix.cu).
 int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const void* d_o, const float* lse, const float* delta,
                      void* q_out, void* do_out, float* lse_out, float* delta_out, cudaStream_t st);

@@ -10,6 +10,9 @@
 //   * items go out heaviest first (the first key tiles are seen by the most queries: all of them where they are sinks or
 //     there is no window), forwards and backwards in turn, so that a CTA's share evens out;
 //   * an item knows its own number of query tiles, possibly none;
+//   * every query sees the sinks, so their key tiles would be walked long after all others are done (4,096 tokens with a
+//     window of 1,024: 128 query tiles against 36). They are shared out over several items, each with a run of the queries
+//     and fp32 dK and dV of its own, which the last kernel adds up in a fixed order (backward of that case 400 -> 2xx us);
 //   * dQ is accumulated in the order of the tiles ([slab][chunk][token][head of the chunk][128]: a tile's rows are one
 //     run of memory), and brought into [B, Hq, Sq, 128] by the kernel that rounds it;
 //   * a thread's key is seen by a run of a tile's columns, so a masked tile costs two comparisons a tile and a select a
@@ -60,8 +63,15 @@ enum {
 };
 #define WB_CODE(role, bar) (LVX_DEV_TIMEOUT_BASE | 0x500 | ((role) << 5) | (bar))
 
+// Key tiles [0, tiles) are walked by `parts` items each.
+struct SinkParts {
+  int tiles, parts;
+};
+
 struct WinBwdParams {
   int sq, skv, hkv, g, slabs, nitems;
+  SinkParts sp;
+  float* parts;                        // [slab][sink tile][part][dK, dV][128][128]
   QTiles qt;
   WindowMask mask;
   const int32_t* kv_valid_len;
@@ -87,6 +97,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   struct Item {
     int slab, kv0, valid, start;
     int blk0, ntot;          // first block of tokens, tiles to walk
+    int part;                // index into `parts`, or -1: the item makes dK and dV itself
   };
   // the CTA's round-th item: forwards and backwards through the list in turn
   auto index_of = [&](int round) {
@@ -95,14 +106,29 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   auto item_of = [&](int w) {
     Item it;
     it.slab = w % p.slabs;
-    it.kv0 = (w / p.slabs) * 128;
+    int tile = w / p.slabs;
+    it.part = -1;
+    const int shared_out = p.sp.tiles * p.sp.parts;
+    if (tile < shared_out) {
+      it.part = it.slab * shared_out + tile;
+      tile /= p.sp.parts;
+    } else {
+      tile += p.sp.tiles - shared_out;
+    }
+    it.kv0 = tile * 128;
     it.valid = p.skv;
     if (p.kv_valid_len) it.valid = min(it.valid, max(0, p.kv_valid_len[it.slab / p.hkv]));
     it.start = p.mask.start >= 0 ? p.mask.start : it.valid - p.sq;
     const int ta = max(0, it.kv0 - it.start);
     const int tb = it.kv0 < p.mask.sinks ? p.sq : min(p.sq, it.kv0 + 127 - it.start + p.mask.window);
     it.blk0 = ta / p.qt.tokens;
-    it.ntot = it.kv0 < it.valid && ta < tb ? ((tb - 1) / p.qt.tokens + 1 - it.blk0) * p.qt.chunks : 0;
+    int blocks = it.kv0 < it.valid && ta < tb ? (tb - 1) / p.qt.tokens + 1 - it.blk0 : 0;
+    if (it.part >= 0) {
+      const int each = (blocks + p.sp.parts - 1) / p.sp.parts, first = it.part % p.sp.parts * each;
+      it.blk0 += first;
+      blocks = max(0, min(each, blocks - first));
+    }
+    it.ntot = blocks * p.qt.chunks;
     return it;
   };
   // first token and chunk of an item's j-th tile
@@ -151,7 +177,10 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
         const Item I = item_of(w);
         if (I.ntot == 0) {      // nothing sees these keys (or they are not valid): their gradients are zero
-          if (warp < 8 && I.kv0 + (tid & 127) < p.skv) {
+          if (I.part >= 0) {
+            float4* dst = reinterpret_cast<float4*>(p.parts + size_t(I.part) * 2 * 128 * 128);
+            for (int i = tid; i < 2 * 128 * 32; i += WB_COMPUTE * 32) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          } else if (warp < 8 && I.kv0 + (tid & 127) < p.skv) {
             uint4* dst = reinterpret_cast<uint4*>((warp < 4 ? p.dk : p.dv) + (size_t(I.slab) * p.skv + I.kv0 + (tid & 127)) * 128);
 #pragma unroll
             for (int i = 0; i < 16; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -309,7 +338,13 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_ld32(tmem_base + (which ? WB_DV : WB_DK) + lane_sel + cg * 32, a);
             tc_wait_ld();
             const float mul = which ? 1.f : p.scale;
-            if (ok_row) {
+            if (I.part >= 0) {
+              float4* dst = reinterpret_cast<float4*>(p.parts + ((size_t(I.part) * 2 + which) * 128 + r) * 128 + cg * 32);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                dst[i] = make_float4(__uint_as_float(a[4 * i]) * mul, __uint_as_float(a[4 * i + 1]) * mul,
+                                     __uint_as_float(a[4 * i + 2]) * mul, __uint_as_float(a[4 * i + 3]) * mul);
+            } else if (ok_row) {
               uint4* dst = reinterpret_cast<uint4*>((which ? p.dv : p.dk) + off);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -529,24 +564,44 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 }
 
 // ---------------------------------------------------------------------------------------------
-// dq[B, Hq, Sq, 128] = cast of the accumulator in tile order. A warp takes one row (16 bytes of fp32 a lane).
+// dq[B, Hq, Sq, 128] = cast of the accumulator in tile order: the grid's second axis walks (slab, chunk), and a warp takes four
+// rows of it at a time (16 bytes of fp32 a lane each). Then the sinks' dK and dV: the sum of their parts.
 template <bool IS_BF16>
 __global__ void __launch_bounds__(256)
-window_dq_kernel(const float* __restrict__ acc, uint16_t* __restrict__ dq, int g, int sq, int heads, int chunks, long rows,
-                 const int* status) {
+window_dq_kernel(const float* __restrict__ acc, uint16_t* __restrict__ dq, int g, int sq, int heads, int chunks, int slabs, const SinkParts sp,
+                 const float* __restrict__ parts, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, int skv, const int* status) {
   if (status && *reinterpret_cast<const volatile int*>(status) != 0) {
     if ((threadIdx.x & 31) == 0) publish_status(status);
     return;
   }
-  const int lane = threadIdx.x & 31;
-  for (long row = (long(blockIdx.x) * 256 + threadIdx.x) >> 5; row < rows; row += long(gridDim.x) * 8) {
-    const long bh = row / sq;                // row of [B*Hq, Sq]
-    const int tok = int(row - bh * sq), head = int(bh % g);
-    const long slab = bh / g;
-    const size_t at = ((size_t(slab) * chunks + head / heads) * sq + tok) * heads + head % heads;
-    const float4 v = reinterpret_cast<const float4*>(acc)[at * 32 + lane];
-    reinterpret_cast<uint2*>(dq)[row * 32 + lane] = IS_BF16 ? make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w))
-                                                            : make_uint2(pack_f16x2(v.x, v.y), pack_f16x2(v.z, v.w));
+  auto cast = [](float4 v) {
+    return IS_BF16 ? make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w)) : make_uint2(pack_f16x2(v.x, v.y), pack_f16x2(v.z, v.w));
+  };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int y = blockIdx.y; y < slabs * chunks; y += gridDim.y) {
+    const int chunk = y % chunks, slab = y / chunks, rows = sq * heads;
+    const float4* src = reinterpret_cast<const float4*>(acc) + size_t(y) * rows * 32;
+    for (int row0 = (blockIdx.x * 8 + warp) * 4; row0 < rows; row0 += gridDim.x * 32) {
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = src[size_t(min(row0 + u, rows - 1)) * 32 + lane];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int row = row0 + u, tok = row / heads, head = chunk * heads + row % heads;
+        if (row < rows && head < g) reinterpret_cast<uint2*>(dq)[((size_t(slab) * g + head) * sq + tok) * 32 + lane] = cast(v[u]);
+      }
+    }
+    const int sink_rows = chunk == 0 ? sp.tiles * 128 * 2 : 0;      // of this slab
+    for (int i = blockIdx.x * 8 + warp; i < sink_rows; i += gridDim.x * 8) {
+      const int r = i & 127, which = (i >> 7) & 1, tile = i >> 8;
+      if (tile * 128 + r >= skv) continue;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < sp.parts; ++c) {
+        const float4 w = reinterpret_cast<const float4*>(parts)[((((size_t(slab) * sp.tiles + tile) * sp.parts + c) * 2 + which) * 128 + r) * 32 + lane];
+        v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+      }
+      reinterpret_cast<uint2*>(which ? dv : dk)[(size_t(slab) * skv + tile * 128 + r) * 32 + lane] = cast(v);
+    }
   }
 }
 
@@ -557,15 +612,35 @@ static int window_num_sms() {
   return 148;
 }
 
+// The key tiles of the sinks that are shared out over several items, and over how many: as many as make an item about as long
+// as those of the other keys.
+static SinkParts sink_parts(const lvx_shape& s, const lvx_window& w) {
+  const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
+  const WindowMask m = make_window_mask(w);
+  SinkParts sp = {0, 1};
+  if (m.window == kNoWindow || m.sinks == 0 || s.Skv == 0) return sp;
+  const long all = (long(s.Sq) + qt.tokens - 1) / qt.tokens, usual = (long(m.window) + 127) / qt.tokens + 1;
+  const long parts = std::min<long>((all + usual - 1) / usual, 32);
+  if (parts < 2) return sp;
+  sp.tiles = int((std::min<long>(m.sinks, s.Skv) + 127) / 128);
+  sp.parts = int(parts);
+  return sp;
+}
+
+size_t window_sink_floats(const lvx_shape& s, const lvx_window& w) {
+  const SinkParts sp = sink_parts(s, w);
+  return size_t(s.B) * s.Hkv * sp.tiles * sp.parts * 2 * 128 * 128;
+}
+
 size_t window_dq_floats(const lvx_shape& s) {
   const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
   return size_t(s.B) * s.Hkv * qt.chunks * s.Sq * qt.heads * 128;
 }
 
-// dq_acc (window_dq_floats, zeroed), then dk and dv.
+// dq_acc (window_dq_floats, zeroed), then dk and dv; `parts`: window_sink_floats.
 int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q, const lvx_view& d_o, const lvx_view& k,
                       const lvx_view& v, const float* lse, const float* delta, const int32_t* kv_valid_len, float sm_scale,
-                      float* dq_acc, void* dk, void* dv, int* status, cudaStream_t st) {
+                      float* dq_acc, float* parts, void* dk, void* dv, int* status, cudaStream_t st) {
   const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
   CUtensorMap tmQ, tmDO, tmK, tmV;
   int rc = make_q_map(&tmQ, s, qt, q);
@@ -579,7 +654,9 @@ int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q
   p.hkv = s.Hkv;
   p.g = s.Hq / s.Hkv;
   p.slabs = s.B * s.Hkv;
-  p.nitems = (s.Skv + 127) / 128 * p.slabs;
+  p.sp = sink_parts(s, w);
+  p.parts = parts;
+  p.nitems = ((s.Skv + 127) / 128 + p.sp.tiles * (p.sp.parts - 1)) * p.slabs;
   p.qt = qt;
   p.mask = make_window_mask(w);
   p.kv_valid_len = kv_valid_len;
@@ -604,12 +681,14 @@ int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "window_bwd_kernel launch");
 }
 
-int launch_window_dq(const lvx_shape& s, const float* acc, void* dq, const int* status, cudaStream_t st) {
+int launch_window_dq(const lvx_shape& s, const lvx_window& w, const float* acc, const float* parts, void* dq, void* dk, void* dv,
+                     const int* status, cudaStream_t st) {
   const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
-  const long rows = long(s.B) * s.Hq * s.Sq;
-  const long blocks = std::min<long>((rows + 7) / 8, 148 * 16);
+  const long all = long(s.B) * s.Hkv * qt.chunks, rows = long(s.Sq) * qt.heads;
+  const dim3 grid(unsigned(std::min<long>((rows + 31) / 32, (148 * 16 + all - 1) / all)), unsigned(std::min<long>(all, 65535)));
   auto go = [&](auto kern) {
-    kern<<<blocks, 256, 0, st>>>(acc, static_cast<uint16_t*>(dq), s.Hq / s.Hkv, s.Sq, qt.heads, qt.chunks, rows, status);
+    kern<<<grid, 256, 0, st>>>(acc, static_cast<uint16_t*>(dq), s.Hq / s.Hkv, s.Sq, qt.heads, qt.chunks, s.B * s.Hkv, sink_parts(s, w), parts,
+                               static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv), s.Skv, status);
   };
   if (s.dtype == LVX_BF16) go(window_dq_kernel<true>);
   else go(window_dq_kernel<false>);

@@ -573,7 +573,7 @@ def _head_norm(q, k, q_weight, k_weight, cos, sin, eps):
                          None if k is None or k_weight is None else k_weight.data_ptr(),
                          None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
                          0 if cos is None or cos.shape[0] == 1 else cos.stride(0), 0 if cos is None else cos.stride(1))
-    return c, [None if t is None else rows_view(t.transpose(1, 2), 4) for t in (q, k)]
+    return c, [None if t is None else rows_view(t.transpose(1, 2), 8) for t in (q, k)]
 
 
 def _ref(view):
@@ -594,7 +594,7 @@ def head_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float):
 def head_norm_rope_bwd(q, k, q_weight, k_weight, cos, sin, eps: float, gq, gk, want):
     """Gradients (dq, dk [B, S, H, 128], dwq, dwk [128]) from the outputs' gradients; `want` says which are made."""
     c, (qv, kv) = _head_norm(q, k, q_weight, k_weight, cos, sin, eps)
-    gv = [None if t is None else rows_view(t, 4) for t in (gq, gk)]
+    gv = [None if t is None else rows_view(t, 8) for t in (gq, gk)]
     dx = [t.new_empty(t.shape) if w else None for t, w in zip((q, k), want[:2])]
     dw = [torch.empty_like(t) if w else None for t, w in zip((q_weight, k_weight), want[2:])]
     with_dw = dw[0] is not None or dw[1] is not None
