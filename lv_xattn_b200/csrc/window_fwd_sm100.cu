@@ -36,6 +36,12 @@ constexpr int WF_OFF_V = WF_OFF_K + WF_NS * WF_TILE;
 constexpr int WF_OFF_BAR = WF_OFF_V + WF_NS * WF_TILE;
 constexpr int WF_SMEM = WF_OFF_BAR + 256 + 1024;  // + barriers + alignment slack
 constexpr int WF_THREADS = 320;
+// PAIR from this many key tiles on. us a call, one warpgroup per query tile -> PAIR, 32 tokens of 32 heads on 8 KV heads, over
+// 512 / 2,048 / 4,096 / 16,384 keys, combine kernel included where there is one:
+//    1 entry      15.7 ->  17.5    16.7 -> 18.9    19.2 ->  19.7     31 ->  27
+//    8 entries    15.9 ->  20.4    30.7 -> 32.3    47.4 ->  42.0    139 -> 103
+//   32 entries    40.5 ->  58.5     101 ->   98     161 ->   142    547 -> 402
+constexpr int kPairTiles = 32;
 
 enum {
   WFB_Q_FULL = 0,
@@ -74,7 +80,10 @@ __device__ __noinline__ void window_plain_values(float* o, const uint16_t* q, co
     axpy32<IS_BF16>(o, ex2f(dot128<IS_BF16>(q, k + key * ks) * c - m), v + key * vs);
 }
 
-template <bool IS_BF16>
+// PAIR: the slab has a single query tile (65 to 128 rows: a token each of 32 requests that share a prefix), and the two
+// warpgroups take turns at its key tiles instead of one of them idling: each has an accumulator and a partial result of its
+// own, and a key tile costs half of the softmax' time, which is then below that of its bytes.
+template <bool IS_BF16, bool PAIR>
 __global__ void __launch_bounds__(WF_THREADS, 1)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const WinFwdParams p) {
@@ -96,7 +105,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int tok0 = (2 * mb / p.qt.chunks) * p.qt.tokens;
   const int tok1 = min(p.sq, (min(2 * mb + 1, p.qt.count - 1) / p.qt.chunks + 1) * p.qt.tokens) - 1;
   const KeyTiles kt = key_tiles(p.mask, valid, start + tok0, start + tok1, 7);
-  const int per_split = (kt.n + p.nsplit - 1) / p.nsplit;
+  const int per_split = (kt.n + gridDim.z - 1) / gridDim.z;
   const int j0 = min(kt.n, split * per_split);
   const int n = min(kt.n, j0 + per_split) - j0;
 
@@ -142,7 +151,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t tS = tmem_base + wg * 128 + lane_sel;
     const uint32_t tO = tmem_base + 256 + wg * 128 + lane_sel;
     const float c = p.scale_log2;
-    const int tile = 2 * mb + wg, tile_tok = (tile / p.qt.chunks) * p.qt.tokens;
+    const int tile = PAIR ? 0 : 2 * mb + wg, tile_tok = (tile / p.qt.chunks) * p.qt.tokens;
     const int tok = tile_tok + r / heads, head = (tile % p.qt.chunks) * heads + r % heads;
     const bool exists = tile < p.qt.count && r < tile_rows && tok < p.sq && head < p.g;
     // this row's keys: [0, sink_end) and [lo, hi]. A row that does not exist sees everything against a reference of 0 (its
@@ -156,10 +165,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int all_sinks = min(p.mask.sinks, all_hi + 1);
     float m = exists ? -INFINITY : 0.f, l = 0.f;
     bool alive = true;
-    for (int j = 0; j < n; ++j) {
+    // this warpgroup's key tiles: all of the CTA's, or every other one
+    constexpr int STEP = PAIR ? 2 : 1;
+    const int first = PAIR ? wg : 0;
+    for (int j = first, t = 0; j < n; j += STEP, ++t) {
       const int key0 = kt.tile(j0 + j) * 128;
       const bool full = key0 + 127 <= all_hi && (key0 >= all_lo || key0 + 128 <= all_sinks);
-      if (!mbar_wait(&bars[WFB_S_FULL + wg], j & 1, abort_flag, p.status, WF_CODE(wg, WFB_S_FULL))) {
+      if (!mbar_wait(&bars[WFB_S_FULL + wg], t & 1, abort_flag, p.status, WF_CODE(wg, WFB_S_FULL))) {
         alive = false;
         break;
       }
@@ -167,7 +179,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // The usual tile: exponentials against the running maximum as it stands (it is only a reference point), P held in
       // registers until the row sums are known to be small. (See fwd_sm100.cu for what each of these costs.)
       bool done = false;
-      if (j > 0 && full) {
+      if (t > 0 && full) {
         uint32_t pk[2][32];
         uint64_t sum_a = f32x2(0.f, 0.f), sum_b = f32x2(0.f, 0.f);
         const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-m, -m);
@@ -230,7 +242,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           m = m_new;
           l *= alpha;
         }
-        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        if (t > 0 && __any_sync(0xffffffffu, grow)) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t o[32];
@@ -266,19 +278,19 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (lane == 0) mbar_arrive(&bars[WFB_P_FULL + wg]);
     }
     // ------------------------------- epilogue -------------------------------
-    if (alive && n > 0) alive = mbar_wait(&bars[WFB_O_DONE + wg], 0, abort_flag, p.status, WF_CODE(wg, WFB_O_DONE));
+    if (alive && n > first) alive = mbar_wait(&bars[WFB_O_DONE + wg], 0, abort_flag, p.status, WF_CODE(wg, WFB_O_DONE));
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
     if (alive) {
       const int qh = kvh * p.g + head;
       const long long row = (static_cast<long long>(batch) * p.hkv * p.g + qh) * p.sq + tok;      // of [B, Hq, Sq]
-      const long long prow = (static_cast<long long>(slab) * p.nsplit + split) * p.g * p.sq + static_cast<long long>(head) * p.sq + tok;
+      const long long prow = (static_cast<long long>(slab) * p.nsplit + (PAIR ? 2 * split + wg : split)) * p.g * p.sq + static_cast<long long>(head) * p.sq + tok;
       const float inv = p.o == nullptr ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         uint32_t o[32];
         float sum = 0.f;
-        if (n > 0) {
+        if (n > first) {
           tmem_ld32(tO + q * 32, o);
           tc_wait_ld();
 #pragma unroll
@@ -293,7 +305,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const uint16_t* qrow = p.q + batch * p.q_b + qh * p.q_h + tok * p.q_s;
           const uint16_t* kb = p.k + batch * p.k_b + kvh * p.k_h;
           const uint16_t* vb = p.v + batch * p.v_b + kvh * p.v_h + q * 32;
-          for (int j = 0; j < n; ++j) {
+          for (int j = first; j < n; j += STEP) {
             const int key0 = kt.tile(j0 + j) * 128, key1 = key0 + 128;
             const int cut = min(key1, sink_end);          // the sinks, then what of the window lies behind them
             window_plain_values<IS_BF16>(again, qrow, kb, vb, p.k_s, p.v_s, key0, cut, c, m == -INFINITY ? 0.f : m);
@@ -335,8 +347,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tma_prefetch_desc(&tmQ);
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
-      mbar_arrive_expect_tx(&bars[WFB_Q_FULL], 2 * tile_rows * 256);
-      for (int t = 0; t < 2; ++t) {
+      mbar_arrive_expect_tx(&bars[WFB_Q_FULL], (PAIR ? 1 : 2) * tile_rows * 256);
+      for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
         const int tile = 2 * mb + t;
         for (int h = 0; h < 2; ++h)
           tma_load_5d(smem + t * WF_TILE + h * WF_HALF, &tmQ, &bars[WFB_Q_FULL], h * 64, (tile % p.qt.chunks) * heads,
@@ -376,7 +388,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     constexpr uint32_t HI = umma_desc_hi(1024);
     const uint32_t sQ = smem_u32(smem), sK = smem_u32(smem + WF_OFF_K), sV = smem_u32(smem + WF_OFF_V);
     auto issue_qk = [&](int i, int stage) {
-      const uint32_t a_lo = umma_desc_lo(sQ + i * WF_TILE, 16);
+      const uint32_t a_lo = umma_desc_lo(sQ + (PAIR ? 0 : i * WF_TILE), 16);
       const uint32_t b_lo = umma_desc_lo(sK + stage * WF_TILE, 16);
       if (elect_one()) {
 #pragma unroll
@@ -404,8 +416,47 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     auto wait = [&](int bar, uint32_t ph) {
       return __all_sync(0xffffffffu, mbar_wait(&bars[bar], ph, abort_flag, p.status, WF_CODE(3, bar)));
     };
+    // rows of V behind the last valid key: whatever they hold is multiplied with zeros
+    auto clear_v = [&](int j, int s) {
+      const int left = valid - kt.tile(j0 + j) * 128;
+      if (left >= 128) return;
+      for (int at = lane; at < (128 - left) * 16; at += 32)
+        *reinterpret_cast<uint4*>(smem + WF_OFF_V + s * WF_TILE + ((at >> 3) & 1) * WF_HALF + (left + (at >> 4)) * 128 + (at & 7) * 16) =
+            make_uint4(0u, 0u, 0u, 0u);
+      fence_async_smem();
+      __syncwarp();
+    };
     bool ok = wait(WFB_Q_FULL, 0) && wait(WFB_K_FULL, 0);
-    if (ok) {
+    if constexpr (PAIR) {
+      // tile j is warpgroup j % 2's; its scores come two tiles ahead
+      for (int j = 0; ok && j < min(n, 2); ++j) {
+        if (j > 0) ok = wait(WFB_K_FULL + j % WF_NS, j / WF_NS & 1);
+        if (!ok) break;
+        tc_fence_after();
+        issue_qk(j, j % WF_NS);
+        commit(&bars[WFB_S_FULL + j]);
+        commit(&bars[WFB_K_EMPTY + j % WF_NS]);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const int i = j & 1, s = j % WF_NS, s2 = (j + 2) % WF_NS;
+        ok = wait(WFB_P_FULL + i, j >> 1 & 1) && wait(WFB_V_FULL + s, j / WF_NS & 1);
+        if (!ok) break;
+        clear_v(j, s);
+        tc_fence_after();
+        issue_pv(i, s, j < 2);
+        commit(&bars[WFB_V_EMPTY + s]);
+        if (j + 2 < n) {
+          ok = wait(WFB_K_FULL + s2, (j + 2) / WF_NS & 1);
+          if (!ok) break;
+          tc_fence_after();
+          issue_qk(i, s2);
+          commit(&bars[WFB_S_FULL + i]);
+          commit(&bars[WFB_K_EMPTY + s2]);
+        } else {
+          commit(&bars[WFB_O_DONE + i]);
+        }
+      }
+    } else if (ok) {
       tc_fence_after();
       issue_qk(0, 0);
       commit(&bars[WFB_S_FULL + 0]);
@@ -413,7 +464,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       commit(&bars[WFB_S_FULL + 1]);
       commit(&bars[WFB_K_EMPTY + 0]);
     }
-    for (int j = 0; ok && j < n; ++j) {
+    for (int j = 0; !PAIR && ok && j < n; ++j) {
       const int s = j % WF_NS, s1 = (j + 1) % WF_NS;
       const uint32_t ph = (j / WF_NS) & 1, ph1 = ((j + 1) / WF_NS) & 1;
 #pragma unroll
@@ -422,15 +473,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = wait(WFB_P_FULL + i, j & 1);
         if (ok && i == 0) {
           ok = wait(WFB_V_FULL + s, ph);
-          // rows of V behind the last valid key: whatever they hold is multiplied with zeros
-          const int left = valid - kt.tile(j0 + j) * 128;
-          if (ok && left < 128) {
-            for (int at = lane; at < (128 - left) * 16; at += 32)
-              *reinterpret_cast<uint4*>(smem + WF_OFF_V + s * WF_TILE + ((at >> 3) & 1) * WF_HALF + (left + (at >> 4)) * 128 +
-                                        (at & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-            fence_async_smem();
-            __syncwarp();
-          }
+          if (ok) clear_v(j, s);
         }
         if (!ok) break;
         tc_fence_after();
@@ -463,19 +506,30 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 }
 
 // ---------------------------------------------------------------------------------------------
+static bool window_pair(const lvx_shape& s, long tiles, bool few) {
+  return !few && tiles >= kPairTiles && make_q_tiles(s.Hq / s.Hkv, s.Sq).count == 1;
+}
+// key tiles that a CTA of this call sees at most: its tokens' windows, and the sinks
+static long window_tiles(const lvx_shape& s, const lvx_window& w, bool few) {
+  const int span = few ? s.Sq : 2 * make_q_tiles(s.Hq / s.Hkv, s.Sq).tokens;
+  const WindowMask m = make_window_mask(w);
+  const long all = (long(s.Skv) + 127) / 128;
+  if (m.window == kNoWindow) return all;
+  return std::min<long>(all, (long(m.window) + span + 126) / 128 + 1 + (long(m.sinks) + 127) / 128);
+}
+
 FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few) {
   FwdPlan p = plan_fwd(s);          // (fp32: as it is)
   const int g = s.Hq / s.Hkv;
   *few = s.dtype != LVX_FP32 && p.rows <= kFewRows;
+  bool pair = false;
   if (s.dtype != LVX_FP32) {
     const QTiles qt = make_q_tiles(g, s.Sq);
     p.m_blocks = *few ? 1 : (qt.count + 1) / 2;
-    // key tiles that a CTA sees at most: its tokens' windows, and the sinks
-    const int span = *few ? s.Sq : 2 * qt.tokens;
-    const WindowMask m = make_window_mask(w);
-    long tiles = p.kv_tiles;
-    if (m.window < kNoWindow) tiles = std::min<long>(tiles, (long(m.window) + span + 126) / 128 + 1 + (long(m.sinks) + 127) / 128);
+    long tiles = window_tiles(s, w, *few);
     const long base = long(p.m_blocks) * s.B * s.Hkv;
+    pair = window_pair(s, tiles, *few);
+    if (pair) tiles = (tiles + 1) / 2;      // what a CTA walks takes half as long
     const long most = std::min<long>(tiles > 0 ? tiles : 1, *few ? 148 : 64);
     double best_cost = 1e300;
     for (int ns = 1; ns <= most; ++ns) {
@@ -488,6 +542,7 @@ FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few) {
       }
     }
     p.tiles_per_split = 0;          // the kernels share out what each CTA turns out to see
+    if (pair) p.nsplit *= 2;        // partial results; the grid has half as many splits
   }
   p.o_part_bytes = (size_t(s.B) * s.Hkv * p.nsplit * p.rows * 512 + 255) & ~size_t(255);
   p.ml_part_bytes = (size_t(s.B) * s.Hkv * p.nsplit * p.rows * 8 + 255) & ~size_t(255);
@@ -546,14 +601,19 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
   p.k_b = k.stride_b; p.k_h = k.stride_h; p.k_s = k.stride_s;
   p.v_b = v.stride_b; p.v_h = v.stride_h; p.v_s = v.stride_s;
   p.status = status;
-  dim3 grid(s.B * s.Hkv, pl.m_blocks, pl.nsplit);
+  const bool pair = window_pair(s, window_tiles(s, w, false), false);
+  dim3 grid(s.B * s.Hkv, pl.m_blocks, pair ? pl.nsplit / 2 : pl.nsplit);
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WF_SMEM);
     if (e == cudaSuccess) kern<<<grid, WF_THREADS, WF_SMEM, st>>>(tmQ, tmK, tmV, p);
   };
-  if (s.dtype == LVX_BF16) go(window_fwd_kernel<true>);
-  else go(window_fwd_kernel<false>);
+  auto pick = [&](auto one, auto two) {
+    if (pair) go(two);
+    else go(one);
+  };
+  if (s.dtype == LVX_BF16) pick(window_fwd_kernel<true, false>, window_fwd_kernel<true, true>);
+  else pick(window_fwd_kernel<false, false>, window_fwd_kernel<false, true>);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(window fwd)");
   e = cudaGetLastError();
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "window_fwd_kernel launch");

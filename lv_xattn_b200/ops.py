@@ -553,9 +553,13 @@ def rows_view(t, align_elements: int, repeats: bool = True):
     """(lvx_view, tensor kept alive) of a [B, H, S, 128] tensor with any strides that keep its rows contiguous and aligned
     to `align_elements` elements; other tensors are copied first, and unless `repeats` those that repeat rows (a stride
     of 0, of which a tensor map does not take any)."""
+    ptr = t.data_ptr()
+    if ptr % 16 == 0 and t.is_contiguous():
+        _, h, s, _ = t.shape
+        return _lib.LvxView(ptr, h * s * 128, s * 128, 128), t
     strides = [0 if n == 1 else st for n, st in zip(t.shape, t.stride())]
     sb, sh, ss, sd = strides
-    if (sd != 1 or (sb | sh | ss) % align_elements or t.data_ptr() % (align_elements * t.element_size())
+    if (sd != 1 or (sb | sh | ss) % align_elements or ptr % (align_elements * t.element_size())
             or not (repeats or all(st or n < 2 for n, st in zip(t.shape, strides)))):
         t = t.clone(memory_format=torch.contiguous_format)
         sb, sh, ss, _ = t.stride()
@@ -573,27 +577,42 @@ def _head_norm(q, k, q_weight, k_weight, cos, sin, eps):
                          None if k is None or k_weight is None else k_weight.data_ptr(),
                          None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
                          0 if cos is None or cos.shape[0] == 1 else cos.stride(0), 0 if cos is None else cos.stride(1))
-    return c, [None if t is None else rows_view(t.transpose(1, 2), 8) for t in (q, k)]
+    return c, _token_view(q), _token_view(k)
+
+
+def _token_view(t):
+    """The same of a [B, S, H, 128] tensor, or None."""
+    if t is None:
+        return None
+    ptr = t.data_ptr()
+    if ptr % 16 == 0 and t.is_contiguous():
+        _, s, h, _ = t.shape
+        return _lib.LvxView(ptr, s * h * 128, 128, h * 128), t
+    return rows_view(t.transpose(1, 2), 8)
 
 
 def _ref(view):
     return None if view is None else ctypes.byref(view[0])
 
 
+def _data(t):
+    return None if t is None else t.data_ptr()
+
+
 def head_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float):
     """(q_out, k_out) [B, H, S, 128] of q, k [B, S, H, 128] (either may be None); cos and sin [1 or B, S, 128]. The caller
     has checked types and shapes; weights and tables are contiguous where a row is."""
-    c, (qv, kv) = _head_norm(q, k, q_weight, k_weight, cos, sin, eps)
-    out = [None if t is None else t.new_empty(c.B, t.shape[2], c.S, 128) for t in (q, k)]
-    _lib.check(_lib.load().lvx_head_norm_rope(ctypes.byref(c), _ref(qv), _ref(kv), *(None if t is None else t.data_ptr() for t in out),
-                                              _lib.stream_int()), "lvx_head_norm_rope")
+    c, qv, kv = _head_norm(q, k, q_weight, k_weight, cos, sin, eps)
+    q_out, k_out = (None if t is None else t.new_empty((c.B, t.shape[2], c.S, 128)) for t in (q, k))
+    _lib.check(_lib.load().lvx_head_norm_rope(ctypes.byref(c), _ref(qv), _ref(kv), _data(q_out), _data(k_out), _lib.stream_int()),
+               "lvx_head_norm_rope")
     _count()
-    return out
+    return q_out, k_out
 
 
 def head_norm_rope_bwd(q, k, q_weight, k_weight, cos, sin, eps: float, gq, gk, want):
     """Gradients (dq, dk [B, S, H, 128], dwq, dwk [128]) from the outputs' gradients; `want` says which are made."""
-    c, (qv, kv) = _head_norm(q, k, q_weight, k_weight, cos, sin, eps)
+    c, qv, kv = _head_norm(q, k, q_weight, k_weight, cos, sin, eps)
     gv = [None if t is None else rows_view(t, 8) for t in (gq, gk)]
     dx = [t.new_empty(t.shape) if w else None for t, w in zip((q, k), want[:2])]
     dw = [torch.empty_like(t) if w else None for t, w in zip((q_weight, k_weight), want[2:])]
@@ -601,7 +620,7 @@ def head_norm_rope_bwd(q, k, q_weight, k_weight, cos, sin, eps: float, gq, gk, w
     scratch = (q if q is not None else k).new_empty(_lib.HEAD_NORM_SCRATCH // 4, dtype=torch.float32) if with_dw else None
     _lib.check(_lib.load().lvx_head_norm_rope_bwd(
         ctypes.byref(c), _ref(qv), _ref(kv), _ref(gv[0]), _ref(gv[1]),
-        *(None if t is None else t.data_ptr() for t in (*dx, *dw, scratch)), _lib.HEAD_NORM_SCRATCH if with_dw else 0,
+        *(_data(t) for t in (*dx, *dw, scratch)), _lib.HEAD_NORM_SCRATCH if with_dw else 0,
         _lib.stream_int()), "lvx_head_norm_rope_bwd")
     _count(2 if with_dw else 1)
     return (*dx, *dw)
@@ -612,7 +631,7 @@ def device_lengths(lengths, batch: int, most: int, device):
     """Valid lengths [batch] of any form as int32 on the device (the kernels clamp them to 0..most), or None."""
     if lengths is None:
         return None
-    t = torch.as_tensor(lengths)
+    t = lengths if torch.is_tensor(lengths) else torch.as_tensor(lengths)
     if t.dtype not in (torch.int32, torch.int64) or t.shape != (batch,):
         raise ValueError(f"valid lengths must be {batch} integers, one per batch entry")
     if not t.is_cuda:
@@ -632,36 +651,34 @@ def _text_view(t):
     return rows_view(t, 8, repeats=False)
 
 
-_window_bytes: dict = {}      # a function of the sizes alone
+_window_calls: dict = {}      # descriptions and scratch sizes, which are functions of the sizes alone
 
 
 def _window_setup(q, k, window, sinks, query_start):
-    shp = shape_of(q, k)
-    win = _lib.LvxWindow(window, sinks, query_start)
-    key = (shp.B, shp.Hq, shp.Hkv, shp.Sq, shp.Skv, shp.dtype, window, sinks)
-    sizes = _window_bytes.get(key)
-    if sizes is None:
+    """(shape, window, forward scratch, backward scratch) of a call, the first two as the library takes them."""
+    key = (q.shape, k.shape, q.dtype, window, sinks, query_start)
+    call = _window_calls.get(key)
+    if call is None:
+        shp, win = ctypes.byref(shape_of(q, k)), ctypes.byref(_lib.LvxWindow(window, sinks, query_start))
         f, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
-        _lib.check(_lib.load().lvx_window_workspace(ctypes.byref(shp), ctypes.byref(win), ctypes.byref(f), ctypes.byref(b)),
-                   "lvx_window_workspace")
-        if len(_window_bytes) >= 4096:
-            _window_bytes.clear()
-        sizes = _window_bytes[key] = f.value, b.value
-    return shp, win, sizes
+        _lib.check(_lib.load().lvx_window_workspace(shp, win, ctypes.byref(f), ctypes.byref(b)), "lvx_window_workspace")
+        if len(_window_calls) >= 4096:
+            _window_calls.clear()
+        call = _window_calls[key] = shp, win, f.value, b.value
+    return call
 
 
 def window_forward(q, k, v, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len):
     """(o [B, Hq, Sq, 128], lse fp32 [B*Hq, Sq]) of causal attention (lvx_window says which keys a query sees). The caller has
     checked the tensors."""
-    shp, win, (nbytes, _) = _window_setup(q, k, window, sinks, query_start)
+    shp, win, nbytes, _ = _window_setup(q, k, window, sinks, query_start)
     qv, kv, vv = _text_view(q), _text_view(k), _text_view(v)
+    B, Hq, Sq, _ = q.shape
     o = q.new_empty(q.shape)
-    lse = q.new_empty(shp.B * shp.Hq, shp.Sq, dtype=torch.float32)
+    lse = q.new_empty((B * Hq, Sq), dtype=torch.float32)
     ws = lse.new_empty(nbytes // 4) if nbytes else None
-    _lib.check(_lib.load().lvx_window_forward(ctypes.byref(shp), ctypes.byref(win), _ref(qv), _ref(kv), _ref(vv),
-                                              None if kv_valid_len is None else kv_valid_len.data_ptr(), sm_scale,
-                                              None if ws is None else ws.data_ptr(), nbytes, o.data_ptr(), lse.data_ptr(),
-                                              _lib.stream_int()), "lvx_window_forward")
+    _lib.check(_lib.load().lvx_window_forward(shp, win, _ref(qv), _ref(kv), _ref(vv), _data(kv_valid_len), sm_scale, _data(ws),
+                                              nbytes, o.data_ptr(), lse.data_ptr(), _lib.stream_int()), "lvx_window_forward")
     _count(2 if nbytes else 1)
     return o, lse
 
@@ -673,71 +690,69 @@ def _dense(t):
 
 def window_backward(do, q, k, v, o, lse, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len):
     """(dq, dk, dv) of window_forward."""
-    shp, win, (_, nbytes) = _window_setup(q, k, window, sinks, query_start)
+    shp, win, _, nbytes = _window_setup(q, k, window, sinks, query_start)
     qv, kv, vv = _text_view(q), _text_view(k), _text_view(v)
     do = _dense(do)
-    dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     ws = lse.new_empty(nbytes // 4)
-    _lib.check(_lib.load().lvx_window_backward(ctypes.byref(shp), ctypes.byref(win), do.data_ptr(), _ref(qv), _ref(kv), _ref(vv),
-                                               o.data_ptr(), lse.data_ptr(),
-                                               None if kv_valid_len is None else kv_valid_len.data_ptr(), sm_scale,
-                                               ws.data_ptr(), nbytes, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    _lib.check(_lib.load().lvx_window_backward(shp, win, do.data_ptr(), _ref(qv), _ref(kv), _ref(vv), o.data_ptr(),
+                                               lse.data_ptr(), _data(kv_valid_len), sm_scale, ws.data_ptr(), nbytes, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                                _lib.stream_int()), "lvx_window_backward")
     _count(2 if q.dtype == torch.float32 else 3)
     return dq, dk, dv
 
 
-_shared_bytes: dict = {}
+_shared_calls: dict = {}
 
 
 def _shared_setup(q, pk, k):
-    shp = _lib.make_shape(q.shape[0], q.shape[1], pk.shape[1], q.shape[2], 0 if k is None else k.shape[2], 128, q.dtype)
-    P, N = pk.shape[0], pk.shape[2]
-    key = (shp.B, shp.Hq, shp.Hkv, shp.Sq, shp.Skv, shp.dtype, P, N)
-    sizes = _shared_bytes.get(key)
-    if sizes is None:
+    """(shape as the library takes it, prefixes, length, forward scratch, backward scratch, launches around the block kernels)"""
+    key = (q.shape, pk.shape, None if k is None else k.shape[2], q.dtype)
+    call = _shared_calls.get(key)
+    if call is None:
+        B, Hq, Sq, _ = q.shape
+        P, Hkv, N, _ = pk.shape
+        Skv = 0 if k is None else k.shape[2]
+        shp = ctypes.byref(_lib.make_shape(B, Hq, Hkv, Sq, Skv, 128, q.dtype))
         f, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
-        _lib.check(_lib.load().lvx_shared_workspace(ctypes.byref(shp), P, N, ctypes.byref(f), ctypes.byref(b)), "lvx_shared_workspace")
-        if len(_shared_bytes) >= 4096:
-            _shared_bytes.clear()
-        sizes = _shared_bytes[key] = f.value, b.value
-    return shp, P, N, sizes
+        _lib.check(_lib.load().lvx_shared_workspace(shp, P, N, ctypes.byref(f), ctypes.byref(b)), "lvx_shared_workspace")
+        if len(_shared_calls) >= 4096:
+            _shared_calls.clear()
+        call = _shared_calls[key] = shp, P, N, f.value, b.value, (P < B and Hkv > 1) + (Skv > 0)
+    return call
 
 
-def _views(*ts):
-    return [None if t is None else _text_view(t) for t in ts]
-
-
-def _data(t):
-    return None if t is None else t.data_ptr()
+def _text_views(*ts):
+    """Views kept alive by the first list, references to them in the second; None for None."""
+    views = [None if t is None else _text_view(t) for t in ts]
+    return views, [_ref(t) for t in views]
 
 
 def shared_forward(q, pk, pv, k, v, sm_scale: float, prefix_valid_len, kv_valid_len):
     """(o [B, Hq, Sq, 128], lse fp32 [B*Hq, Sq]) of attention over shared prefixes and own keys (lvx_shared_forward); k and v may
     be None. The caller has checked the tensors."""
-    shp, P, N, (nbytes, _) = _shared_setup(q, pk, k)
-    views = _views(q, pk, pv, k, v)
+    shp, P, N, nbytes, _, more = _shared_setup(q, pk, k)
+    keep, (qv, pkv, pvv, kv, vv) = _text_views(q, pk, pv, k, v)
+    B, Hq, Sq, _ = q.shape
     o = q.new_empty(q.shape)
-    lse = q.new_empty(shp.B * shp.Hq, shp.Sq, dtype=torch.float32)
+    lse = q.new_empty((B * Hq, Sq), dtype=torch.float32)
     ws = lse.new_empty(nbytes // 4)
-    qv, pkv, pvv, kv, vv = (_ref(t) for t in views)
-    _lib.check(_lib.load().lvx_shared_forward(ctypes.byref(shp), P, N, qv, pkv, pvv, _data(prefix_valid_len), kv, vv,
-                                              _data(kv_valid_len), sm_scale, ws.data_ptr(), nbytes, o.data_ptr(), lse.data_ptr(),
-                                              _lib.stream_int()), "lvx_shared_forward")
-    _count(2 + (P < shp.B and shp.Hkv > 1) + (shp.Skv > 0))
+    _lib.check(_lib.load().lvx_shared_forward(shp, P, N, qv, pkv, pvv, _data(prefix_valid_len), kv, vv, _data(kv_valid_len),
+                                              sm_scale, ws.data_ptr(), nbytes, o.data_ptr(), lse.data_ptr(), _lib.stream_int()),
+               "lvx_shared_forward")
+    _count(2 + more)
     return o, lse
 
 
 def shared_backward(do, q, pk, pv, k, v, o, lse, sm_scale: float, prefix_valid_len, kv_valid_len):
     """(dq, dpk, dpv, dk, dv) of shared_forward."""
-    shp, P, N, (_, nbytes) = _shared_setup(q, pk, k)
-    views = _views(q, pk, pv, k, v)
+    shp, P, N, _, nbytes, more = _shared_setup(q, pk, k)
+    keep, (qv, pkv, pvv, kv, vv) = _text_views(q, pk, pv, k, v)
     do = _dense(do)
     grads = [None if t is None else t.new_empty(t.shape) for t in (q, pk, pv, k, v)]
     ws = lse.new_empty(nbytes // 4)
-    qv, pkv, pvv, kv, vv = (_ref(t) for t in views)
-    _lib.check(_lib.load().lvx_shared_backward(ctypes.byref(shp), P, N, do.data_ptr(), qv, pkv, pvv, _data(prefix_valid_len), kv, vv,
+    _lib.check(_lib.load().lvx_shared_backward(shp, P, N, do.data_ptr(), qv, pkv, pvv, _data(prefix_valid_len), kv, vv,
                                                _data(kv_valid_len), o.data_ptr(), lse.data_ptr(), sm_scale, ws.data_ptr(), nbytes,
                                                *(_data(t) for t in grads), _lib.stream_int()), "lvx_shared_backward")
-    _count(3 + (P < shp.B and shp.Hkv > 1) + (shp.Skv > 0))
+    _count(3 + more)
     return grads

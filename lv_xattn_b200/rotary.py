@@ -15,9 +15,12 @@ from . import _lib, ops
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(t):
     """Makes t's device current for the duration of a call (kernels launch on the current device)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def watch_status(t):
@@ -30,37 +33,37 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
     like = q if q is not None else k
     if like is None:
         raise ValueError("head_norm_rope: q or k must be given")
-    for name, t in (("q", q), ("k", k)):
-        if t is not None and (t.dim() != 4 or t.shape[-1] != 128):
-            raise ValueError(f"head_norm_rope: {name} must be [batch, tokens, heads, 128], got {tuple(t.shape)}")
+    for t in (q, k):
+        if t is not None and (t.dim() != 4 or t.shape[3] != 128):
+            raise ValueError(f"head_norm_rope: q and k must be [batch, tokens, heads, 128], got {tuple(t.shape)}")
     if like.dtype not in _TYPES:
         raise ValueError(f"head_norm_rope: dtype {like.dtype} unsupported; expected bfloat16, float16 or float32")
     if q is not None and k is not None and (q.dtype != k.dtype or q.shape[:2] != k.shape[:2]):
         raise ValueError("head_norm_rope: q and k must agree on dtype, batch and tokens")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
     if (q is None and q_weight is not None) or (k is None and k_weight is not None):
         raise ValueError("head_norm_rope: a weight without the tensor that it scales")
-    for w in weights:
-        if w.shape != (128,) or w.dtype not in (like.dtype, torch.float32) or w.dtype != weights[0].dtype:
+    weight = q_weight if q_weight is not None else k_weight
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (128,) or (w.dtype != like.dtype and w.dtype != torch.float32) or w.dtype != weight.dtype):
             raise ValueError("head_norm_rope: weights must be [128], both fp32 or both in the dtype of q and k")
     if (cos is None) != (sin is None):
         raise ValueError("head_norm_rope: cos and sin go together")
-    if cos is None and not weights:
+    if cos is None and weight is None:
         raise ValueError("head_norm_rope: neither a weight nor cos and sin: nothing to do")
     if cos is not None:
         B, S = like.shape[:2]
         if cos.shape != sin.shape or tuple(cos.shape) not in ((S, 128), (1, S, 128), (B, S, 128)):
             raise ValueError(f"head_norm_rope: cos and sin must be [{S}, 128] or [1 or {B}, {S}, 128], got {tuple(cos.shape)} and {tuple(sin.shape)}")
-        if cos.dtype != sin.dtype or cos.dtype not in (like.dtype, torch.float32):
+        if cos.dtype != sin.dtype or (cos.dtype != like.dtype and cos.dtype != torch.float32):
             raise ValueError("head_norm_rope: cos and sin must be fp32 or in the dtype of q and k")
     if not eps >= 0:
         raise ValueError("head_norm_rope: eps must be non-negative")
-    for t in (q, k, cos, sin, *weights):
-        if t is not None:
+    device = like.device
+    for t in (q, k, cos, sin, q_weight, k_weight):
+        if t is not None and (not t.is_cuda or t.device != device):
             if not t.is_cuda:
                 raise _lib.LvxError("lv_xattn_b200 runs on CUDA tensors only; there is no CPU path")
-            if t.device != like.device:
-                raise ValueError("head_norm_rope: all tensors must be on one device")
+            raise ValueError("head_norm_rope: all tensors must be on one device")
 
 
 def _rows(t):
@@ -77,13 +80,11 @@ class HeadNormRopeFunc(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps):
-        with on_device(q if q is not None else k):
-            out = ops.head_norm_rope(q, k, q_weight, k_weight, cos, sin, eps)
-        # without a norm the gradient does not depend on the input
+        out = ops.head_norm_rope(q, k, q_weight, k_weight, cos, sin, eps)
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
-        return tuple(out)
+        return out
 
     @staticmethod
     def backward(ctx, gq, gk):
@@ -113,5 +114,10 @@ def head_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1
     the weights' are summed in a fixed order."""
     _check(q, k, q_weight, k_weight, cos, sin, eps)
     q_weight, k_weight, cos, sin = (_rows(t) for t in (q_weight, k_weight, cos, sin))
-    watch_status(q if q is not None else k)
-    return HeadNormRopeFunc.apply(q, k, q_weight, k_weight, cos, sin, float(eps))
+    like = q if q is not None else k
+    watch_status(like)
+    args = (q, k, q_weight, k_weight, cos, sin, float(eps))
+    with on_device(like):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+            return HeadNormRopeFunc.apply(*args)
+        return ops.head_norm_rope(*args)

@@ -32,13 +32,16 @@ def _check_attention(who, q, kv):
             raise ValueError(f"{who}: q and {name} must share one dtype")
         if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
             raise ValueError(f"{who}: {q.shape[1]} query heads are not a multiple of the {k.shape[1]} heads of {name}")
-    if max([q.shape[2]] + [k.shape[2] for _, k, _ in kv]) >= _MOST:
+        if k.shape[2] >= _MOST:
+            raise ValueError(f"{who}: lengths must be below {_MOST}")
+    if q.shape[2] >= _MOST:
         raise ValueError(f"{who}: lengths must be below {_MOST}")
-    tensors = [q] + [t for _, k, v in kv for t in (k, v)]
-    if not all(t.is_cuda for t in tensors):
-        raise _lib.LvxError("lv_xattn_b200 runs on CUDA tensors only; there is no CPU path")
-    if any(t.device != q.device for t in tensors):
-        raise ValueError(f"{who}: all tensors must be on one device")
+    device = q.device
+    for name, k, v in kv:
+        if not (q.is_cuda and k.is_cuda and v.is_cuda):
+            raise _lib.LvxError("lv_xattn_b200 runs on CUDA tensors only; there is no CPU path")
+        if k.device != device or v.device != device:
+            raise ValueError(f"{who}: all tensors must be on one device")
 
 
 def _scale(who, sm_scale):
@@ -58,10 +61,13 @@ class WindowAttentionFunc(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, o, lse, kv_valid_len)
         ctx.args = sm_scale, window, sinks, query_start
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return o, lse
 
     @staticmethod
     def backward(ctx, do, _):
+        if do is None:
+            return (None,) * 8
         q, k, v, o, lse, kv_valid_len = ctx.saved_tensors
         with on_device(q):
             grads = ops.window_backward(do, q, k, v, o, lse, *ctx.args, kv_valid_len)
@@ -113,10 +119,13 @@ class SharedPrefixAttentionFunc(torch.autograd.Function):
         ctx.save_for_backward(q, pk, pv, k, v, o, lse, prefix_valid_len, kv_valid_len)
         ctx.sm_scale = sm_scale
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return o, lse
 
     @staticmethod
     def backward(ctx, do, _):
+        if do is None:
+            return (None,) * 8
         q, pk, pv, k, v, o, lse, prefix_valid_len, kv_valid_len = ctx.saved_tensors
         with on_device(q):
             grads = ops.shared_backward(do, q, pk, pv, k, v, o, lse, ctx.sm_scale, prefix_valid_len, kv_valid_len)
