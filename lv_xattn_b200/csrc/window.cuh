@@ -80,6 +80,14 @@ __device__ __forceinline__ uint32_t visible_bits(int key0, int lo, int hi, int s
 // [B, Hq, Sq]); shared by the launchers and the workspace query. nsplit == 1 and not `few`: results are written directly.
 FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few);
 
+// SMs of the current device.
+inline int num_sms() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0)
+    return n;
+  return 148;
+}
+
 // Tensor map of up to five dimensions over 128-byte wide boxes with the 128-byte swizzle; strides in bytes, from the second
 // dimension on.
 int make_tmap_nd(CUtensorMap* out, int dtype, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,

@@ -137,7 +137,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   const bool misaligned = (smem_u32(smem) & 1023u) != 0;      // the operand descriptors assume 1024-byte aligned tiles
   if (misaligned && tid == 0) atomicCAS(p.status, 0, WB_CODE(7, 0));
-  const bool poisoned = misaligned || (*reinterpret_cast<volatile int*>(p.status) != 0);
+  // the status word may be set at any moment: one thread reads it, and the CTA leaves or stays as a whole
+  int word = misaligned;
+  if (tid == 0) word |= *reinterpret_cast<volatile int*>(p.status);
 
   if (tid == 0) {
     for (int b = 0; b < WBB_COUNT; ++b)
@@ -157,7 +159,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  const bool poisoned = __syncthreads_or(word) != 0;
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -605,13 +607,6 @@ window_dq_kernel(const float* __restrict__ acc, uint16_t* __restrict__ dq, int g
   }
 }
 
-static int window_num_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0)
-    return n;
-  return 148;
-}
-
 // The key tiles of the sinks that are shared out over several items, and over how many: as many as make an item about as long
 // as those of the other keys.
 static SinkParts sink_parts(const lvx_shape& s, const lvx_window& w) {
@@ -668,7 +663,7 @@ int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
   p.status = status;
-  const int grid = std::min(p.nitems, window_num_sms());
+  const int grid = std::min(p.nitems, num_sms());
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WB_SMEM);

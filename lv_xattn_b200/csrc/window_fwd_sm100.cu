@@ -33,9 +33,11 @@ constexpr int WF_TILE = 128 * 128 * 2;
 constexpr int WF_HALF = WF_TILE / 2;
 constexpr int WF_OFF_K = 2 * WF_TILE;            // after the two Q tiles
 constexpr int WF_OFF_V = WF_OFF_K + WF_NS * WF_TILE;
-constexpr int WF_OFF_BAR = WF_OFF_V + WF_NS * WF_TILE;
+constexpr int WF_OFF_OUT = WF_OFF_V + WF_NS * WF_TILE;      // 4 KB per softmax warp: its rows of O on their way out
+constexpr int WF_OFF_BAR = WF_OFF_OUT + 8 * 4096;
 constexpr int WF_SMEM = WF_OFF_BAR + 256 + 1024;  // + barriers + alignment slack
-constexpr int WF_THREADS = 320;
+constexpr int WF_THREADS = 384;
+static_assert(WF_SMEM <= 232448, "shared memory budget");
 // PAIR from this many key tiles on. us a call, one warpgroup per query tile -> PAIR, 32 tokens of 32 heads on 8 KV heads, over
 // 512 / 2,048 / 4,096 / 16,384 keys, combine kernel included where there is one:
 //    1 entry      15.7 ->  17.5    16.7 -> 18.9    19.2 ->  19.7     31 ->  27
@@ -45,7 +47,8 @@ constexpr int kPairTiles = 32;
 
 enum {
   WFB_Q_FULL = 0,
-  WFB_K_FULL = 1,
+  WFB_Q_EMPTY,
+  WFB_K_FULL,
   WFB_K_EMPTY = WFB_K_FULL + WF_NS,
   WFB_V_FULL = WFB_K_EMPTY + WF_NS,
   WFB_V_EMPTY = WFB_V_FULL + WF_NS,
@@ -59,6 +62,7 @@ enum {
 
 struct WinFwdParams {
   int sq, skv, hkv, g, m_blocks;
+  int slabs, splits, nitems;      // an item: a pair of query tiles of a slab, and a share of its keys
   QTiles qt;
   WindowMask mask;
   const int32_t* kv_valid_len;
@@ -72,12 +76,36 @@ struct WinFwdParams {
   int* status;
 };
 
-// 32 columns of one row's O over keys [key0, key1), as plain fp32 sums.
+// One row's O as plain fp32 sums over its keys in tiles j = first, first + step, ... < n of `kt` from j0 on, written where the
+// row belongs: in the input type and divided by l (`out16`), or as it is.
+struct PlainRow {
+  const uint16_t *q, *k, *v;
+  uint16_t* out16;
+  float* out;
+  int first, step, n, j0, lo, hi, sink_end;
+  float m, l;
+};
 template <bool IS_BF16>
-__device__ __noinline__ void window_plain_values(float* o, const uint16_t* q, const uint16_t* k, const uint16_t* v, long long ks,
-                                                 long long vs, int key0, int key1, float c, float m) {
-  for (int key = key0; key < key1; ++key)
-    axpy32<IS_BF16>(o, ex2f(dot128<IS_BF16>(q, k + key * ks) * c - m), v + key * vs);
+__device__ __noinline__ void window_plain_row(const WinFwdParams& p, const KeyTiles& kt, const PlainRow& x) {
+  for (int d = 0; d < 128; d += 32) {
+    float o[32];
+    for (int i = 0; i < 32; ++i) o[i] = 0.f;
+    for (int j = x.first; j < x.n; j += x.step) {
+      const int key0 = kt.tile(x.j0 + j) * 128, cut = min(key0 + 128, x.sink_end);
+      for (int key = key0; key < min(key0 + 128, x.hi + 1); ++key)
+        if (key < cut || key >= x.lo)
+          axpy32<IS_BF16>(o, ex2f(dot128<IS_BF16>(x.q, x.k + key * p.k_s) * p.scale_log2 - x.m), x.v + key * p.v_s + d);
+    }
+    for (int i = 0; i < 32; i += 2) {
+      if (x.out16 != nullptr) {
+        const float inv = x.l > 0.f ? 1.f / x.l : 0.f;
+        reinterpret_cast<uint32_t*>(x.out16 + d)[i / 2] = IS_BF16 ? pack_bf16x2(o[i] * inv, o[i + 1] * inv) : pack_f16x2(o[i] * inv, o[i + 1] * inv);
+      } else {
+        x.out[d + i] = o[i];
+        x.out[d + i + 1] = o[i + 1];
+      }
+    }
+  }
 }
 
 // PAIR: the slab has a single query tile (65 to 128 rows: a token each of 32 requests that share a prefix), and the two
@@ -94,25 +122,42 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int slab = blockIdx.x, mb = p.m_blocks - 1 - int(blockIdx.y), split = blockIdx.z;
-  const int batch = slab / p.hkv, kvh = slab % p.hkv;
   const int heads = p.qt.heads, tile_rows = heads * p.qt.tokens;
+  struct Item {
+    int mb, slab, split, valid, start;
+    KeyTiles kt;
+    int j0, n;               // its share of the key tiles
+  };
+  // the CTA's round-th item: forwards and backwards through the list in turn
+  auto index_of = [&](int round) {
+    return round * int(gridDim.x) + ((round & 1) ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x));
+  };
+  auto item_of = [&](int w) {
+    Item it;
+    it.slab = w % p.slabs;
+    const int rest = w / p.slabs;
+    it.split = rest / p.m_blocks;
+    it.mb = p.m_blocks - 1 - rest % p.m_blocks;
+    it.valid = p.skv;
+    if (p.kv_valid_len) it.valid = min(it.valid, max(0, p.kv_valid_len[it.slab / p.hkv]));
+    it.start = p.mask.start >= 0 ? p.mask.start : it.valid - p.sq;
+    // token range of the two tiles (the second may not exist: its rows do not then, and its tile is loaded as zeros)
+    const int tok0 = (2 * it.mb / p.qt.chunks) * p.qt.tokens;
+    const int tok1 = min(p.sq, (min(2 * it.mb + 1, p.qt.count - 1) / p.qt.chunks + 1) * p.qt.tokens) - 1;
+    it.kt = key_tiles(p.mask, it.valid, it.start + tok0, it.start + tok1, 7);
+    const int per_split = (it.kt.n + p.splits - 1) / p.splits;
+    it.j0 = min(it.kt.n, it.split * per_split);
+    it.n = min(it.kt.n, it.j0 + per_split) - it.j0;
+    return it;
+  };
 
-  int valid = p.skv;
-  if (p.kv_valid_len) valid = min(valid, max(0, p.kv_valid_len[batch]));
-  const int start = p.mask.start >= 0 ? p.mask.start : valid - p.sq;
-  // token range of the CTA's two tiles (the second may not exist: its rows do not then, and its tile is loaded as zeros)
-  const int tok0 = (2 * mb / p.qt.chunks) * p.qt.tokens;
-  const int tok1 = min(p.sq, (min(2 * mb + 1, p.qt.count - 1) / p.qt.chunks + 1) * p.qt.tokens) - 1;
-  const KeyTiles kt = key_tiles(p.mask, valid, start + tok0, start + tok1, 7);
-  const int per_split = (kt.n + gridDim.z - 1) / gridDim.z;
-  const int j0 = min(kt.n, split * per_split);
-  const int n = min(kt.n, j0 + per_split) - j0;
-
-  const bool poisoned = (*reinterpret_cast<volatile int*>(p.status) != 0);
+  // the status word may be set at any moment: one thread reads it, and the CTA leaves or stays as a whole
+  int word = 0;
+  if (tid == 0) word = *reinterpret_cast<volatile int*>(p.status);
 
   if (tid == 0) {
     mbar_init(&bars[WFB_Q_FULL], 1);
+    mbar_init(&bars[WFB_Q_EMPTY], 1);
     for (int s = 0; s < WF_NS; ++s) {
       mbar_init(&bars[WFB_K_FULL + s], 1);
       mbar_init(&bars[WFB_K_EMPTY + s], 1);
@@ -139,39 +184,45 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  const bool poisoned = __syncthreads_or(word) != 0;
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-
-  if (!poisoned && warp < 8) {
+  // Every role walks the same items in the same order and keeps the same counters: `it` = items with key tiles done, `jj0` =
+  // key tiles done before the current item (PAIR: t0, those of one warpgroup). All barrier phases follow from them.
+  // Registers: 384 threads are launched with 168 each; 256 x 208 + 128 x 88 is the same number of them.
+  if (warp < 8) {
     // =========================== softmax warpgroups ===========================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
     const int wg = warp >> 2;
     const int r = (warp & 3) * 32 + lane;            // row of the tile, TMEM lane
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem_base + wg * 128 + lane_sel;
     const uint32_t tO = tmem_base + 256 + wg * 128 + lane_sel;
     const float c = p.scale_log2;
-    const int tile = PAIR ? 0 : 2 * mb + wg, tile_tok = (tile / p.qt.chunks) * p.qt.tokens;
-    const int tok = tile_tok + r / heads, head = (tile % p.qt.chunks) * heads + r % heads;
+    // this warpgroup's key tiles: all of an item's, or every other one
+    constexpr int STEP = PAIR ? 2 : 1;
+    const int first = PAIR ? wg : 0;
+    bool alive = !poisoned;
+    int done_items = 0, t0 = 0;      // items with tiles of this warpgroup, and those tiles
+    for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
+    const Item I = item_of(w);
+    const int tile = PAIR ? 0 : 2 * I.mb + wg;
+    const int tok = (tile / p.qt.chunks) * p.qt.tokens + r / heads, head = (tile % p.qt.chunks) * heads + r % heads;
     const bool exists = tile < p.qt.count && r < tile_rows && tok < p.sq && head < p.g;
     // this row's keys: [0, sink_end) and [lo, hi]. A row that does not exist sees everything against a reference of 0 (its
     // scores are zeros), so that it never holds up its warp.
-    const int pos = start + tok;
-    const int hi = exists ? min(pos, valid - 1) : valid - 1;
-    const int lo = exists ? max(0, pos - p.mask.window + 1) : 0;
+    const int hi = exists ? min(I.start + tok, I.valid - 1) : I.valid - 1;
+    const int lo = exists ? max(0, I.start + tok - p.mask.window + 1) : 0;
     const int sink_end = min(p.mask.sinks, hi + 1);
     // keys that every row of the warp sees: [0, all_sinks) and [all_lo, all_hi]
     const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
     const int all_sinks = min(p.mask.sinks, all_hi + 1);
     float m = exists ? -INFINITY : 0.f, l = 0.f;
-    bool alive = true;
-    // this warpgroup's key tiles: all of the CTA's, or every other one
-    constexpr int STEP = PAIR ? 2 : 1;
-    const int first = PAIR ? wg : 0;
-    for (int j = first, t = 0; j < n; j += STEP, ++t) {
-      const int key0 = kt.tile(j0 + j) * 128;
+    int t = 0;                       // tiles of this warpgroup in the item
+    for (int j = first; j < I.n; j += STEP, ++t) {
+      const int key0 = I.kt.tile(I.j0 + j) * 128;
       const bool full = key0 + 127 <= all_hi && (key0 >= all_lo || key0 + 128 <= all_sinks);
-      if (!mbar_wait(&bars[WFB_S_FULL + wg], t & 1, abort_flag, p.status, WF_CODE(wg, WFB_S_FULL))) {
+      if (!mbar_wait(&bars[WFB_S_FULL + wg], (t0 + t) & 1, abort_flag, p.status, WF_CODE(wg, WFB_S_FULL))) {
         alive = false;
         break;
       }
@@ -216,24 +267,38 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
       if (!done) {
+        // The first tile, tiles that are seen in part, and scores that jumped: with the row maximum. A warp's rows are few
+        // tokens, so of a partly seen tile's four groups of 32 keys all but one or two are seen by all of its rows or by none;
+        // those that none sees are zeros without an exponential, and only the mixed ones are masked.
         uint32_t s[4][32];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, s[q]);
-        tc_wait_ld();
+        uint32_t none = 0;      // bit q: group q is seen by no row of the warp
         if (!full) {
+          uint32_t seen[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const uint32_t seen = visible_bits(key0 + q * 32, lo, hi, sink_end);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(seen & (1u << i))) s[q][i] = 0xff800000u;  // -inf
+            seen[q] = visible_bits(key0 + q * 32, lo, hi, sink_end);
+            if (!__any_sync(0xffffffffu, seen[q] != 0u)) none |= 1u << q;
           }
+          tc_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (!(none >> q & 1) && !__all_sync(0xffffffffu, seen[q] == 0xffffffffu)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(seen[q] & (1u << i))) s[q][i] = 0xff800000u;  // -inf
+            }
+        } else {
+          tc_wait_ld();
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int q = 0; q < 4; ++q)
+          if (!(none >> q & 1)) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], __uint_as_float(s[q][i]));
+            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[q][i]));
+          }
         const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
         const bool grow = m_new > m + 8.f;       // raised only when it would grow by more than 2^8: P stays below 256
         float alpha = 1.f;
@@ -254,22 +319,28 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         }
         const float moff = (m == -INFINITY) ? 0.f : m;
-        float sum0 = 0.f, sum1 = 0.f;
+        const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-moff, -moff);
+        uint64_t sum = f32x2(0.f, 0.f);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pk[16];
+          if (none >> q & 1) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+            for (int i = 0; i < 16; ++i) pk[i] = 0u;
+          } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float a0 = ex2f(fmaf(__uint_as_float(s[2 * h + e][2 * i]), c, -moff));
-              const float a1 = ex2f(fmaf(__uint_as_float(s[2 * h + e][2 * i + 1]), c, -moff));
-              sum0 += a0;
-              sum1 += a1;
-              pk[e * 16 + i] = IS_BF16 ? pack_bf16x2(a0, a1) : pack_f16x2(a0, a1);
+              float x0, x1;
+              f32x2_get(fma2(f32x2(__uint_as_float(s[q][2 * i]), __uint_as_float(s[q][2 * i + 1])), c2, nm2), x0, x1);
+              const float e0 = ex2f(x0), e1 = ex2f(x1);
+              sum = add2(sum, f32x2(e0, e1));
+              pk[i] = IS_BF16 ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1);
             }
-          tmem_st32(tS + h * 32, pk);
+          }
+          tmem_st16(tS + q * 16, pk);
         }
+        float sum0, sum1;
+        f32x2_get(sum, sum0, sum1);
         l += sum0 + sum1;
       }
       tc_wait_st();
@@ -278,109 +349,165 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (lane == 0) mbar_arrive(&bars[WFB_P_FULL + wg]);
     }
     // ------------------------------- epilogue -------------------------------
-    if (alive && n > first) alive = mbar_wait(&bars[WFB_O_DONE + wg], 0, abort_flag, p.status, WF_CODE(wg, WFB_O_DONE));
+    if (alive && t > 0) alive = mbar_wait(&bars[WFB_O_DONE + wg], done_items & 1, abort_flag, p.status, WF_CODE(wg, WFB_O_DONE));
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
     if (alive) {
-      const int qh = kvh * p.g + head;
-      const long long row = (static_cast<long long>(batch) * p.hkv * p.g + qh) * p.sq + tok;      // of [B, Hq, Sq]
-      const long long prow = (static_cast<long long>(slab) * p.nsplit + (PAIR ? 2 * split + wg : split)) * p.g * p.sq + static_cast<long long>(head) * p.sq + tok;
-      const float inv = p.o == nullptr ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
+      uint32_t o[4][32];
+      uint64_t sum2[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        uint32_t o[32];
-        float sum = 0.f;
-        if (n > first) {
-          tmem_ld32(tO + q * 32, o);
-          tc_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) sum += __uint_as_float(o[i]);
+        if (t > 0) {
+          tmem_ld32(tO + q * 32, o[q]);
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
+          for (int i = 0; i < 32; ++i) o[q][i] = 0u;
         }
-        if (exists && isnan(sum) && l < INFINITY) {
-          float again[32];
-          for (int i = 0; i < 32; ++i) again[i] = 0.f;
-          const uint16_t* qrow = p.q + batch * p.q_b + qh * p.q_h + tok * p.q_s;
-          const uint16_t* kb = p.k + batch * p.k_b + kvh * p.k_h;
-          const uint16_t* vb = p.v + batch * p.v_b + kvh * p.v_h + q * 32;
-          for (int j = first; j < n; j += STEP) {
-            const int key0 = kt.tile(j0 + j) * 128, key1 = key0 + 128;
-            const int cut = min(key1, sink_end);          // the sinks, then what of the window lies behind them
-            window_plain_values<IS_BF16>(again, qrow, kb, vb, p.k_s, p.v_s, key0, cut, c, m == -INFINITY ? 0.f : m);
-            window_plain_values<IS_BF16>(again, qrow, kb, vb, p.k_s, p.v_s, max(max(key0, cut), lo), min(key1, hi + 1), c,
-                                         m == -INFINITY ? 0.f : m);
-          }
+      }
+      tc_wait_ld();
+      tc_fence_before();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(again[i]);
+      for (int q = 0; q < 4; ++q) {
+        sum2[q] = 0ull;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum2[q] = add2(sum2[q], f32x2(__uint_as_float(o[q][2 * i]), __uint_as_float(o[q][2 * i + 1])));
+      }
+      float sum_a, sum_b;
+      f32x2_get(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_a, sum_b);
+      const bool again = exists && isnan(sum_a + sum_b) && l < INFINITY;
+      // The warp's rows go through shared memory, 128 bytes of each at a time (16-byte pieces, rotated by row against bank
+      // conflicts), so that a store covers whole sectors: written by row they are 32 pieces of 16 bytes, 256 bytes apart.
+      const int row = head * p.sq + tok;         // of the slab
+      const unsigned here = __ballot_sync(0xffffffffu, exists);
+      uint8_t* out = smem + WF_OFF_OUT + warp * 4096;
+      const bool direct = p.o != nullptr;
+      const size_t slab_rows = size_t(p.g) * p.sq;
+      uint8_t* base;
+      int row_bytes;
+      if (direct) {
+        base = static_cast<uint8_t*>(p.o) + size_t(I.slab) * slab_rows * 256;
+        row_bytes = 256;
+      } else {
+        base = reinterpret_cast<uint8_t*>(p.o_part) + (size_t(I.slab) * p.nsplit + (PAIR ? 2 * I.split + wg : I.split)) * slab_rows * 512;
+        row_bytes = 512;
+      }
+      auto store = [&](int at) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = i * 4 + (lane >> 3), piece = lane & 7;
+          const int to = __shfl_sync(0xffffffffu, row, rr);
+          if (here >> rr & 1)
+            *reinterpret_cast<uint4*>(base + size_t(to) * row_bytes + at + piece * 16) =
+                *reinterpret_cast<const uint4*>(out + rr * 128 + ((piece ^ (rr & 7)) << 4));
         }
-        if (exists && p.o != nullptr) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + row * 128 + q * 32);
+        __syncwarp();
+      };
+      if (direct) {
+        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
+            uint32_t w4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float a = __uint_as_float(o[8 * i + 2 * e]) * inv, b = __uint_as_float(o[8 * i + 2 * e + 1]) * inv;
-              w[e] = IS_BF16 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
+              const float x = __uint_as_float(o[q][8 * i + 2 * e]) * inv, y = __uint_as_float(o[q][8 * i + 2 * e + 1]) * inv;
+              w4[e] = IS_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
             }
-            dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(out + lane * 128 + ((((q & 1) * 4 + i) ^ (lane & 7)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
           }
-        } else if (exists) {
-          float4* dst = reinterpret_cast<float4*>(p.o_part + prow * 128 + q * 32);
+          if (q & 1) store((q >> 1) * 128);
+        }
+        if (exists) p.lse[size_t(I.slab) * slab_rows + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                                 __uint_as_float(o[4 * i + 3]));
+            *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[q][4 * i], o[q][4 * i + 1], o[q][4 * i + 2], o[q][4 * i + 3]);
+          store(q * 128);
         }
-        __syncwarp();      // the next load of TMEM wants the whole warp
+        if (exists)
+          reinterpret_cast<float2*>(p.ml_part)[(size_t(I.slab) * p.nsplit + (PAIR ? 2 * I.split + wg : I.split)) * slab_rows + row] = make_float2(m, l);
       }
-      if (exists) {
-        if (p.o != nullptr) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-        else *reinterpret_cast<float2*>(p.ml_part + prow * 2) = make_float2(m, l);
+      if (again) {
+        const int batch = I.slab / p.hkv, kvh = I.slab % p.hkv;
+        PlainRow x;
+        x.q = p.q + batch * p.q_b + (kvh * p.g + head) * p.q_h + tok * p.q_s;
+        x.k = p.k + batch * p.k_b + kvh * p.k_h;
+        x.v = p.v + batch * p.v_b + kvh * p.v_h;
+        x.out16 = direct ? reinterpret_cast<uint16_t*>(base + size_t(row) * 256) : nullptr;
+        x.out = reinterpret_cast<float*>(base + size_t(row) * 512);
+        x.first = first;
+        x.step = STEP;
+        x.n = I.n;
+        x.j0 = I.j0;
+        x.lo = lo;
+        x.hi = hi;
+        x.sink_end = sink_end;
+        x.m = m == -INFINITY ? 0.f : m;
+        x.l = l;
+        window_plain_row<IS_BF16>(p, I.kt, x);
       }
+      __syncwarp();
     }
-  } else if (!poisoned && warp == 8 && n > 0) {
-    // =========================== TMA producer ===========================
-    if (lane == 0) {
+    done_items += t > 0;
+    t0 += t;
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
+    if (warp == 8 && lane == 0 && !poisoned) {
+      // =========================== TMA producer ===========================
       tma_prefetch_desc(&tmQ);
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
-      mbar_arrive_expect_tx(&bars[WFB_Q_FULL], (PAIR ? 1 : 2) * tile_rows * 256);
-      for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
-        const int tile = 2 * mb + t;
-        for (int h = 0; h < 2; ++h)
-          tma_load_5d(smem + t * WF_TILE + h * WF_HALF, &tmQ, &bars[WFB_Q_FULL], h * 64, (tile % p.qt.chunks) * heads,
-                      (tile / p.qt.chunks) * p.qt.tokens, kvh, batch);
-      }
-      int k_issued = 0, v_issued = 0;
-      for (int j = 0; j < n; ++j) {
-        const int s = j % WF_NS;
-        const uint32_t ph = (j / WF_NS) & 1;
-        const int y = kt.tile(j0 + j) * 128;
-        if (!mbar_wait(&bars[WFB_K_EMPTY + s], ph ^ 1, abort_flag, p.status, WF_CODE(2, WFB_K_EMPTY))) break;
-        mbar_arrive_expect_tx(&bars[WFB_K_FULL + s], WF_TILE);
-        tma_load_4d(smem + WF_OFF_K + s * WF_TILE, &tmK, &bars[WFB_K_FULL + s], 0, y, kvh, batch);
-        tma_load_4d(smem + WF_OFF_K + s * WF_TILE + WF_HALF, &tmK, &bars[WFB_K_FULL + s], 64, y, kvh, batch);
-        k_issued = j + 1;
-        if (!mbar_wait(&bars[WFB_V_EMPTY + s], ph ^ 1, abort_flag, p.status, WF_CODE(2, WFB_V_EMPTY))) break;
-        mbar_arrive_expect_tx(&bars[WFB_V_FULL + s], WF_TILE);
-        tma_load_4d(smem + WF_OFF_V + s * WF_TILE, &tmV, &bars[WFB_V_FULL + s], 0, y, kvh, batch);
-        tma_load_4d(smem + WF_OFF_V + s * WF_TILE + WF_HALF, &tmV, &bars[WFB_V_FULL + s], 64, y, kvh, batch);
-        v_issued = j + 1;
+      int it = 0, jj0 = 0, k_issued = 0, v_issued = 0;
+      bool alive = true;
+      for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
+        const Item I = item_of(w);
+        if (I.n == 0) continue;
+        const int batch = I.slab / p.hkv, kvh = I.slab % p.hkv;
+        // the previous item's last scores have been made: its Q is done with, while its last softmax still runs
+        if (it > 0 && !mbar_wait(&bars[WFB_Q_EMPTY], (it - 1) & 1, abort_flag, p.status, WF_CODE(2, WFB_Q_EMPTY))) break;
+        mbar_arrive_expect_tx(&bars[WFB_Q_FULL], (PAIR ? 1 : 2) * tile_rows * 256);
+        for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
+          const int tile = 2 * I.mb + t;
+          for (int h = 0; h < 2; ++h)
+            tma_load_5d(smem + t * WF_TILE + h * WF_HALF, &tmQ, &bars[WFB_Q_FULL], h * 64, (tile % p.qt.chunks) * heads,
+                        (tile / p.qt.chunks) * p.qt.tokens, kvh, batch);
+        }
+        ++it;
+        for (int j = 0; j < I.n; ++j) {
+          const int jj = jj0 + j, s = jj % WF_NS;
+          const uint32_t ph = (jj / WF_NS) & 1;
+          const int y = I.kt.tile(I.j0 + j) * 128;
+          alive = mbar_wait(&bars[WFB_K_EMPTY + s], ph ^ 1, abort_flag, p.status, WF_CODE(2, WFB_K_EMPTY));
+          if (!alive) break;
+          mbar_arrive_expect_tx(&bars[WFB_K_FULL + s], WF_TILE);
+          tma_load_4d(smem + WF_OFF_K + s * WF_TILE, &tmK, &bars[WFB_K_FULL + s], 0, y, kvh, batch);
+          tma_load_4d(smem + WF_OFF_K + s * WF_TILE + WF_HALF, &tmK, &bars[WFB_K_FULL + s], 64, y, kvh, batch);
+          k_issued = jj + 1;
+          alive = mbar_wait(&bars[WFB_V_EMPTY + s], ph ^ 1, abort_flag, p.status, WF_CODE(2, WFB_V_EMPTY));
+          if (!alive) break;
+          mbar_arrive_expect_tx(&bars[WFB_V_FULL + s], WF_TILE);
+          tma_load_4d(smem + WF_OFF_V + s * WF_TILE, &tmV, &bars[WFB_V_FULL + s], 0, y, kvh, batch);
+          tma_load_4d(smem + WF_OFF_V + s * WF_TILE + WF_HALF, &tmV, &bars[WFB_V_FULL + s], 64, y, kvh, batch);
+          v_issued = jj + 1;
+        }
+        jj0 += I.n;
       }
       if (*abort_flag) {      // a CTA that is giving up must not leave while a copy into its shared memory is in flight
         auto drain = [&](uint64_t* bar, uint32_t ph) {
           const long long t0 = clock64();
           while (!mbar_try_wait(bar, ph) && clock64() - t0 < LVX_SPIN_LIMIT_CYCLES) {}
         };
-        drain(&bars[WFB_Q_FULL], 0);
+        if (it > 0) drain(&bars[WFB_Q_FULL], (it - 1) & 1);
         for (int j = max(0, k_issued - WF_NS); j < k_issued; ++j) drain(&bars[WFB_K_FULL + j % WF_NS], (j / WF_NS) & 1);
         for (int j = max(0, v_issued - WF_NS); j < v_issued; ++j) drain(&bars[WFB_V_FULL + j % WF_NS], (j / WF_NS) & 1);
       }
     }
-  } else if (!poisoned && warp == 9 && n > 0) {
+    if (warp == 9 && !poisoned) {
     // =========================== MMA issuer (the whole warp walks, one elected lane issues) ===========================
     constexpr uint32_t FMT = IS_BF16 ? UMMA_BF16 : UMMA_F16;
     constexpr uint32_t IDESC_QK = umma_idesc(FMT, UMMA_K_MAJOR, UMMA_K_MAJOR, 128, 128);
@@ -416,85 +543,107 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     auto wait = [&](int bar, uint32_t ph) {
       return __all_sync(0xffffffffu, mbar_wait(&bars[bar], ph, abort_flag, p.status, WF_CODE(3, bar)));
     };
-    // rows of V behind the last valid key: whatever they hold is multiplied with zeros
-    auto clear_v = [&](int j, int s) {
-      const int left = valid - kt.tile(j0 + j) * 128;
-      if (left >= 128) return;
-      for (int at = lane; at < (128 - left) * 16; at += 32)
-        *reinterpret_cast<uint4*>(smem + WF_OFF_V + s * WF_TILE + ((at >> 3) & 1) * WF_HALF + (left + (at >> 4)) * 128 + (at & 7) * 16) =
-            make_uint4(0u, 0u, 0u, 0u);
-      fence_async_smem();
-      __syncwarp();
-    };
-    bool ok = wait(WFB_Q_FULL, 0) && wait(WFB_K_FULL, 0);
-    if constexpr (PAIR) {
-      // tile j is warpgroup j % 2's; its scores come two tiles ahead
-      for (int j = 0; ok && j < min(n, 2); ++j) {
-        if (j > 0) ok = wait(WFB_K_FULL + j % WF_NS, j / WF_NS & 1);
-        if (!ok) break;
-        tc_fence_after();
-        issue_qk(j, j % WF_NS);
-        commit(&bars[WFB_S_FULL + j]);
-        commit(&bars[WFB_K_EMPTY + j % WF_NS]);
-      }
-      for (int j = 0; ok && j < n; ++j) {
-        const int i = j & 1, s = j % WF_NS, s2 = (j + 2) % WF_NS;
-        ok = wait(WFB_P_FULL + i, j >> 1 & 1) && wait(WFB_V_FULL + s, j / WF_NS & 1);
-        if (!ok) break;
-        clear_v(j, s);
-        tc_fence_after();
-        issue_pv(i, s, j < 2);
-        commit(&bars[WFB_V_EMPTY + s]);
-        if (j + 2 < n) {
-          ok = wait(WFB_K_FULL + s2, (j + 2) / WF_NS & 1);
+    bool ok = true;
+    int it = 0, jj0 = 0, t0[2] = {0, 0};      // t0: tiles of each warpgroup done
+    for (int round = 0, w; ok && (w = index_of(round)) < p.nitems; ++round) {
+      const Item I = item_of(w);
+      const int n = I.n;
+      if (n == 0) continue;
+      auto k_full = [&](int j) { return wait(WFB_K_FULL + (jj0 + j) % WF_NS, (jj0 + j) / WF_NS & 1); };
+      auto v_full = [&](int j) { return wait(WFB_V_FULL + (jj0 + j) % WF_NS, (jj0 + j) / WF_NS & 1); };
+      auto stage = [&](int j) { return (jj0 + j) % WF_NS; };
+      // rows of V behind the last valid key: whatever they hold is multiplied with zeros
+      auto clear_v = [&](int j) {
+        const int left = I.valid - I.kt.tile(I.j0 + j) * 128;
+        if (left >= 128) return;
+        for (int at = lane; at < (128 - left) * 16; at += 32)
+          *reinterpret_cast<uint4*>(smem + WF_OFF_V + stage(j) * WF_TILE + ((at >> 3) & 1) * WF_HALF + (left + (at >> 4)) * 128 +
+                                    (at & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_smem();
+        __syncwarp();
+      };
+      // the item's first scores: S is free (the tensor pipe runs in order behind the last product with P)
+      ok = wait(WFB_Q_FULL, it & 1) && k_full(0);
+      if constexpr (PAIR) {
+        // tile j is warpgroup j % 2's; its scores come two tiles ahead
+        for (int j = 0; ok && j < min(n, 2); ++j) {
+          if (j > 0) ok = k_full(j);
           if (!ok) break;
           tc_fence_after();
-          issue_qk(i, s2);
-          commit(&bars[WFB_S_FULL + i]);
-          commit(&bars[WFB_K_EMPTY + s2]);
-        } else {
-          commit(&bars[WFB_O_DONE + i]);
+          issue_qk(j, stage(j));
+          commit(&bars[WFB_S_FULL + j]);
+          commit(&bars[WFB_K_EMPTY + stage(j)]);
+          if (j == n - 1) commit(&bars[WFB_Q_EMPTY]);
         }
-      }
-    } else if (ok) {
-      tc_fence_after();
-      issue_qk(0, 0);
-      commit(&bars[WFB_S_FULL + 0]);
-      issue_qk(1, 0);
-      commit(&bars[WFB_S_FULL + 1]);
-      commit(&bars[WFB_K_EMPTY + 0]);
-    }
-    for (int j = 0; !PAIR && ok && j < n; ++j) {
-      const int s = j % WF_NS, s1 = (j + 1) % WF_NS;
-      const uint32_t ph = (j / WF_NS) & 1, ph1 = ((j + 1) / WF_NS) & 1;
+        for (int j = 0; ok && j < n; ++j) {
+          const int i = j & 1;
+          ok = wait(WFB_P_FULL + i, (t0[i] + (j >> 1)) & 1) && v_full(j);
+          if (!ok) break;
+          clear_v(j);
+          tc_fence_after();
+          issue_pv(i, stage(j), j < 2);
+          commit(&bars[WFB_V_EMPTY + stage(j)]);
+          if (j + 2 < n) {
+            ok = k_full(j + 2);
+            if (!ok) break;
+            tc_fence_after();
+            issue_qk(i, stage(j + 2));
+            commit(&bars[WFB_S_FULL + i]);
+            commit(&bars[WFB_K_EMPTY + stage(j + 2)]);
+            if (j + 2 == n - 1) commit(&bars[WFB_Q_EMPTY]);
+          } else {
+            commit(&bars[WFB_O_DONE + i]);
+          }
+        }
+        t0[0] += (n + 1) / 2;
+        t0[1] += n / 2;
+      } else {
+        if (ok) {
+          tc_fence_after();
+          issue_qk(0, stage(0));
+          commit(&bars[WFB_S_FULL + 0]);
+          issue_qk(1, stage(0));
+          commit(&bars[WFB_S_FULL + 1]);
+          commit(&bars[WFB_K_EMPTY + stage(0)]);
+          if (n == 1) commit(&bars[WFB_Q_EMPTY]);
+        }
+        for (int j = 0; ok && j < n; ++j) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (!ok) break;
-        ok = wait(WFB_P_FULL + i, j & 1);
-        if (ok && i == 0) {
-          ok = wait(WFB_V_FULL + s, ph);
-          if (ok) clear_v(j, s);
-        }
-        if (!ok) break;
-        tc_fence_after();
-        issue_pv(i, s, j == 0);
-        if (i == 1) commit(&bars[WFB_V_EMPTY + s]);
-        if (j + 1 < n) {
-          if (i == 0) ok = wait(WFB_K_FULL + s1, ph1);
-          if (!ok) break;
-          tc_fence_after();
-          issue_qk(i, s1);
-          commit(&bars[WFB_S_FULL + i]);
-          if (i == 1) commit(&bars[WFB_K_EMPTY + s1]);
-        } else {
-          commit(&bars[WFB_O_DONE + i]);
+          for (int i = 0; i < 2; ++i) {
+            if (!ok) break;
+            ok = wait(WFB_P_FULL + i, (jj0 + j) & 1);
+            if (ok && i == 0) {
+              ok = v_full(j);
+              if (ok) clear_v(j);
+            }
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(i, stage(j), j == 0);
+            if (i == 1) commit(&bars[WFB_V_EMPTY + stage(j)]);
+            if (j + 1 < n) {
+              if (i == 0) ok = k_full(j + 1);
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(i, stage(j + 1));
+              commit(&bars[WFB_S_FULL + i]);
+              if (i == 1) {
+                commit(&bars[WFB_K_EMPTY + stage(j + 1)]);
+                if (j + 1 == n - 1) commit(&bars[WFB_Q_EMPTY]);
+              }
+            } else {
+              commit(&bars[WFB_O_DONE + i]);
+            }
+          }
         }
       }
+      ++it;
+      jj0 += n;
     }
     if (!ok) {      // wind down: let every MMA already issued finish before TMEM is released
       commit(&bars[WFB_DRAIN]);
       const long long t0 = clock64();
       while (!mbar_try_wait(&bars[WFB_DRAIN], 0) && clock64() - t0 < LVX_SPIN_LIMIT_CYCLES) {}
+    }
     }
   }
 
@@ -602,7 +751,12 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
   p.v_b = v.stride_b; p.v_h = v.stride_h; p.v_s = v.stride_s;
   p.status = status;
   const bool pair = window_pair(s, window_tiles(s, w, false), false);
-  dim3 grid(s.B * s.Hkv, pl.m_blocks, pair ? pl.nsplit / 2 : pl.nsplit);
+  p.slabs = s.B * s.Hkv;
+  p.splits = pair ? pl.nsplit / 2 : pl.nsplit;
+  const long items = long(p.slabs) * pl.m_blocks * p.splits;
+  if (items >= (1l << 30)) return fail(LVX_ERR_LIMIT, "window_fwd: %ld work items", items);
+  p.nitems = int(items);
+  const unsigned grid = unsigned(std::min<long>(items, num_sms()));      // persistent: one CTA per SM
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WF_SMEM);
