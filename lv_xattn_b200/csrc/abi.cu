@@ -658,15 +658,23 @@ static int check_qkv_views(const lvx_shape* s, const lvx_view* q, const lvx_view
   return LVX_OK;
 }
 
+static size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+static size_t window_fwd_bytes(const lvx_shape* s, const FwdPlan& p, bool few) {
+  const bool direct = !few && p.nsplit == 1 && s->dtype != LVX_FP32;
+  return direct ? 0 : p.o_part_bytes + p.ml_part_bytes;
+}
+static size_t window_bwd_bytes(const lvx_shape* s, const lvx_window* w) {
+  return round256(size_t(s->B) * s->Hq * s->Sq * 4) +
+         (s->dtype == LVX_FP32 ? 0 : (window_dq_floats(*s) + window_sink_floats(*s, *w)) * 4);
+}
+
 int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_bytes, size_t* bwd_bytes) {
   const int rc = check_window(s, w, "lvx_window_workspace");
   if (rc) return rc;
   bool few;
   const FwdPlan p = plan_window(*s, *w, &few);
-  const bool direct = !few && p.nsplit == 1 && s->dtype != LVX_FP32;
-  if (fwd_bytes) *fwd_bytes = direct ? 0 : p.o_part_bytes + p.ml_part_bytes;
-  const size_t delta = ((size_t(s->B) * s->Hq * s->Sq * 4 + 255) & ~size_t(255));
-  if (bwd_bytes) *bwd_bytes = delta + (s->dtype == LVX_FP32 ? 0 : (window_dq_floats(*s) + window_sink_floats(*s, *w)) * 4);
+  if (fwd_bytes) *fwd_bytes = window_fwd_bytes(s, p, few);
+  if (bwd_bytes) *bwd_bytes = window_bwd_bytes(s, w);
   return LVX_OK;
 }
 
@@ -691,14 +699,13 @@ int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* 
   if (!(sm_scale > 0.f)) return fail(LVX_ERR_SHAPE, "%s: sm_scale must be positive", who);
   LVX_REQUIRE_PTR(o, who);
   LVX_REQUIRE_PTR(lse, who);
-  size_t need = 0;
-  if ((rc = lvx_window_workspace(s, w, &need, nullptr))) return rc;
+  bool few;
+  const FwdPlan p = plan_window(*s, *w, &few);
+  const size_t need = window_fwd_bytes(s, p, few);
   if (need) LVX_REQUIRE_PTR(workspace, who);
   if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
   int* sp = status_ptr();
   if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
-  bool few;
-  const FwdPlan p = plan_window(*s, *w, &few);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (need == 0) return window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, nullptr, nullptr, o, lse, sp, st);
   float* o_part = static_cast<float*>(workspace);
@@ -725,8 +732,7 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
     LVX_REQUIRE_PTR(dk, who);
     LVX_REQUIRE_PTR(dv, who);
   }
-  size_t need = 0;
-  if ((rc = lvx_window_workspace(s, w, nullptr, &need))) return rc;
+  const size_t need = window_bwd_bytes(s, w);
   if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
   int* sp = status_ptr();
   if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
@@ -734,7 +740,7 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
   const bool direct = s->dtype == LVX_FP32;      // dQ is accumulated where it is wanted
   const size_t rows = size_t(s->B) * s->Hq * s->Sq;
   float* delta = static_cast<float*>(workspace);
-  float* dq_acc = direct ? static_cast<float*>(dq) : reinterpret_cast<float*>(static_cast<char*>(workspace) + ((rows * 4 + 255) & ~size_t(255)));
+  float* dq_acc = direct ? static_cast<float*>(dq) : reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(rows * 4));
   float* parts = direct ? nullptr : dq_acc + window_dq_floats(*s);
   if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
   const cudaError_t e = cudaMemsetAsync(dq_acc, 0, direct ? rows * 512 : window_dq_floats(*s) * 4, st);
@@ -757,7 +763,6 @@ struct SharedCall {
   bool packed;              // the packed order is another one than q's
   size_t rows;              // B * Hq * Sq
 };
-static size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 static int shared_call(SharedCall* c, const lvx_shape* s, int prefixes, int prefix_len, const char* who) {
   c->own_win = lvx_window{0, 0, -1};
   int rc = check_window(s, &c->own_win, who);
@@ -773,26 +778,34 @@ static int shared_call(SharedCall* c, const lvx_shape* s, int prefixes, int pref
   c->pre.Skv = prefix_len;
   c->pre_win = lvx_window{0, 0, prefix_len};      // every row stands behind all keys
   if ((rc = check_window(&c->pre, &c->pre_win, who))) return rc;
-  c->pre_plan = plan_window(c->pre, c->pre_win, &c->pre_few);
-  c->own_plan = plan_window(*s, c->own_win, &c->own_few);
   c->packed = s->B != prefixes && s->Hkv > 1;
   c->rows = size_t(s->B) * s->Hq * s->Sq;
   return LVX_OK;
+}
+
+// Forward: its plans, and the scratch.
+static size_t shared_fwd_plan(SharedCall* c, const lvx_shape* s) {
+  c->pre_plan = plan_window(c->pre, c->pre_win, &c->pre_few);
+  size_t n = c->pre_plan.o_part_bytes + c->pre_plan.ml_part_bytes + round256(c->rows * 128 * elt_size(s->dtype));
+  if (s->Skv > 0) {
+    c->own_plan = plan_window(*s, c->own_win, &c->own_few);
+    n += c->own_plan.o_part_bytes + c->own_plan.ml_part_bytes;
+  }
+  return n;
+}
+static size_t shared_bwd_bytes(const SharedCall& c, const lvx_shape* s) {
+  const bool f32 = s->dtype == LVX_FP32;
+  const size_t acc = f32 ? c.rows * 512 : window_dq_floats(c.pre) * 4;
+  const size_t acc_own = s->Skv == 0 ? 0 : f32 ? c.rows * 512 : window_dq_floats(*s) * 4;
+  return 3 * round256(c.rows * 4) + 2 * round256(c.rows * 128 * elt_size(s->dtype)) + round256(acc) + acc_own;
 }
 
 int lvx_shared_workspace(const lvx_shape* s, int prefixes, int prefix_len, size_t* fwd_bytes, size_t* bwd_bytes) {
   SharedCall c;
   const int rc = shared_call(&c, s, prefixes, prefix_len, "lvx_shared_workspace");
   if (rc) return rc;
-  const size_t es = elt_size(s->dtype), row_bytes = round256(c.rows * 128 * es), stat = round256(c.rows * 4);
-  const size_t own = s->Skv > 0 ? c.own_plan.o_part_bytes + c.own_plan.ml_part_bytes : 0;
-  if (fwd_bytes) *fwd_bytes = c.pre_plan.o_part_bytes + c.pre_plan.ml_part_bytes + own + row_bytes;
-  if (bwd_bytes) {
-    const bool f32 = s->dtype == LVX_FP32;
-    const size_t acc = f32 ? c.rows * 512 : window_dq_floats(c.pre) * 4;
-    const size_t acc_own = s->Skv == 0 ? 0 : f32 ? c.rows * 512 : window_dq_floats(*s) * 4;
-    *bwd_bytes = 3 * stat + 2 * row_bytes + round256(acc) + acc_own;
-  }
+  if (fwd_bytes) *fwd_bytes = shared_fwd_plan(&c, s);
+  if (bwd_bytes) *bwd_bytes = shared_bwd_bytes(c, s);
   return LVX_OK;
 }
 
@@ -810,8 +823,7 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
   LVX_REQUIRE_PTR(o, who);
   LVX_REQUIRE_PTR(lse, who);
   LVX_REQUIRE_PTR(workspace, who);
-  size_t need = 0;
-  if ((rc = lvx_shared_workspace(s, prefixes, prefix_len, &need, nullptr))) return rc;
+  const size_t need = shared_fwd_plan(&c, s);
   if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
   int* sp = status_ptr();
   if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
@@ -867,8 +879,7 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
     LVX_REQUIRE_PTR(dk, who);
     LVX_REQUIRE_PTR(dv, who);
   }
-  size_t need = 0;
-  if ((rc = lvx_shared_workspace(s, prefixes, prefix_len, nullptr, &need))) return rc;
+  const size_t need = shared_bwd_bytes(c, s);
   if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
   int* sp = status_ptr();
   if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);

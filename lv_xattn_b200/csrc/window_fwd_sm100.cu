@@ -25,6 +25,7 @@
 #include "window.cuh"
 #include <math.h>
 #include <algorithm>
+#include <limits>
 
 namespace lvx {
 
@@ -128,24 +129,27 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     KeyTiles kt;
     int j0, n;               // its share of the key tiles
   };
+  // block of tokens and chunk of heads of a tile (an integer division costs the roles' common start of an item dearly)
+  auto block_of = [&](int tile) { return p.qt.chunks == 1 ? tile : tile / p.qt.chunks; };
+  auto chunk_of = [&](int tile) { return p.qt.chunks == 1 ? 0 : tile % p.qt.chunks; };
   // the CTA's round-th item: forwards and backwards through the list in turn
   auto index_of = [&](int round) {
     return round * int(gridDim.x) + ((round & 1) ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x));
   };
   auto item_of = [&](int w) {
     Item it;
-    it.slab = w % p.slabs;
     const int rest = w / p.slabs;
-    it.split = rest / p.m_blocks;
-    it.mb = p.m_blocks - 1 - rest % p.m_blocks;
+    it.slab = w - rest * p.slabs;
+    it.split = p.splits == 1 ? 0 : rest / p.m_blocks;
+    it.mb = p.m_blocks - 1 - (rest - it.split * p.m_blocks);
     it.valid = p.skv;
     if (p.kv_valid_len) it.valid = min(it.valid, max(0, p.kv_valid_len[it.slab / p.hkv]));
     it.start = p.mask.start >= 0 ? p.mask.start : it.valid - p.sq;
     // token range of the two tiles (the second may not exist: its rows do not then, and its tile is loaded as zeros)
-    const int tok0 = (2 * it.mb / p.qt.chunks) * p.qt.tokens;
-    const int tok1 = min(p.sq, (min(2 * it.mb + 1, p.qt.count - 1) / p.qt.chunks + 1) * p.qt.tokens) - 1;
+    const int tok0 = block_of(2 * it.mb) * p.qt.tokens;
+    const int tok1 = min(p.sq, (block_of(min(2 * it.mb + 1, p.qt.count - 1)) + 1) * p.qt.tokens) - 1;
     it.kt = key_tiles(p.mask, it.valid, it.start + tok0, it.start + tok1, 7);
-    const int per_split = (it.kt.n + p.splits - 1) / p.splits;
+    const int per_split = p.splits == 1 ? it.kt.n : (it.kt.n + p.splits - 1) / p.splits;
     it.j0 = min(it.kt.n, it.split * per_split);
     it.n = min(it.kt.n, it.j0 + per_split) - it.j0;
     return it;
@@ -195,6 +199,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
     const int wg = warp >> 2;
     const int r = (warp & 3) * 32 + lane;            // row of the tile, TMEM lane
+    const int r_tok = r / heads, r_head = r - r_tok * heads;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem_base + wg * 128 + lane_sel;
     const uint32_t tO = tmem_base + 256 + wg * 128 + lane_sel;
@@ -207,7 +212,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
     const Item I = item_of(w);
     const int tile = PAIR ? 0 : 2 * I.mb + wg;
-    const int tok = (tile / p.qt.chunks) * p.qt.tokens + r / heads, head = (tile % p.qt.chunks) * heads + r % heads;
+    const int tok = block_of(tile) * p.qt.tokens + r_tok, head = chunk_of(tile) * heads + r_head;
     const bool exists = tile < p.qt.count && r < tile_rows && tok < p.sq && head < p.g;
     // this row's keys: [0, sink_end) and [lo, hi]. A row that does not exist sees everything against a reference of 0 (its
     // scores are zeros), so that it never holds up its warp.
@@ -474,8 +479,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
           const int tile = 2 * I.mb + t;
           for (int h = 0; h < 2; ++h)
-            tma_load_5d(smem + t * WF_TILE + h * WF_HALF, &tmQ, &bars[WFB_Q_FULL], h * 64, (tile % p.qt.chunks) * heads,
-                        (tile / p.qt.chunks) * p.qt.tokens, kvh, batch);
+            tma_load_5d(smem + t * WF_TILE + h * WF_HALF, &tmQ, &bars[WFB_Q_FULL], h * 64, chunk_of(tile) * heads,
+                        block_of(tile) * p.qt.tokens, kvh, batch);
         }
         ++it;
         for (int j = 0; j < I.n; ++j) {
@@ -668,31 +673,33 @@ static long window_tiles(const lvx_shape& s, const lvx_window& w, bool few) {
 }
 
 FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few) {
-  FwdPlan p = plan_fwd(s);          // (fp32: as it is)
+  *few = false;
+  if (s.dtype == LVX_FP32) return plan_fwd(s);
   const int g = s.Hq / s.Hkv;
-  *few = s.dtype != LVX_FP32 && p.rows <= kFewRows;
-  bool pair = false;
-  if (s.dtype != LVX_FP32) {
-    const QTiles qt = make_q_tiles(g, s.Sq);
-    p.m_blocks = *few ? 1 : (qt.count + 1) / 2;
-    long tiles = window_tiles(s, w, *few);
-    const long base = long(p.m_blocks) * s.B * s.Hkv;
-    pair = window_pair(s, tiles, *few);
-    if (pair) tiles = (tiles + 1) / 2;      // what a CTA walks takes half as long
-    const long most = std::min<long>(tiles > 0 ? tiles : 1, *few ? 148 : 64);
-    double best_cost = 1e300;
-    for (int ns = 1; ns <= most; ++ns) {
-      const long waves = (base * ns + 147) / 148, per = (tiles + ns - 1) / ns;
-      // 3 tiles' worth of fixed cost per CTA, and 4 for a second kernel where one would do without
-      const double cost = double(waves) * (per + 3.0) + (ns > 1 && !*few ? 4.0 : 0.0);
-      if (cost < best_cost * 0.995) {
-        best_cost = cost;
-        p.nsplit = ns;
-      }
+  FwdPlan p;
+  p.rows = g * s.Sq;
+  p.kv_tiles = (s.Skv + 127) / 128;
+  *few = p.rows <= kFewRows;
+  p.m_blocks = *few ? 1 : (make_q_tiles(g, s.Sq).count + 1) / 2;
+  long tiles = window_tiles(s, w, *few);
+  const long base = long(p.m_blocks) * s.B * s.Hkv;
+  const bool pair = window_pair(s, tiles, *few);
+  if (pair) tiles = (tiles + 1) / 2;      // what a CTA walks takes half as long
+  const long most = std::min<long>(tiles > 0 ? tiles : 1, *few ? 148 : 64);
+  // Splits that fill whole rounds of 148 SMs, eight rounds at most (the fixed cost then outweighs what a partly filled last round
+  // wastes): 3 tiles' worth of fixed cost per item, and 4 for a second kernel where one would do without.
+  long best_cost = std::numeric_limits<long>::max();
+  p.nsplit = 1;
+  for (long ns = 1; ns <= most && (ns == 1 || base * ns <= 148 * 8); ++ns) {
+    const long rounds = (base * ns + 147) / 148, per = (tiles + ns - 1) / ns;
+    const long cost = rounds * (per + 3) + (ns > 1 && !*few ? 4 : 0);
+    if (cost < best_cost) {
+      best_cost = cost;
+      p.nsplit = int(ns);
     }
-    p.tiles_per_split = 0;          // the kernels share out what each CTA turns out to see
-    if (pair) p.nsplit *= 2;        // partial results; the grid has half as many splits
   }
+  p.tiles_per_split = 0;          // the kernels share out what each CTA turns out to see
+  if (pair) p.nsplit *= 2;        // partial results; there are half as many items
   p.o_part_bytes = (size_t(s.B) * s.Hkv * p.nsplit * p.rows * 512 + 255) & ~size_t(255);
   p.ml_part_bytes = (size_t(s.B) * s.Hkv * p.nsplit * p.rows * 8 + 255) & ~size_t(255);
   return p;
