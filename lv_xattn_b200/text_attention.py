@@ -17,31 +17,41 @@ _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MOST = 1 << 28          # lengths and positions are below this
 
 
-def _check_attention(who, q, kv):
-    """q against every (name, k, v) of `kv`."""
-    if q.dim() != 4 or q.shape[-1] != 128:
-        raise ValueError(f"{who}: q must be [batch, heads, tokens, 128], got {tuple(q.shape)}")
-    if q.dtype not in _TYPES:
-        raise ValueError(f"{who}: dtype {q.dtype} unsupported; expected bfloat16, float16 or float32")
-    if 0 in q.shape:
-        raise ValueError(f"{who}: q is empty, {tuple(q.shape)}")
-    for name, k, v in kv:
-        if k.dim() != 4 or k.shape != v.shape or k.shape[-1] != 128:
-            raise ValueError(f"{who}: {name} must be two tensors [batch, KV heads, keys, 128] of one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
-            raise ValueError(f"{who}: q and {name} must share one dtype")
-        if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
-            raise ValueError(f"{who}: {q.shape[1]} query heads are not a multiple of the {k.shape[1]} heads of {name}")
-        if k.shape[2] >= _MOST:
-            raise ValueError(f"{who}: lengths must be below {_MOST}")
-    if q.shape[2] >= _MOST:
+def _check_q(who, q):
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 4 or shape[3] != 128:
+        raise ValueError(f"{who}: q must be [batch, heads, tokens, 128], got {tuple(shape)}")
+    if dtype not in _TYPES:
+        raise ValueError(f"{who}: dtype {dtype} unsupported; expected bfloat16, float16 or float32")
+    if 0 in shape:
+        raise ValueError(f"{who}: q is empty, {tuple(shape)}")
+    if shape[2] >= _MOST:
         raise ValueError(f"{who}: lengths must be below {_MOST}")
+    return shape, dtype
+
+
+def _check_kv(who, name, k, v, q_heads, dtype):
+    """The shape of keys and values, which `name` calls them."""
+    shape = k.shape
+    if len(shape) != 4 or shape[3] != 128 or shape != v.shape:
+        raise ValueError(f"{who}: {name} must be two tensors [batch, KV heads, keys, 128] of one shape, got {tuple(shape)} and {tuple(v.shape)}")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"{who}: q and {name} must share one dtype")
+    if shape[1] == 0 or q_heads % shape[1]:
+        raise ValueError(f"{who}: {q_heads} query heads are not a multiple of the {shape[1]} heads of {name}")
+    if shape[2] >= _MOST:
+        raise ValueError(f"{who}: lengths must be below {_MOST}")
+    return shape
+
+
+def _check_devices(who, q, *kv):
     device = q.device
-    for name, k, v in kv:
-        if not (q.is_cuda and k.is_cuda and v.is_cuda):
-            raise _lib.LvxError("lv_xattn_b200 runs on CUDA tensors only; there is no CPU path")
-        if k.device != device or v.device != device:
+    for t in kv:
+        if t.device != device:
             raise ValueError(f"{who}: all tensors must be on one device")
+    if not q.is_cuda:
+        raise _lib.LvxError("lv_xattn_b200 runs on CUDA tensors only; there is no CPU path")
+    return device
 
 
 def _scale(who, sm_scale):
@@ -95,12 +105,14 @@ def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=
         raise ValueError(f"{who}: sinks must not be negative, got {sinks}")
     if query_start is not None and not 0 <= query_start < _MOST:
         raise ValueError(f"{who}: query_start must lie in 0..{_MOST - 1}, got {query_start}")
-    if k.dim() == q.dim() == 4 and k.shape[0] != q.shape[0]:
-        raise ValueError(f"{who}: q has {q.shape[0]} batch entries, k and v {k.shape[0]}")
-    _check_attention(who, q, [("k and v", k, v)])
+    q_shape, dtype = _check_q(who, q)
+    k_shape = _check_kv(who, "k and v", k, v, q_shape[1], dtype)
+    if k_shape[0] != q_shape[0]:
+        raise ValueError(f"{who}: q has {q_shape[0]} batch entries, k and v {k_shape[0]}")
+    device = _check_devices(who, q, k, v)
     watch_status(q)
     with on_device(q):
-        lengths = ops.device_lengths(kv_valid_len, q.shape[0], k.shape[2], q.device)
+        lengths = ops.device_lengths(kv_valid_len, q_shape[0], k_shape[2], device)
         args = (q, k, v, sm_scale, 0 if window is None or window >= _MOST else int(window), min(int(sinks), _MOST),
                 -1 if query_start is None else int(query_start), lengths)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -150,20 +162,26 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k=None, v=None, sm_scale=None
         raise ValueError(f"{who}: k and v go together")
     if k is None and kv_valid_len is not None:
         raise ValueError(f"{who}: valid lengths of own keys that are not there")
-    if q.dim() == k_prefix.dim() == 4:
-        if k_prefix.shape[0] == 0 or q.shape[0] % k_prefix.shape[0]:
-            raise ValueError(f"{who}: {q.shape[0]} requests are not a multiple of {k_prefix.shape[0]} prefixes")
-        if k_prefix.shape[2] == 0:
-            raise ValueError(f"{who}: the prefix is empty")
-        if k is not None and k.dim() == 4 and (k.shape[0] != q.shape[0] or k.shape[1] != k_prefix.shape[1]):
-            raise ValueError(f"{who}: own keys {tuple(k.shape)} for {q.shape[0]} requests and {k_prefix.shape[1]} KV heads")
-    _check_attention(who, q, [("the prefix", k_prefix, v_prefix)] + ([] if k is None else [("k and v", k, v)]))
+    q_shape, dtype = _check_q(who, q)
+    B, P, _, N = q_shape[0], *_check_kv(who, "the prefix", k_prefix, v_prefix, q_shape[1], dtype)[:3]
+    if P == 0 or B % P:
+        raise ValueError(f"{who}: {B} requests are not a multiple of {P} prefixes")
+    if N == 0:
+        raise ValueError(f"{who}: the prefix is empty")
+    if k is None:
+        own = 0
+        device = _check_devices(who, q, k_prefix, v_prefix)
+    else:
+        b, heads, own, _ = _check_kv(who, "k and v", k, v, q_shape[1], dtype)
+        if b != B or heads != k_prefix.shape[1]:
+            raise ValueError(f"{who}: own keys {tuple(k.shape)} for {B} requests and {k_prefix.shape[1]} KV heads")
+        device = _check_devices(who, q, k_prefix, v_prefix, k, v)
     watch_status(q)
     with on_device(q):
-        prefix_lengths = ops.device_lengths(prefix_valid_len, k_prefix.shape[0], k_prefix.shape[2], q.device)
-        lengths = ops.device_lengths(kv_valid_len, q.shape[0], 0 if k is None else k.shape[2], q.device)
-        args = (q, k_prefix, v_prefix, k, v, sm_scale, prefix_lengths, lengths)
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+        args = (q, k_prefix, v_prefix, k, v, sm_scale, ops.device_lengths(prefix_valid_len, P, N, device),
+                ops.device_lengths(kv_valid_len, B, own, device))
+        if torch.is_grad_enabled() and (q.requires_grad or k_prefix.requires_grad or v_prefix.requires_grad
+                                        or (k is not None and (k.requires_grad or v.requires_grad))):
             o, lse = SharedPrefixAttentionFunc.apply(*args)
         else:
             o, lse = ops.shared_forward(*args)
