@@ -12,14 +12,19 @@
 //   * an item knows its own number of query tiles, possibly none;
 //   * every query sees the sinks, so their key tiles would be walked long after all others are done (4,096 tokens with a
 //     window of 1,024: 128 query tiles against 36). They are shared out over several items, each with a run of the queries
-//     and fp32 dK and dV of its own, which the last kernel adds up in a fixed order (backward of that case 400 -> 2xx us);
+//     and fp32 dK and dV of its own, which the last kernel adds up in a fixed order (backward kernel of that case 400 -> 257 us);
 //   * dQ is accumulated in the order of the tiles ([slab][chunk][token][head of the chunk][128]: a tile's rows are one
 //     run of memory), and brought into [B, Hq, Sq, 128] by the kernel that rounds it;
 //   * a thread's key is seen by a run of a tile's columns, so a masked tile costs two comparisons a tile and a select a
 //     value; tiles seen whole cost none;
 //   * rows of K and V behind the last valid key are cleared in shared memory: they may hold anything, and zero times
 //     that would reach dQ. (A key inside must be finite: in a backward there is no other answer than NaN.)
-// P and dS are rounded to 16 bits for their products, as in the backward block.
+//   * P is rounded to 16 bits for its product with dO, but dS is made from the fp32 P (dQ and dK then err by 2.4e-3 in bf16,
+//     1.7e-3 of which is their own rounding; with P taken back from its 16 bits 3.0e-3). That P has to outlive the wait for
+//     dP^T, 16 registers more in the compute warps. They come from the producer's and the issuer's warpgroup: 896 threads
+//     are launched with 72 registers each, 512 x 80 + 256 x 72 + 128 x 40 is the same number of them. The issuer makes its
+//     descriptors anew for every product, or it would not fit 40 (spilled, that cost 11 %; the drain warps with 64 instead of
+//     72 cost 60 %). 258 -> 252 us for 4,096 tokens with a window of 1,024.
 #include "lvx_internal.h"
 #include "sm100_prims.cuh"
 #include "window.cuh"
@@ -39,7 +44,7 @@ constexpr int WB_OFF_BAR = WB_OFF_STAT + 2 * 256 * 4;
 constexpr int WB_SMEM = WB_OFF_BAR + 256;
 constexpr int WB_COMPUTE = 16, WB_DRAIN_WARPS = 8;
 constexpr int WB_WARP_TMA = WB_COMPUTE + WB_DRAIN_WARPS, WB_WARP_MMA = WB_WARP_TMA + 1;
-constexpr int WB_THREADS = (WB_WARP_MMA + 1) * 32;
+constexpr int WB_THREADS = (WB_WARP_MMA + 3) * 32;      // two idle warps make the last warpgroup whole (setmaxnreg)
 static_assert(WB_SMEM <= 232448, "shared memory budget");
 constexpr uint32_t WB_DK = 0, WB_DV = 128, WB_X = 256, WB_Y = 384;
 
@@ -165,16 +170,17 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   // Every role walks the same items in the same order and keeps the same counters: `it` = items with tiles done, `jj0` =
   // tiles done before the current item, `cleaned` = items whose K and V were cleared in part.
-  if (!poisoned) {
+  {
     if (warp < WB_COMPUTE) {
       // =========================== compute warps ===========================
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 80;" ::: "memory");
       const int quarter = warp & 3;                         // TMEM lane quarter
       const int cg = warp >> 2;                             // 32-column group of the query tile
       const int r = quarter * 32 + lane;                    // key inside the tile
       const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
       const uint32_t tX = tmem_base + WB_X + lane_sel, tY = tmem_base + WB_Y + lane_sel;
       const float c = p.scale_log2;
-      bool alive = true;
+      bool alive = !poisoned;
       int it = 0, jj0 = 0;
       for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
         const Item I = item_of(w);
@@ -257,23 +263,24 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const bool masked = __any_sync(0xffffffffu, seen != 0xffffffffu);
           const float4* sl = reinterpret_cast<const float4*>(s_stat + (jj & 1) * 256 + cg * 32);
           const float4* sd = reinterpret_cast<const float4*>(s_stat + (jj & 1) * 256 + 128 + cg * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {      // s becomes P, which stays in fp32 for dS
+            const float4 l2 = sl[i];
+            s[4 * i] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i]), c, -l2.x)));
+            s[4 * i + 1] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 1]), c, -l2.y)));
+            s[4 * i + 2] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 2]), c, -l2.z)));
+            s[4 * i + 3] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 3]), c, -l2.w)));
+          }
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(seen & (1u << i))) s[i] = 0u;
+          }
           uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 l2 = sl[i];
-            float p0 = ex2f(fmaf(__uint_as_float(s[4 * i]), c, -l2.x));
-            float p1 = ex2f(fmaf(__uint_as_float(s[4 * i + 1]), c, -l2.y));
-            float p2 = ex2f(fmaf(__uint_as_float(s[4 * i + 2]), c, -l2.z));
-            float p3 = ex2f(fmaf(__uint_as_float(s[4 * i + 3]), c, -l2.w));
-            if (masked) {
-              if (!(seen & (1u << (4 * i)))) p0 = 0.f;
-              if (!(seen & (2u << (4 * i)))) p1 = 0.f;
-              if (!(seen & (4u << (4 * i)))) p2 = 0.f;
-              if (!(seen & (8u << (4 * i)))) p3 = 0.f;
-            }
-            pk[2 * i] = IS_BF16 ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
-            pk[2 * i + 1] = IS_BF16 ? pack_bf16x2(p2, p3) : pack_f16x2(p2, p3);
-          }
+          for (int i = 0; i < 16; ++i)
+            pk[i] = IS_BF16 ? pack_bf16x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]))
+                            : pack_f16x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
           // P^T overwrites S^T in X: wait until every warp has taken its S^T columns out.
           if (!mbar_wait(&bars[WBB_X_LOADED], jj & 1, abort_flag, p.status, WB_CODE(0, WBB_X_LOADED))) {
             alive = false;
@@ -298,13 +305,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              // P as the dV product uses it: only its 16 packed registers live across the wait for dP^T
               const float4 dl = sd[h * 4 + i];
-              const float2 pa = unpack16x2<IS_BF16>(pk[h * 8 + 2 * i]), pb = unpack16x2<IS_BF16>(pk[h * 8 + 2 * i + 1]);
-              const float d0 = pa.x * (__uint_as_float(dp[4 * i]) - dl.x);
-              const float d1 = pa.y * (__uint_as_float(dp[4 * i + 1]) - dl.y);
-              const float d2 = pb.x * (__uint_as_float(dp[4 * i + 2]) - dl.z);
-              const float d3 = pb.y * (__uint_as_float(dp[4 * i + 3]) - dl.w);
+              const float d0 = __uint_as_float(s[h * 16 + 4 * i]) * (__uint_as_float(dp[4 * i]) - dl.x);
+              const float d1 = __uint_as_float(s[h * 16 + 4 * i + 1]) * (__uint_as_float(dp[4 * i + 1]) - dl.y);
+              const float d2 = __uint_as_float(s[h * 16 + 4 * i + 2]) * (__uint_as_float(dp[4 * i + 2]) - dl.z);
+              const float d3 = __uint_as_float(s[h * 16 + 4 * i + 3]) * (__uint_as_float(dp[4 * i + 3]) - dl.w);
               dsk[h * 8 + 2 * i] = IS_BF16 ? pack_bf16x2(d0, d1) : pack_f16x2(d0, d1);
               dsk[h * 8 + 2 * i + 1] = IS_BF16 ? pack_bf16x2(d2, d3) : pack_f16x2(d2, d3);
             }
@@ -372,7 +377,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int ch = (warp - WB_COMPUTE) >> 2;              // which 64 query columns
       const int d = quarter * 32 + lane;                    // head-dim index = TMEM lane of dQ^T
       const uint32_t tY = tmem_base + WB_Y + (static_cast<uint32_t>(quarter * 32) << 16);
-      bool alive = true;
+      bool alive = !poisoned;
       int jj0 = 0;
       for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
         const Item I = item_of(w);
@@ -399,9 +404,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         jj0 += I.ntot;
       }
-    } else if (warp == WB_WARP_TMA) {
+    } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;" ::: "memory");
+    if (warp == WB_WARP_TMA) {
       // =========================== TMA producer ===========================
-      if (lane == 0) {
+      if (lane == 0 && !poisoned) {
         tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmDO);
         tma_prefetch_desc(&tmK);
@@ -454,9 +461,9 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int jj = max(0, issued - 2); jj < issued; ++jj) drain(&bars[WBB_Q_FULL + (jj & 1)], (jj >> 1) & 1);
         }
       }
-    } else {
+    } else if (warp == WB_WARP_MMA) {
       // =========================== MMA issuer ===========================
-      if (lane == 0) {
+      if (lane == 0 && !poisoned) {
         constexpr uint32_t FMT = IS_BF16 ? UMMA_BF16 : UMMA_F16;
         constexpr uint32_t IDESC_ST = umma_idesc(FMT, UMMA_K_MAJOR, UMMA_K_MAJOR, 128, 128);
         constexpr uint32_t IDESC_ACC = umma_idesc(FMT, UMMA_K_MAJOR, UMMA_MN_MAJOR, 128, 128);
@@ -465,9 +472,16 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t sK = smem_u32(smem + WB_OFF_K), sV = smem_u32(smem + WB_OFF_V);
         const uint32_t sQ0 = smem_u32(smem + WB_OFF_Q), sDS = smem_u32(smem + WB_OFF_DS);
         auto q_at = [&](int jj) { return sQ0 + (jj & 1) * 2 * WB_TILE; };
+        // The descriptors are made anew for every product (one addition an instruction): kept over the loop, as the compiler
+        // would have them, they do not fit this warp's registers.
+        auto desc = [](uint32_t smem_addr, uint32_t lead) {
+          uint32_t lo = umma_desc_lo(smem_addr, lead);
+          asm volatile("" : "+r"(lo));
+          return lo;
+        };
         // D[128 kv, 128 q] = A[128 kv, 128 d] * B[128 q, 128 d]^T, both K-major
         auto issue_st = [&](uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem) {
-          const uint32_t a_lo = umma_desc_lo(a_smem, 16), b_lo = umma_desc_lo(b_smem, 16);
+          const uint32_t a_lo = desc(a_smem, 16), b_lo = desc(b_smem, 16);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) {
             const uint32_t off = ((kk >> 2) * WB_HALF + (kk & 3) * 32) >> 4;
@@ -476,7 +490,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         };
         // dV[128 kv, 128 d] += P^T (TMEM) * dO (MN-major: rows are q)
         auto issue_dv = [&](uint32_t b_smem, bool first) {
-          const uint32_t b_lo = umma_desc_lo(b_smem, WB_HALF);
+          const uint32_t b_lo = desc(b_smem, WB_HALF);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             umma_ts_f16(tmem_base + WB_DV, tmem_base + WB_X + kk * 8, umma_desc_join(b_lo + ((kk * 2048) >> 4), HI), IDESC_ACC,
@@ -484,15 +498,15 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         };
         // dK[128 kv, 128 d] += dS^T (shared memory, K-major) * Q (MN-major)
         auto issue_dk = [&](uint32_t b_smem, bool first) {
-          const uint32_t a_lo = umma_desc_lo(sDS, 16), b_lo = umma_desc_lo(b_smem, WB_HALF);
+          const uint32_t a_lo = desc(sDS, 16), b_lo = desc(b_smem, WB_HALF);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             umma_ss_f16(tmem_base + WB_DK, umma_desc_join(a_lo + (((kk >> 2) * WB_HALF + (kk & 3) * 32) >> 4), HI),
                         umma_desc_join(b_lo + ((kk * 2048) >> 4), HI), IDESC_ACC, (!first) || kk > 0);
         };
         // dQ^T[128 d, 128 q] = K^T * dS^T (both MN-major: rows are kv)
-        const uint32_t kT_lo = umma_desc_lo(sK, WB_HALF), ds_lo = umma_desc_lo(sDS, WB_HALF);
         auto issue_dq = [&]() {
+          const uint32_t kT_lo = desc(sK, WB_HALF), ds_lo = desc(sDS, WB_HALF);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             umma_ss_f16(tmem_base + WB_Y, umma_desc_join(kT_lo + ((kk * 2048) >> 4), HI),
@@ -557,6 +571,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           while (!mbar_try_wait(&bars[WBB_DRAIN], 0) && clock64() - t0 < LVX_SPIN_LIMIT_CYCLES) {}
         }
       }
+    }
     }
   }
 
