@@ -770,7 +770,8 @@ static int shared_call(SharedCall* c, const lvx_shape* s, int prefixes, int pref
   if (prefixes < 1 || s->B % prefixes) return fail(LVX_ERR_SHAPE, "%s: %d requests are not a multiple of %d prefixes", who, s->B, prefixes);
   if (prefix_len < 1 || prefix_len >= kWindowMaxLen) return fail(LVX_ERR_SHAPE, "%s: a prefix of %d keys", who, prefix_len);
   const int64_t rows = int64_t(s->B / prefixes) * (s->Hq / s->Hkv) * s->Sq;      // of a prefix' KV head
-  if (rows * s->Hkv > (int64_t(1) << 30)) return fail(LVX_ERR_SHAPE, "%s: dimension too large", who);
+  // all rows are counted in 32 bits, with room for a tile's last ones
+  if (rows * s->Hkv * prefixes > (int64_t(1) << 30)) return fail(LVX_ERR_SHAPE, "%s: dimension too large", who);
   c->pre = *s;
   c->pre.B = prefixes;
   c->pre.Hq = int32_t(rows * s->Hkv);
@@ -918,7 +919,7 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
              : launch_window_bwd(*s, c.own_win, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, acc_own, nullptr, dk, dv, sp, st);
   if (rc) return rc;
   const QTiles pt = make_q_tiles(c.pre.Hq / c.pre.Hkv, 1);
-  const long pre_slab_rows = f32 ? c.pre.Hq / c.pre.Hkv : long(pt.chunks) * pt.heads;
+  const int pre_slab_rows = f32 ? c.pre.Hq / c.pre.Hkv : pt.chunks * pt.heads;
   return launch_shared_dq(*s, prefixes, acc, pre_slab_rows, acc_own, dq, st);
 }
 

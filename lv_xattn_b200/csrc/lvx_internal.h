@@ -90,7 +90,7 @@ int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const 
                      void* q_out, void* do_out, float* lse_out, float* delta_out, cudaStream_t st);
 int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
                           const float* ml_own, int ns_own, void* o, float* lse, cudaStream_t st);
-int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, long pre_slab_rows, const float* acc_own, void* dq,
+int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int pre_slab_rows, const float* acc_own, void* dq,
                      cudaStream_t st);
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,

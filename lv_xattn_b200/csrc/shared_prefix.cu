@@ -17,50 +17,60 @@
 
 namespace lvx {
 
-// A row of [B, Hq, Sq] in the packed order [P, Hkv, per, g, Sq], per = B / P.
+// A row of [B, Hq, Sq] in the packed order [P, Hkv, per, g, Sq], per = B / P. Rows are counted in 32 bits (checked on the
+// host): 64-bit divisions are most of what these kernels would execute.
 struct PackOrder {
   int hkv, g, sq, per;
-  __device__ __forceinline__ void split(long row, long& slab, int& in_slab) const {      // (KV head of a request, row in it)
+  __device__ __forceinline__ void split(int row, int& slab, int& in_slab) const {      // (KV head of a request, row in it)
     const int rows = g * sq;
     slab = row / rows;
-    in_slab = int(row - slab * rows);
+    in_slab = row - slab * rows;
   }
   // packed row: of slab p * hkv + kvh
-  __device__ __forceinline__ void packed(long slab, int in_slab, long& pslab, int& prow) const {
-    const long b = slab / hkv;
-    const int kvh = int(slab - b * hkv);
-    const long p = b / per;
+  __device__ __forceinline__ void packed(int slab, int in_slab, int& pslab, int& prow) const {
+    const int b = slab / hkv, kvh = slab - b * hkv, p = b / per;
     pslab = p * hkv + kvh;
-    prow = int(b - p * per) * g * sq + in_slab;
+    prow = (b - p * per) * g * sq + in_slab;
   }
-  __device__ __forceinline__ long packed_rows() const { return long(per) * g * sq; }
+  __device__ __forceinline__ int packed_rows() const { return per * g * sq; }
 };
 static PackOrder pack_order(const lvx_shape& s, int prefixes) { return PackOrder{s.Hkv, s.Hq / s.Hkv, s.Sq, s.B / prefixes}; }
 
-// ROW16: 16-byte pieces of a row (16: 16-bit types, 32: fp32). One piece a thread.
+// ROW16: 16-byte pieces of a row (16: 16-bit types, 32: fp32), one a thread; a thread takes that piece of four rows, which are
+// in flight together (42,624 rows of bf16: 10 -> 6 us against one row a thread and 64-bit arithmetic).
 template <int ROW16>
 __global__ void __launch_bounds__(256)
 pack_rows_kernel(const char* __restrict__ q, long long q_b, long long q_h, long long q_s, const uint4* __restrict__ d_o,
                  const float* __restrict__ lse, const float* __restrict__ delta, uint4* __restrict__ q_out, uint4* __restrict__ do_out,
-                 float* __restrict__ lse_out, float* __restrict__ delta_out, PackOrder order, long rows, const int* status) {
+                 float* __restrict__ lse_out, float* __restrict__ delta_out, PackOrder order, int rows, const int* status) {
   if (poisoned(status)) return;
-  const long at = long(blockIdx.x) * 256 + threadIdx.x;
-  const long row = at / ROW16;
-  const int piece = int(at % ROW16);
-  if (row >= rows) return;
-  long slab, pslab;
-  int in_slab, prow;
-  order.split(row, slab, in_slab);
-  order.packed(slab, in_slab, pslab, prow);
-  const long to = pslab * order.packed_rows() + prow;
-  const long bh = row / order.sq, b = slab / order.hkv;
-  const int h = int(bh - b * order.hkv * order.g), tok = int(row - bh * order.sq);
-  q_out[to * ROW16 + piece] = *reinterpret_cast<const uint4*>(q + b * q_b + h * q_h + tok * q_s + piece * 16);
-  if (d_o != nullptr) {
-    do_out[to * ROW16 + piece] = d_o[at];
-    if (piece == 0) {
-      lse_out[to] = lse[row];
-      delta_out[to] = delta[row];
+  constexpr int U = 4, PER = 256 / ROW16;      // rows of a thread, rows of a block at a time
+  const int piece = threadIdx.x % ROW16, row0 = blockIdx.x * PER * U + threadIdx.x / ROW16;
+  uint4 v[U], w[U];
+  int to[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int row = min(row0 + u * PER, rows - 1);
+    int slab, in_slab, pslab, prow;
+    order.split(row, slab, in_slab);
+    order.packed(slab, in_slab, pslab, prow);
+    to[u] = pslab * order.packed_rows() + prow;
+    const int b = slab / order.hkv, head = in_slab / order.sq, tok = in_slab - head * order.sq;
+    const int h = (slab - b * order.hkv) * order.g + head;
+    v[u] = *reinterpret_cast<const uint4*>(q + b * q_b + h * q_h + tok * q_s + piece * 16);
+    if (d_o != nullptr) w[u] = d_o[size_t(row) * ROW16 + piece];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int row = row0 + u * PER;
+    if (row >= rows) return;
+    q_out[size_t(to[u]) * ROW16 + piece] = v[u];
+    if (d_o != nullptr) {
+      do_out[size_t(to[u]) * ROW16 + piece] = w[u];
+      if (piece == 0) {
+        lse_out[to[u]] = lse[row];
+        delta_out[to[u]] = delta[row];
+      }
     }
   }
 }
@@ -69,23 +79,23 @@ template <int OUT, int WPR>
 __global__ void __launch_bounds__(256)
 shared_combine_kernel(const float* __restrict__ o_pre, const float* __restrict__ ml_pre, int ns_pre, const float* __restrict__ o_own,
                       const float* __restrict__ ml_own, int ns_own, PackOrder order, void* __restrict__ o_out,
-                      float* __restrict__ lse_out, long rows, const int* status) {
+                      float* __restrict__ lse_out, int rows, const int* status) {
   const int bad = status ? *reinterpret_cast<const volatile int*>(status) : 0;
   const int lane = threadIdx.x & 31, part = (threadIdx.x >> 5) % WPR;
-  const long row = ((long(blockIdx.x) * blockDim.x + threadIdx.x) >> 5) / WPR;
+  const int row = (blockIdx.x * 8 + (threadIdx.x >> 5)) / WPR;
   if (row >= rows) return;                 // WPR > 1: a block is one row, so its warps leave together
-  long slab, pslab;
-  int in_slab, prow;
+  int slab, in_slab, pslab, prow;
   order.split(row, slab, in_slab);
   order.packed(slab, in_slab, pslab, prow);
   RowAcc a;
   a.m = -INFINITY;
   a.l = 0.f;
   a.v = make_float4(0.f, 0.f, 0.f, 0.f);
+  // four partials at a time in flight (eight: 53 -> 73 us for 42,624 rows of seven and one, with half the warps an SM)
   const int groups = (ns_pre + 3) >> 2, own_groups = (ns_own + 3) >> 2;
   for (int i = part; i < groups + own_groups; i += WPR) {
-    if (i < groups) row_four(a, o_pre, ml_pre, size_t(pslab), ns_pre, int(order.packed_rows()), prow, i * 4, lane);
-    else row_four(a, o_own, ml_own, size_t(slab), ns_own, order.g * order.sq, in_slab, (i - groups) * 4, lane);
+    if (i < groups) row_four(a, o_pre, ml_pre, pslab, ns_pre, order.packed_rows(), prow, i * 4, lane);
+    else row_four(a, o_own, ml_own, slab, ns_own, order.g * order.sq, in_slab, (i - groups) * 4, lane);
   }
   if constexpr (WPR > 1) {
     __shared__ float4 s_v[WPR][32];
@@ -116,19 +126,18 @@ shared_combine_kernel(const float* __restrict__ o_pre, const float* __restrict__
 // one in the order of window_bwd_sm100.cu's tiles (heads of a tile, chunks).
 template <int OUT>
 __global__ void __launch_bounds__(256)
-shared_dq_kernel(const float* __restrict__ acc_pre, long pre_slab_rows, const float* __restrict__ acc_own, int heads, int chunks,
-                 PackOrder order, void* __restrict__ dq, long rows, const int* status) {
+shared_dq_kernel(const float* __restrict__ acc_pre, int pre_slab_rows, const float* __restrict__ acc_own, int heads, int chunks,
+                 PackOrder order, void* __restrict__ dq, int rows, const int* status) {
   if (poisoned(status)) {
     if ((threadIdx.x & 31) == 0) publish_status(status);
     return;
   }
   const int lane = threadIdx.x & 31;
-  for (long row = (long(blockIdx.x) * 256 + threadIdx.x) >> 5; row < rows; row += long(gridDim.x) * 8) {
-    long slab, pslab;
-    int in_slab, prow;
+  for (int row = blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8) {
+    int slab, in_slab, pslab, prow;
     order.split(row, slab, in_slab);
     order.packed(slab, in_slab, pslab, prow);
-    float4 v = reinterpret_cast<const float4*>(acc_pre)[(pslab * pre_slab_rows + prow) * 32 + lane];
+    float4 v = reinterpret_cast<const float4*>(acc_pre)[(size_t(pslab) * pre_slab_rows + prow) * 32 + lane];
     if (acc_own != nullptr) {
       const int head = in_slab / order.sq, tok = in_slab - head * order.sq;
       const size_t at = ((size_t(slab) * chunks + head / heads) * order.sq + tok) * heads + head % heads;
@@ -141,10 +150,10 @@ shared_dq_kernel(const float* __restrict__ acc_pre, long pre_slab_rows, const fl
 
 int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const void* d_o, const float* lse, const float* delta,
                      void* q_out, void* do_out, float* lse_out, float* delta_out, cudaStream_t st) {
-  const long rows = long(s.B) * s.Hq * s.Sq;
+  const int rows = s.B * s.Hq * s.Sq;
   const int es = elt_size(s.dtype), pieces = es * 8;
   auto go = [&](auto kern) {
-    kern<<<(rows * pieces + 255) / 256, 256, 0, st>>>(static_cast<const char*>(q.data), q.stride_b * es, q.stride_h * es,
+    kern<<<(rows + 1024 / pieces - 1) / (1024 / pieces), 256, 0, st>>>(static_cast<const char*>(q.data), q.stride_b * es, q.stride_h * es,
                                                       q.stride_s * es, static_cast<const uint4*>(d_o), lse, delta,
                                                       static_cast<uint4*>(q_out), static_cast<uint4*>(do_out), lse_out, delta_out,
                                                       pack_order(s, prefixes), rows, device_status_ptr());
@@ -157,12 +166,12 @@ int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const 
 
 int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
                           const float* ml_own, int ns_own, void* o, float* lse, cudaStream_t st) {
-  const long rows = long(s.B) * s.Hq * s.Sq;
+  const int rows = s.B * s.Hq * s.Sq;
   // as in launch_fwd_combine: eight warps a row while the rows alone leave SMs empty and one warp's walk is long
   const bool wide = rows <= 148 * 8 && ns_pre + ns_own > 8;
   auto go = [&](auto one, auto eight) {
     if (wide) eight<<<rows, 256, 0, st>>>(o_pre, ml_pre, ns_pre, o_own, ml_own, ns_own, pack_order(s, prefixes), o, lse, rows, device_status_ptr());
-    else one<<<(rows + 7) / 8, 256, 0, st>>>(o_pre, ml_pre, ns_pre, o_own, ml_own, ns_own, pack_order(s, prefixes), o, lse, rows, device_status_ptr());
+    else one<<<(rows - 1) / 8 + 1, 256, 0, st>>>(o_pre, ml_pre, ns_pre, o_own, ml_own, ns_own, pack_order(s, prefixes), o, lse, rows, device_status_ptr());
   };
   if (s.dtype == LVX_BF16) go(shared_combine_kernel<0, 1>, shared_combine_kernel<0, 8>);
   else if (s.dtype == LVX_FP16) go(shared_combine_kernel<1, 1>, shared_combine_kernel<1, 8>);
@@ -171,13 +180,13 @@ int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, 
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "shared_combine launch");
 }
 
-int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, long pre_slab_rows, const float* acc_own, void* dq,
+int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int pre_slab_rows, const float* acc_own, void* dq,
                      cudaStream_t st) {
-  const long rows = long(s.B) * s.Hq * s.Sq;
+  const int rows = s.B * s.Hq * s.Sq;
   const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
   // the general kernel accumulates in the order of [B, Hq, Sq]: one head a chunk
   const int heads = s.dtype == LVX_FP32 ? 1 : qt.heads, chunks = s.dtype == LVX_FP32 ? s.Hq / s.Hkv : qt.chunks;
-  const long blocks = std::min<long>((rows + 7) / 8, 148 * 16);
+  const int blocks = std::min((rows - 1) / 8 + 1, 148 * 16);
   auto go = [&](auto kern) {
     kern<<<blocks, 256, 0, st>>>(acc_pre, pre_slab_rows, acc_own, heads, chunks, pack_order(s, prefixes), dq, rows, device_status_ptr());
   };
