@@ -64,6 +64,7 @@ enum {
 struct WinFwdParams {
   int sq, skv, hkv, g, m_blocks;
   int slabs, splits, nitems;      // an item: a pair of query tiles of a slab, and a share of its keys
+  int run_tiles;                  // > 0: items are shared out as runs of key tiles, run_tiles to a pair of query tiles
   QTiles qt;
   WindowMask mask;
   const int32_t* kv_valid_len;
@@ -125,15 +126,27 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int heads = p.qt.heads, tile_rows = heads * p.qt.tokens;
   struct Item {
-    int mb, slab, split, valid, start;
+    int mb, slab, split, valid, start;      // split: number of the partial result
     KeyTiles kt;
     int j0, n;               // its share of the key tiles
+    bool last;               // runs: the last share of its query tiles (partial results that nobody makes are up to it)
   };
   // block of tokens and chunk of heads of a tile (an integer division costs the roles' common start of an item dearly)
   auto block_of = [&](int tile) { return p.qt.chunks == 1 ? tile : tile / p.qt.chunks; };
   auto chunk_of = [&](int tile) { return p.qt.chunks == 1 ? 0 : tile % p.qt.chunks; };
+  // Runs: the key tiles of all pairs of query tiles in one row, of which every CTA takes an equal stretch [run0, run1).
+  const long long run_all = static_cast<long long>(p.nitems) * p.run_tiles;
+  long long run0 = 0, run1 = 0;
+  int run_first = 0, run_end = 0;
+  if (p.run_tiles > 0) {
+    run0 = blockIdx.x * run_all / gridDim.x;
+    run1 = (blockIdx.x + 1) * run_all / gridDim.x;
+    run_first = int(run0 / p.run_tiles);
+    run_end = int((run1 - 1) / p.run_tiles);
+  }
   // the CTA's round-th item: forwards and backwards through the list in turn
   auto index_of = [&](int round) {
+    if (p.run_tiles > 0) return run_first + round <= run_end ? run_first + round : p.nitems;
     return round * int(gridDim.x) + ((round & 1) ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x));
   };
   auto item_of = [&](int w) {
@@ -149,6 +162,18 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int tok0 = block_of(2 * it.mb) * p.qt.tokens;
     const int tok1 = min(p.sq, (block_of(min(2 * it.mb + 1, p.qt.count - 1)) + 1) * p.qt.tokens) - 1;
     it.kt = key_tiles(p.mask, it.valid, it.start + tok0, it.start + tok1, 7);
+    it.last = false;
+    if (p.run_tiles > 0) {
+      // the stretch's part of this item, in proportion to the tiles that there turn out to be
+      const long long at = static_cast<long long>(w) * p.run_tiles;
+      const int a = int(max(run0 - at, 0ll)), b = int(min(run1 - at, static_cast<long long>(p.run_tiles)));
+      it.j0 = int(static_cast<long long>(a) * it.kt.n / p.run_tiles);
+      it.n = int(static_cast<long long>(b) * it.kt.n / p.run_tiles) - it.j0;
+      it.last = b == p.run_tiles;
+      // its number: CTAs since the one whose stretch holds the item's first tile (CTA c's begins at floor(c * all / CTAs))
+      it.split = a == 0 ? 0 : int(blockIdx.x) - int(((at + 1) * gridDim.x + run_all - 1) / run_all - 1);
+      return it;
+    }
     const int per_split = p.splits == 1 ? it.kt.n : (it.kt.n + p.splits - 1) / p.splits;
     it.j0 = min(it.kt.n, it.split * per_split);
     it.n = min(it.kt.n, it.j0 + per_split) - it.j0;
@@ -433,8 +458,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[q][4 * i], o[q][4 * i + 1], o[q][4 * i + 2], o[q][4 * i + 3]);
           store(q * 128);
         }
-        if (exists)
-          reinterpret_cast<float2*>(p.ml_part)[(size_t(I.slab) * p.nsplit + (PAIR ? 2 * I.split + wg : I.split)) * slab_rows + row] = make_float2(m, l);
+        if (exists) {
+          float2* ml = reinterpret_cast<float2*>(p.ml_part) + size_t(I.slab) * p.nsplit * slab_rows + row;
+          ml[(PAIR ? 2 * I.split + wg : I.split) * slab_rows] = make_float2(m, l);
+          if (I.last)      // the partial results that no CTA makes
+            for (int k = PAIR ? 2 * I.split + 2 + wg : I.split + 1; k < p.nsplit; k += STEP) ml[k * slab_rows] = make_float2(-INFINITY, 0.f);
+        }
       }
       if (again) {
         const int batch = I.slab / p.hkv, kvh = I.slab % p.hkv;
@@ -672,6 +701,11 @@ static long window_tiles(const lvx_shape& s, const lvx_window& w, bool few) {
   return std::min<long>(all, (long(m.window) + span + 126) / 128 + 1 + (long(m.sinks) + 127) / 128);
 }
 
+// Whether all pairs of query tiles see about the same number of key tiles: a prefix, a few tokens behind a long cache.
+static bool window_even(const lvx_shape& s, const lvx_window& w, long tiles) {
+  return w.query_start >= s.Skv || 8l * s.Sq <= tiles * 128;
+}
+
 FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few) {
   *few = false;
   if (s.dtype == LVX_FP32) return plan_fwd(s);
@@ -699,6 +733,17 @@ FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few) {
     }
   }
   p.tiles_per_split = 0;          // the kernels share out what each CTA turns out to see
+  // Runs, where the pairs of query tiles see about the same number of keys: equal stretches for 148 CTAs instead of whole
+  // rounds of equal shares, which leave the last round partly filled, pay the fixed cost for every share and write as many
+  // partial results. (168 pairs of 201 tiles: 547 -> 535 us, and their merge 48 -> 30; 80 pairs: 285 -> 270 and 23 -> 16; 8
+  // pairs, which are 18 or 19 shares each way: even.) A pair is met by 148 / pairs CTAs, and one more where it does not divide.
+  if (!*few && tiles > 0 && window_even(s, w, tiles) && base * tiles >= 148) {
+    const long cost = (base * tiles + 147) / 148 + 3 * (base / 148 + 2) + 4;
+    if (cost < best_cost) {
+      p.tiles_per_split = int(tiles);
+      p.nsplit = int((148 + base - 1) / base + (148 % base != 0 || 148 < base));
+    }
+  }
   if (pair) p.nsplit *= 2;        // partial results; there are half as many items
   p.o_part_bytes = (size_t(s.B) * s.Hkv * p.nsplit * p.rows * 512 + 255) & ~size_t(255);
   p.ml_part_bytes = (size_t(s.B) * s.Hkv * p.nsplit * p.rows * 8 + 255) & ~size_t(255);
@@ -759,11 +804,13 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
   p.status = status;
   const bool pair = window_pair(s, window_tiles(s, w, false), false);
   p.slabs = s.B * s.Hkv;
-  p.splits = pair ? pl.nsplit / 2 : pl.nsplit;
+  p.run_tiles = pl.tiles_per_split;
+  p.splits = p.run_tiles > 0 ? 1 : pair ? pl.nsplit / 2 : pl.nsplit;
   const long items = long(p.slabs) * pl.m_blocks * p.splits;
   if (items >= (1l << 30)) return fail(LVX_ERR_LIMIT, "window_fwd: %ld work items", items);
   p.nitems = int(items);
-  const unsigned grid = unsigned(std::min<long>(items, num_sms()));      // persistent: one CTA per SM
+  // persistent: one CTA per SM; runs are planned for 148
+  const unsigned grid = p.run_tiles > 0 ? 148 : unsigned(std::min<long>(items, num_sms()));
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WF_SMEM);
