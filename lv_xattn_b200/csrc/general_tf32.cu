@@ -715,7 +715,7 @@ int launch_bwd_block_general(const lvx_shape& s, const void* q, const void* d_o,
     // 512 tokens, 32 heads, window 128: 528 us with a CTA per key tile, which waited for the sinks' 32 row tiles.
     const long tiles = (p.rows + 63) / 64, keys = long(grid.x) * grid.y;
     const long seen = std::min<long>(tiles, p.mask.window < kNoWindow ? (long(p.mask.window) + 126) * (p.rows / s.Sq) / 64 + 2 : tiles);
-    p.share = int(std::max<long>(2, (keys * seen + 295) / 296));
+    p.share = int(std::max<long>(std::max<long>(2, (tiles + 65534) / 65535), (keys * seen + 295) / 296));
     grid.z = unsigned((tiles + p.share - 1) / p.share);
     if (grid.z > 1) {
       const size_t n = size_t(s.B) * s.Hkv * s.Skv * 128 * sizeof(float);

@@ -170,252 +170,251 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   // Every role walks the same items in the same order and keeps the same counters: `it` = items with tiles done, `jj0` =
   // tiles done before the current item, `cleaned` = items whose K and V were cleared in part.
-  {
-    if (warp < WB_COMPUTE) {
-      // =========================== compute warps ===========================
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 80;" ::: "memory");
-      const int quarter = warp & 3;                         // TMEM lane quarter
-      const int cg = warp >> 2;                             // 32-column group of the query tile
-      const int r = quarter * 32 + lane;                    // key inside the tile
-      const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
-      const uint32_t tX = tmem_base + WB_X + lane_sel, tY = tmem_base + WB_Y + lane_sel;
-      const float c = p.scale_log2;
-      bool alive = !poisoned;
-      int it = 0, jj0 = 0;
-      for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
-        const Item I = item_of(w);
-        if (I.ntot == 0) {      // nothing sees these keys (or they are not valid): their gradients are zero
-          if (I.part >= 0) {
-            float4* dst = reinterpret_cast<float4*>(p.parts + size_t(I.part) * 2 * 128 * 128);
-            for (int i = tid; i < 2 * 128 * 32; i += WB_COMPUTE * 32) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          } else if (warp < 8 && I.kv0 + (tid & 127) < p.skv) {
-            uint4* dst = reinterpret_cast<uint4*>((warp < 4 ? p.dk : p.dv) + (size_t(I.slab) * p.skv + I.kv0 + (tid & 127)) * 128);
+  if (warp < WB_COMPUTE) {
+    // =========================== compute warps ===========================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 80;" ::: "memory");
+    const int quarter = warp & 3;                         // TMEM lane quarter
+    const int cg = warp >> 2;                             // 32-column group of the query tile
+    const int r = quarter * 32 + lane;                    // key inside the tile
+    const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tX = tmem_base + WB_X + lane_sel, tY = tmem_base + WB_Y + lane_sel;
+    const float c = p.scale_log2;
+    bool alive = !poisoned;
+    int it = 0, jj0 = 0;
+    for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
+      const Item I = item_of(w);
+      if (I.ntot == 0) {      // nothing sees these keys (or they are not valid): their gradients are zero
+        if (I.part >= 0) {
+          float4* dst = reinterpret_cast<float4*>(p.parts + size_t(I.part) * 2 * 128 * 128);
+          for (int i = tid; i < 2 * 128 * 32; i += WB_COMPUTE * 32) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else if (warp < 8 && I.kv0 + (tid & 127) < p.skv) {
+          uint4* dst = reinterpret_cast<uint4*>((warp < 4 ? p.dk : p.dv) + (size_t(I.slab) * p.skv + I.kv0 + (tid & 127)) * 128);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
-          }
-          continue;
+          for (int i = 0; i < 16; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
         }
-        // Statistics of a tile's columns: threads 0-127 fetch lse, 128-255 delta.
-        auto fetch_stat = [&](int j) -> float {
-          if (tid >= 256) return 0.f;
-          const int col = tid & 127, tok = tile_tok(I, j) + col / heads, head = tile_chunk(j) * heads + col % heads;
-          const bool exists = col < tile_rows && tok < p.sq && head < p.g;
-          const size_t at = (size_t(I.slab) * p.g + head) * p.sq + tok;
-          if (tid >= 128) return exists ? p.delta[at] : 0.f;
-          float v = INFINITY;       // +inf => P = 0: a query that does not exist, or that sees nothing
-          if (exists) {
-            v = p.lse[at] * 1.4426950408889634f;
-            if (v == -INFINITY) v = INFINITY;
-          }
-          return v;
-        };
-        auto put_stat = [&](int jj, float v) {
-          if (tid >= 256) return;
-          s_stat[(jj & 1) * 256 + tid] = v;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[WBB_STAT_FULL + (jj & 1)]);
-        };
-        put_stat(jj0, fetch_stat(0));
-        float stat_next = I.ntot > 1 ? fetch_stat(1) : 0.f;
-        if (I.valid < min(p.skv, I.kv0 + 128)) {      // rows that are there but not valid
-          if (!mbar_wait(&bars[WBB_KV_FULL], it & 1, abort_flag, p.status, WB_CODE(0, WBB_KV_FULL))) {
-            alive = false;
-            break;
-          }
-          const int left = I.valid - I.kv0;
-          for (int i = tid; i < (128 - left) * 8 * 4; i += WB_COMPUTE * 32)
-            reinterpret_cast<uint4*>(smem + WB_OFF_K + (i & 3) * WB_HALF)[left * 8 + (i >> 2)] = make_uint4(0u, 0u, 0u, 0u);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[WBB_KV_CLEAN]);
+        continue;
+      }
+      // Statistics of a tile's columns: threads 0-127 fetch lse, 128-255 delta.
+      auto fetch_stat = [&](int j) -> float {
+        if (tid >= 256) return 0.f;
+        const int col = tid & 127, tok = tile_tok(I, j) + col / heads, head = tile_chunk(j) * heads + col % heads;
+        const bool exists = col < tile_rows && tok < p.sq && head < p.g;
+        const size_t at = (size_t(I.slab) * p.g + head) * p.sq + tok;
+        if (tid >= 128) return exists ? p.delta[at] : 0.f;
+        float v = INFINITY;       // +inf => P = 0: a query that does not exist, or that sees nothing
+        if (exists) {
+          v = p.lse[at] * 1.4426950408889634f;
+          if (v == -INFINITY) v = INFINITY;
         }
-        // The queries that see this thread's key: tokens from `from` on, up to `to`.
-        const int key = I.kv0 + r;
-        const int from = key < I.valid ? key - I.start : kNoWindow;
-        const int to = key < p.mask.sinks ? kNoWindow : key - I.start + p.mask.window;
-        for (int j = 0; j < I.ntot; ++j) {
-          const int jj = jj0 + j;
-          float stat_after = 0.f;
-          if (j + 2 < I.ntot) stat_after = fetch_stat(j + 2);
-          // ---------------- P^T half: needs S^T only ----------------
-          if (!mbar_wait(&bars[WBB_S_FULL], jj & 1, abort_flag, p.status, WB_CODE(0, WBB_S_FULL))) {
-            alive = false;
-            break;
-          }
-          tc_fence_after();
-          uint32_t s[32];
-          tmem_ld32(tX + cg * 32, s);
+        return v;
+      };
+      auto put_stat = [&](int jj, float v) {
+        if (tid >= 256) return;
+        s_stat[(jj & 1) * 256 + tid] = v;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[WBB_STAT_FULL + (jj & 1)]);
+      };
+      put_stat(jj0, fetch_stat(0));
+      float stat_next = I.ntot > 1 ? fetch_stat(1) : 0.f;
+      if (I.valid < min(p.skv, I.kv0 + 128)) {      // rows that are there but not valid
+        if (!mbar_wait(&bars[WBB_KV_FULL], it & 1, abort_flag, p.status, WB_CODE(0, WBB_KV_FULL))) {
+          alive = false;
+          break;
+        }
+        const int left = I.valid - I.kv0;
+        for (int i = tid; i < (128 - left) * 8 * 4; i += WB_COMPUTE * 32)
+          reinterpret_cast<uint4*>(smem + WB_OFF_K + (i & 3) * WB_HALF)[left * 8 + (i >> 2)] = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[WBB_KV_CLEAN]);
+      }
+      // The queries that see this thread's key: tokens from `from` on, up to `to`.
+      const int key = I.kv0 + r;
+      const int from = key < I.valid ? key - I.start : kNoWindow;
+      const int to = key < p.mask.sinks ? kNoWindow : key - I.start + p.mask.window;
+      for (int j = 0; j < I.ntot; ++j) {
+        const int jj = jj0 + j;
+        float stat_after = 0.f;
+        if (j + 2 < I.ntot) stat_after = fetch_stat(j + 2);
+        // ---------------- P^T half: needs S^T only ----------------
+        if (!mbar_wait(&bars[WBB_S_FULL], jj & 1, abort_flag, p.status, WB_CODE(0, WBB_S_FULL))) {
+          alive = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[32];
+        tmem_ld32(tX + cg * 32, s);
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[WBB_X_LOADED]);
+        if (!mbar_wait(&bars[WBB_STAT_FULL + (jj & 1)], (jj >> 1) & 1, abort_flag, p.status, WB_CODE(0, WBB_STAT_FULL))) {
+          alive = false;
+          break;
+        }
+        // of the warp's 32 columns, those that see the key; a tile that all see is not masked
+        uint32_t seen;
+        {
+          const int tok0 = tile_tok(I, j);
+          const int c0 = min(max(from - tok0, 0), 128) * heads - cg * 32, c1 = min(max(to - tok0, 0), 128) * heads - cg * 32;
+          seen = low_bits(clamp32(c1)) & ~low_bits(clamp32(c0));
+        }
+        const bool masked = __any_sync(0xffffffffu, seen != 0xffffffffu);
+        const float4* sl = reinterpret_cast<const float4*>(s_stat + (jj & 1) * 256 + cg * 32);
+        const float4* sd = reinterpret_cast<const float4*>(s_stat + (jj & 1) * 256 + 128 + cg * 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {      // s becomes P, which stays in fp32 for dS
+          const float4 l2 = sl[i];
+          s[4 * i] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i]), c, -l2.x)));
+          s[4 * i + 1] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 1]), c, -l2.y)));
+          s[4 * i + 2] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 2]), c, -l2.z)));
+          s[4 * i + 3] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 3]), c, -l2.w)));
+        }
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(seen & (1u << i))) s[i] = 0u;
+        }
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          pk[i] = IS_BF16 ? pack_bf16x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]))
+                          : pack_f16x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+        // P^T overwrites S^T in X: wait until every warp has taken its S^T columns out.
+        if (!mbar_wait(&bars[WBB_X_LOADED], jj & 1, abort_flag, p.status, WB_CODE(0, WBB_X_LOADED))) {
+          alive = false;
+          break;
+        }
+        tmem_st16(tX + cg * 16, pk);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[WBB_P_FULL]);      // dV of this tile may start
+        // ---------------- dS^T half: needs dP^T ----------------
+        if (!mbar_wait(&bars[WBB_DP_FULL], jj & 1, abort_flag, p.status, WB_CODE(0, WBB_DP_FULL))) {
+          alive = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t dsk[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t dp[16];
+          tmem_ld16(tY + cg * 32 + h * 16, dp);
           tc_wait_ld();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[WBB_X_LOADED]);
-          if (!mbar_wait(&bars[WBB_STAT_FULL + (jj & 1)], (jj >> 1) & 1, abort_flag, p.status, WB_CODE(0, WBB_STAT_FULL))) {
-            alive = false;
-            break;
-          }
-          // of the warp's 32 columns, those that see the key; a tile that all see is not masked
-          uint32_t seen;
-          {
-            const int tok0 = tile_tok(I, j);
-            const int c0 = min(max(from - tok0, 0), 128) * heads - cg * 32, c1 = min(max(to - tok0, 0), 128) * heads - cg * 32;
-            seen = low_bits(clamp32(c1)) & ~low_bits(clamp32(c0));
-          }
-          const bool masked = __any_sync(0xffffffffu, seen != 0xffffffffu);
-          const float4* sl = reinterpret_cast<const float4*>(s_stat + (jj & 1) * 256 + cg * 32);
-          const float4* sd = reinterpret_cast<const float4*>(s_stat + (jj & 1) * 256 + 128 + cg * 32);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {      // s becomes P, which stays in fp32 for dS
-            const float4 l2 = sl[i];
-            s[4 * i] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i]), c, -l2.x)));
-            s[4 * i + 1] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 1]), c, -l2.y)));
-            s[4 * i + 2] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 2]), c, -l2.z)));
-            s[4 * i + 3] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[4 * i + 3]), c, -l2.w)));
+          for (int i = 0; i < 4; ++i) {
+            const float4 dl = sd[h * 4 + i];
+            const float d0 = __uint_as_float(s[h * 16 + 4 * i]) * (__uint_as_float(dp[4 * i]) - dl.x);
+            const float d1 = __uint_as_float(s[h * 16 + 4 * i + 1]) * (__uint_as_float(dp[4 * i + 1]) - dl.y);
+            const float d2 = __uint_as_float(s[h * 16 + 4 * i + 2]) * (__uint_as_float(dp[4 * i + 2]) - dl.z);
+            const float d3 = __uint_as_float(s[h * 16 + 4 * i + 3]) * (__uint_as_float(dp[4 * i + 3]) - dl.w);
+            dsk[h * 8 + 2 * i] = IS_BF16 ? pack_bf16x2(d0, d1) : pack_f16x2(d0, d1);
+            dsk[h * 8 + 2 * i + 1] = IS_BF16 ? pack_bf16x2(d2, d3) : pack_f16x2(d2, d3);
           }
-          if (masked) {
+        }
+        tc_fence_before();
+        if (jj > 0 && !mbar_wait(&bars[WBB_DS_FREE], (jj - 1) & 1, abort_flag, p.status, WB_CODE(0, WBB_DS_FREE))) {
+          alive = false;
+          break;
+        }
+        {
+          uint8_t* rowp = smem + WB_OFF_DS + (cg >> 1) * WB_HALF + r * 128;
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(seen & (1u << i))) s[i] = 0u;
-          }
-          uint32_t pk[16];
+          for (int ch = 0; ch < 4; ++ch)
+            *reinterpret_cast<uint4*>(rowp + ((((cg & 1) * 4 + ch) ^ (r & 7)) << 4)) =
+                make_uint4(dsk[4 * ch], dsk[4 * ch + 1], dsk[4 * ch + 2], dsk[4 * ch + 3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[WBB_PDS_FULL]);
+        if (j + 1 < I.ntot) put_stat(jj + 1, stat_next);
+        stat_next = stat_after;
+      }
+      // ------------------------------- dK / dV of the item -------------------------------
+      if (alive) alive = mbar_wait(&bars[WBB_ACC_DONE], it & 1, abort_flag, p.status, WB_CODE(0, WBB_ACC_DONE));
+      alive = __all_sync(0xffffffffu, alive);
+      tc_fence_after();
+      if (alive) {
+        // A thread's 64 bytes of a row go through the warp's own part of the dS^T tile (which nothing reads until this warp
+        // writes it again), so that a store covers whole sectors. Written by row they were 16-byte pieces 256 bytes apart,
+        // and the write-out took 12,000 cycles beside the reduce-adds instead of 3,000.
+        uint8_t* stage = smem + WB_OFF_DS + (cg >> 1) * WB_HALF + quarter * 32 * 128;
+        const size_t off = (size_t(I.slab) * p.skv + I.kv0 + quarter * 32) * 128 + cg * 32;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            pk[i] = IS_BF16 ? pack_bf16x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]))
-                            : pack_f16x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-          // P^T overwrites S^T in X: wait until every warp has taken its S^T columns out.
-          if (!mbar_wait(&bars[WBB_X_LOADED], jj & 1, abort_flag, p.status, WB_CODE(0, WBB_X_LOADED))) {
-            alive = false;
-            break;
-          }
-          tmem_st16(tX + cg * 16, pk);
-          tc_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[WBB_P_FULL]);      // dV of this tile may start
-          // ---------------- dS^T half: needs dP^T ----------------
-          if (!mbar_wait(&bars[WBB_DP_FULL], jj & 1, abort_flag, p.status, WB_CODE(0, WBB_DP_FULL))) {
-            alive = false;
-            break;
-          }
-          tc_fence_after();
-          uint32_t dsk[16];
+        for (int which = 0; which < 2; ++which) {
+          uint32_t a[32];
+          tmem_ld32(tmem_base + (which ? WB_DV : WB_DK) + lane_sel + cg * 32, a);
+          tc_wait_ld();
+          const float mul = which ? 1.f : p.scale;
+          if (I.part >= 0) {
+            float4* dst = reinterpret_cast<float4*>(p.parts + ((size_t(I.part) * 2 + which) * 128 + r) * 128 + cg * 32);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t dp[16];
-            tmem_ld16(tY + cg * 32 + h * 16, dp);
-            tc_wait_ld();
+            for (int i = 0; i < 8; ++i)
+              dst[i] = make_float4(__uint_as_float(a[4 * i]) * mul, __uint_as_float(a[4 * i + 1]) * mul,
+                                   __uint_as_float(a[4 * i + 2]) * mul, __uint_as_float(a[4 * i + 3]) * mul);
+          } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float4 dl = sd[h * 4 + i];
-              const float d0 = __uint_as_float(s[h * 16 + 4 * i]) * (__uint_as_float(dp[4 * i]) - dl.x);
-              const float d1 = __uint_as_float(s[h * 16 + 4 * i + 1]) * (__uint_as_float(dp[4 * i + 1]) - dl.y);
-              const float d2 = __uint_as_float(s[h * 16 + 4 * i + 2]) * (__uint_as_float(dp[4 * i + 2]) - dl.z);
-              const float d3 = __uint_as_float(s[h * 16 + 4 * i + 3]) * (__uint_as_float(dp[4 * i + 3]) - dl.w);
-              dsk[h * 8 + 2 * i] = IS_BF16 ? pack_bf16x2(d0, d1) : pack_f16x2(d0, d1);
-              dsk[h * 8 + 2 * i + 1] = IS_BF16 ? pack_bf16x2(d2, d3) : pack_f16x2(d2, d3);
-            }
-          }
-          tc_fence_before();
-          if (jj > 0 && !mbar_wait(&bars[WBB_DS_FREE], (jj - 1) & 1, abort_flag, p.status, WB_CODE(0, WBB_DS_FREE))) {
-            alive = false;
-            break;
-          }
-          {
-            uint8_t* rowp = smem + WB_OFF_DS + (cg >> 1) * WB_HALF + r * 128;
+              uint32_t wd[4];
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch)
-              *reinterpret_cast<uint4*>(rowp + ((((cg & 1) * 4 + ch) ^ (r & 7)) << 4)) =
-                  make_uint4(dsk[4 * ch], dsk[4 * ch + 1], dsk[4 * ch + 2], dsk[4 * ch + 3]);
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[WBB_PDS_FULL]);
-          if (j + 1 < I.ntot) put_stat(jj + 1, stat_next);
-          stat_next = stat_after;
-        }
-        // ------------------------------- dK / dV of the item -------------------------------
-        if (alive) alive = mbar_wait(&bars[WBB_ACC_DONE], it & 1, abort_flag, p.status, WB_CODE(0, WBB_ACC_DONE));
-        alive = __all_sync(0xffffffffu, alive);
-        tc_fence_after();
-        if (alive) {
-          // A thread's 64 bytes of a row go through the warp's own part of the dS^T tile (which nothing reads until this warp
-          // writes it again), so that a store covers whole sectors. Written by row they were 16-byte pieces 256 bytes apart,
-          // and the write-out took 12,000 cycles beside the reduce-adds instead of 3,000.
-          uint8_t* stage = smem + WB_OFF_DS + (cg >> 1) * WB_HALF + quarter * 32 * 128;
-          const size_t off = (size_t(I.slab) * p.skv + I.kv0 + quarter * 32) * 128 + cg * 32;
-#pragma unroll
-          for (int which = 0; which < 2; ++which) {
-            uint32_t a[32];
-            tmem_ld32(tmem_base + (which ? WB_DV : WB_DK) + lane_sel + cg * 32, a);
-            tc_wait_ld();
-            const float mul = which ? 1.f : p.scale;
-            if (I.part >= 0) {
-              float4* dst = reinterpret_cast<float4*>(p.parts + ((size_t(I.part) * 2 + which) * 128 + r) * 128 + cg * 32);
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                dst[i] = make_float4(__uint_as_float(a[4 * i]) * mul, __uint_as_float(a[4 * i + 1]) * mul,
-                                     __uint_as_float(a[4 * i + 2]) * mul, __uint_as_float(a[4 * i + 3]) * mul);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t wd[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float lo = __uint_as_float(a[8 * i + 2 * e]) * mul, hi = __uint_as_float(a[8 * i + 2 * e + 1]) * mul;
-                  wd[e] = IS_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
-                }
-                *reinterpret_cast<uint4*>(stage + lane * 128 + ((((cg & 1) * 4 + i) ^ (lane & 7)) << 4)) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+              for (int e = 0; e < 4; ++e) {
+                const float lo = __uint_as_float(a[8 * i + 2 * e]) * mul, hi = __uint_as_float(a[8 * i + 2 * e + 1]) * mul;
+                wd[e] = IS_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
               }
-              __syncwarp();
-              uint16_t* dst = (which ? p.dv : p.dk) + off;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int rr = i * 8 + (lane >> 2), piece = lane & 3;
-                if (I.kv0 + quarter * 32 + rr < p.skv)
-                  *reinterpret_cast<uint4*>(dst + rr * 128 + piece * 8) =
-                      *reinterpret_cast<const uint4*>(stage + rr * 128 + ((((cg & 1) * 4 + piece) ^ (rr & 7)) << 4));
-              }
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((((cg & 1) * 4 + i) ^ (lane & 7)) << 4)) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
             }
             __syncwarp();
-          }
-          tc_fence_before();
-        }
-        ++it;
-        jj0 += I.ntot;
-      }
-    } else if (warp < WB_WARP_TMA) {
-      // =========================== dQ drain warps ===========================
-      const int quarter = warp & 3;
-      const int ch = (warp - WB_COMPUTE) >> 2;              // which 64 query columns
-      const int d = quarter * 32 + lane;                    // head-dim index = TMEM lane of dQ^T
-      const uint32_t tY = tmem_base + WB_Y + (static_cast<uint32_t>(quarter * 32) << 16);
-      bool alive = !poisoned;
-      int jj0 = 0;
-      for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
-        const Item I = item_of(w);
-        for (int j = 0; j < I.ntot; ++j) {
-          const int jj = jj0 + j;
-          if (!mbar_wait(&bars[WBB_DQ_FULL], jj & 1, abort_flag, p.status, WB_CODE(1, WBB_DQ_FULL))) {
-            alive = false;
-            break;
-          }
-          tc_fence_after();
-          uint32_t v[2][32];
-          tmem_ld32(tY + ch * 64, v[0]);
-          tmem_ld32(tY + ch * 64 + 32, v[1]);
-          tc_wait_ld();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[WBB_DQ_FREE]);     // Y is free for the next tile's dP^T
-          const int tok0 = tile_tok(I, j);
-          const int ncols = min(tile_rows, (p.sq - tok0) * heads) - ch * 64;
-          float* dst = p.dq_acc + ((size_t(I.slab) * p.qt.chunks + tile_chunk(j)) * p.sq * heads + size_t(tok0) * heads + ch * 64) * 128 + d;
+            uint16_t* dst = (which ? p.dv : p.dk) + off;
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i < ncols) atomicAdd(dst + size_t(i) * 128, __uint_as_float(v[i >> 5][i & 31]) * p.scale);
+            for (int i = 0; i < 4; ++i) {
+              const int rr = i * 8 + (lane >> 2), piece = lane & 3;
+              if (I.kv0 + quarter * 32 + rr < p.skv)
+                *reinterpret_cast<uint4*>(dst + rr * 128 + piece * 8) =
+                    *reinterpret_cast<const uint4*>(stage + rr * 128 + ((((cg & 1) * 4 + piece) ^ (rr & 7)) << 4));
+            }
+          }
+          __syncwarp();
         }
-        jj0 += I.ntot;
+        tc_fence_before();
       }
-    } else {
+      ++it;
+      jj0 += I.ntot;
+    }
+  } else if (warp < WB_WARP_TMA) {
+    // =========================== dQ drain warps ===========================
+    const int quarter = warp & 3;
+    const int ch = (warp - WB_COMPUTE) >> 2;              // which 64 query columns
+    const int d = quarter * 32 + lane;                    // head-dim index = TMEM lane of dQ^T
+    const uint32_t tY = tmem_base + WB_Y + (static_cast<uint32_t>(quarter * 32) << 16);
+    bool alive = !poisoned;
+    int jj0 = 0;
+    for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
+      const Item I = item_of(w);
+      for (int j = 0; j < I.ntot; ++j) {
+        const int jj = jj0 + j;
+        if (!mbar_wait(&bars[WBB_DQ_FULL], jj & 1, abort_flag, p.status, WB_CODE(1, WBB_DQ_FULL))) {
+          alive = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t v[2][32];
+        tmem_ld32(tY + ch * 64, v[0]);
+        tmem_ld32(tY + ch * 64 + 32, v[1]);
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[WBB_DQ_FREE]);     // Y is free for the next tile's dP^T
+        const int tok0 = tile_tok(I, j);
+        const int ncols = min(tile_rows, (p.sq - tok0) * heads) - ch * 64;
+        float* dst = p.dq_acc + ((size_t(I.slab) * p.qt.chunks + tile_chunk(j)) * p.sq * heads + size_t(tok0) * heads + ch * 64) * 128 + d;
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (i < ncols) atomicAdd(dst + size_t(i) * 128, __uint_as_float(v[i >> 5][i & 31]) * p.scale);
+      }
+      jj0 += I.ntot;
+    }
+  } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;" ::: "memory");
     if (warp == WB_WARP_TMA) {
       // =========================== TMA producer ===========================
@@ -583,7 +582,6 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
     }
-    }
   }
 
   tc_fence_before();
@@ -641,9 +639,12 @@ static SinkParts sink_parts(const lvx_shape& s, const lvx_window& w) {
   SinkParts sp = {0, 1};
   if (m.window == kNoWindow || m.sinks == 0 || s.Skv == 0) return sp;
   const long all = (long(s.Sq) + qt.tokens - 1) / qt.tokens, usual = (long(m.window) + 127) / qt.tokens + 1;
-  const long parts = std::min<long>((all + usual - 1) / usual, 32);
+  const long tiles = (std::min<long>(m.sinks, s.Skv) + 127) / 128;
+  // (and no more than fill the GPU four times over: many sinks are many items as it is, and every part is 128 KB of scratch)
+  const long enough = (4 * 148 + s.B * s.Hkv * tiles - 1) / (s.B * s.Hkv * tiles);
+  const long parts = std::min((all + usual - 1) / usual, enough);
   if (parts < 2) return sp;
-  sp.tiles = int((std::min<long>(m.sinks, s.Skv) + 127) / 128);
+  sp.tiles = int(tiles);
   sp.parts = int(parts);
   return sp;
 }

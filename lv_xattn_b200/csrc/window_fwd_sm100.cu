@@ -235,259 +235,259 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     bool alive = !poisoned;
     int done_items = 0, t0 = 0;      // items with tiles of this warpgroup, and those tiles
     for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
-    const Item I = item_of(w);
-    const int tile = PAIR ? 0 : 2 * I.mb + wg;
-    const int tok = block_of(tile) * p.qt.tokens + r_tok, head = chunk_of(tile) * heads + r_head;
-    const bool exists = tile < p.qt.count && r < tile_rows && tok < p.sq && head < p.g;
-    // this row's keys: [0, sink_end) and [lo, hi]. A row that does not exist sees everything against a reference of 0 (its
-    // scores are zeros), so that it never holds up its warp.
-    const int hi = exists ? min(I.start + tok, I.valid - 1) : I.valid - 1;
-    const int lo = exists ? max(0, I.start + tok - p.mask.window + 1) : 0;
-    const int sink_end = min(p.mask.sinks, hi + 1);
-    // keys that every row of the warp sees: [0, all_sinks) and [all_lo, all_hi]
-    const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
-    const int all_sinks = min(p.mask.sinks, all_hi + 1);
-    float m = exists ? -INFINITY : 0.f, l = 0.f;
-    int t = 0;                       // tiles of this warpgroup in the item
-    for (int j = first; j < I.n; j += STEP, ++t) {
-      const int key0 = I.kt.tile(I.j0 + j) * 128;
-      const bool full = key0 + 127 <= all_hi && (key0 >= all_lo || key0 + 128 <= all_sinks);
-      if (!mbar_wait(&bars[WFB_S_FULL + wg], (t0 + t) & 1, abort_flag, p.status, WF_CODE(wg, WFB_S_FULL))) {
-        alive = false;
-        break;
-      }
-      tc_fence_after();
-      // The usual tile: exponentials against the running maximum as it stands (it is only a reference point), P held in
-      // registers until the row sums are known to be small. (See fwd_sm100.cu for what each of these costs.)
-      bool done = false;
-      if (t > 0 && full) {
-        uint32_t pk[2][32];
-        uint64_t sum_a = f32x2(0.f, 0.f), sum_b = f32x2(0.f, 0.f);
-        const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-m, -m);
-        auto chunk = [&](const uint32_t (&b)[32], uint32_t* out) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float x0, x1, x2, x3;
-            f32x2_get(fma2(f32x2(__uint_as_float(b[4 * i]), __uint_as_float(b[4 * i + 1])), c2, nm2), x0, x1);
-            f32x2_get(fma2(f32x2(__uint_as_float(b[4 * i + 2]), __uint_as_float(b[4 * i + 3])), c2, nm2), x2, x3);
-            const float e0 = ex2f(x0), e1 = ex2f(x1), e2 = ex2f(x2), e3 = ex2f(x3);
-            sum_a = add2(sum_a, f32x2(e0, e1));
-            sum_b = add2(sum_b, f32x2(e2, e3));
-            out[2 * i] = IS_BF16 ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1);
-            out[2 * i + 1] = IS_BF16 ? pack_bf16x2(e2, e3) : pack_f16x2(e2, e3);
-          }
-        };
-        {
-          uint32_t sv[4][32];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, sv[q]);
-          tc_wait_ld();
-#pragma unroll
-          for (int q = 0; q < 4; ++q) chunk(sv[q], &pk[0][0] + q * 16);
+      const Item I = item_of(w);
+      const int tile = PAIR ? 0 : 2 * I.mb + wg;
+      const int tok = block_of(tile) * p.qt.tokens + r_tok, head = chunk_of(tile) * heads + r_head;
+      const bool exists = tile < p.qt.count && r < tile_rows && tok < p.sq && head < p.g;
+      // this row's keys: [0, sink_end) and [lo, hi]. A row that does not exist sees everything against a reference of 0 (its
+      // scores are zeros), so that it never holds up its warp.
+      const int hi = exists ? min(I.start + tok, I.valid - 1) : I.valid - 1;
+      const int lo = exists ? max(0, I.start + tok - p.mask.window + 1) : 0;
+      const int sink_end = min(p.mask.sinks, hi + 1);
+      // keys that every row of the warp sees: [0, all_sinks) and [all_lo, all_hi]
+      const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
+      const int all_sinks = min(p.mask.sinks, all_hi + 1);
+      float m = exists ? -INFINITY : 0.f, l = 0.f;
+      int t = 0;                       // tiles of this warpgroup in the item
+      for (int j = first; j < I.n; j += STEP, ++t) {
+        const int key0 = I.kt.tile(I.j0 + j) * 128;
+        const bool full = key0 + 127 <= all_hi && (key0 >= all_lo || key0 + 128 <= all_sinks);
+        if (!mbar_wait(&bars[WFB_S_FULL + wg], (t0 + t) & 1, abort_flag, p.status, WF_CODE(wg, WFB_S_FULL))) {
+          alive = false;
+          break;
         }
-        float t0, t1, t2, t3;
-        f32x2_get(sum_a, t0, t1);
-        f32x2_get(sum_b, t2, t3);
-        const float tile_sum = (t0 + t1) + (t2 + t3);
-        if (__all_sync(0xffffffffu, tile_sum <= 16384.f)) {      // bounds each P; false for infinities and NaN
-          tmem_st32(tS + 0, pk[0]);
-          tmem_st32(tS + 32, pk[1]);
-          l += tile_sum;
-          done = true;
-        }
-      }
-      if (!done) {
-        // The first tile, tiles that are seen in part, and scores that jumped: with the row maximum. A warp's rows are few
-        // tokens, so of a partly seen tile's four groups of 32 keys all but one or two are seen by all of its rows or by none;
-        // those that none sees are zeros without an exponential, and only the mixed ones are masked.
-        uint32_t s[4][32];
+        tc_fence_after();
+        // The usual tile: exponentials against the running maximum as it stands (it is only a reference point), P held in
+        // registers until the row sums are known to be small. (See fwd_sm100.cu for what each of these costs.)
+        bool done = false;
+        if (t > 0 && full) {
+          uint32_t pk[2][32];
+          uint64_t sum_a = f32x2(0.f, 0.f), sum_b = f32x2(0.f, 0.f);
+          const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-m, -m);
+          auto chunk = [&](const uint32_t (&b)[32], uint32_t* out) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, s[q]);
-        uint32_t none = 0;      // bit q: group q is seen by no row of the warp
-        if (!full) {
-          uint32_t seen[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            seen[q] = visible_bits(key0 + q * 32, lo, hi, sink_end);
-            if (!__any_sync(0xffffffffu, seen[q] != 0u)) none |= 1u << q;
-          }
-          tc_wait_ld();
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (!(none >> q & 1) && !__all_sync(0xffffffffu, seen[q] == 0xffffffffu)) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(seen[q] & (1u << i))) s[q][i] = 0xff800000u;  // -inf
+            for (int i = 0; i < 8; ++i) {
+              float x0, x1, x2, x3;
+              f32x2_get(fma2(f32x2(__uint_as_float(b[4 * i]), __uint_as_float(b[4 * i + 1])), c2, nm2), x0, x1);
+              f32x2_get(fma2(f32x2(__uint_as_float(b[4 * i + 2]), __uint_as_float(b[4 * i + 3])), c2, nm2), x2, x3);
+              const float e0 = ex2f(x0), e1 = ex2f(x1), e2 = ex2f(x2), e3 = ex2f(x3);
+              sum_a = add2(sum_a, f32x2(e0, e1));
+              sum_b = add2(sum_b, f32x2(e2, e3));
+              out[2 * i] = IS_BF16 ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1);
+              out[2 * i + 1] = IS_BF16 ? pack_bf16x2(e2, e3) : pack_f16x2(e2, e3);
             }
-        } else {
-          tc_wait_ld();
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          };
+          {
+            uint32_t sv[4][32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (!(none >> q & 1)) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[q][i]));
-          }
-        const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
-        const bool grow = m_new > m + 8.f;       // raised only when it would grow by more than 2^8: P stays below 256
-        float alpha = 1.f;
-        if (grow) {
-          alpha = ex2f(m - m_new);
-          m = m_new;
-          l *= alpha;
-        }
-        if (t > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t o[32];
-            tmem_ld32(tO + q * 32, o);
+            for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, sv[q]);
             tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st32(tO + q * 32, o);
+            for (int q = 0; q < 4; ++q) chunk(sv[q], &pk[0][0] + q * 16);
+          }
+          float s0, s1, s2, s3;
+          f32x2_get(sum_a, s0, s1);
+          f32x2_get(sum_b, s2, s3);
+          const float tile_sum = (s0 + s1) + (s2 + s3);
+          if (__all_sync(0xffffffffu, tile_sum <= 16384.f)) {      // bounds each P; false for infinities and NaN
+            tmem_st32(tS + 0, pk[0]);
+            tmem_st32(tS + 32, pk[1]);
+            l += tile_sum;
+            done = true;
           }
         }
-        const float moff = (m == -INFINITY) ? 0.f : m;
-        const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-moff, -moff);
-        uint64_t sum = f32x2(0.f, 0.f);
+        if (!done) {
+          // The first tile, tiles that are seen in part, and scores that jumped: with the row maximum. A warp's rows are few
+          // tokens, so of a partly seen tile's four groups of 32 keys all but one or two are seen by all of its rows or by none;
+          // those that none sees are zeros without an exponential, and only the mixed ones are masked.
+          uint32_t s[4][32];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, s[q]);
+          uint32_t none = 0;      // bit q: group q is seen by no row of the warp
+          if (!full) {
+            uint32_t seen[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              seen[q] = visible_bits(key0 + q * 32, lo, hi, sink_end);
+              if (!__any_sync(0xffffffffu, seen[q] != 0u)) none |= 1u << q;
+            }
+            tc_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (!(none >> q & 1) && !__all_sync(0xffffffffu, seen[q] == 0xffffffffu)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!(seen[q] & (1u << i))) s[q][i] = 0xff800000u;  // -inf
+              }
+          } else {
+            tc_wait_ld();
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (!(none >> q & 1)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[q][i]));
+            }
+          const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
+          const bool grow = m_new > m + 8.f;       // raised only when it would grow by more than 2^8: P stays below 256
+          float alpha = 1.f;
+          if (grow) {
+            alpha = ex2f(m - m_new);
+            m = m_new;
+            l *= alpha;
+          }
+          if (t > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t o[32];
+              tmem_ld32(tO + q * 32, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st32(tO + q * 32, o);
+            }
+          }
+          const float moff = (m == -INFINITY) ? 0.f : m;
+          const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-moff, -moff);
+          uint64_t sum = f32x2(0.f, 0.f);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[16];
+            if (none >> q & 1) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = 0u;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float x0, x1;
+                f32x2_get(fma2(f32x2(__uint_as_float(s[q][2 * i]), __uint_as_float(s[q][2 * i + 1])), c2, nm2), x0, x1);
+                const float e0 = ex2f(x0), e1 = ex2f(x1);
+                sum = add2(sum, f32x2(e0, e1));
+                pk[i] = IS_BF16 ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1);
+              }
+            }
+            tmem_st16(tS + q * 16, pk);
+          }
+          float sum0, sum1;
+          f32x2_get(sum, sum0, sum1);
+          l += sum0 + sum1;
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[WFB_P_FULL + wg]);
+      }
+      // ------------------------------- epilogue -------------------------------
+      if (alive && t > 0) alive = mbar_wait(&bars[WFB_O_DONE + wg], done_items & 1, abort_flag, p.status, WF_CODE(wg, WFB_O_DONE));
+      alive = __all_sync(0xffffffffu, alive);
+      tc_fence_after();
+      if (alive) {
+        uint32_t o[4][32];
+        uint64_t sum2[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint32_t pk[16];
-          if (none >> q & 1) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = 0u;
+          if (t > 0) {
+            tmem_ld32(tO + q * 32, o[q]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float x0, x1;
-              f32x2_get(fma2(f32x2(__uint_as_float(s[q][2 * i]), __uint_as_float(s[q][2 * i + 1])), c2, nm2), x0, x1);
-              const float e0 = ex2f(x0), e1 = ex2f(x1);
-              sum = add2(sum, f32x2(e0, e1));
-              pk[i] = IS_BF16 ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1);
-            }
+            for (int i = 0; i < 32; ++i) o[q][i] = 0u;
           }
-          tmem_st16(tS + q * 16, pk);
         }
-        float sum0, sum1;
-        f32x2_get(sum, sum0, sum1);
-        l += sum0 + sum1;
-      }
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[WFB_P_FULL + wg]);
-    }
-    // ------------------------------- epilogue -------------------------------
-    if (alive && t > 0) alive = mbar_wait(&bars[WFB_O_DONE + wg], done_items & 1, abort_flag, p.status, WF_CODE(wg, WFB_O_DONE));
-    alive = __all_sync(0xffffffffu, alive);
-    tc_fence_after();
-    if (alive) {
-      uint32_t o[4][32];
-      uint64_t sum2[4];
+        tc_wait_ld();
+        tc_fence_before();
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (t > 0) {
-          tmem_ld32(tO + q * 32, o[q]);
+        for (int q = 0; q < 4; ++q) {
+          sum2[q] = 0ull;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum2[q] = add2(sum2[q], f32x2(__uint_as_float(o[q][2 * i]), __uint_as_float(o[q][2 * i + 1])));
+        }
+        float sum_a, sum_b;
+        f32x2_get(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_a, sum_b);
+        const bool again = exists && isnan(sum_a + sum_b) && l < INFINITY;
+        // The warp's rows go through shared memory, 128 bytes of each at a time (16-byte pieces, rotated by row against bank
+        // conflicts), so that a store covers whole sectors: written by row they are 32 pieces of 16 bytes, 256 bytes apart.
+        const int row = head * p.sq + tok;         // of the slab
+        const unsigned here = __ballot_sync(0xffffffffu, exists);
+        uint8_t* out = smem + WF_OFF_OUT + warp * 4096;
+        const bool direct = p.o != nullptr;
+        const size_t slab_rows = size_t(p.g) * p.sq;
+        uint8_t* base;
+        int row_bytes;
+        if (direct) {
+          base = static_cast<uint8_t*>(p.o) + size_t(I.slab) * slab_rows * 256;
+          row_bytes = 256;
+        } else {
+          base = reinterpret_cast<uint8_t*>(p.o_part) + (size_t(I.slab) * p.nsplit + (PAIR ? 2 * I.split + wg : I.split)) * slab_rows * 512;
+          row_bytes = 512;
+        }
+        auto store = [&](int at) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = i * 4 + (lane >> 3), piece = lane & 7;
+            const int to = __shfl_sync(0xffffffffu, row, rr);
+            if (here >> rr & 1)
+              *reinterpret_cast<uint4*>(base + size_t(to) * row_bytes + at + piece * 16) =
+                  *reinterpret_cast<const uint4*>(out + rr * 128 + ((piece ^ (rr & 7)) << 4));
+          }
+          __syncwarp();
+        };
+        if (direct) {
+          const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w4[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = __uint_as_float(o[q][8 * i + 2 * e]) * inv, y = __uint_as_float(o[q][8 * i + 2 * e + 1]) * inv;
+                w4[e] = IS_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+              }
+              *reinterpret_cast<uint4*>(out + lane * 128 + ((((q & 1) * 4 + i) ^ (lane & 7)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+            }
+            if (q & 1) store((q >> 1) * 128);
+          }
+          if (exists) p.lse[size_t(I.slab) * slab_rows + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[q][i] = 0u;
-        }
-      }
-      tc_wait_ld();
-      tc_fence_before();
+          for (int q = 0; q < 4; ++q) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        sum2[q] = 0ull;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum2[q] = add2(sum2[q], f32x2(__uint_as_float(o[q][2 * i]), __uint_as_float(o[q][2 * i + 1])));
-      }
-      float sum_a, sum_b;
-      f32x2_get(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_a, sum_b);
-      const bool again = exists && isnan(sum_a + sum_b) && l < INFINITY;
-      // The warp's rows go through shared memory, 128 bytes of each at a time (16-byte pieces, rotated by row against bank
-      // conflicts), so that a store covers whole sectors: written by row they are 32 pieces of 16 bytes, 256 bytes apart.
-      const int row = head * p.sq + tok;         // of the slab
-      const unsigned here = __ballot_sync(0xffffffffu, exists);
-      uint8_t* out = smem + WF_OFF_OUT + warp * 4096;
-      const bool direct = p.o != nullptr;
-      const size_t slab_rows = size_t(p.g) * p.sq;
-      uint8_t* base;
-      int row_bytes;
-      if (direct) {
-        base = static_cast<uint8_t*>(p.o) + size_t(I.slab) * slab_rows * 256;
-        row_bytes = 256;
-      } else {
-        base = reinterpret_cast<uint8_t*>(p.o_part) + (size_t(I.slab) * p.nsplit + (PAIR ? 2 * I.split + wg : I.split)) * slab_rows * 512;
-        row_bytes = 512;
-      }
-      auto store = [&](int at) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int rr = i * 4 + (lane >> 3), piece = lane & 7;
-          const int to = __shfl_sync(0xffffffffu, row, rr);
-          if (here >> rr & 1)
-            *reinterpret_cast<uint4*>(base + size_t(to) * row_bytes + at + piece * 16) =
-                *reinterpret_cast<const uint4*>(out + rr * 128 + ((piece ^ (rr & 7)) << 4));
-        }
-        __syncwarp();
-      };
-      if (direct) {
-        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w4[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = __uint_as_float(o[q][8 * i + 2 * e]) * inv, y = __uint_as_float(o[q][8 * i + 2 * e + 1]) * inv;
-              w4[e] = IS_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
-            }
-            *reinterpret_cast<uint4*>(out + lane * 128 + ((((q & 1) * 4 + i) ^ (lane & 7)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[q][4 * i], o[q][4 * i + 1], o[q][4 * i + 2], o[q][4 * i + 3]);
+            store(q * 128);
           }
-          if (q & 1) store((q >> 1) * 128);
+          if (exists) {
+            float2* ml = reinterpret_cast<float2*>(p.ml_part) + size_t(I.slab) * p.nsplit * slab_rows + row;
+            ml[(PAIR ? 2 * I.split + wg : I.split) * slab_rows] = make_float2(m, l);
+            if (I.last)      // the partial results that no CTA makes
+              for (int k = PAIR ? 2 * I.split + 2 + wg : I.split + 1; k < p.nsplit; k += STEP) ml[k * slab_rows] = make_float2(-INFINITY, 0.f);
+          }
         }
-        if (exists) p.lse[size_t(I.slab) * slab_rows + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[q][4 * i], o[q][4 * i + 1], o[q][4 * i + 2], o[q][4 * i + 3]);
-          store(q * 128);
+        if (again) {
+          const int batch = I.slab / p.hkv, kvh = I.slab % p.hkv;
+          PlainRow x;
+          x.q = p.q + batch * p.q_b + (kvh * p.g + head) * p.q_h + tok * p.q_s;
+          x.k = p.k + batch * p.k_b + kvh * p.k_h;
+          x.v = p.v + batch * p.v_b + kvh * p.v_h;
+          x.out16 = direct ? reinterpret_cast<uint16_t*>(base + size_t(row) * 256) : nullptr;
+          x.out = reinterpret_cast<float*>(base + size_t(row) * 512);
+          x.first = first;
+          x.step = STEP;
+          x.n = I.n;
+          x.j0 = I.j0;
+          x.lo = lo;
+          x.hi = hi;
+          x.sink_end = sink_end;
+          x.m = m == -INFINITY ? 0.f : m;
+          x.l = l;
+          window_plain_row<IS_BF16>(p, I.kt, x);
         }
-        if (exists) {
-          float2* ml = reinterpret_cast<float2*>(p.ml_part) + size_t(I.slab) * p.nsplit * slab_rows + row;
-          ml[(PAIR ? 2 * I.split + wg : I.split) * slab_rows] = make_float2(m, l);
-          if (I.last)      // the partial results that no CTA makes
-            for (int k = PAIR ? 2 * I.split + 2 + wg : I.split + 1; k < p.nsplit; k += STEP) ml[k * slab_rows] = make_float2(-INFINITY, 0.f);
-        }
+        __syncwarp();
       }
-      if (again) {
-        const int batch = I.slab / p.hkv, kvh = I.slab % p.hkv;
-        PlainRow x;
-        x.q = p.q + batch * p.q_b + (kvh * p.g + head) * p.q_h + tok * p.q_s;
-        x.k = p.k + batch * p.k_b + kvh * p.k_h;
-        x.v = p.v + batch * p.v_b + kvh * p.v_h;
-        x.out16 = direct ? reinterpret_cast<uint16_t*>(base + size_t(row) * 256) : nullptr;
-        x.out = reinterpret_cast<float*>(base + size_t(row) * 512);
-        x.first = first;
-        x.step = STEP;
-        x.n = I.n;
-        x.j0 = I.j0;
-        x.lo = lo;
-        x.hi = hi;
-        x.sink_end = sink_end;
-        x.m = m == -INFINITY ? 0.f : m;
-        x.l = l;
-        window_plain_row<IS_BF16>(p, I.kt, x);
-      }
-      __syncwarp();
-    }
-    done_items += t > 0;
-    t0 += t;
+      done_items += t > 0;
+      t0 += t;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
@@ -542,142 +542,142 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     }
     if (warp == 9 && !poisoned) {
-    // =========================== MMA issuer (the whole warp walks, one elected lane issues) ===========================
-    constexpr uint32_t FMT = IS_BF16 ? UMMA_BF16 : UMMA_F16;
-    constexpr uint32_t IDESC_QK = umma_idesc(FMT, UMMA_K_MAJOR, UMMA_K_MAJOR, 128, 128);
-    constexpr uint32_t IDESC_PV = umma_idesc(FMT, UMMA_K_MAJOR, UMMA_MN_MAJOR, 128, 128);
-    constexpr uint32_t HI = umma_desc_hi(1024);
-    const uint32_t sQ = smem_u32(smem), sK = smem_u32(smem + WF_OFF_K), sV = smem_u32(smem + WF_OFF_V);
-    auto issue_qk = [&](int i, int stage) {
-      const uint32_t a_lo = umma_desc_lo(sQ + (PAIR ? 0 : i * WF_TILE), 16);
-      const uint32_t b_lo = umma_desc_lo(sK + stage * WF_TILE, 16);
-      if (elect_one()) {
+      // =========================== MMA issuer (the whole warp walks, one elected lane issues) ===========================
+      constexpr uint32_t FMT = IS_BF16 ? UMMA_BF16 : UMMA_F16;
+      constexpr uint32_t IDESC_QK = umma_idesc(FMT, UMMA_K_MAJOR, UMMA_K_MAJOR, 128, 128);
+      constexpr uint32_t IDESC_PV = umma_idesc(FMT, UMMA_K_MAJOR, UMMA_MN_MAJOR, 128, 128);
+      constexpr uint32_t HI = umma_desc_hi(1024);
+      const uint32_t sQ = smem_u32(smem), sK = smem_u32(smem + WF_OFF_K), sV = smem_u32(smem + WF_OFF_V);
+      auto issue_qk = [&](int i, int stage) {
+        const uint32_t a_lo = umma_desc_lo(sQ + (PAIR ? 0 : i * WF_TILE), 16);
+        const uint32_t b_lo = umma_desc_lo(sK + stage * WF_TILE, 16);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint32_t off = ((kk >> 2) * WF_HALF + (kk & 3) * 32) >> 4;
-          umma_ss_f16(tmem_base + i * 128, umma_desc_join(a_lo + off, HI), umma_desc_join(b_lo + off, HI), IDESC_QK, kk > 0);
-        }
-      }
-      __syncwarp();
-    };
-    auto issue_pv = [&](int i, int stage, bool first) {
-      const uint32_t b_lo = umma_desc_lo(sV + stage * WF_TILE, WF_HALF);
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_ts_f16(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, umma_desc_join(b_lo + ((kk * 2048) >> 4), HI),
-                      IDESC_PV, (!first) || kk > 0);
-      }
-      __syncwarp();
-    };
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) tc_commit(bar);
-      __syncwarp();
-    };
-    auto wait = [&](int bar, uint32_t ph) {
-      return __all_sync(0xffffffffu, mbar_wait(&bars[bar], ph, abort_flag, p.status, WF_CODE(3, bar)));
-    };
-    bool ok = true;
-    int it = 0, jj0 = 0, t0[2] = {0, 0};      // t0: tiles of each warpgroup done
-    for (int round = 0, w; ok && (w = index_of(round)) < p.nitems; ++round) {
-      const Item I = item_of(w);
-      const int n = I.n;
-      if (n == 0) continue;
-      auto k_full = [&](int j) { return wait(WFB_K_FULL + (jj0 + j) % WF_NS, (jj0 + j) / WF_NS & 1); };
-      auto v_full = [&](int j) { return wait(WFB_V_FULL + (jj0 + j) % WF_NS, (jj0 + j) / WF_NS & 1); };
-      auto stage = [&](int j) { return (jj0 + j) % WF_NS; };
-      // rows of V behind the last valid key: whatever they hold is multiplied with zeros
-      auto clear_v = [&](int j) {
-        const int left = I.valid - I.kt.tile(I.j0 + j) * 128;
-        if (left >= 128) return;
-        for (int at = lane; at < (128 - left) * 16; at += 32)
-          *reinterpret_cast<uint4*>(smem + WF_OFF_V + stage(j) * WF_TILE + ((at >> 3) & 1) * WF_HALF + (left + (at >> 4)) * 128 +
-                                    (at & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-        fence_async_smem();
-        __syncwarp();
-      };
-      // the item's first scores: S is free (the tensor pipe runs in order behind the last product with P)
-      ok = wait(WFB_Q_FULL, it & 1) && k_full(0);
-      if constexpr (PAIR) {
-        // tile j is warpgroup j % 2's; its scores come two tiles ahead
-        for (int j = 0; ok && j < min(n, 2); ++j) {
-          if (j > 0) ok = k_full(j);
-          if (!ok) break;
-          tc_fence_after();
-          issue_qk(j, stage(j));
-          commit(&bars[WFB_S_FULL + j]);
-          commit(&bars[WFB_K_EMPTY + stage(j)]);
-          if (j == n - 1) commit(&bars[WFB_Q_EMPTY]);
-        }
-        for (int j = 0; ok && j < n; ++j) {
-          const int i = j & 1;
-          ok = wait(WFB_P_FULL + i, (t0[i] + (j >> 1)) & 1) && v_full(j);
-          if (!ok) break;
-          clear_v(j);
-          tc_fence_after();
-          issue_pv(i, stage(j), j < 2);
-          commit(&bars[WFB_V_EMPTY + stage(j)]);
-          if (j + 2 < n) {
-            ok = k_full(j + 2);
-            if (!ok) break;
-            tc_fence_after();
-            issue_qk(i, stage(j + 2));
-            commit(&bars[WFB_S_FULL + i]);
-            commit(&bars[WFB_K_EMPTY + stage(j + 2)]);
-            if (j + 2 == n - 1) commit(&bars[WFB_Q_EMPTY]);
-          } else {
-            commit(&bars[WFB_O_DONE + i]);
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = ((kk >> 2) * WF_HALF + (kk & 3) * 32) >> 4;
+            umma_ss_f16(tmem_base + i * 128, umma_desc_join(a_lo + off, HI), umma_desc_join(b_lo + off, HI), IDESC_QK, kk > 0);
           }
         }
-        t0[0] += (n + 1) / 2;
-        t0[1] += n / 2;
-      } else {
-        if (ok) {
-          tc_fence_after();
-          issue_qk(0, stage(0));
-          commit(&bars[WFB_S_FULL + 0]);
-          issue_qk(1, stage(0));
-          commit(&bars[WFB_S_FULL + 1]);
-          commit(&bars[WFB_K_EMPTY + stage(0)]);
-          if (n == 1) commit(&bars[WFB_Q_EMPTY]);
-        }
-        for (int j = 0; ok && j < n; ++j) {
+        __syncwarp();
+      };
+      auto issue_pv = [&](int i, int stage, bool first) {
+        const uint32_t b_lo = umma_desc_lo(sV + stage * WF_TILE, WF_HALF);
+        if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (!ok) break;
-            ok = wait(WFB_P_FULL + i, (jj0 + j) & 1);
-            if (ok && i == 0) {
-              ok = v_full(j);
-              if (ok) clear_v(j);
-            }
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ts_f16(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, umma_desc_join(b_lo + ((kk * 2048) >> 4), HI),
+                        IDESC_PV, (!first) || kk > 0);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
+      };
+      auto wait = [&](int bar, uint32_t ph) {
+        return __all_sync(0xffffffffu, mbar_wait(&bars[bar], ph, abort_flag, p.status, WF_CODE(3, bar)));
+      };
+      bool ok = true;
+      int it = 0, jj0 = 0, t0[2] = {0, 0};      // t0: tiles of each warpgroup done
+      for (int round = 0, w; ok && (w = index_of(round)) < p.nitems; ++round) {
+        const Item I = item_of(w);
+        const int n = I.n;
+        if (n == 0) continue;
+        auto k_full = [&](int j) { return wait(WFB_K_FULL + (jj0 + j) % WF_NS, (jj0 + j) / WF_NS & 1); };
+        auto v_full = [&](int j) { return wait(WFB_V_FULL + (jj0 + j) % WF_NS, (jj0 + j) / WF_NS & 1); };
+        auto stage = [&](int j) { return (jj0 + j) % WF_NS; };
+        // rows of V behind the last valid key: whatever they hold is multiplied with zeros
+        auto clear_v = [&](int j) {
+          const int left = I.valid - I.kt.tile(I.j0 + j) * 128;
+          if (left >= 128) return;
+          for (int at = lane; at < (128 - left) * 16; at += 32)
+            *reinterpret_cast<uint4*>(smem + WF_OFF_V + stage(j) * WF_TILE + ((at >> 3) & 1) * WF_HALF + (left + (at >> 4)) * 128 +
+                                      (at & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_async_smem();
+          __syncwarp();
+        };
+        // the item's first scores: S is free (the tensor pipe runs in order behind the last product with P)
+        ok = wait(WFB_Q_FULL, it & 1) && k_full(0);
+        if constexpr (PAIR) {
+          // tile j is warpgroup j % 2's; its scores come two tiles ahead
+          for (int j = 0; ok && j < min(n, 2); ++j) {
+            if (j > 0) ok = k_full(j);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(i, stage(j), j == 0);
-            if (i == 1) commit(&bars[WFB_V_EMPTY + stage(j)]);
-            if (j + 1 < n) {
-              if (i == 0) ok = k_full(j + 1);
+            issue_qk(j, stage(j));
+            commit(&bars[WFB_S_FULL + j]);
+            commit(&bars[WFB_K_EMPTY + stage(j)]);
+            if (j == n - 1) commit(&bars[WFB_Q_EMPTY]);
+          }
+          for (int j = 0; ok && j < n; ++j) {
+            const int i = j & 1;
+            ok = wait(WFB_P_FULL + i, (t0[i] + (j >> 1)) & 1) && v_full(j);
+            if (!ok) break;
+            clear_v(j);
+            tc_fence_after();
+            issue_pv(i, stage(j), j < 2);
+            commit(&bars[WFB_V_EMPTY + stage(j)]);
+            if (j + 2 < n) {
+              ok = k_full(j + 2);
               if (!ok) break;
               tc_fence_after();
-              issue_qk(i, stage(j + 1));
+              issue_qk(i, stage(j + 2));
               commit(&bars[WFB_S_FULL + i]);
-              if (i == 1) {
-                commit(&bars[WFB_K_EMPTY + stage(j + 1)]);
-                if (j + 1 == n - 1) commit(&bars[WFB_Q_EMPTY]);
-              }
+              commit(&bars[WFB_K_EMPTY + stage(j + 2)]);
+              if (j + 2 == n - 1) commit(&bars[WFB_Q_EMPTY]);
             } else {
               commit(&bars[WFB_O_DONE + i]);
             }
           }
+          t0[0] += (n + 1) / 2;
+          t0[1] += n / 2;
+        } else {
+          if (ok) {
+            tc_fence_after();
+            issue_qk(0, stage(0));
+            commit(&bars[WFB_S_FULL + 0]);
+            issue_qk(1, stage(0));
+            commit(&bars[WFB_S_FULL + 1]);
+            commit(&bars[WFB_K_EMPTY + stage(0)]);
+            if (n == 1) commit(&bars[WFB_Q_EMPTY]);
+          }
+          for (int j = 0; ok && j < n; ++j) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (!ok) break;
+              ok = wait(WFB_P_FULL + i, (jj0 + j) & 1);
+              if (ok && i == 0) {
+                ok = v_full(j);
+                if (ok) clear_v(j);
+              }
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(i, stage(j), j == 0);
+              if (i == 1) commit(&bars[WFB_V_EMPTY + stage(j)]);
+              if (j + 1 < n) {
+                if (i == 0) ok = k_full(j + 1);
+                if (!ok) break;
+                tc_fence_after();
+                issue_qk(i, stage(j + 1));
+                commit(&bars[WFB_S_FULL + i]);
+                if (i == 1) {
+                  commit(&bars[WFB_K_EMPTY + stage(j + 1)]);
+                  if (j + 1 == n - 1) commit(&bars[WFB_Q_EMPTY]);
+                }
+              } else {
+                commit(&bars[WFB_O_DONE + i]);
+              }
+            }
+          }
         }
+        ++it;
+        jj0 += n;
       }
-      ++it;
-      jj0 += n;
-    }
-    if (!ok) {      // wind down: let every MMA already issued finish before TMEM is released
-      commit(&bars[WFB_DRAIN]);
-      const long long t0 = clock64();
-      while (!mbar_try_wait(&bars[WFB_DRAIN], 0) && clock64() - t0 < LVX_SPIN_LIMIT_CYCLES) {}
-    }
+      if (!ok) {      // wind down: let every MMA already issued finish before TMEM is released
+        commit(&bars[WFB_DRAIN]);
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&bars[WFB_DRAIN], 0) && clock64() - t0 < LVX_SPIN_LIMIT_CYCLES) {}
+      }
     }
   }
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 
@@ -24,7 +25,8 @@ def on_device(t):
 
 
 def watch_status(t):
-    """Start of a call: raises if a kernel of an earlier call gave up on a bounded wait (see peer_memory.StatusWatch)."""
+    """Start of a call, with t's device current: raises if a kernel of an earlier call gave up on a bounded wait (see
+    peer_memory.StatusWatch)."""
     from .peer_memory import status_watch
     status_watch.watch(t.device.index)
 
@@ -87,6 +89,7 @@ class HeadNormRopeFunc(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, cos, sin = ctx.saved_tensors
         want = list(ctx.needs_input_grad[:4])
@@ -115,9 +118,9 @@ def head_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1
     _check(q, k, q_weight, k_weight, cos, sin, eps)
     q_weight, k_weight, cos, sin = (_rows(t) for t in (q_weight, k_weight, cos, sin))
     like = q if q is not None else k
-    watch_status(like)
     args = (q, k, q_weight, k_weight, cos, sin, float(eps))
     with on_device(like):
+        watch_status(like)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
             return HeadNormRopeFunc.apply(*args)
         return ops.head_norm_rope(*args)

@@ -9,6 +9,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from .rotary import on_device, watch_status
@@ -75,6 +76,7 @@ class WindowAttentionFunc(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do, _):
         if do is None:
             return (None,) * 8
@@ -110,8 +112,8 @@ def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=
     if k_shape[0] != q_shape[0]:
         raise ValueError(f"{who}: q has {q_shape[0]} batch entries, k and v {k_shape[0]}")
     device = _check_devices(who, q, k, v)
-    watch_status(q)
     with on_device(q):
+        watch_status(q)
         lengths = ops.device_lengths(kv_valid_len, q_shape[0], k_shape[2], device)
         args = (q, k, v, sm_scale, 0 if window is None or window >= _MOST else int(window), min(int(sinks), _MOST),
                 -1 if query_start is None else int(query_start), lengths)
@@ -135,6 +137,7 @@ class SharedPrefixAttentionFunc(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do, _):
         if do is None:
             return (None,) * 8
@@ -176,8 +179,8 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k=None, v=None, sm_scale=None
         if b != B or heads != k_prefix.shape[1]:
             raise ValueError(f"{who}: own keys {tuple(k.shape)} for {B} requests and {k_prefix.shape[1]} KV heads")
         device = _check_devices(who, q, k_prefix, v_prefix, k, v)
-    watch_status(q)
     with on_device(q):
+        watch_status(q)
         args = (q, k_prefix, v_prefix, k, v, sm_scale, ops.device_lengths(prefix_valid_len, P, N, device),
                 ops.device_lengths(kv_valid_len, B, own, device))
         if torch.is_grad_enabled() and (q.requires_grad or k_prefix.requires_grad or v_prefix.requires_grad

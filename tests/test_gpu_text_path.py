@@ -151,3 +151,72 @@ def test_windowed_self_attention_hook(cuda_device):
     assert rel(xb.grad, xr.grad) <= 3e-2, rel(xb.grad, xr.grad)
     for (n, p), (_, pr) in zip(mod.named_parameters(), ref_mod.named_parameters()):
         assert p.grad is not None and rel(p.grad, pr.grad) <= 3e-2, (n, rel(p.grad, pr.grad))
+
+
+def test_two_threads_on_two_streams(cuda_device):
+    """Calls that two threads launch at the same time, each on its own stream, give what they give one after the other (dQ up to
+    the order of its additions: one rounding)."""
+    import threading
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    r = lambda *s: torch.randn(*s, device=cuda_device, generator=g).bfloat16()
+    inputs = []
+    for S, N in ((150, 900), (77, 2500)):
+        inputs.append([r(2, S, 8, 128), r(2, S, 2, 128), r(128), r(128), r(2, 2, S, 128), r(1, 2, N, 128), r(1, 2, N, 128), r(2, 8, S, 128)])
+    cs = [t.float() for t in tables(torch.arange(200, device=cuda_device))]
+
+    def work(xq, xk, wq, wk, v, pk, pv, do):
+        S = xq.shape[1]
+        leaves = [t.detach().requires_grad_() for t in (xq, xk, wq, wk, v, pk, pv)]
+        q, k = lvx.head_norm_rope(*leaves[:4], cs[0][:S], cs[1][:S])
+        o = lvx.window_attention(q, k, leaves[4], window=40, sinks=4) + lvx.shared_prefix_attention(q, *leaves[5:], k, leaves[4])
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    alone = [work(*x) for x in inputs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(12):
+                got[i].append(work(*inputs[i]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 12
+        for outs in got[i]:
+            assert torch.equal(outs[0], alone[i][0])
+            # what dQ's order reaches: the queries' and their weight's gradients; two roundings of 2^-8 of the largest at most
+            for j, (a, b) in enumerate(zip(outs[1:], alone[i][1:])):
+                if j in (0, 2):
+                    assert (a.float() - b.float()).abs().max() <= 2.0 ** -6 * b.float().abs().max(), j
+                else:
+                    assert torch.equal(a, b), j
+
+
+def test_no_second_derivatives(cuda_device):
+    x = torch.randn(1, 8, 2, 128, device=cuda_device, requires_grad=True)
+    cs = [t.float() for t in tables(torch.arange(8, device=cuda_device))]
+    for out in (lvx.head_norm_rope(x, None, cos=cs[0], sin=cs[1])[0], lvx.window_attention(x, x, x, window=3),
+                lvx.shared_prefix_attention(x, x, x)):
+        (g,) = torch.autograd.grad((out * out).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
+def test_broadcast_gradients_and_unused_outputs(cuda_device):
+    """An upstream gradient of one repeated value (what .sum() gives), and a result whose log-sum-exp alone is used."""
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    x = torch.randn(1, 4, 70, 128, device=cuda_device, generator=g).bfloat16().requires_grad_()
+    for f in (lambda t: lvx.window_attention(t, t, t, window=9), lambda t: lvx.shared_prefix_attention(t, t, t, t, t),
+              lambda t: lvx.head_norm_rope(t, None, torch.ones(128, device=cuda_device))[0]):
+        (a,) = torch.autograd.grad(f(x).sum(), x)
+        out = f(x)
+        (b,) = torch.autograd.grad(out, x, torch.ones_like(out))
+        assert (a.float() - b.float()).abs().max() <= 2.0 ** -6 * b.float().abs().max()
+    _, lse = lvx.window_attention(x, x, x, window=9, return_lse=True)
+    assert not lse.requires_grad

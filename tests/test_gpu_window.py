@@ -239,3 +239,25 @@ def test_word_already_set(cuda_device):
             lib.lvx_p2p_set_timeout(120.0)
             _lib.device_status()
         assert torch.equal(lvx.window_attention(*leaves, window=64), good)
+
+
+@pytest.mark.parametrize("Sq", [1, 70])
+def test_offsets_past_32_bits(cuda_device, Sq):
+    """A cache of 2.2 million keys: 2^31 values lie before its last head. What is compared is that head, at its end."""
+    Skv, Hkv, window, sinks = 2_200_000, 8, 300, 4
+    q, small_k, small_v, do = inputs(cuda_device, 1, 2 * Hkv, Hkv, Sq, 1024, torch.bfloat16, 23)
+    k, v = (torch.zeros(1, Hkv, Skv, 128, device=cuda_device, dtype=torch.bfloat16) for _ in range(2))
+    for big, small in ((k, small_k), (v, small_v)):
+        big[:, :, :512], big[:, :, -512:] = small[:, :, :512], small[:, :, 512:]
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = lvx.window_attention(*leaves, SCALE, window=window, sinks=sinks)
+    grads = torch.autograd.grad(o, leaves, do)
+    seen = oracle.visible(1024, Sq, 1024, window, sinks, None).to(cuda_device)      # the keys between have no part in it
+    h, kv = 2 * Hkv - 1, Hkv - 1
+    parts = [oracle.masked_attention(q[0, i], small_k[0, kv], small_v[0, kv], seen, SCALE, do[0, i]) for i in (h - 1, h)]
+    oracle.check(o[0, h].detach(), *parts[1]["o"], "o")
+    oracle.check(grads[0][0, h], *parts[1]["dq"], "dq")
+    for name, got in zip(("dk", "dv"), grads[1:]):
+        ref, bar = (parts[0][name][i] + parts[1][name][i] for i in range(2))
+        oracle.check(torch.cat([got[0, kv, :512], got[0, kv, -512:]]), ref, bar, name)
+        assert not got[0, kv, 512:-512].any()
