@@ -3,17 +3,26 @@
 // Softmax(scale Q K^T) V over the keys that window.cuh describes, with the running maximum and sum of an online softmax.
 // A CTA owns two 128-row query tiles of one KV head (neighbours, so that both see nearly the same keys: the heads of a
 // group lie side by side in a tile, and with four heads two tiles span 64 tokens) and walks the key tiles that either of
-// them sees: those of the sinks, then those of the window. Only a tile that some row sees in part is masked; the others
-// take the path without a mask and without a row maximum. What lies outside costs nothing.
+// them sees: those of the sinks, then those of the window. Only a tile that some row sees in part is masked. What lies
+// outside costs nothing.
 //
-// The anatomy is that of the forward block (320 threads: two softmax warpgroups, thread = row = TMEM lane; a TMA
-// producer; a tcgen05 issuer that interleaves the two tiles, P overwriting S in TMEM), with its measured reasons: the
-// softmax is what a tile waits for, so that the two tiles take turns in the tensor core. What differs:
+// The anatomy is that of the forward block (two softmax warpgroups, thread = row = TMEM lane; a TMA producer; a tcgen05
+// issuer that interleaves the two tiles, P overwriting S in TMEM): scores, softmax and product with V of a tile follow one
+// another, so that a tile waits for its softmax and the two tiles take turns in the tensor core. What differs:
+//   * P is handed over in halves, the first while the second is made, and the reference maximum is settled before the
+//     exponentials (three-operand maxima: 64 instructions a row), so that no half has to be taken back. A tile pair then
+//     takes 3,390 cycles instead of 3,720 (2,048 of which the tensor core and the exponentials need each): 304 K rows on 4,096
+//     keys 540 -> 490 us, 1,300 TFLOP/s. A quarter of the exponentials as polynomials beside the others: no change;
+//   * the epilogue and the rescaling work through fewer columns at a time than fit the registers of a loop of their own: what
+//     does not spill around the tile loop, and a shorter way through the instruction cache, is worth more (the same rows with
+//     a window of 9.4 tiles: 203 us before, 190 with halves, 178 without the spills, 174 with the short epilogue);
+//   * CTAs are persistent, and the producer fetches the next item's Q and keys while the last softmax of this one runs;
 //   * tiles come through tensor maps of rank 5 and 4, so that q, k and v may have any strides (a cache of more rows
 //     than are valid, the projections' [B, S, H, 128]);
 //   * key ranges are short, so that a CTA normally sees all of its keys and writes O (rounded once) and lse itself;
 //     only where the tiles do not fill the GPU are they split, and the combine kernel merges the parts;
-//   * CTAs with the latest queries, which see the most keys, are started first;
+//   * the items with the latest queries, which see the most keys, come first, and CTAs walk the list forwards and backwards
+//     in turn;
 //   * what lies behind the last valid key may hold anything: scores are replaced, and the rows of V that the last valid
 //     tile shares with it are cleared before they are multiplied with a probability of zero. A key inside that a row
 //     does not see, but another row of the tile does, may hold an infinity or a NaN too: such a row ends with NaN
@@ -41,9 +50,9 @@ constexpr int WF_THREADS = 384;
 static_assert(WF_SMEM <= 232448, "shared memory budget");
 // PAIR from this many key tiles on. us a call, one warpgroup per query tile -> PAIR, 32 tokens of 32 heads on 8 KV heads, over
 // 512 / 2,048 / 4,096 / 16,384 keys, combine kernel included where there is one:
-//    1 entry      15.7 ->  17.5    16.7 -> 18.9    19.2 ->  19.7     31 ->  27
-//    8 entries    15.9 ->  20.4    30.7 -> 32.3    47.4 ->  42.0    139 -> 103
-//   32 entries    40.5 ->  58.5     101 ->   98     161 ->   142    547 -> 402
+//    1 entry      15.0 -> 15.1    16.7 -> 16.7    19.0 -> 17.7     30 ->  25
+//    8 entries    15.5 -> 18.0    28.8 -> 29.5    44.8 -> 40.3    128 -> 107
+//   32 entries    28.6 -> 39.5      74 ->   78     140 ->  121    482 -> 370
 constexpr int kPairTiles = 32;
 
 enum {
@@ -55,7 +64,7 @@ enum {
   WFB_V_EMPTY = WFB_V_FULL + WF_NS,
   WFB_S_FULL = WFB_V_EMPTY + WF_NS,
   WFB_P_FULL = WFB_S_FULL + 2,
-  WFB_O_DONE = WFB_P_FULL + 2,
+  WFB_O_DONE = WFB_P_FULL + 4,
   WFB_DRAIN = WFB_O_DONE + 2,
   WFB_COUNT = WFB_DRAIN + 1
 };
@@ -77,6 +86,13 @@ struct WinFwdParams {
   long long q_b, q_h, q_s, k_b, k_h, k_s, v_b, v_h, v_s;
   int* status;
 };
+
+// (ignores NaN, like fmaxf)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // One row's O as plain fp32 sums over its keys in tiles j = first, first + step, ... < n of `kt` from j0 on, written where the
 // row belongs: in the input type and divided by l (`out16`), or as it is.
@@ -116,7 +132,7 @@ __device__ __noinline__ void window_plain_row(const WinFwdParams& p, const KeyTi
 template <bool IS_BF16, bool PAIR>
 __global__ void __launch_bounds__(WF_THREADS, 1)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const WinFwdParams p) {
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WinFwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WF_OFF_BAR);
@@ -195,7 +211,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[WFB_S_FULL + i], 1);
-      mbar_init(&bars[WFB_P_FULL + i], 4);      // one arrival per softmax warp
+      for (int h = 0; h < 2; ++h) mbar_init(&bars[WFB_P_FULL + 2 * i + h], 4);      // one arrival per softmax warp
       mbar_init(&bars[WFB_O_DONE + i], 1);
     }
     mbar_init(&bars[WFB_DRAIN], 1);
@@ -232,6 +248,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     // this warpgroup's key tiles: all of an item's, or every other one
     constexpr int STEP = PAIR ? 2 : 1;
     const int first = PAIR ? wg : 0;
+    auto hand_over = [&](int half) {      // of P, to the tensor core
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[WFB_P_FULL + 2 * wg + half]);
+    };
     bool alive = !poisoned;
     int done_items = 0, t0 = 0;      // items with tiles of this warpgroup, and those tiles
     for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
@@ -257,42 +279,46 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           break;
         }
         tc_fence_after();
-        // The usual tile: exponentials against the running maximum as it stands (it is only a reference point), P held in
-        // registers until the row sums are known to be small. (See fwd_sm100.cu for what each of these costs.)
+        // The usual tile: exponentials against the running maximum as it stands (it is only a reference point). The first half
+        // of P is handed to the tensor core while the second is made.
         bool done = false;
         if (t > 0 && full) {
-          uint32_t pk[2][32];
-          uint64_t sum_a = f32x2(0.f, 0.f), sum_b = f32x2(0.f, 0.f);
-          const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-m, -m);
-          auto chunk = [&](const uint32_t (&b)[32], uint32_t* out) {
+          uint32_t sv[4][32];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float x0, x1, x2, x3;
-              f32x2_get(fma2(f32x2(__uint_as_float(b[4 * i]), __uint_as_float(b[4 * i + 1])), c2, nm2), x0, x1);
-              f32x2_get(fma2(f32x2(__uint_as_float(b[4 * i + 2]), __uint_as_float(b[4 * i + 3])), c2, nm2), x2, x3);
-              const float e0 = ex2f(x0), e1 = ex2f(x1), e2 = ex2f(x2), e3 = ex2f(x3);
-              sum_a = add2(sum_a, f32x2(e0, e1));
-              sum_b = add2(sum_b, f32x2(e2, e3));
-              out[2 * i] = IS_BF16 ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1);
-              out[2 * i + 1] = IS_BF16 ? pack_bf16x2(e2, e3) : pack_f16x2(e2, e3);
+          for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, sv[q]);
+          tc_wait_ld();
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx[i & 3] = max3(mx[i & 3], __uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1]));
+          const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
+          if (!__any_sync(0xffffffffu, top > m + 8.f)) {
+            const float moff = m == -INFINITY ? 0.f : m;
+            uint64_t sum_a = f32x2(0.f, 0.f), sum_b = f32x2(0.f, 0.f);
+            const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-moff, -moff);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t pk[32];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const uint32_t* b = &sv[2 * h + i / 8][4 * (i % 8)];
+                float x0, x1, x2, x3;
+                f32x2_get(fma2(f32x2(__uint_as_float(b[0]), __uint_as_float(b[1])), c2, nm2), x0, x1);
+                f32x2_get(fma2(f32x2(__uint_as_float(b[2]), __uint_as_float(b[3])), c2, nm2), x2, x3);
+                const float e0 = ex2f(x0), e1 = ex2f(x1), e2 = ex2f(x2), e3 = ex2f(x3);
+                sum_a = add2(sum_a, f32x2(e0, e1));
+                sum_b = add2(sum_b, f32x2(e2, e3));
+                pk[2 * i] = IS_BF16 ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1);
+                pk[2 * i + 1] = IS_BF16 ? pack_bf16x2(e2, e3) : pack_f16x2(e2, e3);
+              }
+              tmem_st32(tS + h * 32, pk);
+              hand_over(h);
             }
-          };
-          {
-            uint32_t sv[4][32];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) tmem_ld32(tS + q * 32, sv[q]);
-            tc_wait_ld();
-#pragma unroll
-            for (int q = 0; q < 4; ++q) chunk(sv[q], &pk[0][0] + q * 16);
-          }
-          float s0, s1, s2, s3;
-          f32x2_get(sum_a, s0, s1);
-          f32x2_get(sum_b, s2, s3);
-          const float tile_sum = (s0 + s1) + (s2 + s3);
-          if (__all_sync(0xffffffffu, tile_sum <= 16384.f)) {      // bounds each P; false for infinities and NaN
-            tmem_st32(tS + 0, pk[0]);
-            tmem_st32(tS + 32, pk[1]);
-            l += tile_sum;
+            float s0, s1, s2, s3;
+            f32x2_get(sum_a, s0, s1);
+            f32x2_get(sum_b, s2, s3);
+            l += (s0 + s1) + (s2 + s3);
             done = true;
           }
         }
@@ -327,7 +353,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int q = 0; q < 4; ++q)
             if (!(none >> q & 1)) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[q][i]));
+              for (int i = 0; i < 16; ++i) mx[i & 3] = max3(mx[i & 3], __uint_as_float(s[q][2 * i]), __uint_as_float(s[q][2 * i + 1]));
             }
           const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
           const bool grow = m_new > m + 8.f;       // raised only when it would grow by more than 2^8: P stays below 256
@@ -339,13 +365,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           if (t > 0 && __any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t o[32];
-              tmem_ld32(tO + q * 32, o);
+            for (int q = 0; q < 8; ++q) {      // (32 columns at a time do not fit beside the scores)
+              uint32_t o[16];
+              tmem_ld16(tO + q * 16, o);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st32(tO + q * 32, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(tO + q * 16, o);
             }
           }
           const float moff = (m == -INFINITY) ? 0.f : m;
@@ -368,43 +394,19 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               }
             }
             tmem_st16(tS + q * 16, pk);
+            if (q == 1) hand_over(0);
           }
           float sum0, sum1;
           f32x2_get(sum, sum0, sum1);
           l += sum0 + sum1;
+          hand_over(1);
         }
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[WFB_P_FULL + wg]);
       }
       // ------------------------------- epilogue -------------------------------
       if (alive && t > 0) alive = mbar_wait(&bars[WFB_O_DONE + wg], done_items & 1, abort_flag, p.status, WF_CODE(wg, WFB_O_DONE));
       alive = __all_sync(0xffffffffu, alive);
       tc_fence_after();
       if (alive) {
-        uint32_t o[4][32];
-        uint64_t sum2[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (t > 0) {
-            tmem_ld32(tO + q * 32, o[q]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[q][i] = 0u;
-          }
-        }
-        tc_wait_ld();
-        tc_fence_before();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          sum2[q] = 0ull;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sum2[q] = add2(sum2[q], f32x2(__uint_as_float(o[q][2 * i]), __uint_as_float(o[q][2 * i + 1])));
-        }
-        float sum_a, sum_b;
-        f32x2_get(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_a, sum_b);
-        const bool again = exists && isnan(sum_a + sum_b) && l < INFINITY;
         // The warp's rows go through shared memory, 128 bytes of each at a time (16-byte pieces, rotated by row against bank
         // conflicts), so that a store covers whole sectors: written by row they are 32 pieces of 16 bytes, 256 bytes apart.
         const int row = head * p.sq + tok;         // of the slab
@@ -433,29 +435,54 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           __syncwarp();
         };
+        auto load = [&](int col, uint32_t (&o)[32]) {
+          if (t > 0) {
+            tmem_ld32(tO + col, o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+        };
+        uint64_t sum2 = 0ull;
+        auto bad = [&](const uint32_t (&o)[32]) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum2 = add2(sum2, f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
+        };
         if (direct) {
           const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t o[2][32];
+            load(h * 64, o[0]);
+            load(h * 64 + 32, o[1]);
+            tc_wait_ld();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 2; ++q) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t w4[4];
+              for (int i = 0; i < 4; ++i) {
+                uint32_t w4[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = __uint_as_float(o[q][8 * i + 2 * e]) * inv, y = __uint_as_float(o[q][8 * i + 2 * e + 1]) * inv;
-                w4[e] = IS_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                for (int e = 0; e < 4; ++e) {
+                  const float x = __uint_as_float(o[q][8 * i + 2 * e]) * inv, y = __uint_as_float(o[q][8 * i + 2 * e + 1]) * inv;
+                  w4[e] = IS_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                }
+                *reinterpret_cast<uint4*>(out + lane * 128 + (((q * 4 + i) ^ (lane & 7)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
               }
-              *reinterpret_cast<uint4*>(out + lane * 128 + ((((q & 1) * 4 + i) ^ (lane & 7)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+              bad(o[q]);
             }
-            if (q & 1) store((q >> 1) * 128);
+            store(h * 128);
           }
           if (exists) p.lse[size_t(I.slab) * slab_rows + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         } else {
-#pragma unroll
+#pragma unroll 1
           for (int q = 0; q < 4; ++q) {
+            uint32_t o[32];
+            load(q * 32, o);
+            tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[q][4 * i], o[q][4 * i + 1], o[q][4 * i + 2], o[q][4 * i + 3]);
+              *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            bad(o);
             store(q * 128);
           }
           if (exists) {
@@ -465,7 +492,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               for (int k = PAIR ? 2 * I.split + 2 + wg : I.split + 1; k < p.nsplit; k += STEP) ml[k * slab_rows] = make_float2(-INFINITY, 0.f);
           }
         }
-        if (again) {
+        tc_fence_before();
+        float sum_a, sum_b;
+        f32x2_get(sum2, sum_a, sum_b);
+        if (exists && isnan(sum_a + sum_b) && l < INFINITY) {
           const int batch = I.slab / p.hkv, kvh = I.slab % p.hkv;
           PlainRow x;
           x.q = p.q + batch * p.q_b + (kvh * p.g + head) * p.q_h + tok * p.q_s;
@@ -482,7 +512,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           x.sink_end = sink_end;
           x.m = m == -INFINITY ? 0.f : m;
           x.l = l;
-          window_plain_row<IS_BF16>(p, I.kt, x);
+          const KeyTiles kt = I.kt;
+          window_plain_row<IS_BF16>(p, kt, x);
         }
         __syncwarp();
       }
@@ -560,11 +591,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         __syncwarp();
       };
-      auto issue_pv = [&](int i, int stage, bool first) {
+      auto issue_pv = [&](int i, int stage, int h, bool first) {
         const uint32_t b_lo = umma_desc_lo(sV + stage * WF_TILE, WF_HALF);
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
+          for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
             umma_ts_f16(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, umma_desc_join(b_lo + ((kk * 2048) >> 4), HI),
                         IDESC_PV, (!first) || kk > 0);
         }
@@ -611,11 +642,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           for (int j = 0; ok && j < n; ++j) {
             const int i = j & 1;
-            ok = wait(WFB_P_FULL + i, (t0[i] + (j >> 1)) & 1) && v_full(j);
+            ok = v_full(j);
+            if (ok) clear_v(j);
+            for (int h = 0; h < 2; ++h) {
+              ok = ok && wait(WFB_P_FULL + 2 * i + h, (t0[i] + (j >> 1)) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(i, stage(j), h, j < 2);
+            }
             if (!ok) break;
-            clear_v(j);
-            tc_fence_after();
-            issue_pv(i, stage(j), j < 2);
             commit(&bars[WFB_V_EMPTY + stage(j)]);
             if (j + 2 < n) {
               ok = k_full(j + 2);
@@ -645,14 +680,17 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               if (!ok) break;
-              ok = wait(WFB_P_FULL + i, (jj0 + j) & 1);
-              if (ok && i == 0) {
+              if (i == 0) {
                 ok = v_full(j);
                 if (ok) clear_v(j);
               }
+              for (int h = 0; h < 2; ++h) {
+                ok = ok && wait(WFB_P_FULL + 2 * i + h, (jj0 + j) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                issue_pv(i, stage(j), h, j == 0);
+              }
               if (!ok) break;
-              tc_fence_after();
-              issue_pv(i, stage(j), j == 0);
               if (i == 1) commit(&bars[WFB_V_EMPTY + stage(j)]);
               if (j + 1 < n) {
                 if (i == 0) ok = k_full(j + 1);
