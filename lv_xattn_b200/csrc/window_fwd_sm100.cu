@@ -26,7 +26,7 @@
 //   * what lies behind the last valid key may hold anything: scores are replaced, and the rows of V that the last valid
 //     tile shares with it are cleared before they are multiplied with a probability of zero. A key inside that a row
 //     does not see, but another row of the tile does, may hold an infinity or a NaN too: such a row ends with NaN
-//     although its sum is finite, and is made again from the keys that it sees (plain_values; nothing else pays for it).
+//     although its sum is finite, and is made again from the keys that it sees (window_plain_row; nothing else pays for it).
 // P is rounded to 16 bits for its product, as in the forward block (O then errs by 2.3e-3 in bf16, 1.7e-3 of which is the
 // rounding of O itself); the sum is taken before that.
 #include "lvx_internal.h"
@@ -82,7 +82,7 @@ struct WinFwdParams {
   void* o;              // [B, Hq, Sq, 128] in the input type, with lse; nullptr: partials
   float* lse;
   float *o_part, *ml_part;
-  const uint16_t *q, *k, *v;      // for plain_values
+  const uint16_t *q, *k, *v;      // for window_plain_row
   long long q_b, q_h, q_s, k_b, k_h, k_s, v_b, v_h, v_s;
   int* status;
 };
