@@ -7,6 +7,7 @@ single tokens of a generation. The layouts are those of `attention`: q [B, Hq, S
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -63,6 +64,13 @@ def _scale(who, sm_scale):
     return float(sm_scale)
 
 
+def _whole(who, name, n):
+    try:
+        return operator.index(n)
+    except TypeError:
+        raise ValueError(f"{who}: {name} must be an integer, got {n!r}") from None
+
+
 class WindowAttentionFunc(torch.autograd.Function):
     """(q, k, v, sm_scale, window, sinks, query_start, kv_valid_len on the device) -> (o, lse)."""
 
@@ -101,6 +109,11 @@ def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=
     sm_scale scales the scores (None: 1 / sqrt(128)). Gradients flow into q, k and v."""
     who = "window_attention"
     sm_scale = _scale(who, sm_scale)
+    sinks = _whole(who, "sinks", sinks)
+    if window is not None:
+        window = _whole(who, "window", window)
+    if query_start is not None:
+        query_start = _whole(who, "query_start", query_start)
     if window is not None and window < 1:
         raise ValueError(f"{who}: window must be at least 1 (a query's own position), got {window}")
     if sinks < 0:
@@ -115,8 +128,8 @@ def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=
     with on_device(q):
         watch_status(q)
         lengths = ops.device_lengths(kv_valid_len, q_shape[0], k_shape[2], device)
-        args = (q, k, v, sm_scale, 0 if window is None or window >= _MOST else int(window), min(int(sinks), _MOST),
-                -1 if query_start is None else int(query_start), lengths)
+        args = (q, k, v, sm_scale, 0 if window is None or window >= _MOST else window, min(sinks, _MOST),
+                -1 if query_start is None else query_start, lengths)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             o, lse = WindowAttentionFunc.apply(*args)
         else:

@@ -89,3 +89,15 @@ def test_hook_refusals():
         with pytest.raises(ValueError):
             hf_patch.install_hooks("lv_xattn", **args)
     assert before == (mllama.MllamaTextCrossAttention.forward, mllama.MllamaTextSelfAttention.forward)
+
+
+@pytest.mark.parametrize("args", [dict(window=2.5), dict(window="4"), dict(sinks=0.5), dict(sinks=None), dict(query_start=1.0)])
+def test_whole_numbers(args):
+    with pytest.raises(ValueError, match="integer"):
+        lvx.window_attention(Q, K, K, **args)
+
+
+def test_whole_numbers_of_any_kind():
+    """Integers of other kinds are taken: the call ends at the missing CPU path, not at its arguments."""
+    with pytest.raises(LvxError):
+        lvx.window_attention(Q, K, K, window=torch.tensor(4), sinks=torch.tensor(2), query_start=torch.tensor(6))
