@@ -681,11 +681,11 @@ int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_by
 // The partials of a windowed forward, or where they are not needed (and o is given) its results.
 static int window_forward(const lvx_shape* s, const lvx_window* w, const FwdPlan& p, bool few, const lvx_view* q, const lvx_view* k,
                           const lvx_view* v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                          float* lse, int* sp, cudaStream_t st) {
+                          float* lse, int* sp, bool overlap, cudaStream_t st) {
   if (s->dtype == LVX_FP32)
     return launch_fwd_block_general(*s, p, q->data, k->data, v->data, kv_valid_len, nullptr, sm_scale, o_part, ml_part, st, w);
-  if (few) return launch_window_rows(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, sp, st);
-  return launch_window_fwd(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, lse, sp, st);
+  if (few) return launch_window_rows(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, sp, overlap, st);
+  return launch_window_fwd(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, lse, sp, overlap, st);
 }
 
 int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* q, const lvx_view* k, const lvx_view* v,
@@ -707,11 +707,11 @@ int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* 
   int* sp = status_ptr();
   if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (need == 0) return window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, nullptr, nullptr, o, lse, sp, st);
+  if (need == 0) return window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, nullptr, nullptr, o, lse, sp, false, st);
   float* o_part = static_cast<float*>(workspace);
   float* ml_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_part_bytes);
-  rc = window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, o_part, ml_part, nullptr, nullptr, sp, st);
-  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st);
+  rc = window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, o_part, ml_part, nullptr, nullptr, sp, false, st);
+  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st, true);
 }
 
 int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o, const lvx_view* q, const lvx_view* k,
@@ -742,9 +742,9 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
   float* delta = static_cast<float*>(workspace);
   float* dq_acc = direct ? static_cast<float*>(dq) : reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(rows * 4));
   float* parts = direct ? nullptr : dq_acc + window_dq_floats(*s);
-  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
   const cudaError_t e = cudaMemsetAsync(dq_acc, 0, direct ? rows * 512 : window_dq_floats(*s) * 4, st);
   if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dq)");
+  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
   if (s->Skv > 0) {
     const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
     rc = direct ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, dq_acc,
@@ -841,18 +841,19 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
   // q as it lies serves where the orders agree, if it is dense
   const bool dense = q->stride_s == 128 && q->stride_h == int64_t(s->Sq) * 128 && q->stride_b == int64_t(s->Hq) * s->Sq * 128;
   lvx_view pq = packed_q;
-  if (c.packed || !dense) {
+  const bool pack = c.packed || !dense;
+  if (pack) {
     pq.data = workspace;
-    if ((rc = launch_pack_rows(*s, prefixes, *q, nullptr, nullptr, nullptr, workspace, nullptr, nullptr, nullptr, st))) return rc;
+    if ((rc = launch_pack_rows(*s, prefixes, *q, nullptr, nullptr, nullptr, workspace, nullptr, nullptr, nullptr, false, st))) return rc;
   }
   if (s->Skv > 0) {
     o_own = take(c.own_plan.o_part_bytes);
     ml_own = take(c.own_plan.ml_part_bytes);
-    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, sp, st)))
+    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, sp, pack, st)))
       return rc;
   }
   if ((rc = window_forward(&c.pre, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre,
-                           nullptr, nullptr, sp, st)))
+                           nullptr, nullptr, sp, pack || s->Skv > 0, st)))
     return rc;
   return launch_shared_combine(*s, prefixes, o_pre, ml_pre, c.pre_plan.nsplit, o_own, ml_own, o_own ? c.own_plan.nsplit : 0, o, lse, st);
 }
@@ -901,12 +902,12 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
   float* acc = reinterpret_cast<float*>(at);
   const size_t acc_bytes = round256(f32 ? c.rows * 512 : window_dq_floats(c.pre) * 4);
   float* acc_own = s->Skv > 0 ? reinterpret_cast<float*>(at + acc_bytes) : nullptr;
-  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
   const cudaError_t e = cudaMemsetAsync(acc, 0, static_cast<char*>(workspace) + need - at, st);
   if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dq)");
+  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
   const bool dense = q->stride_s == 128 && q->stride_h == int64_t(s->Sq) * 128 && q->stride_b == int64_t(s->Hq) * s->Sq * 128;
   const bool pack = c.packed || !dense;
-  if (pack && (rc = launch_pack_rows(*s, prefixes, *q, d_o, lse, delta, q_p, do_p, lse_p, delta_p, st))) return rc;
+  if (pack && (rc = launch_pack_rows(*s, prefixes, *q, d_o, lse, delta, q_p, do_p, lse_p, delta_p, true, st))) return rc;
   const lvx_view pq = dense_view(pack ? q_p : q->data, c.pre.Hq, 1), pdo = dense_view(pack ? do_p : d_o, c.pre.Hq, 1);
   const float *pl = pack ? lse_p : lse, *pd = pack ? delta_p : delta;
   const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);

@@ -23,6 +23,9 @@ __global__ void __launch_bounds__(256)
 fwd_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ ml_part, const float* __restrict__ o_in,
                    const float* __restrict__ lse_in, void* __restrict__ o_out, float* __restrict__ lse_out,
                    int rows_per_slab, int nsplit, long total_rows, const int* status) {
+  grid_dep_wait();
+  grid_dep_read(o_part);
+  grid_dep_read(ml_part);
   const int bad = status ? *reinterpret_cast<const volatile int*>(status) : 0;
   const int lane = threadIdx.x & 31, part = (threadIdx.x >> 5) % WPR;
   const long grow = ((long(blockIdx.x) * blockDim.x + threadIdx.x) >> 5) / WPR;
@@ -92,7 +95,7 @@ fwd_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ m
 
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
-                       cudaStream_t st) {
+                       cudaStream_t st, bool overlap) {
   const long total_rows = long(q_blocks_of(s)) * s.B * s.Hq * s.Sq;
   const int threads = 256;
   const int* sp = device_status_ptr();
@@ -101,13 +104,12 @@ int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part
   // Eight warps per row while the rows alone leave SMs empty and a warp would walk more than two groups of four splits.
   const bool wide = total_rows <= 148 * 8 && p.nsplit > 8;
   auto go = [&](auto one, auto eight) {
-    if (wide) eight<<<total_rows, threads, 0, st>>>(o_part, ml_part, o_in, lse_in, o_out, lse_out, p.rows, p.nsplit, total_rows, sp);
-    else one<<<blocks, threads, 0, st>>>(o_part, ml_part, o_in, lse_in, o_out, lse_out, p.rows, p.nsplit, total_rows, sp);
+    return launch_kernel(overlap, wide ? eight : one, dim3(unsigned(wide ? total_rows : blocks)), threads, 0, st, o_part, ml_part, o_in,
+                         lse_in, o_out, lse_out, p.rows, p.nsplit, total_rows, sp);
   };
-  if (out == LVX_BF16) go(fwd_combine_kernel<0, 1>, fwd_combine_kernel<0, 8>);
-  else if (out == LVX_FP16) go(fwd_combine_kernel<1, 1>, fwd_combine_kernel<1, 8>);
-  else go(fwd_combine_kernel<2, 1>, fwd_combine_kernel<2, 8>);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = out == LVX_BF16   ? go(fwd_combine_kernel<0, 1>, fwd_combine_kernel<0, 8>)
+                        : out == LVX_FP16 ? go(fwd_combine_kernel<1, 1>, fwd_combine_kernel<1, 8>)
+                                          : go(fwd_combine_kernel<2, 1>, fwd_combine_kernel<2, 8>);
   if (e != cudaSuccess) return cuda_fail(e, "fwd_combine launch");
   return LVX_OK;
 }
@@ -168,6 +170,7 @@ __global__ void __launch_bounds__(256)
 bwd_prep_kernel(const void* __restrict__ o, const void* __restrict__ d_o, float* __restrict__ delta, long total_rows,
                 const int* status) {
   constexpr int LANES = IN == 2 ? 32 : 16, GROUPS = 256 / LANES, U = 4;
+  grid_dep_launch();
   const int bad = status ? *reinterpret_cast<const volatile int*>(status) : 0;
   const int l = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const long row0 = long(blockIdx.x) * (GROUPS * U) + grp;

@@ -70,12 +70,28 @@ int launch_fwd_rows(const lvx_shape& s, const FwdPlan& p, const void* q, const v
                     const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
                     cudaStream_t st);
 // Windowed causal attention (window.cuh): few packed rows (partials), and the kernel for more (partials, or O and lse).
+// Launches a kernel; with `overlap` it may come onto the SMs while the kernel before it in the stream still runs, and has to
+// call grid_dep_wait before it touches memory (sm100_prims.cuh).
+template <class... P, class... A>
+inline cudaError_t launch_kernel(bool overlap, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  c.attrs = &attr;
+  c.numAttrs = overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
 int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
                        const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
-                       cudaStream_t st);
+                       bool overlap, cudaStream_t st);
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                      float* lse, int* status, cudaStream_t st);
+                      float* lse, int* status, bool overlap, cudaStream_t st);
 // Its backward for 16-bit types: dq_acc (window_dq_floats of them, zeroed) is in tile order, launch_window_dq rounds it and
 // adds up the parts (window_sink_floats of them) of the sinks' dK and dV.
 size_t window_dq_floats(const lvx_shape& s);
@@ -87,14 +103,14 @@ int launch_window_dq(const lvx_shape& s, const lvx_window& w, const float* acc, 
                      const int* status, cudaStream_t st);
 // Around the windowed kernels for a batch that shares prefixes (shared_prefix.cu).
 int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const void* d_o, const float* lse, const float* delta,
-                     void* q_out, void* do_out, float* lse_out, float* delta_out, cudaStream_t st);
+                     void* q_out, void* do_out, float* lse_out, float* delta_out, bool overlap, cudaStream_t st);
 int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
                           const float* ml_own, int ns_own, void* o, float* lse, cudaStream_t st);
 int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int pre_slab_rows, const float* acc_own, void* dq,
                      cudaStream_t st);
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
-                       cudaStream_t st);
+                       cudaStream_t st, bool overlap = false);
 int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st);
 int launch_bwd_block(const lvx_shape& s, const void* q, const void* d_o, const float* lse, const float* delta,
                      const void* k, const void* v, const int32_t* kv_valid_len, float sm_scale, float* dq_acc,

@@ -43,6 +43,9 @@ __global__ void __launch_bounds__(256)
 pack_rows_kernel(const char* __restrict__ q, long long q_b, long long q_h, long long q_s, const uint4* __restrict__ d_o,
                  const float* __restrict__ lse, const float* __restrict__ delta, uint4* __restrict__ q_out, uint4* __restrict__ do_out,
                  float* __restrict__ lse_out, float* __restrict__ delta_out, PackOrder order, int rows, const int* status) {
+  grid_dep_launch();
+  grid_dep_wait();
+  grid_dep_read(delta);
   if (poisoned(status)) return;
   constexpr int U = 4, PER = 256 / ROW16;      // rows of a thread, rows of a block at a time
   const int piece = threadIdx.x % ROW16, row0 = blockIdx.x * PER * U + threadIdx.x / ROW16;
@@ -80,6 +83,11 @@ __global__ void __launch_bounds__(256)
 shared_combine_kernel(const float* __restrict__ o_pre, const float* __restrict__ ml_pre, int ns_pre, const float* __restrict__ o_own,
                       const float* __restrict__ ml_own, int ns_own, PackOrder order, void* __restrict__ o_out,
                       float* __restrict__ lse_out, int rows, const int* status) {
+  grid_dep_wait();
+  grid_dep_read(o_pre);
+  grid_dep_read(ml_pre);
+  grid_dep_read(o_own);
+  grid_dep_read(ml_own);
   const int bad = status ? *reinterpret_cast<const volatile int*>(status) : 0;
   const int lane = threadIdx.x & 31, part = (threadIdx.x >> 5) % WPR;
   const int row = (blockIdx.x * 8 + (threadIdx.x >> 5)) / WPR;
@@ -128,6 +136,9 @@ template <int OUT>
 __global__ void __launch_bounds__(256)
 shared_dq_kernel(const float* __restrict__ acc_pre, int pre_slab_rows, const float* __restrict__ acc_own, int heads, int chunks,
                  PackOrder order, void* __restrict__ dq, int rows, const int* status) {
+  grid_dep_wait();
+  grid_dep_read(acc_pre);
+  grid_dep_read(acc_own);
   if (poisoned(status)) {
     if ((threadIdx.x & 31) == 0) publish_status(status);
     return;
@@ -149,18 +160,16 @@ shared_dq_kernel(const float* __restrict__ acc_pre, int pre_slab_rows, const flo
 }
 
 int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const void* d_o, const float* lse, const float* delta,
-                     void* q_out, void* do_out, float* lse_out, float* delta_out, cudaStream_t st) {
+                     void* q_out, void* do_out, float* lse_out, float* delta_out, bool overlap, cudaStream_t st) {
   const int rows = s.B * s.Hq * s.Sq;
   const int es = elt_size(s.dtype), pieces = es * 8;
   auto go = [&](auto kern) {
-    kern<<<(rows + 1024 / pieces - 1) / (1024 / pieces), 256, 0, st>>>(static_cast<const char*>(q.data), q.stride_b * es, q.stride_h * es,
-                                                      q.stride_s * es, static_cast<const uint4*>(d_o), lse, delta,
-                                                      static_cast<uint4*>(q_out), static_cast<uint4*>(do_out), lse_out, delta_out,
-                                                      pack_order(s, prefixes), rows, device_status_ptr());
+    return launch_kernel(overlap, kern, dim3((rows + 1024 / pieces - 1) / (1024 / pieces)), 256, 0, st, static_cast<const char*>(q.data),
+                         q.stride_b * es, q.stride_h * es, q.stride_s * es, static_cast<const uint4*>(d_o), lse, delta,
+                         static_cast<uint4*>(q_out), static_cast<uint4*>(do_out), lse_out, delta_out, pack_order(s, prefixes), rows,
+                         device_status_ptr());
   };
-  if (es == 2) go(pack_rows_kernel<16>);
-  else go(pack_rows_kernel<32>);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = es == 2 ? go(pack_rows_kernel<16>) : go(pack_rows_kernel<32>);
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "pack_rows launch");
 }
 
@@ -170,13 +179,12 @@ int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, 
   // as in launch_fwd_combine: eight warps a row while the rows alone leave SMs empty and one warp's walk is long
   const bool wide = rows <= 148 * 8 && ns_pre + ns_own > 8;
   auto go = [&](auto one, auto eight) {
-    if (wide) eight<<<rows, 256, 0, st>>>(o_pre, ml_pre, ns_pre, o_own, ml_own, ns_own, pack_order(s, prefixes), o, lse, rows, device_status_ptr());
-    else one<<<(rows - 1) / 8 + 1, 256, 0, st>>>(o_pre, ml_pre, ns_pre, o_own, ml_own, ns_own, pack_order(s, prefixes), o, lse, rows, device_status_ptr());
+    return launch_kernel(true, wide ? eight : one, dim3(wide ? rows : (rows - 1) / 8 + 1), 256, 0, st, o_pre, ml_pre, ns_pre, o_own, ml_own,
+                         ns_own, pack_order(s, prefixes), o, lse, rows, device_status_ptr());
   };
-  if (s.dtype == LVX_BF16) go(shared_combine_kernel<0, 1>, shared_combine_kernel<0, 8>);
-  else if (s.dtype == LVX_FP16) go(shared_combine_kernel<1, 1>, shared_combine_kernel<1, 8>);
-  else go(shared_combine_kernel<2, 1>, shared_combine_kernel<2, 8>);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = s.dtype == LVX_BF16   ? go(shared_combine_kernel<0, 1>, shared_combine_kernel<0, 8>)
+                        : s.dtype == LVX_FP16 ? go(shared_combine_kernel<1, 1>, shared_combine_kernel<1, 8>)
+                                              : go(shared_combine_kernel<2, 1>, shared_combine_kernel<2, 8>);
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "shared_combine launch");
 }
 
@@ -188,12 +196,12 @@ int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int
   const int heads = s.dtype == LVX_FP32 ? 1 : qt.heads, chunks = s.dtype == LVX_FP32 ? s.Hq / s.Hkv : qt.chunks;
   const int blocks = std::min((rows - 1) / 8 + 1, 148 * 16);
   auto go = [&](auto kern) {
-    kern<<<blocks, 256, 0, st>>>(acc_pre, pre_slab_rows, acc_own, heads, chunks, pack_order(s, prefixes), dq, rows, device_status_ptr());
+    return launch_kernel(true, kern, dim3(blocks), 256, 0, st, acc_pre, pre_slab_rows, acc_own, heads, chunks, pack_order(s, prefixes), dq,
+                         rows, device_status_ptr());
   };
-  if (s.dtype == LVX_BF16) go(shared_dq_kernel<0>);
-  else if (s.dtype == LVX_FP16) go(shared_dq_kernel<1>);
-  else go(shared_dq_kernel<2>);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = s.dtype == LVX_BF16   ? go(shared_dq_kernel<0>)
+                        : s.dtype == LVX_FP16 ? go(shared_dq_kernel<1>)
+                                              : go(shared_dq_kernel<2>);
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "shared_dq launch");
 }
 

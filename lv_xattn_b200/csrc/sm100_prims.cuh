@@ -364,6 +364,14 @@ __device__ __forceinline__ void publish_status(const int* status) {
     __threadfence_system();
   }
 }
+// Kernels of one call that follow one another (launch_kernel's `overlap`): the next one is brought onto the SMs while this
+// one still runs, from grid_dep_launch on, and waits in grid_dep_wait until all before it in the stream is complete and
+// visible. Each of them waits, so that completion is passed on along the call. Pointers that the kernel reads through the
+// non-coherent path go through the wait, so that no read of them can be moved before it.
+__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class P>
+__device__ __forceinline__ void grid_dep_read(P& p) { asm volatile("" : "+l"(p) : : "memory"); }
 // Product of two 128-wide 16-bit rows in fp32.
 template <bool IS_BF16>
 __device__ __forceinline__ float dot128(const void* a, const void* b) {

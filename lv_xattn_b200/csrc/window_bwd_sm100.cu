@@ -98,6 +98,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   float* s_stat = reinterpret_cast<float*>(smem + WB_OFF_STAT);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  grid_dep_launch();
+  grid_dep_wait();
   const int heads = p.qt.heads, tile_rows = heads * p.qt.tokens;
   struct Item {
     int slab, kv0, valid, start;
@@ -596,6 +598,9 @@ template <bool IS_BF16>
 __global__ void __launch_bounds__(256)
 window_dq_kernel(const float* __restrict__ acc, uint16_t* __restrict__ dq, int g, int sq, int heads, int chunks, int slabs, const SinkParts sp,
                  const float* __restrict__ parts, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, int skv, const int* status) {
+  grid_dep_wait();
+  grid_dep_read(acc);
+  grid_dep_read(parts);
   if (status && *reinterpret_cast<const volatile int*>(status) != 0) {
     if ((threadIdx.x & 31) == 0) publish_status(status);
     return;
@@ -694,7 +699,7 @@ int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WB_SMEM);
-    if (e == cudaSuccess) kern<<<grid, WB_THREADS, WB_SMEM, st>>>(tmQ, tmDO, tmK, tmV, p);
+    if (e == cudaSuccess) e = launch_kernel(true, kern, grid, WB_THREADS, WB_SMEM, st, tmQ, tmDO, tmK, tmV, p);
   };
   if (s.dtype == LVX_BF16) go(window_bwd_kernel<true>);
   else go(window_bwd_kernel<false>);
@@ -709,12 +714,10 @@ int launch_window_dq(const lvx_shape& s, const lvx_window& w, const float* acc, 
   const long all = long(s.B) * s.Hkv * qt.chunks, rows = long(s.Sq) * qt.heads;
   const dim3 grid(unsigned(std::min<long>((rows + 31) / 32, (148 * 16 + all - 1) / all)), unsigned(std::min<long>(all, 65535)));
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, st>>>(acc, static_cast<uint16_t*>(dq), s.Hq / s.Hkv, s.Sq, qt.heads, qt.chunks, s.B * s.Hkv, sink_parts(s, w), parts,
-                               static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv), s.Skv, status);
+    return launch_kernel(true, kern, grid, 256, 0, st, acc, static_cast<uint16_t*>(dq), s.Hq / s.Hkv, s.Sq, qt.heads, qt.chunks,
+                         s.B * s.Hkv, sink_parts(s, w), parts, static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv), s.Skv, status);
   };
-  if (s.dtype == LVX_BF16) go(window_dq_kernel<true>);
-  else go(window_dq_kernel<false>);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = s.dtype == LVX_BF16 ? go(window_dq_kernel<true>) : go(window_dq_kernel<false>);
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "window_dq launch");
 }
 

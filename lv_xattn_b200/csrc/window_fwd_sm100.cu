@@ -140,6 +140,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  grid_dep_launch();
+  grid_dep_wait();
   const int heads = p.qt.heads, tile_rows = heads * p.qt.tokens;
   struct Item {
     int mb, slab, split, valid, start;      // split: number of the partial result
@@ -811,7 +813,7 @@ int make_kv_map(CUtensorMap* out, const lvx_shape& s, const lvx_view& v, const l
 
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                      float* lse, int* status, cudaStream_t st) {
+                      float* lse, int* status, bool overlap, cudaStream_t st) {
   const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
   CUtensorMap tmQ, tmK, tmV;
   int rc = make_q_map(&tmQ, s, qt, q);
@@ -852,7 +854,7 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WF_SMEM);
-    if (e == cudaSuccess) kern<<<grid, WF_THREADS, WF_SMEM, st>>>(tmQ, tmK, tmV, p);
+    if (e == cudaSuccess) e = launch_kernel(overlap, kern, grid, WF_THREADS, WF_SMEM, st, tmQ, tmK, tmV, p);
   };
   auto pick = [&](auto one, auto two) {
     if (pair) go(two);
