@@ -681,11 +681,11 @@ int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_by
 // The partials of a windowed forward, or where they are not needed (and o is given) its results.
 static int window_forward(const lvx_shape* s, const lvx_window* w, const FwdPlan& p, bool few, const lvx_view* q, const lvx_view* k,
                           const lvx_view* v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                          float* lse, int* sp, bool overlap, cudaStream_t st) {
+                          float* lse, int* sp, Order order, cudaStream_t st) {
   if (s->dtype == LVX_FP32)
     return launch_fwd_block_general(*s, p, q->data, k->data, v->data, kv_valid_len, nullptr, sm_scale, o_part, ml_part, st, w);
-  if (few) return launch_window_rows(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, sp, overlap, st);
-  return launch_window_fwd(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, lse, sp, overlap, st);
+  if (few) return launch_window_rows(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, sp, order, st);
+  return launch_window_fwd(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, lse, sp, order, st);
 }
 
 int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* q, const lvx_view* k, const lvx_view* v,
@@ -707,11 +707,11 @@ int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* 
   int* sp = status_ptr();
   if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (need == 0) return window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, nullptr, nullptr, o, lse, sp, false, st);
+  if (need == 0) return window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, nullptr, nullptr, o, lse, sp, ORDER_AFTER, st);
   float* o_part = static_cast<float*>(workspace);
   float* ml_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_part_bytes);
-  rc = window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, o_part, ml_part, nullptr, nullptr, sp, false, st);
-  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st, true);
+  rc = window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, o_part, ml_part, nullptr, nullptr, sp, ORDER_AFTER, st);
+  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st, ORDER_OVERLAP);
 }
 
 int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o, const lvx_view* q, const lvx_view* k,
@@ -749,7 +749,7 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
     const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
     rc = direct ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, dq_acc,
                                            dk, dv, 2, st, w)
-                : launch_window_bwd(*s, *w, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, dq_acc, parts, dk, dv, sp, st);
+                : launch_window_bwd(*s, *w, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, dq_acc, parts, dk, dv, sp, ORDER_OVERLAP, st);
   }
   return rc || direct ? rc : launch_window_dq(*s, *w, dq_acc, parts, dq, dk, dv, sp, st);
 }
@@ -844,16 +844,16 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
   const bool pack = c.packed || !dense;
   if (pack) {
     pq.data = workspace;
-    if ((rc = launch_pack_rows(*s, prefixes, *q, nullptr, nullptr, nullptr, workspace, nullptr, nullptr, nullptr, false, st))) return rc;
+    if ((rc = launch_pack_rows(*s, prefixes, *q, nullptr, nullptr, nullptr, workspace, nullptr, nullptr, nullptr, ORDER_AFTER, st))) return rc;
   }
   if (s->Skv > 0) {
     o_own = take(c.own_plan.o_part_bytes);
     ml_own = take(c.own_plan.ml_part_bytes);
-    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, sp, pack, st)))
+    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, sp, pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
       return rc;
   }
   if ((rc = window_forward(&c.pre, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre,
-                           nullptr, nullptr, sp, pack || s->Skv > 0, st)))
+                           nullptr, nullptr, sp, s->Skv > 0 ? ORDER_BESIDE : pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
     return rc;
   return launch_shared_combine(*s, prefixes, o_pre, ml_pre, c.pre_plan.nsplit, o_own, ml_own, o_own ? c.own_plan.nsplit : 0, o, lse, st);
 }
@@ -907,17 +907,17 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
   if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
   const bool dense = q->stride_s == 128 && q->stride_h == int64_t(s->Sq) * 128 && q->stride_b == int64_t(s->Hq) * s->Sq * 128;
   const bool pack = c.packed || !dense;
-  if (pack && (rc = launch_pack_rows(*s, prefixes, *q, d_o, lse, delta, q_p, do_p, lse_p, delta_p, true, st))) return rc;
+  if (pack && (rc = launch_pack_rows(*s, prefixes, *q, d_o, lse, delta, q_p, do_p, lse_p, delta_p, ORDER_OVERLAP, st))) return rc;
   const lvx_view pq = dense_view(pack ? q_p : q->data, c.pre.Hq, 1), pdo = dense_view(pack ? do_p : d_o, c.pre.Hq, 1);
   const float *pl = pack ? lse_p : lse, *pd = pack ? delta_p : delta;
   const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
   rc = f32 ? launch_bwd_block_general(c.pre, pq.data, pdo.data, pl, pd, pk->data, pv->data, prefix_valid_len, nullptr, sm_scale, acc,
                                       dpk, dpv, 2, st, &c.pre_win)
-           : launch_window_bwd(c.pre, c.pre_win, pq, pdo, *pk, *pv, pl, pd, prefix_valid_len, sm_scale, acc, nullptr, dpk, dpv, sp, st);
+           : launch_window_bwd(c.pre, c.pre_win, pq, pdo, *pk, *pv, pl, pd, prefix_valid_len, sm_scale, acc, nullptr, dpk, dpv, sp, ORDER_OVERLAP, st);
   if (!rc && s->Skv > 0)
     rc = f32 ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, acc_own, dk,
                                         dv, 2, st, &c.own_win)
-             : launch_window_bwd(*s, c.own_win, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, acc_own, nullptr, dk, dv, sp, st);
+             : launch_window_bwd(*s, c.own_win, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, acc_own, nullptr, dk, dv, sp, ORDER_BESIDE, st);
   if (rc) return rc;
   const QTiles pt = make_q_tiles(c.pre.Hq / c.pre.Hkv, 1);
   const int pre_slab_rows = f32 ? c.pre.Hq / c.pre.Hkv : pt.chunks * pt.heads;

@@ -95,7 +95,7 @@ fwd_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ m
 
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
-                       cudaStream_t st, bool overlap) {
+                       cudaStream_t st, Order order) {
   const long total_rows = long(q_blocks_of(s)) * s.B * s.Hq * s.Sq;
   const int threads = 256;
   const int* sp = device_status_ptr();
@@ -104,7 +104,7 @@ int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part
   // Eight warps per row while the rows alone leave SMs empty and a warp would walk more than two groups of four splits.
   const bool wide = total_rows <= 148 * 8 && p.nsplit > 8;
   auto go = [&](auto one, auto eight) {
-    return launch_kernel(overlap, wide ? eight : one, dim3(unsigned(wide ? total_rows : blocks)), threads, 0, st, o_part, ml_part, o_in,
+    return launch_kernel(order, wide ? eight : one, dim3(unsigned(wide ? total_rows : blocks)), threads, 0, st, o_part, ml_part, o_in,
                          lse_in, o_out, lse_out, p.rows, p.nsplit, total_rows, sp);
   };
   const cudaError_t e = out == LVX_BF16   ? go(fwd_combine_kernel<0, 1>, fwd_combine_kernel<0, 8>)
@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(256)
 bwd_prep_kernel(const void* __restrict__ o, const void* __restrict__ d_o, float* __restrict__ delta, long total_rows,
                 const int* status) {
   constexpr int LANES = IN == 2 ? 32 : 16, GROUPS = 256 / LANES, U = 4;
+  grid_dep_wait();
   grid_dep_launch();
   const int bad = status ? *reinterpret_cast<const volatile int*>(status) : 0;
   const int l = threadIdx.x % LANES, grp = threadIdx.x / LANES;

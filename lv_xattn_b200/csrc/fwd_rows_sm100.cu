@@ -54,6 +54,7 @@ struct RowsParams {
   int* status;
   // WIN
   WindowMask mask;
+  bool beside;            // ORDER_BESIDE
   int sq, g;
   const void *k, *v;
   long long q_b, q_h, q_s, k_b, k_h, k_s, v_b, v_h, v_s;
@@ -106,10 +107,7 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.x, slab = blockIdx.y;
-  if constexpr (WIN) {
-    grid_dep_launch();
-    grid_dep_wait();
-  }
+  GridDep dep(WIN && p.beside);
   // The status word may be set by another CTA or stream at any moment: one thread reads it, and the CTA leaves or stays as
   // a whole. Warps that went on alone would meet barriers that nobody initialised and wait for the others at bar.sync.
   int word = 0;
@@ -465,7 +463,7 @@ int launch_fwd_rows(const lvx_shape& s, const FwdPlan& pl, const void* q, const 
 
 int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl, const lvx_view& q, const lvx_view& k,
                        const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
-                       bool overlap, cudaStream_t st) {
+                       Order order, cudaStream_t st) {
   CUtensorMap tmK, tmV;
   int rc = make_kv_map(&tmK, s, k, q);
   if (!rc) rc = make_kv_map(&tmV, s, v, q);
@@ -482,6 +480,7 @@ int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p
   p.ml_part = ml_part;
   p.status = status;
   p.mask = make_window_mask(w);
+  p.beside = order == ORDER_BESIDE;
   p.sq = s.Sq;
   p.g = s.Hq / s.Hkv;
   p.k = k.data;
@@ -493,7 +492,7 @@ int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FR_SMEM);
-    if (e == cudaSuccess) e = launch_kernel(overlap, kern, grid, FR_THREADS, FR_SMEM, st, tmK, tmV, p);
+    if (e == cudaSuccess) e = launch_kernel(order, kern, grid, FR_THREADS, FR_SMEM, st, tmK, tmV, p);
   };
   auto pick = [&](auto bf16) {
     constexpr bool B16 = decltype(bf16)::value;

@@ -70,10 +70,13 @@ int launch_fwd_rows(const lvx_shape& s, const FwdPlan& p, const void* q, const v
                     const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
                     cudaStream_t st);
 // Windowed causal attention (window.cuh): few packed rows (partials), and the kernel for more (partials, or O and lse).
-// Launches a kernel; with `overlap` it may come onto the SMs while the kernel before it in the stream still runs, and has to
-// call grid_dep_wait before it touches memory (sm100_prims.cuh).
+// How a kernel stands to the one before it in the stream: it starts when that one is complete; or comes onto the SMs while that
+// one, of the same call, still runs, and waits for it itself, at its start or, needing none of its results, at its end
+// (sm100_prims.cuh). The kernels of own keys and of a shared prefix stand beside each other: one token of 32 requests with 2,048
+// own keys behind 102,464 134 -> 128 us, 77 tokens of eight requests behind 25,616 274 -> 270, 333 of four even.
+enum Order { ORDER_AFTER, ORDER_OVERLAP, ORDER_BESIDE };
 template <class... P, class... A>
-inline cudaError_t launch_kernel(bool overlap, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
+inline cudaError_t launch_kernel(Order order, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -83,34 +86,34 @@ inline cudaError_t launch_kernel(bool overlap, void (*kernel)(P...), dim3 grid, 
   c.dynamicSmemBytes = smem;
   c.stream = st;
   c.attrs = &attr;
-  c.numAttrs = overlap ? 1 : 0;
+  c.numAttrs = order == ORDER_AFTER ? 0 : 1;
   return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
 }
 int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
                        const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
-                       bool overlap, cudaStream_t st);
+                       Order order, cudaStream_t st);
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                      float* lse, int* status, bool overlap, cudaStream_t st);
+                      float* lse, int* status, Order order, cudaStream_t st);
 // Its backward for 16-bit types: dq_acc (window_dq_floats of them, zeroed) is in tile order, launch_window_dq rounds it and
 // adds up the parts (window_sink_floats of them) of the sinks' dK and dV.
 size_t window_dq_floats(const lvx_shape& s);
 size_t window_sink_floats(const lvx_shape& s, const lvx_window& w);
 int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q, const lvx_view& d_o, const lvx_view& k,
                       const lvx_view& v, const float* lse, const float* delta, const int32_t* kv_valid_len, float sm_scale,
-                      float* dq_acc, float* parts, void* dk, void* dv, int* status, cudaStream_t st);
+                      float* dq_acc, float* parts, void* dk, void* dv, int* status, Order order, cudaStream_t st);
 int launch_window_dq(const lvx_shape& s, const lvx_window& w, const float* acc, const float* parts, void* dq, void* dk, void* dv,
                      const int* status, cudaStream_t st);
 // Around the windowed kernels for a batch that shares prefixes (shared_prefix.cu).
 int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const void* d_o, const float* lse, const float* delta,
-                     void* q_out, void* do_out, float* lse_out, float* delta_out, bool overlap, cudaStream_t st);
+                     void* q_out, void* do_out, float* lse_out, float* delta_out, Order order, cudaStream_t st);
 int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
                           const float* ml_own, int ns_own, void* o, float* lse, cudaStream_t st);
 int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int pre_slab_rows, const float* acc_own, void* dq,
                      cudaStream_t st);
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
-                       cudaStream_t st, bool overlap = false);
+                       cudaStream_t st, Order order = ORDER_AFTER);
 int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st);
 int launch_bwd_block(const lvx_shape& s, const void* q, const void* d_o, const float* lse, const float* delta,
                      const void* k, const void* v, const int32_t* kv_valid_len, float sm_scale, float* dq_acc,

@@ -43,8 +43,8 @@ __global__ void __launch_bounds__(256)
 pack_rows_kernel(const char* __restrict__ q, long long q_b, long long q_h, long long q_s, const uint4* __restrict__ d_o,
                  const float* __restrict__ lse, const float* __restrict__ delta, uint4* __restrict__ q_out, uint4* __restrict__ do_out,
                  float* __restrict__ lse_out, float* __restrict__ delta_out, PackOrder order, int rows, const int* status) {
-  grid_dep_launch();
   grid_dep_wait();
+  grid_dep_launch();
   grid_dep_read(delta);
   if (poisoned(status)) return;
   constexpr int U = 4, PER = 256 / ROW16;      // rows of a thread, rows of a block at a time
@@ -160,11 +160,11 @@ shared_dq_kernel(const float* __restrict__ acc_pre, int pre_slab_rows, const flo
 }
 
 int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const void* d_o, const float* lse, const float* delta,
-                     void* q_out, void* do_out, float* lse_out, float* delta_out, bool overlap, cudaStream_t st) {
+                     void* q_out, void* do_out, float* lse_out, float* delta_out, Order order, cudaStream_t st) {
   const int rows = s.B * s.Hq * s.Sq;
   const int es = elt_size(s.dtype), pieces = es * 8;
   auto go = [&](auto kern) {
-    return launch_kernel(overlap, kern, dim3((rows + 1024 / pieces - 1) / (1024 / pieces)), 256, 0, st, static_cast<const char*>(q.data),
+    return launch_kernel(order, kern, dim3((rows + 1024 / pieces - 1) / (1024 / pieces)), 256, 0, st, static_cast<const char*>(q.data),
                          q.stride_b * es, q.stride_h * es, q.stride_s * es, static_cast<const uint4*>(d_o), lse, delta,
                          static_cast<uint4*>(q_out), static_cast<uint4*>(do_out), lse_out, delta_out, pack_order(s, prefixes), rows,
                          device_status_ptr());
@@ -179,7 +179,7 @@ int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, 
   // as in launch_fwd_combine: eight warps a row while the rows alone leave SMs empty and one warp's walk is long
   const bool wide = rows <= 148 * 8 && ns_pre + ns_own > 8;
   auto go = [&](auto one, auto eight) {
-    return launch_kernel(true, wide ? eight : one, dim3(wide ? rows : (rows - 1) / 8 + 1), 256, 0, st, o_pre, ml_pre, ns_pre, o_own, ml_own,
+    return launch_kernel(ORDER_OVERLAP, wide ? eight : one, dim3(wide ? rows : (rows - 1) / 8 + 1), 256, 0, st, o_pre, ml_pre, ns_pre, o_own, ml_own,
                          ns_own, pack_order(s, prefixes), o, lse, rows, device_status_ptr());
   };
   const cudaError_t e = s.dtype == LVX_BF16   ? go(shared_combine_kernel<0, 1>, shared_combine_kernel<0, 8>)
@@ -196,7 +196,7 @@ int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int
   const int heads = s.dtype == LVX_FP32 ? 1 : qt.heads, chunks = s.dtype == LVX_FP32 ? s.Hq / s.Hkv : qt.chunks;
   const int blocks = std::min((rows - 1) / 8 + 1, 148 * 16);
   auto go = [&](auto kern) {
-    return launch_kernel(true, kern, dim3(blocks), 256, 0, st, acc_pre, pre_slab_rows, acc_own, heads, chunks, pack_order(s, prefixes), dq,
+    return launch_kernel(ORDER_OVERLAP, kern, dim3(blocks), 256, 0, st, acc_pre, pre_slab_rows, acc_own, heads, chunks, pack_order(s, prefixes), dq,
                          rows, device_status_ptr());
   };
   const cudaError_t e = s.dtype == LVX_BF16   ? go(shared_dq_kernel<0>)

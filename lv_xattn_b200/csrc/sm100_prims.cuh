@@ -364,12 +364,24 @@ __device__ __forceinline__ void publish_status(const int* status) {
     __threadfence_system();
   }
 }
-// Kernels of one call that follow one another (launch_kernel's `overlap`): the next one is brought onto the SMs while this
-// one still runs, from grid_dep_launch on, and waits in grid_dep_wait until all before it in the stream is complete and
-// visible. Each of them waits, so that completion is passed on along the call. Pointers that the kernel reads through the
-// non-coherent path go through the wait, so that no read of them can be moved before it.
+// Kernels of one call that follow one another (enum Order): the next one is brought onto the SMs while this one still runs,
+// when all CTAs of this one have called grid_dep_launch or left, and waits in grid_dep_wait until this one is complete and
+// visible. Every kernel waits before it ends, so that completion is passed on along the call, and calls grid_dep_launch
+// after its wait, so that a kernel that follows one whose results it does not need finds all before that one complete:
+// it puts its wait off to its end (GridDep), and fills the SMs that the other one's last CTAs leave idle. Pointers that a
+// kernel reads through the non-coherent path go through grid_dep_read, so that no read of them can be moved before the wait.
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+struct GridDep {      // at the top of a kernel; `late`: launched with ORDER_BESIDE
+  bool late;
+  __device__ __forceinline__ explicit GridDep(bool l) : late(l) {
+    if (!late) grid_dep_wait();
+    grid_dep_launch();
+  }
+  __device__ __forceinline__ ~GridDep() {
+    if (late) grid_dep_wait();
+  }
+};
 template <class P>
 __device__ __forceinline__ void grid_dep_read(P& p) { asm volatile("" : "+l"(p) : : "memory"); }
 // Product of two 128-wide 16-bit rows in fp32.

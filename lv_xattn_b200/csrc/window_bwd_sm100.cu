@@ -76,6 +76,7 @@ struct SinkParts {
 struct WinBwdParams {
   int sq, skv, hkv, g, slabs, nitems;
   SinkParts sp;
+  bool beside;                         // ORDER_BESIDE
   float* parts;                        // [slab][sink tile][part][dK, dV][128][128]
   QTiles qt;
   WindowMask mask;
@@ -98,8 +99,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   float* s_stat = reinterpret_cast<float*>(smem + WB_OFF_STAT);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  grid_dep_launch();
-  grid_dep_wait();
+  GridDep dep(p.beside);
   const int heads = p.qt.heads, tile_rows = heads * p.qt.tokens;
   struct Item {
     int slab, kv0, valid, start;
@@ -667,7 +667,7 @@ size_t window_dq_floats(const lvx_shape& s) {
 // dq_acc (window_dq_floats, zeroed), then dk and dv; `parts`: window_sink_floats.
 int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q, const lvx_view& d_o, const lvx_view& k,
                       const lvx_view& v, const float* lse, const float* delta, const int32_t* kv_valid_len, float sm_scale,
-                      float* dq_acc, float* parts, void* dk, void* dv, int* status, cudaStream_t st) {
+                      float* dq_acc, float* parts, void* dk, void* dv, int* status, Order order, cudaStream_t st) {
   const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
   CUtensorMap tmQ, tmDO, tmK, tmV;
   int rc = make_q_map(&tmQ, s, qt, q);
@@ -683,6 +683,7 @@ int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q
   p.slabs = s.B * s.Hkv;
   p.sp = sink_parts(s, w);
   p.parts = parts;
+  p.beside = order == ORDER_BESIDE;
   p.nitems = ((s.Skv + 127) / 128 + p.sp.tiles * (p.sp.parts - 1)) * p.slabs;
   p.qt = qt;
   p.mask = make_window_mask(w);
@@ -699,7 +700,7 @@ int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WB_SMEM);
-    if (e == cudaSuccess) e = launch_kernel(true, kern, grid, WB_THREADS, WB_SMEM, st, tmQ, tmDO, tmK, tmV, p);
+    if (e == cudaSuccess) e = launch_kernel(order, kern, grid, WB_THREADS, WB_SMEM, st, tmQ, tmDO, tmK, tmV, p);
   };
   if (s.dtype == LVX_BF16) go(window_bwd_kernel<true>);
   else go(window_bwd_kernel<false>);
@@ -714,7 +715,7 @@ int launch_window_dq(const lvx_shape& s, const lvx_window& w, const float* acc, 
   const long all = long(s.B) * s.Hkv * qt.chunks, rows = long(s.Sq) * qt.heads;
   const dim3 grid(unsigned(std::min<long>((rows + 31) / 32, (148 * 16 + all - 1) / all)), unsigned(std::min<long>(all, 65535)));
   auto go = [&](auto kern) {
-    return launch_kernel(true, kern, grid, 256, 0, st, acc, static_cast<uint16_t*>(dq), s.Hq / s.Hkv, s.Sq, qt.heads, qt.chunks,
+    return launch_kernel(ORDER_OVERLAP, kern, grid, 256, 0, st, acc, static_cast<uint16_t*>(dq), s.Hq / s.Hkv, s.Sq, qt.heads, qt.chunks,
                          s.B * s.Hkv, sink_parts(s, w), parts, static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv), s.Skv, status);
   };
   const cudaError_t e = s.dtype == LVX_BF16 ? go(window_dq_kernel<true>) : go(window_dq_kernel<false>);

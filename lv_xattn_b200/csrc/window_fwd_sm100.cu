@@ -79,6 +79,7 @@ struct WinFwdParams {
   const int32_t* kv_valid_len;
   float scale_log2;
   int nsplit;
+  bool beside;          // ORDER_BESIDE
   void* o;              // [B, Hq, Sq, 128] in the input type, with lse; nullptr: partials
   float* lse;
   float *o_part, *ml_part;
@@ -140,8 +141,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  grid_dep_launch();
-  grid_dep_wait();
+  GridDep dep(p.beside);
   const int heads = p.qt.heads, tile_rows = heads * p.qt.tokens;
   struct Item {
     int mb, slab, split, valid, start;      // split: number of the partial result
@@ -813,7 +813,7 @@ int make_kv_map(CUtensorMap* out, const lvx_shape& s, const lvx_view& v, const l
 
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                      float* lse, int* status, bool overlap, cudaStream_t st) {
+                      float* lse, int* status, Order order, cudaStream_t st) {
   const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
   CUtensorMap tmQ, tmK, tmV;
   int rc = make_q_map(&tmQ, s, qt, q);
@@ -831,6 +831,7 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
   p.kv_valid_len = kv_valid_len;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.nsplit = pl.nsplit;
+  p.beside = order == ORDER_BESIDE;
   p.o = o;
   p.lse = lse;
   p.o_part = o_part;
@@ -854,7 +855,7 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WF_SMEM);
-    if (e == cudaSuccess) e = launch_kernel(overlap, kern, grid, WF_THREADS, WF_SMEM, st, tmQ, tmK, tmV, p);
+    if (e == cudaSuccess) e = launch_kernel(order, kern, grid, WF_THREADS, WF_SMEM, st, tmQ, tmK, tmV, p);
   };
   auto pick = [&](auto one, auto two) {
     if (pair) go(two);
