@@ -17,8 +17,9 @@
 // value an instruction and 64-bit divisions. Registers are what decides: four heads a unit and two blocks an SM in the
 // backward 68 us (three blocks, which spill: 79 with two heads, 113 with four; one block 108), eight lanes a row 82; forward
 // 38 us with four heads and four blocks (eight heads and three blocks 35, but a call of four tokens then takes 4.3 us instead of
-// 3.3, on fewer SMs; five blocks, which spill, 52). A block works on queries or on keys; dw is kept in registers over its walk through the units, summed per block and then
-// by a second kernel in a fixed order: atomics on its 128 addresses would cost time, and another result every time.
+// 3.3, on fewer SMs; five blocks, which spill, 52). A block works on queries or on keys; dw is kept in registers over its walk
+// through the units, summed per block and then by a second kernel in a fixed order: atomics on its 128 addresses would cost
+// time, and another result every time.
 #include "lvx_internal.h"
 #include "sm100_prims.cuh"
 #include <algorithm>
