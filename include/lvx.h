@@ -367,13 +367,17 @@ typedef struct lvx_window {
 /* Scratch of lvx_window_forward and lvx_window_backward for these sizes. */
 int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_bytes, size_t* bwd_bytes);
 /* o dense [B, Hq, Sq, 128] in shape.dtype, lse fp32 [B*Hq, Sq] (a row without keys: zeros and -inf). q, k, v may have any
- * strides for 16-bit types, and are dense for fp32. Keys from n_b on are never looked at, whatever they hold. */
+ * strides for 16-bit types, and are dense for fp32. Keys from n_b on are never looked at, whatever they hold.
+ * o_low: [B*Hq, LVX_LOW_ROWS, 128] in o's type, or NULL (always for fp32): what rounding O to 16 bits dropped, of the rows at
+ * positions below LVX_LOW_ROWS, by position; others are left as they were. With it the backward's gradients are more accurate
+ * where rows see few keys. */
+#define LVX_LOW_ROWS 256
 int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* q, const lvx_view* k, const lvx_view* v,
-                       const int32_t* kv_valid_len, float sm_scale, void* workspace, size_t workspace_bytes, void* o, float* lse,
-                       void* stream);
-/* dq, dk, dv dense, in shape.dtype; o, d_o dense. */
+                       const int32_t* kv_valid_len, float sm_scale, void* workspace, size_t workspace_bytes, void* o, void* o_low,
+                       float* lse, void* stream);
+/* dq, dk, dv dense, in shape.dtype; o, d_o dense; o_low: the forward's, or NULL. */
 int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o, const lvx_view* q, const lvx_view* k,
-                        const lvx_view* v, const void* o, const float* lse, const int32_t* kv_valid_len, float sm_scale,
+                        const lvx_view* v, const void* o, const void* o_low, const float* lse, const int32_t* kv_valid_len, float sm_scale,
                         void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream);
 
 /* Attention for a batch that shares long prefixes: the B requests of `s` (a multiple of `prefixes`; the first B / prefixes

@@ -32,6 +32,7 @@ SYMBOLS = [
 MAX_PEERS = 16      # LVX_MAX_PEERS
 P2P_SLOTS = 8       # LVX_P2P_SLOTS
 HEAD_NORM_SCRATCH = 606208      # LVX_HEAD_NORM_SCRATCH
+LOW_ROWS = 256                  # LVX_LOW_ROWS
 
 
 class LvxShape(ctypes.Structure):
@@ -128,8 +129,8 @@ def load():
     lib.lvx_head_norm_rope_bwd.argtypes = [hp, viewp, viewp, viewp, viewp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
     winp, szp = ctypes.POINTER(LvxWindow), ctypes.POINTER(ctypes.c_size_t)
     lib.lvx_window_workspace.argtypes = [sp, winp, szp, szp]
-    lib.lvx_window_forward.argtypes = [sp, winp, viewp, viewp, viewp, vp, ctypes.c_float, vp, ctypes.c_size_t, vp, vp, vp]
-    lib.lvx_window_backward.argtypes = [sp, winp, vp, viewp, viewp, viewp, vp, vp, vp, ctypes.c_float, vp, ctypes.c_size_t, vp, vp,
+    lib.lvx_window_forward.argtypes = [sp, winp, viewp, viewp, viewp, vp, ctypes.c_float, vp, ctypes.c_size_t, vp, vp, vp, vp]
+    lib.lvx_window_backward.argtypes = [sp, winp, vp, viewp, viewp, viewp, vp, vp, vp, vp, ctypes.c_float, vp, ctypes.c_size_t, vp, vp,
                                         vp, vp]
     i32, sz = ctypes.c_int, ctypes.c_size_t
     lib.lvx_shared_workspace.argtypes = [sp, i32, i32, szp, szp]

@@ -681,16 +681,20 @@ int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_by
 // The partials of a windowed forward, or where they are not needed (and o is given) its results.
 static int window_forward(const lvx_shape* s, const lvx_window* w, const FwdPlan& p, bool few, const lvx_view* q, const lvx_view* k,
                           const lvx_view* v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                          float* lse, int* sp, Order order, cudaStream_t st) {
+                          void* o_low, float* lse, int* sp, Order order, cudaStream_t st) {
   if (s->dtype == LVX_FP32)
     return launch_fwd_block_general(*s, p, q->data, k->data, v->data, kv_valid_len, nullptr, sm_scale, o_part, ml_part, st, w);
   if (few) return launch_window_rows(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, sp, order, st);
-  return launch_window_fwd(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, lse, sp, order, st);
+  return launch_window_fwd(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, o_low, lse, sp, order, st);
+}
+
+static LowRows low_rows(const lvx_shape* s, const lvx_window* w, void* o_low, const int32_t* kv_valid_len) {
+  return {static_cast<uint16_t*>(o_low), kv_valid_len, w->query_start, s->Skv, s->Sq, s->Hq};
 }
 
 int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* q, const lvx_view* k, const lvx_view* v,
-                       const int32_t* kv_valid_len, float sm_scale, void* workspace, size_t workspace_bytes, void* o, float* lse,
-                       void* stream) {
+                       const int32_t* kv_valid_len, float sm_scale, void* workspace, size_t workspace_bytes, void* o, void* o_low,
+                       float* lse, void* stream) {
   const char* who = "lvx_window_forward";
   int rc = check_window(s, w, who);
   if (!rc) rc = check_qkv_views(s, q, k, v, who);
@@ -698,6 +702,7 @@ int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* 
   if (rc) return rc;
   if (!(sm_scale > 0.f)) return fail(LVX_ERR_SHAPE, "%s: sm_scale must be positive", who);
   LVX_REQUIRE_PTR(o, who);
+  if (o_low && s->dtype == LVX_FP32) return fail(LVX_ERR_DTYPE, "%s: nothing of O is dropped in fp32", who);
   LVX_REQUIRE_PTR(lse, who);
   bool few;
   const FwdPlan p = plan_window(*s, *w, &few);
@@ -707,16 +712,16 @@ int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* 
   int* sp = status_ptr();
   if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (need == 0) return window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, nullptr, nullptr, o, lse, sp, ORDER_AFTER, st);
+  if (need == 0) return window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, nullptr, nullptr, o, o_low, lse, sp, ORDER_AFTER, st);
   float* o_part = static_cast<float*>(workspace);
   float* ml_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_part_bytes);
-  rc = window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, o_part, ml_part, nullptr, nullptr, sp, ORDER_AFTER, st);
-  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st, ORDER_OVERLAP);
+  rc = window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, o_part, ml_part, nullptr, nullptr, nullptr, sp, ORDER_AFTER, st);
+  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st, ORDER_OVERLAP, low_rows(s, w, o_low, kv_valid_len));
 }
 
 int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o, const lvx_view* q, const lvx_view* k,
-                        const lvx_view* v, const void* o, const float* lse, const int32_t* kv_valid_len, float sm_scale,
-                        void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream) {
+                        const lvx_view* v, const void* o, const void* o_low, const float* lse, const int32_t* kv_valid_len,
+                        float sm_scale, void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream) {
   const char* who = "lvx_window_backward";
   int rc = check_window(s, w, who);
   if (!rc) rc = check_qkv_views(s, q, k, v, who);
@@ -725,6 +730,7 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
   if (!(sm_scale > 0.f)) return fail(LVX_ERR_SHAPE, "%s: sm_scale must be positive", who);
   LVX_REQUIRE_PTR(d_o, who);
   LVX_REQUIRE_PTR(o, who);
+  if (o_low && s->dtype == LVX_FP32) return fail(LVX_ERR_DTYPE, "%s: nothing of O is dropped in fp32", who);
   LVX_REQUIRE_PTR(lse, who);
   LVX_REQUIRE_PTR(dq, who);
   LVX_REQUIRE_PTR(workspace, who);
@@ -744,7 +750,7 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
   float* parts = direct ? nullptr : dq_acc + window_dq_floats(*s);
   const cudaError_t e = cudaMemsetAsync(dq_acc, 0, direct ? rows * 512 : window_dq_floats(*s) * 4, st);
   if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dq)");
-  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
+  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st, low_rows(s, w, const_cast<void*>(o_low), kv_valid_len)))) return rc;
   if (s->Skv > 0) {
     const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
     rc = direct ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, dq_acc,
@@ -849,11 +855,11 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
   if (s->Skv > 0) {
     o_own = take(c.own_plan.o_part_bytes);
     ml_own = take(c.own_plan.ml_part_bytes);
-    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, sp, pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
+    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, nullptr, sp, pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
       return rc;
   }
   if ((rc = window_forward(&c.pre, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre,
-                           nullptr, nullptr, sp, s->Skv > 0 ? ORDER_BESIDE : pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
+                           nullptr, nullptr, nullptr, sp, s->Skv > 0 ? ORDER_BESIDE : pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
     return rc;
   return launch_shared_combine(*s, prefixes, o_pre, ml_pre, c.pre_plan.nsplit, o_own, ml_own, o_own ? c.own_plan.nsplit : 0, o, lse, st);
 }

@@ -22,7 +22,7 @@ template <int OUT, int WPR>
 __global__ void __launch_bounds__(256)
 fwd_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ ml_part, const float* __restrict__ o_in,
                    const float* __restrict__ lse_in, void* __restrict__ o_out, float* __restrict__ lse_out,
-                   int rows_per_slab, int nsplit, long total_rows, const int* status) {
+                   int rows_per_slab, int nsplit, long total_rows, const int* status, const LowRows low) {
   grid_dep_wait();
   grid_dep_read(o_part);
   grid_dep_read(ml_part);
@@ -90,12 +90,20 @@ fwd_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ m
     }
   }
   store4<OUT>(o_out, size_t(grow) * 32 + lane, acc);
+  if constexpr (OUT < 2) {
+    if (low.data != nullptr) {
+      const int bh = unsigned(grow) / unsigned(low.sq);
+      if (uint16_t* dst = low.row(bh, int(grow) - bh * low.sq))
+        reinterpret_cast<uint2*>(dst)[lane] = make_uint2(rest16x2<OUT == 0>(acc.x, acc.y, pack16x2<OUT == 0>(acc.x, acc.y)),
+                                                         rest16x2<OUT == 0>(acc.z, acc.w, pack16x2<OUT == 0>(acc.z, acc.w)));
+    }
+  }
   if (lane == 0) lse_out[grow] = lse_new;
 }
 
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
-                       cudaStream_t st, Order order) {
+                       cudaStream_t st, Order order, const LowRows& low) {
   const long total_rows = long(q_blocks_of(s)) * s.B * s.Hq * s.Sq;
   const int threads = 256;
   const int* sp = device_status_ptr();
@@ -105,7 +113,7 @@ int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part
   const bool wide = total_rows <= 148 * 8 && p.nsplit > 8;
   auto go = [&](auto one, auto eight) {
     return launch_kernel(order, wide ? eight : one, dim3(unsigned(wide ? total_rows : blocks)), threads, 0, st, o_part, ml_part, o_in,
-                         lse_in, o_out, lse_out, p.rows, p.nsplit, total_rows, sp);
+                         lse_in, o_out, lse_out, p.rows, p.nsplit, total_rows, sp, low);
   };
   const cudaError_t e = out == LVX_BF16   ? go(fwd_combine_kernel<0, 1>, fwd_combine_kernel<0, 8>)
                         : out == LVX_FP16 ? go(fwd_combine_kernel<1, 1>, fwd_combine_kernel<1, 8>)
@@ -165,10 +173,11 @@ int launch_fwd_merge_parts(const lvx_shape& s, const float* o_parts, const float
 // ---------------------------------------------------------------------------------------------
 // delta = rowsum(O * dO): 16 bytes a lane (a half-warp per 16-bit row), four rows in flight per lane group: 65,536 rows of
 // bf16 in 7.6 us against 23 with one row per warp.
-template <int IN>
+// LOW: rows at early positions have an O in two parts (LowRows).
+template <int IN, bool LOW = false>
 __global__ void __launch_bounds__(256)
 bwd_prep_kernel(const void* __restrict__ o, const void* __restrict__ d_o, float* __restrict__ delta, long total_rows,
-                const int* status) {
+                const int* status, const LowRows low) {
   constexpr int LANES = IN == 2 ? 32 : 16, GROUPS = 256 / LANES, U = 4;
   grid_dep_wait();
   grid_dep_launch();
@@ -186,6 +195,19 @@ bwd_prep_kernel(const void* __restrict__ o, const void* __restrict__ d_o, float*
   for (int u = 0; u < U; ++u) {
     const uint32_t x[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, y[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
     float v = 0.f;
+    if constexpr (LOW) {
+      const int row = int(min(row0 + u * GROUPS, total_rows - 1)), bh = unsigned(row) / unsigned(low.sq);      // (below 2^31: 256 bytes each)
+      if (const uint16_t* rest = low.row(bh, row - bh * low.sq)) {
+        const uint4 c = reinterpret_cast<const uint4*>(rest)[l];
+        const uint32_t z[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 r = unpack16x2<IN == 0>(z[i]), q = unpack16x2<IN == 0>(y[i]);
+          v = fmaf(r.x, q.x, v);
+          v = fmaf(r.y, q.y, v);
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (IN == 2) {
@@ -202,15 +224,16 @@ bwd_prep_kernel(const void* __restrict__ o, const void* __restrict__ d_o, float*
   }
 }
 
-int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st) {
+int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st, const LowRows& low) {
   const long total_rows = long(q_blocks_of(s)) * s.B * s.Hq * s.Sq;
   const int threads = 256;
   const int* sp = device_status_ptr();
   const long per_block = (s.dtype == LVX_FP32 ? 8 : 16) * 4;
   const long blocks = (total_rows + per_block - 1) / per_block;
-  if (s.dtype == LVX_BF16) bwd_prep_kernel<0><<<blocks, threads, 0, st>>>(o, d_o, delta, total_rows, sp);
-  else if (s.dtype == LVX_FP16) bwd_prep_kernel<1><<<blocks, threads, 0, st>>>(o, d_o, delta, total_rows, sp);
-  else bwd_prep_kernel<2><<<blocks, threads, 0, st>>>(o, d_o, delta, total_rows, sp);
+  auto go = [&](auto kern) { kern<<<blocks, threads, 0, st>>>(o, d_o, delta, total_rows, sp, low); };
+  if (s.dtype == LVX_BF16) low.data ? go(bwd_prep_kernel<0, true>) : go(bwd_prep_kernel<0>);
+  else if (s.dtype == LVX_FP16) low.data ? go(bwd_prep_kernel<1, true>) : go(bwd_prep_kernel<1>);
+  else go(bwd_prep_kernel<2>);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "bwd_prep launch");
   return LVX_OK;

@@ -70,6 +70,23 @@ int launch_fwd_rows(const lvx_shape& s, const FwdPlan& p, const void* q, const v
                     const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
                     cudaStream_t st);
 // Windowed causal attention (window.cuh): few packed rows (partials), and the kernel for more (partials, or O and lse).
+// What the rounding of O to 16 bits dropped, of the rows at the first kLowRows positions of a text: [B * Hq][kLowRows][128], by
+// position, in O's type. The backward makes delta from both parts there: such rows see few keys, and in dS the error of a rounded
+// O is then as large as the rounding of dS itself (texts of 16 tokens, bf16: gradients off by 2.80e-3 -> 2.41e-3, of 300
+// 2.49e-3 -> 2.38e-3). Rows behind that many positions hardly change it, and the parts of all rows cost 4 to 6 % of a training pass.
+constexpr int kLowRows = LVX_LOW_ROWS;
+struct LowRows {
+  uint16_t* data;                // nullptr: not kept
+  const int32_t* kv_valid_len;
+  int start, skv, sq, heads;     // start: query_start; heads: Hq
+  // the part of row `tok` of (batch entry, head) `bh`, or nullptr
+  __device__ __forceinline__ uint16_t* row(int bh, int tok) const {
+    if (data == nullptr) return nullptr;
+    const int valid = kv_valid_len ? min(skv, max(0, kv_valid_len[bh / heads])) : skv;
+    const int pos = (start >= 0 ? start : valid - sq) + tok;
+    return pos >= 0 && pos < kLowRows ? data + (size_t(bh) * kLowRows + pos) * 128 : nullptr;
+  }
+};
 // How a kernel stands to the one before it in the stream: it starts when that one is complete; or comes onto the SMs while that
 // one, of the same call, still runs, and waits for it itself, at its start or, needing none of its results, at its end
 // (sm100_prims.cuh). The kernels of own keys and of a shared prefix stand beside each other: one token of 32 requests with 2,048
@@ -94,7 +111,7 @@ int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p
                        Order order, cudaStream_t st);
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                      float* lse, int* status, Order order, cudaStream_t st);
+                      void* o_low, float* lse, int* status, Order order, cudaStream_t st);
 // Its backward for 16-bit types: dq_acc (window_dq_floats of them, zeroed) is in tile order, launch_window_dq rounds it and
 // adds up the parts (window_sink_floats of them) of the sinks' dK and dV.
 size_t window_dq_floats(const lvx_shape& s);
@@ -113,8 +130,8 @@ int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int
                      cudaStream_t st);
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
-                       cudaStream_t st, Order order = ORDER_AFTER);
-int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st);
+                       cudaStream_t st, Order order = ORDER_AFTER, const LowRows& low = {});
+int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st, const LowRows& low = {});
 int launch_bwd_block(const lvx_shape& s, const void* q, const void* d_o, const float* lse, const float* delta,
                      const void* k, const void* v, const int32_t* kv_valid_len, float sm_scale, float* dq_acc,
                      float* dk_acc, float* dv_acc, int accumulate_dkdv, int* status, cudaStream_t st,

@@ -352,6 +352,14 @@ __device__ __forceinline__ float2 unpack16x2(uint32_t v) {
   if (IS_BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
+template <bool IS_BF16>
+__device__ __forceinline__ uint32_t pack16x2(float lo, float hi) { return IS_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi); }
+// What the rounding of (lo, hi) to `packed` dropped, rounded itself.
+template <bool IS_BF16>
+__device__ __forceinline__ uint32_t rest16x2(float lo, float hi, uint32_t packed) {
+  const float2 f = unpack16x2<IS_BF16>(packed);
+  return pack16x2<IS_BF16>(lo - f.x, hi - f.y);
+}
 // The last kernel of a forward or backward pass (combine, add_cast, the general backward where dQ needs no cast) also tells
 // the host: status[2..3] hold the address of the host's copy of the word where the library has set one up, and every warp
 // that found the word set and left its work undone writes it there (the word may be set while the kernel runs, so that no

@@ -81,6 +81,7 @@ struct WinFwdParams {
   int nsplit;
   bool beside;          // ORDER_BESIDE
   void* o;              // [B, Hq, Sq, 128] in the input type, with lse; nullptr: partials
+  uint16_t* o_low;      // LOW
   float* lse;
   float *o_part, *ml_part;
   const uint16_t *q, *k, *v;      // for window_plain_row
@@ -99,7 +100,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // row belongs: in the input type and divided by l (`out16`), or as it is.
 struct PlainRow {
   const uint16_t *q, *k, *v;
-  uint16_t* out16;
+  uint16_t *out16, *low16;
   float* out;
   int first, step, n, j0, lo, hi, sink_end;
   float m, l;
@@ -118,7 +119,9 @@ __device__ __noinline__ void window_plain_row(const WinFwdParams& p, const KeyTi
     for (int i = 0; i < 32; i += 2) {
       if (x.out16 != nullptr) {
         const float inv = x.l > 0.f ? 1.f / x.l : 0.f;
-        reinterpret_cast<uint32_t*>(x.out16 + d)[i / 2] = IS_BF16 ? pack_bf16x2(o[i] * inv, o[i + 1] * inv) : pack_f16x2(o[i] * inv, o[i + 1] * inv);
+        const uint32_t high = pack16x2<IS_BF16>(o[i] * inv, o[i + 1] * inv);
+        reinterpret_cast<uint32_t*>(x.out16 + d)[i / 2] = high;
+        if (x.low16 != nullptr) reinterpret_cast<uint32_t*>(x.low16 + d)[i / 2] = rest16x2<IS_BF16>(o[i] * inv, o[i + 1] * inv, high);
       } else {
         x.out[d + i] = o[i];
         x.out[d + i + 1] = o[i + 1];
@@ -130,7 +133,8 @@ __device__ __noinline__ void window_plain_row(const WinFwdParams& p, const KeyTi
 // PAIR: the slab has a single query tile (65 to 128 rows: a token each of 32 requests that share a prefix), and the two
 // warpgroups take turns at its key tiles instead of one of them idling: each has an accumulator and a partial result of its
 // own, and a key tile costs half of the softmax' time, which is then below that of its bytes.
-template <bool IS_BF16, bool PAIR>
+// LOW: what O's rounding drops of early rows is kept (LowRows); a form of its own, since the mere question costs the others 2 %.
+template <bool IS_BF16, bool PAIR, bool LOW = false>
 __global__ void __launch_bounds__(WF_THREADS, 1)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WinFwdParams p) {
@@ -450,6 +454,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 16; ++i) sum2 = add2(sum2, f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
         };
+        auto low_row = [&] {
+          const int pos = I.start + tok;
+          return LOW && exists && pos >= 0 && pos < kLowRows ? p.o_low + ((size_t(I.slab) * p.g + head) * kLowRows + pos) * 128 : nullptr;
+        };
         if (direct) {
           const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
 #pragma unroll 1
@@ -466,13 +474,29 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const float x = __uint_as_float(o[q][8 * i + 2 * e]) * inv, y = __uint_as_float(o[q][8 * i + 2 * e + 1]) * inv;
-                  w4[e] = IS_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                  w4[e] = pack16x2<IS_BF16>(x, y);
                 }
                 *reinterpret_cast<uint4*>(out + lane * 128 + (((q * 4 + i) ^ (lane & 7)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
               }
               bad(o[q]);
             }
             store(h * 128);
+            if constexpr (LOW) {
+              if (uint16_t* low = low_row()) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    uint32_t w4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                      const float x = __uint_as_float(o[q][8 * i + 2 * e]) * inv, y = __uint_as_float(o[q][8 * i + 2 * e + 1]) * inv;
+                      w4[e] = rest16x2<IS_BF16>(x, y, pack16x2<IS_BF16>(x, y));
+                    }
+                    reinterpret_cast<uint4*>(low + h * 64)[q * 4 + i] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                  }
+              }
+            }
           }
           if (exists) p.lse[size_t(I.slab) * slab_rows + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         } else {
@@ -503,6 +527,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           x.q = p.q + batch * p.q_b + (kvh * p.g + head) * p.q_h + tok * p.q_s;
           x.k = p.k + batch * p.k_b + kvh * p.k_h;
           x.v = p.v + batch * p.v_b + kvh * p.v_h;
+          x.low16 = low_row();
           x.out16 = direct ? reinterpret_cast<uint16_t*>(base + size_t(row) * 256) : nullptr;
           x.out = reinterpret_cast<float*>(base + size_t(row) * 512);
           x.first = first;
@@ -813,7 +838,7 @@ int make_kv_map(CUtensorMap* out, const lvx_shape& s, const lvx_view& v, const l
 
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
-                      float* lse, int* status, Order order, cudaStream_t st) {
+                      void* o_low, float* lse, int* status, Order order, cudaStream_t st) {
   const QTiles qt = make_q_tiles(s.Hq / s.Hkv, s.Sq);
   CUtensorMap tmQ, tmK, tmV;
   int rc = make_q_map(&tmQ, s, qt, q);
@@ -833,6 +858,7 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
   p.nsplit = pl.nsplit;
   p.beside = order == ORDER_BESIDE;
   p.o = o;
+  p.o_low = static_cast<uint16_t*>(o_low);
   p.lse = lse;
   p.o_part = o_part;
   p.ml_part = ml_part;
@@ -857,12 +883,13 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WF_SMEM);
     if (e == cudaSuccess) e = launch_kernel(order, kern, grid, WF_THREADS, WF_SMEM, st, tmQ, tmK, tmV, p);
   };
-  auto pick = [&](auto one, auto two) {
+  auto pick = [&](auto one, auto two, auto low) {
     if (pair) go(two);
+    else if (o != nullptr && o_low != nullptr) go(low);
     else go(one);
   };
-  if (s.dtype == LVX_BF16) pick(window_fwd_kernel<true, false>, window_fwd_kernel<true, true>);
-  else pick(window_fwd_kernel<false, false>, window_fwd_kernel<false, true>);
+  if (s.dtype == LVX_BF16) pick(window_fwd_kernel<true, false>, window_fwd_kernel<true, true>, window_fwd_kernel<true, false, true>);
+  else pick(window_fwd_kernel<false, false>, window_fwd_kernel<false, true>, window_fwd_kernel<false, false, true>);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(window fwd)");
   e = cudaGetLastError();
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "window_fwd_kernel launch");

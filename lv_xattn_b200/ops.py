@@ -668,19 +668,28 @@ def _window_setup(q, k, window, sinks, query_start):
     return call
 
 
-def window_forward(q, k, v, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len):
-    """(o [B, Hq, Sq, 128], lse fp32 [B*Hq, Sq]) of causal attention (lvx_window says which keys a query sees). The caller has
-    checked the tensors."""
+# Longer texts do without the dropped part of O's early rows: their gradients' error is that of the other rows (4,096 tokens with
+# a window of 1,024, bf16: 2.46e-3 -> 2.38e-3), and the forward that keeps it is slower (79 -> 86 us there; 2 x 2,048 tokens 46 ->
+# 48 us, shorter texts wait for the host).
+_LOW_TOKENS = 2048
+
+
+def window_forward(q, k, v, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len, training: bool = False):
+    """(o [B, Hq, Sq, 128], lse fp32 [B*Hq, Sq]) of causal attention (lvx_window says which keys a query sees), and with
+    `training` what o's rounding dropped of early rows, for the backward (None where there are none). The caller has checked
+    the tensors."""
     shp, win, nbytes, _ = _window_setup(q, k, window, sinks, query_start)
     qv, kv, vv = _text_view(q), _text_view(k), _text_view(v)
     B, Hq, Sq, _ = q.shape
     o = q.new_empty(q.shape)
     lse = q.new_empty((B * Hq, Sq), dtype=torch.float32)
     ws = lse.new_empty(nbytes // 4) if nbytes else None
+    early = training and q.dtype != torch.float32 and Sq <= _LOW_TOKENS and query_start < _lib.LOW_ROWS      # (-1: the lengths decide)
+    low = q.new_empty((B * Hq, _lib.LOW_ROWS, 128)) if early else None
     _lib.check(_lib.load().lvx_window_forward(shp, win, _ref(qv), _ref(kv), _ref(vv), _data(kv_valid_len), sm_scale, _data(ws),
-                                              nbytes, o.data_ptr(), lse.data_ptr(), _lib.stream_int()), "lvx_window_forward")
+                                              nbytes, o.data_ptr(), _data(low), lse.data_ptr(), _lib.stream_int()), "lvx_window_forward")
     _count(2 if nbytes else 1)
-    return o, lse
+    return (o, lse, low) if training else (o, lse)
 
 
 def _dense(t):
@@ -688,14 +697,14 @@ def _dense(t):
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def window_backward(do, q, k, v, o, lse, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len):
-    """(dq, dk, dv) of window_forward."""
+def window_backward(do, q, k, v, o, low, lse, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len):
+    """(dq, dk, dv) of window_forward; `low`: the third that it returned, or None."""
     shp, win, _, nbytes = _window_setup(q, k, window, sinks, query_start)
     qv, kv, vv = _text_view(q), _text_view(k), _text_view(v)
     do = _dense(do)
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     ws = lse.new_empty(nbytes // 4)
-    _lib.check(_lib.load().lvx_window_backward(shp, win, do.data_ptr(), _ref(qv), _ref(kv), _ref(vv), o.data_ptr(),
+    _lib.check(_lib.load().lvx_window_backward(shp, win, do.data_ptr(), _ref(qv), _ref(kv), _ref(vv), o.data_ptr(), _data(low),
                                                lse.data_ptr(), _data(kv_valid_len), sm_scale, ws.data_ptr(), nbytes, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                                _lib.stream_int()), "lvx_window_backward")
     _count(2 if q.dtype == torch.float32 else 3)

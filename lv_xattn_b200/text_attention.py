@@ -76,8 +76,8 @@ class WindowAttentionFunc(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, sm_scale, window, sinks, query_start, kv_valid_len):
-        o, lse = ops.window_forward(q, k, v, sm_scale, window, sinks, query_start, kv_valid_len)
-        ctx.save_for_backward(q, k, v, o, lse, kv_valid_len)
+        o, lse, low = ops.window_forward(q, k, v, sm_scale, window, sinks, query_start, kv_valid_len, True)
+        ctx.save_for_backward(q, k, v, o, low, lse, kv_valid_len)
         ctx.args = sm_scale, window, sinks, query_start
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -88,9 +88,9 @@ class WindowAttentionFunc(torch.autograd.Function):
     def backward(ctx, do, _):
         if do is None:
             return (None,) * 8
-        q, k, v, o, lse, kv_valid_len = ctx.saved_tensors
+        q, k, v, o, low, lse, kv_valid_len = ctx.saved_tensors
         with on_device(q):
-            grads = ops.window_backward(do, q, k, v, o, lse, *ctx.args, kv_valid_len)
+            grads = ops.window_backward(do, q, k, v, o, low, lse, *ctx.args, kv_valid_len)
         return (*(g if want else None for g, want in zip(grads, ctx.needs_input_grad)), None, None, None, None, None)
 
 
