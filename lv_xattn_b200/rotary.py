@@ -35,34 +35,37 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
     like = q if q is not None else k
     if like is None:
         raise ValueError("head_norm_rope: q or k must be given")
+    dtype, device = like.dtype, like.device
     for t in (q, k):
         if t is not None and (t.dim() != 4 or t.shape[3] != 128):
             raise ValueError(f"head_norm_rope: q and k must be [batch, tokens, heads, 128], got {tuple(t.shape)}")
-    if like.dtype not in _TYPES:
-        raise ValueError(f"head_norm_rope: dtype {like.dtype} unsupported; expected bfloat16, float16 or float32")
-    if q is not None and k is not None and (q.dtype != k.dtype or q.shape[:2] != k.shape[:2]):
+    if dtype not in _TYPES:
+        raise ValueError(f"head_norm_rope: dtype {dtype} unsupported; expected bfloat16, float16 or float32")
+    B, S = like.shape[:2]
+    if q is not None and k is not None and (k.dtype != dtype or k.shape[:2] != (B, S)):
         raise ValueError("head_norm_rope: q and k must agree on dtype, batch and tokens")
     if (q is None and q_weight is not None) or (k is None and k_weight is not None):
         raise ValueError("head_norm_rope: a weight without the tensor that it scales")
     weight = q_weight if q_weight is not None else k_weight
-    for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (128,) or (w.dtype != like.dtype and w.dtype != torch.float32) or w.dtype != weight.dtype):
-            raise ValueError("head_norm_rope: weights must be [128], both fp32 or both in the dtype of q and k")
+    if weight is not None:
+        kind = weight.dtype
+        for w in (q_weight, k_weight):
+            if w is not None and (w.shape != (128,) or (kind != dtype and kind != torch.float32) or w.dtype != kind):
+                raise ValueError("head_norm_rope: weights must be [128], both fp32 or both in the dtype of q and k")
     if (cos is None) != (sin is None):
         raise ValueError("head_norm_rope: cos and sin go together")
-    if cos is None and weight is None:
-        raise ValueError("head_norm_rope: neither a weight nor cos and sin: nothing to do")
     if cos is not None:
-        B, S = like.shape[:2]
-        if cos.shape != sin.shape or tuple(cos.shape) not in ((S, 128), (1, S, 128), (B, S, 128)):
+        shape, kind = cos.shape, cos.dtype
+        if sin.shape != shape or not (shape == (B, S, 128) or shape == (S, 128) or shape == (1, S, 128)):
             raise ValueError(f"head_norm_rope: cos and sin must be [{S}, 128] or [1 or {B}, {S}, 128], got {tuple(cos.shape)} and {tuple(sin.shape)}")
-        if cos.dtype != sin.dtype or (cos.dtype != like.dtype and cos.dtype != torch.float32):
+        if sin.dtype != kind or (kind != dtype and kind != torch.float32):
             raise ValueError("head_norm_rope: cos and sin must be fp32 or in the dtype of q and k")
+    elif weight is None:
+        raise ValueError("head_norm_rope: neither a weight nor cos and sin: nothing to do")
     if not eps >= 0:
         raise ValueError("head_norm_rope: eps must be non-negative")
-    device = like.device
     for t in (q, k, cos, sin, q_weight, k_weight):
-        if t is not None and (not t.is_cuda or t.device != device):
+        if t is not None and (t.device != device or not t.is_cuda):
             if not t.is_cuda:
                 raise _lib.LvxError("lv_xattn_b200 runs on CUDA tensors only; there is no CPU path")
             raise ValueError("head_norm_rope: all tensors must be on one device")
@@ -121,6 +124,8 @@ def head_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1
     args = (q, k, q_weight, k_weight, cos, sin, float(eps))
     with on_device(like):
         watch_status(like)
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)
+                                        or (q_weight is not None and q_weight.requires_grad)
+                                        or (k_weight is not None and k_weight.requires_grad)):
             return HeadNormRopeFunc.apply(*args)
         return ops.head_norm_rope(*args)
