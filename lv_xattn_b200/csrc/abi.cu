@@ -748,9 +748,9 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
   float* delta = static_cast<float*>(workspace);
   float* dq_acc = direct ? static_cast<float*>(dq) : reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(rows * 4));
   float* parts = direct ? nullptr : dq_acc + window_dq_floats(*s);
-  const cudaError_t e = cudaMemsetAsync(dq_acc, 0, direct ? rows * 512 : window_dq_floats(*s) * 4, st);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dq)");
-  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st, low_rows(s, w, const_cast<void*>(o_low), kv_valid_len)))) return rc;
+  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st, low_rows(s, w, const_cast<void*>(o_low), kv_valid_len), dq_acc,
+                            direct ? rows * 512 : window_dq_floats(*s) * 4)))
+    return rc;
   if (s->Skv > 0) {
     const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
     rc = direct ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, dq_acc,
@@ -908,9 +908,7 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
   float* acc = reinterpret_cast<float*>(at);
   const size_t acc_bytes = round256(f32 ? c.rows * 512 : window_dq_floats(c.pre) * 4);
   float* acc_own = s->Skv > 0 ? reinterpret_cast<float*>(at + acc_bytes) : nullptr;
-  const cudaError_t e = cudaMemsetAsync(acc, 0, static_cast<char*>(workspace) + need - at, st);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dq)");
-  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st))) return rc;
+  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st, {}, acc, static_cast<char*>(workspace) + need - at))) return rc;
   const bool dense = q->stride_s == 128 && q->stride_h == int64_t(s->Sq) * 128 && q->stride_b == int64_t(s->Hq) * s->Sq * 128;
   const bool pack = c.packed || !dense;
   if (pack && (rc = launch_pack_rows(*s, prefixes, *q, d_o, lse, delta, q_p, do_p, lse_p, delta_p, ORDER_OVERLAP, st))) return rc;

@@ -173,11 +173,13 @@ int launch_fwd_merge_parts(const lvx_shape& s, const float* o_parts, const float
 // ---------------------------------------------------------------------------------------------
 // delta = rowsum(O * dO): 16 bytes a lane (a half-warp per 16-bit row), four rows in flight per lane group: 65,536 rows of
 // bf16 in 7.6 us against 23 with one row per warp.
-// LOW: rows at early positions have an O in two parts (LowRows).
-template <int IN, bool LOW = false>
+// TEXT: rows at early positions have an O in two parts (LowRows), and the accumulator of dQ is cleared on the way: its writes beside
+// the reads here instead of a launch of their own (backward of 4,096 tokens with a window of 1,024 284 -> 280 us, of 2 x 2,048
+// 140 -> 135, of 100 36 -> 32).
+template <int IN, bool TEXT = false>
 __global__ void __launch_bounds__(256)
 bwd_prep_kernel(const void* __restrict__ o, const void* __restrict__ d_o, float* __restrict__ delta, long total_rows,
-                const int* status, const LowRows low) {
+                const int* status, const LowRows low, uint4* __restrict__ zero, size_t zero_pieces) {
   constexpr int LANES = IN == 2 ? 32 : 16, GROUPS = 256 / LANES, U = 4;
   grid_dep_wait();
   grid_dep_launch();
@@ -191,11 +193,13 @@ bwd_prep_kernel(const void* __restrict__ o, const void* __restrict__ d_o, float*
     a[u] = reinterpret_cast<const uint4*>(o)[at];
     b[u] = reinterpret_cast<const uint4*>(d_o)[at];
   }
+  if constexpr (TEXT)
+    for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < zero_pieces; i += size_t(gridDim.x) * 256) zero[i] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t x[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, y[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
     float v = 0.f;
-    if constexpr (LOW) {
+    if (TEXT && IN < 2 && low.data != nullptr) {
       const int row = int(min(row0 + u * GROUPS, total_rows - 1)), bh = unsigned(row) / unsigned(low.sq);      // (below 2^31: 256 bytes each)
       if (const uint16_t* rest = low.row(bh, row - bh * low.sq)) {
         const uint4 c = reinterpret_cast<const uint4*>(rest)[l];
@@ -224,16 +228,17 @@ bwd_prep_kernel(const void* __restrict__ o, const void* __restrict__ d_o, float*
   }
 }
 
-int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st, const LowRows& low) {
+int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st, const LowRows& low, void* zero,
+                    size_t zero_bytes) {
   const long total_rows = long(q_blocks_of(s)) * s.B * s.Hq * s.Sq;
   const int threads = 256;
   const int* sp = device_status_ptr();
   const long per_block = (s.dtype == LVX_FP32 ? 8 : 16) * 4;
   const long blocks = (total_rows + per_block - 1) / per_block;
-  auto go = [&](auto kern) { kern<<<blocks, threads, 0, st>>>(o, d_o, delta, total_rows, sp, low); };
-  if (s.dtype == LVX_BF16) low.data ? go(bwd_prep_kernel<0, true>) : go(bwd_prep_kernel<0>);
-  else if (s.dtype == LVX_FP16) low.data ? go(bwd_prep_kernel<1, true>) : go(bwd_prep_kernel<1>);
-  else go(bwd_prep_kernel<2>);
+  auto go = [&](auto kern) { kern<<<blocks, threads, 0, st>>>(o, d_o, delta, total_rows, sp, low, static_cast<uint4*>(zero), zero_bytes / 16); };
+  if (s.dtype == LVX_BF16) zero ? go(bwd_prep_kernel<0, true>) : go(bwd_prep_kernel<0>);
+  else if (s.dtype == LVX_FP16) zero ? go(bwd_prep_kernel<1, true>) : go(bwd_prep_kernel<1>);
+  else zero ? go(bwd_prep_kernel<2, true>) : go(bwd_prep_kernel<2>);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "bwd_prep launch");
   return LVX_OK;

@@ -131,7 +131,8 @@ int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int
 int launch_fwd_combine(const lvx_shape& s, const FwdPlan& p, const float* o_part, const float* ml_part,
                        const float* o_in, const float* lse_in, void* o_out, float* lse_out, int out_is_final,
                        cudaStream_t st, Order order = ORDER_AFTER, const LowRows& low = {});
-int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st, const LowRows& low = {});
+int launch_bwd_prep(const lvx_shape& s, const void* o, const void* d_o, float* delta, cudaStream_t st, const LowRows& low = {},
+                    void* zero = nullptr, size_t zero_bytes = 0);      // memory to be cleared on the way, a multiple of 16 bytes
 int launch_bwd_block(const lvx_shape& s, const void* q, const void* d_o, const float* lse, const float* delta,
                      const void* k, const void* v, const int32_t* kv_valid_len, float sm_scale, float* dq_acc,
                      float* dk_acc, float* dv_acc, int accumulate_dkdv, int* status, cudaStream_t st,
