@@ -659,8 +659,8 @@ static int check_qkv_views(const lvx_shape* s, const lvx_view* q, const lvx_view
 }
 
 static size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
-static size_t window_fwd_bytes(const lvx_shape* s, const FwdPlan& p, bool few) {
-  const bool direct = !few && p.nsplit == 1 && s->dtype != LVX_FP32;
+static size_t window_fwd_bytes(const lvx_shape* s, const FwdPlan& p) {
+  const bool direct = p.nsplit == 1 && s->dtype != LVX_FP32;
   return direct ? 0 : p.o_part_bytes + p.ml_part_bytes;
 }
 static size_t window_bwd_bytes(const lvx_shape* s, const lvx_window* w) {
@@ -673,7 +673,7 @@ int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_by
   if (rc) return rc;
   bool few;
   const FwdPlan p = plan_window(*s, *w, &few);
-  if (fwd_bytes) *fwd_bytes = window_fwd_bytes(s, p, few);
+  if (fwd_bytes) *fwd_bytes = window_fwd_bytes(s, p);
   if (bwd_bytes) *bwd_bytes = window_bwd_bytes(s, w);
   return LVX_OK;
 }
@@ -684,12 +684,8 @@ static int window_forward(const lvx_shape* s, const lvx_window* w, const FwdPlan
                           void* o_low, float* lse, int* sp, Order order, cudaStream_t st) {
   if (s->dtype == LVX_FP32)
     return launch_fwd_block_general(*s, p, q->data, k->data, v->data, kv_valid_len, nullptr, sm_scale, o_part, ml_part, st, w);
-  if (few) return launch_window_rows(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, sp, order, st);
+  if (few) return launch_window_rows(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, o_low, lse, sp, order, st);
   return launch_window_fwd(*s, *w, p, *q, *k, *v, kv_valid_len, sm_scale, o_part, ml_part, o, o_low, lse, sp, order, st);
-}
-
-static LowRows low_rows(const lvx_shape* s, const lvx_window* w, void* o_low, const int32_t* kv_valid_len) {
-  return {static_cast<uint16_t*>(o_low), kv_valid_len, w->query_start, s->Skv, s->Sq, s->Hq};
 }
 
 int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* q, const lvx_view* k, const lvx_view* v,
@@ -706,7 +702,7 @@ int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* 
   LVX_REQUIRE_PTR(lse, who);
   bool few;
   const FwdPlan p = plan_window(*s, *w, &few);
-  const size_t need = window_fwd_bytes(s, p, few);
+  const size_t need = window_fwd_bytes(s, p);
   if (need) LVX_REQUIRE_PTR(workspace, who);
   if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
   int* sp = status_ptr();
@@ -716,7 +712,7 @@ int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* 
   float* o_part = static_cast<float*>(workspace);
   float* ml_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_part_bytes);
   rc = window_forward(s, w, p, few, q, k, v, kv_valid_len, sm_scale, o_part, ml_part, nullptr, nullptr, nullptr, sp, ORDER_AFTER, st);
-  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st, ORDER_OVERLAP, low_rows(s, w, o_low, kv_valid_len));
+  return rc ? rc : launch_fwd_combine(*s, p, o_part, ml_part, nullptr, nullptr, o, lse, 1, st, ORDER_OVERLAP, low_rows(*s, *w, o_low, kv_valid_len));
 }
 
 int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o, const lvx_view* q, const lvx_view* k,
@@ -748,7 +744,7 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
   float* delta = static_cast<float*>(workspace);
   float* dq_acc = direct ? static_cast<float*>(dq) : reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(rows * 4));
   float* parts = direct ? nullptr : dq_acc + window_dq_floats(*s);
-  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st, low_rows(s, w, const_cast<void*>(o_low), kv_valid_len), dq_acc,
+  if ((rc = launch_bwd_prep(*s, o, d_o, delta, st, low_rows(*s, *w, const_cast<void*>(o_low), kv_valid_len), dq_acc,
                             direct ? rows * 512 : window_dq_floats(*s) * 4)))
     return rc;
   if (s->Skv > 0) {
@@ -792,10 +788,10 @@ static int shared_call(SharedCall* c, const lvx_shape* s, int prefixes, int pref
 
 // Forward: its plans, and the scratch.
 static size_t shared_fwd_plan(SharedCall* c, const lvx_shape* s) {
-  c->pre_plan = plan_window(c->pre, c->pre_win, &c->pre_few);
+  c->pre_plan = plan_window(c->pre, c->pre_win, &c->pre_few, true);
   size_t n = c->pre_plan.o_part_bytes + c->pre_plan.ml_part_bytes + round256(c->rows * 128 * elt_size(s->dtype));
   if (s->Skv > 0) {
-    c->own_plan = plan_window(*s, c->own_win, &c->own_few);
+    c->own_plan = plan_window(*s, c->own_win, &c->own_few, true);
     n += c->own_plan.o_part_bytes + c->own_plan.ml_part_bytes;
   }
   return n;

@@ -66,6 +66,9 @@ fwd_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ m
     const float inv = 1.f / lsum;
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
     lse_loc = (mmax + log2f(lsum)) * kLn2;
+  } else if (low.sq > 0 && lsum != 0.f) {      // a text call: NaN stays
+    acc = make_float4(lsum, lsum, lsum, lsum);
+    lse_loc = lsum;
   } else {
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
   }

@@ -87,6 +87,9 @@ struct LowRows {
     return pos >= 0 && pos < kLowRows ? data + (size_t(bh) * kLowRows + pos) * 128 : nullptr;
   }
 };
+inline LowRows low_rows(const lvx_shape& s, const lvx_window& w, void* o_low, const int32_t* kv_valid_len) {
+  return {static_cast<uint16_t*>(o_low), kv_valid_len, w.query_start, s.Skv, s.Sq, s.Hq};
+}
 // How a kernel stands to the one before it in the stream: it starts when that one is complete; or comes onto the SMs while that
 // one, of the same call, still runs, and waits for it itself, at its start or, needing none of its results, at its end
 // (sm100_prims.cuh). The kernels of own keys and of a shared prefix stand beside each other: one token of 32 requests with 2,048
@@ -107,7 +110,7 @@ inline cudaError_t launch_kernel(Order order, void (*kernel)(P...), dim3 grid, u
   return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
 }
 int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
-                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
+                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o, void* o_low, float* lse, int* status,
                        Order order, cudaStream_t st);
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,

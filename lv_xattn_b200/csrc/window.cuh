@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t visible_bits(int key0, int lo, int hi, int s
 
 // Split of the key tiles over CTAs, and the layout of the partial results (FwdPlan's, with rows in the order of
 // [B, Hq, Sq]); shared by the launchers and the workspace query. nsplit == 1 and not `few`: results are written directly.
-FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few);
+FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few, bool merged = false);
 
 // SMs of the current device.
 inline int num_sms() {

@@ -771,7 +771,8 @@ static bool window_even(const lvx_shape& s, const lvx_window& w, long tiles) {
   return w.query_start >= s.Skv || 8l * s.Sq <= tiles * 128;
 }
 
-FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few) {
+// `merged`: the parts are merged with others in any case.
+FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few, bool merged) {
   *few = false;
   if (s.dtype == LVX_FP32) return plan_fwd(s);
   const int g = s.Hq / s.Hkv;
@@ -791,7 +792,7 @@ FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few) {
   p.nsplit = 1;
   for (long ns = 1; ns <= most && (ns == 1 || base * ns <= 148 * 8); ++ns) {
     const long rounds = (base * ns + 147) / 148, per = (tiles + ns - 1) / ns;
-    const long cost = rounds * (per + 3) + (ns > 1 && !*few ? 4 : 0);
+    const long cost = rounds * (per + 3) + (ns > 1 && !(merged && *few) ? 4 : 0);
     if (cost < best_cost) {
       best_cost = cost;
       p.nsplit = int(ns);
