@@ -659,8 +659,8 @@ static int check_qkv_views(const lvx_shape* s, const lvx_view* q, const lvx_view
 }
 
 static size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
-static size_t window_fwd_bytes(const lvx_shape* s, const FwdPlan& p) {
-  const bool direct = p.nsplit == 1 && s->dtype != LVX_FP32;
+static size_t window_fwd_bytes(const lvx_shape* s, const FwdPlan& p, bool few) {
+  const bool direct = p.nsplit <= (few ? kRowCluster : 1) && s->dtype != LVX_FP32;
   return direct ? 0 : p.o_part_bytes + p.ml_part_bytes;
 }
 static size_t window_bwd_bytes(const lvx_shape* s, const lvx_window* w) {
@@ -673,7 +673,7 @@ int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_by
   if (rc) return rc;
   bool few;
   const FwdPlan p = plan_window(*s, *w, &few);
-  if (fwd_bytes) *fwd_bytes = window_fwd_bytes(s, p);
+  if (fwd_bytes) *fwd_bytes = window_fwd_bytes(s, p, few);
   if (bwd_bytes) *bwd_bytes = window_bwd_bytes(s, w);
   return LVX_OK;
 }
@@ -702,7 +702,7 @@ int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* 
   LVX_REQUIRE_PTR(lse, who);
   bool few;
   const FwdPlan p = plan_window(*s, *w, &few);
-  const size_t need = window_fwd_bytes(s, p);
+  const size_t need = window_fwd_bytes(s, p, few);
   if (need) LVX_REQUIRE_PTR(workspace, who);
   if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
   int* sp = status_ptr();

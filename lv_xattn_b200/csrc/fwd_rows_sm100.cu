@@ -24,8 +24,11 @@
 // and v of any strides. The CTAs of a slab share out the key tiles that its queries turn out to see. What lies behind
 // the last valid key may hold anything: its scores are replaced and its rows of V cleared in shared memory (each warp its
 // own keys' rows). Where keys that only some rows see hold an infinity or a NaN, the others' outputs are made again as
-// plain sums (rows_plain_values), as in window_fwd_sm100.cu. A CTA that walks all of its slab's keys writes O and lse itself,
-// without scratch and a second kernel: eight tokens behind 512 keys 22 -> 18.4 us a call, 32 behind 8,192 164 -> 156.
+// plain sums (rows_plain_values), as in window_fwd_sm100.cu. Up to eight CTAs that share out a slab's keys are a cluster: they read
+// one another's (max, sum, O) in shared memory, merge them in the order of the keys, a share of the rows each, and write O and
+// lse; a CTA that walks all of them writes its own. That needs no scratch and no second kernel. us a call, and on the GPU
+// (a captured one): eight tokens behind 512 keys (one CTA a slab) 22 / 7.1 -> 18 / 6.8, behind 4,096 (two) 29.3 / 25.6 -> 27.9 /
+// 25.0; one token behind 1,024 (eight) 22 / 7.0 -> 18 / 6.5, behind 8,192 (eight instead of seventeen) 22.6 / 9.3 -> 18 / 12.
 #include "lvx_internal.h"
 #include "sm100_prims.cuh"
 #include "window.cuh"
@@ -56,7 +59,7 @@ struct RowsParams {
   // WIN
   WindowMask mask;
   bool beside;            // ORDER_BESIDE
-  void* o;                // one split: O [slab][rows][128] in the input type and lse [slab][rows]; nullptr: partials
+  void* o;                // a cluster a slab: O [slab][rows][128] in the input type and lse [slab][rows]; nullptr: partials
   float* lse;
   LowRows low;
   int sq, g;
@@ -75,6 +78,57 @@ __device__ __noinline__ float4 rows_plain_values(float4 o, const uint16_t* q, co
     o = make_float4(fmaf(w, a.x, o.x), fmaf(w, a.y, o.y), fmaf(w, b.x, o.z), fmaf(w, b.y, o.w));
   }
   return o;
+}
+
+// Four columns of a row's O, and its lse.
+template <bool IS_BF16>
+__device__ __forceinline__ void rows_result(const RowsParams& p, int slab, int row, int c4, float m, float l, float4 x) {
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
+  x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  const size_t at = size_t(slab) * p.rows + row;
+  const uint2 high = make_uint2(pack16x2<IS_BF16>(x.x, x.y), pack16x2<IS_BF16>(x.z, x.w));
+  static_cast<uint2*>(p.o)[at * 32 + c4] = high;
+  if (c4 == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  if (uint16_t* low = p.low.row(slab * p.g + row / p.sq, row % p.sq))
+    reinterpret_cast<uint2*>(low)[c4] = make_uint2(rest16x2<IS_BF16>(x.x, x.y, high.x), rest16x2<IS_BF16>(x.z, x.w, high.y));
+}
+// The end of a CTA of a cluster: its (max, sum, O) lie in the third stage, if it got as far. The cluster's CTAs stay until all of
+// them have read what they need.
+constexpr int FR_OFF_PART = 2 * FR_STAGE, FR_OFF_PART_ML = FR_OFF_PART + 64 * 512;
+template <bool IS_BF16>
+__device__ __forceinline__ void rows_merge_cluster(const RowsParams& p, uint8_t* smem, int* cta_ok, int slab, int rank, bool ok) {
+  const int tid = threadIdx.x;
+  if (tid == 0) *cta_ok = ok;
+  __syncwarp();
+  cluster_sync();
+  bool all = true;
+  for (int r = 0; r < p.nsplit; ++r) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(smem_u32(cta_ok), r)) : "memory");
+    all = all && v != 0;
+  }
+  if (!all && tid == 0) publish_status(p.status);      // this is the call's last kernel
+  const int mine = rank < p.rows ? (p.rows - 1 - rank) / p.nsplit + 1 : 0;
+  if (all && tid < FR_WARPS * 32)
+    for (int i = tid; i < mine * 32; i += FR_WARPS * 32) {
+      const int row = rank + (i >> 5) * p.nsplit, c4 = i & 31;
+      const uint32_t part = smem_u32(smem + FR_OFF_PART) + row * 512 + c4 * 16, ml = smem_u32(smem + FR_OFF_PART_ML) + row * 8;
+      float m = -INFINITY;
+      for (int r = 0; r < p.nsplit; ++r) m = fmaxf(m, cluster_ld2(cluster_addr(ml, r)).x);
+      const float moff = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int r = 0; r < p.nsplit; ++r) {
+        const float2 s = cluster_ld2(cluster_addr(ml, r));
+        const float4 v = cluster_ld4(cluster_addr(part, r));
+        const float w = ex2f(s.x - moff);
+        l = fmaf(s.y, w, l);
+        x = make_float4(fmaf(v.x, w, x.x), fmaf(v.y, w, x.y), fmaf(v.z, w, x.z), fmaf(v.w, w, x.w));
+      }
+      rows_result<IS_BF16>(p, slab, row, c4, m, l, x);
+    }
+  __syncwarp();
+  cluster_sync();
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -143,23 +197,23 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     *abort_flag = 0;
     fence_mbar_init();
   }
+  const bool merge = WIN && p.o != nullptr;
+  int* cta_ok = const_cast<int*>(abort_flag) + 1;
   if (__syncthreads_or(word)) {
-    if (WIN && p.o != nullptr && tid == 0) publish_status(p.status);      // this is the call's last kernel
+    if (merge) rows_merge_cluster<IS_BF16>(p, smem, cta_ok, slab, split, false);
     return;
   }
 
   float* o_dst = p.o_part + (size_t(slab) * p.nsplit + split) * p.rows * 128;
   float* ml_dst = p.ml_part + (size_t(slab) * p.nsplit + split) * p.rows * 2;
-  if (WIN && n == 0 && p.o != nullptr) {
-    for (int i = tid; i < p.rows * 16; i += FR_THREADS) static_cast<uint4*>(p.o)[size_t(slab) * p.rows * 16 + i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int i = tid; i < p.rows; i += FR_THREADS) p.lse[size_t(slab) * p.rows + i] = -INFINITY;
-    for (int i = tid; i < p.rows * 16; i += FR_THREADS)
-      if (uint16_t* low = p.low.row(slab * p.g + (i >> 4) / p.sq, (i >> 4) % p.sq)) reinterpret_cast<uint4*>(low)[i & 15] = make_uint4(0u, 0u, 0u, 0u);
-    return;
+  if (merge) {
+    o_dst = reinterpret_cast<float*>(smem + FR_OFF_PART);
+    ml_dst = reinterpret_cast<float*>(smem + FR_OFF_PART_ML);
   }
   if (n == 0) {      // nothing valid in this key range: the empty partial (O = 0, max = -inf, sum = 0)
     for (int i = tid; i < p.rows * 32; i += FR_THREADS) reinterpret_cast<float4*>(o_dst)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = tid; i < p.rows; i += FR_THREADS) reinterpret_cast<float2*>(ml_dst)[i] = make_float2(-INFINITY, 0.f);
+    if (merge) rows_merge_cluster<IS_BF16>(p, smem, cta_ok, slab, split, true);
     return;
   }
 
@@ -377,7 +431,7 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   float* mml = mo + FR_WARPS * 16 * FR_LDO;
   asm volatile("bar.sync 1, %0;" ::"n"(FR_WARPS * 32) : "memory");
   if (*abort_flag) {
-    if (WIN && p.o != nullptr && tid == 0) publish_status(p.status);
+    if (merge) rows_merge_cluster<IS_BF16>(p, smem, cta_ok, slab, split, false);
     return;
   }
   {
@@ -431,22 +485,14 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         }
       }
     }
-    if constexpr (WIN) {
-      if (p.o != nullptr) {
-        const float inv = ls > 0.f ? 1.f / ls : ls == 0.f ? 0.f : ls;      // (NaN stays)
-        const size_t at = size_t(slab) * p.rows + row;
-        const float4 x = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-        const uint2 high = make_uint2(pack16x2<IS_BF16>(x.x, x.y), pack16x2<IS_BF16>(x.z, x.w));
-        static_cast<uint2*>(p.o)[at * 32 + c4] = high;
-        if (c4 == 0) p.lse[at] = ls == 0.f ? -INFINITY : (mm + log2f(ls)) * 0.6931471805599453f;
-        if (uint16_t* low = p.low.row(slab * p.g + row / p.sq, row % p.sq))
-          reinterpret_cast<uint2*>(low)[c4] = make_uint2(rest16x2<IS_BF16>(x.x, x.y, high.x), rest16x2<IS_BF16>(x.z, x.w, high.y));
-        continue;
-      }
+    if (merge && p.nsplit == 1) {
+      rows_result<IS_BF16>(p, slab, row, c4, mm, ls, acc);
+      continue;
     }
     reinterpret_cast<float4*>(o_dst)[row * 32 + c4] = acc;
     if (c4 == 0) *reinterpret_cast<float2*>(ml_dst + row * 2) = make_float2(mm, ls);
   }
+  if (merge && p.nsplit > 1) rows_merge_cluster<IS_BF16>(p, smem, cta_ok, slab, split, true);
 }
 
 int launch_fwd_rows(const lvx_shape& s, const FwdPlan& pl, const void* q, const void* k, const void* v,
@@ -525,7 +571,23 @@ int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FR_SMEM);
-    if (e == cudaSuccess) e = launch_kernel(order, kern, grid, FR_THREADS, FR_SMEM, st, tmK, tmV, p);
+    if (e != cudaSuccess) return;
+    if (o == nullptr) {
+      e = launch_kernel(order, kern, grid, FR_THREADS, FR_SMEM, st, tmK, tmV, p);
+      return;
+    }
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = grid.x;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3(FR_THREADS);
+    c.dynamicSmemBytes = FR_SMEM;
+    c.stream = st;
+    c.attrs = &attr;
+    c.numAttrs = 1;
+    e = cudaLaunchKernelEx(&c, kern, tmK, tmV, p);
   };
   auto pick = [&](auto bf16) {
     constexpr bool B16 = decltype(bf16)::value;

@@ -69,7 +69,6 @@ constexpr int kFewRows = 64;
 int launch_fwd_rows(const lvx_shape& s, const FwdPlan& p, const void* q, const void* k, const void* v,
                     const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, int* status,
                     cudaStream_t st);
-// Windowed causal attention (window.cuh): few packed rows (partials), and the kernel for more (partials, or O and lse).
 // What the rounding of O to 16 bits dropped, of the rows at the first kLowRows positions of a text: [B * Hq][kLowRows][128], by
 // position, in O's type. The backward makes delta from both parts there: such rows see few keys, and in dS the error of a rounded
 // O is then as large as the rounding of dS itself (texts of 16 tokens, bf16: gradients off by 2.80e-3 -> 2.41e-3, of 300
@@ -109,9 +108,12 @@ inline cudaError_t launch_kernel(Order order, void (*kernel)(P...), dim3 grid, u
   c.numAttrs = order == ORDER_AFTER ? 0 : 1;
   return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
 }
+// Windowed causal attention (window.cuh): few packed rows (partials; or O and lse, where plan_window has a slab's keys shared out over
+// a cluster of at most kRowCluster CTAs), and the kernel for more (partials, or O and lse).
+constexpr int kRowCluster = 8;
 int launch_window_rows(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
-                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o, void* o_low, float* lse, int* status,
-                       Order order, cudaStream_t st);
+                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
+                       void* o_low, float* lse, int* status, Order order, cudaStream_t st);
 int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& p, const lvx_view& q, const lvx_view& k,
                       const lvx_view& v, const int32_t* kv_valid_len, float sm_scale, float* o_part, float* ml_part, void* o,
                       void* o_low, float* lse, int* status, Order order, cudaStream_t st);

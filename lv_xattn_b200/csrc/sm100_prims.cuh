@@ -392,6 +392,25 @@ struct GridDep {      // at the top of a kernel; `late`: launched with ORDER_BES
 };
 template <class P>
 __device__ __forceinline__ void grid_dep_read(P& p) { asm volatile("" : "+l"(p) : : "memory"); }
+// Barrier of all threads of a cluster that have not exited (whole warps), and reads of another CTA's shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t smem_addr, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 cluster_ld2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 // Product of two 128-wide 16-bit rows in fp32.
 template <bool IS_BF16>
 __device__ __forceinline__ float dot128(const void* a, const void* b) {

@@ -787,12 +787,16 @@ FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few, bool mer
   if (pair) tiles = (tiles + 1) / 2;      // what a CTA walks takes half as long
   const long most = std::min<long>(tiles > 0 ? tiles : 1, *few ? 148 : 64);
   // Splits that fill whole rounds of 148 SMs, eight rounds at most (the fixed cost then outweighs what a partly filled last round
-  // wastes): 3 tiles' worth of fixed cost per item, and 4 for a second kernel where one would do without.
+  // wastes): 3 tiles' worth of fixed cost per item, and 4 for a second kernel where one would do without. Few rows do without it
+  // as a cluster, which lies within one of eight groups of about 18 SMs (32 tokens behind 8,192 keys as 256 clusters of four: 172 us
+  // instead of 152 as 256 CTAs).
   long best_cost = std::numeric_limits<long>::max();
   p.nsplit = 1;
   for (long ns = 1; ns <= most && (ns == 1 || base * ns <= 148 * 8); ++ns) {
-    const long rounds = (base * ns + 147) / 148, per = (tiles + ns - 1) / ns;
-    const long cost = rounds * (per + 3) + (ns > 1 && !(merged && *few) ? 4 : 0);
+    const bool cluster = *few && !merged && ns > 1 && ns <= kRowCluster;
+    const long at_once = cluster ? 8 * (18 / ns) * ns : 148;
+    const long rounds = (base * ns + at_once - 1) / at_once, per = (tiles + ns - 1) / ns;
+    const long cost = rounds * (per + 3) + (ns == 1 || cluster || (*few && merged) ? 0 : 4);
     if (cost < best_cost) {
       best_cost = cost;
       p.nsplit = int(ns);

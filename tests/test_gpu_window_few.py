@@ -70,3 +70,24 @@ def test_nan_in_a_key(cuda_device, B, heads, Sq, Skv, window, dtype):
     assert hit.any()
     assert (o.isnan().all(-1) == hit).all() and (o.isnan().any(-1) == hit).all()
     assert (lse.view(B, heads[0], Sq).isnan() == hit).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("B,heads,Sq,Skv,window,sinks", [
+    (2, (8, 2), 1, 300, None, 0), (2, (8, 2), 8, 2000, None, 0), (2, (32, 2), 4, 1100, 500, 130), (1, (1, 1), 1, 20000, None, 0), (3, (16, 16), 64, 900, None, 0),
+])
+def test_shared_out(cuda_device, B, heads, Sq, Skv, window, sinks, dtype):
+    """Keys of a KV head shared out over CTAs that merge what they have, some of them without a key; the same result every time."""
+    q, k, v = inputs(cuda_device, B, *heads, Sq, Skv, dtype, Skv)
+    for valid in ([Skv] * B, [0] + [Skv // 2] * (B - 1), [1] + [Skv - 1] * (B - 1), [129] * B):
+        m = seen(Sq, Skv, valid, window, sinks, cuda_device)
+        o, lse = lvx.window_attention(q, k, v, window=window, sinks=sinks, kv_valid_len=valid, return_lse=True)
+        again, lse_again = lvx.window_attention(q, k, v, window=window, sinks=sinks, kv_valid_len=valid, return_lse=True)
+        assert torch.equal(o, again) and torch.equal(lse, lse_again)
+        ro, rl = exact(q, k, v, m)
+        assert v.abs().max() < 6
+        assert ((o.double() - ro).abs() <= torch.finfo(dtype).eps * 6).all()      # as above
+        empty = (~m.any(-1)).expand(B, heads[0], Sq)
+        lse = lse.view(B, heads[0], Sq).double()
+        assert (lse[empty] == float("-inf")).all() and (o[empty] == 0).all()
+        assert ((lse - rl)[~empty].abs() < 1e-4).all()
