@@ -759,6 +759,8 @@ int lvx_window_backward(const lvx_shape* s, const lvx_window* w, const void* d_o
 // The pieces of a call with shared prefixes: the prefix as an attention of packed rows, and the layout of the scratch.
 struct SharedCall {
   lvx_shape pre;            // B = prefixes, one "head" per packed row, Sq = 1
+  lvx_shape fwd;            // the same for the forward, which reads a single token's rows where they are: a "token" per request
+  bool in_place;            // that it does
   lvx_window pre_win, own_win;
   FwdPlan pre_plan, own_plan;
   bool pre_few, own_few;
@@ -788,8 +790,14 @@ static int shared_call(SharedCall* c, const lvx_shape* s, int prefixes, int pref
 
 // Forward: its plans, and the scratch.
 static size_t shared_fwd_plan(SharedCall* c, const lvx_shape* s) {
-  c->pre_plan = plan_window(c->pre, c->pre_win, &c->pre_few, true);
-  size_t n = c->pre_plan.o_part_bytes + c->pre_plan.ml_part_bytes + round256(c->rows * 128 * elt_size(s->dtype));
+  c->fwd = c->pre;
+  c->in_place = c->packed && s->Sq == 1 && s->dtype != LVX_FP32;      // (the fp32 kernels read dense rows)
+  if (c->in_place) {
+    c->fwd.Hq = s->Hq;
+    c->fwd.Sq = s->B / c->pre.B;
+  }
+  c->pre_plan = plan_window(c->fwd, c->pre_win, &c->pre_few, true);
+  size_t n = c->pre_plan.o_part_bytes + c->pre_plan.ml_part_bytes + (c->in_place ? 0 : round256(c->rows * 128 * elt_size(s->dtype)));
   if (s->Skv > 0) {
     c->own_plan = plan_window(*s, c->own_win, &c->own_few, true);
     n += c->own_plan.o_part_bytes + c->own_plan.ml_part_bytes;
@@ -820,18 +828,19 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
   int rc = shared_call(&c, s, prefixes, prefix_len, who);
   if (!rc) rc = check_qkv_views(s, q, s->Skv > 0 ? k : q, s->Skv > 0 ? v : q, who);
   if (rc) return rc;
-  const lvx_view packed_q = dense_view(c.packed ? workspace : q->data, c.pre.Hq, 1);
-  if ((rc = check_qkv_views(&c.pre, &packed_q, pk, pv, who)) || (rc = check_arch())) return rc;
+  const size_t need = shared_fwd_plan(&c, s);
+  const lvx_view packed_q = c.in_place ? lvx_view{q->data, (s->B / prefixes) * q->stride_b, q->stride_h, q->stride_b}
+                                       : dense_view(c.packed ? workspace : q->data, c.pre.Hq, 1);
+  if ((rc = check_qkv_views(&c.fwd, &packed_q, pk, pv, who)) || (rc = check_arch())) return rc;
   if (!(sm_scale > 0.f)) return fail(LVX_ERR_SHAPE, "%s: sm_scale must be positive", who);
   LVX_REQUIRE_PTR(o, who);
   LVX_REQUIRE_PTR(lse, who);
   LVX_REQUIRE_PTR(workspace, who);
-  const size_t need = shared_fwd_plan(&c, s);
   if (workspace_bytes < need) return fail(LVX_ERR_WORKSPACE, "%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, need);
   int* sp = status_ptr();
   if (!sp) return fail(LVX_ERR_DRIVER, "%s: status word unavailable", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  char* at = static_cast<char*>(workspace) + round256(c.rows * 128 * elt_size(s->dtype));
+  char* at = static_cast<char*>(workspace) + (c.in_place ? 0 : round256(c.rows * 128 * elt_size(s->dtype)));
   auto take = [&](size_t n) {
     float* p = reinterpret_cast<float*>(at);
     at += n;
@@ -843,7 +852,7 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
   // q as it lies serves where the orders agree, if it is dense
   const bool dense = q->stride_s == 128 && q->stride_h == int64_t(s->Sq) * 128 && q->stride_b == int64_t(s->Hq) * s->Sq * 128;
   lvx_view pq = packed_q;
-  const bool pack = c.packed || !dense;
+  const bool pack = !c.in_place && (c.packed || !dense);
   if (pack) {
     pq.data = workspace;
     if ((rc = launch_pack_rows(*s, prefixes, *q, nullptr, nullptr, nullptr, workspace, nullptr, nullptr, nullptr, ORDER_AFTER, st))) return rc;
@@ -854,10 +863,10 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
     if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, nullptr, sp, pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
       return rc;
   }
-  if ((rc = window_forward(&c.pre, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre,
+  if ((rc = window_forward(&c.fwd, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre,
                            nullptr, nullptr, nullptr, sp, s->Skv > 0 ? ORDER_BESIDE : pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
     return rc;
-  return launch_shared_combine(*s, prefixes, o_pre, ml_pre, c.pre_plan.nsplit, o_own, ml_own, o_own ? c.own_plan.nsplit : 0, o, lse, st);
+  return launch_shared_combine(*s, prefixes, c.in_place, o_pre, ml_pre, c.pre_plan.nsplit, o_own, ml_own, o_own ? c.own_plan.nsplit : 0, o, lse, st);
 }
 
 int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const void* d_o, const lvx_view* q, const lvx_view* pk,

@@ -129,7 +129,7 @@ int launch_window_dq(const lvx_shape& s, const lvx_window& w, const float* acc, 
 // Around the windowed kernels for a batch that shares prefixes (shared_prefix.cu).
 int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const void* d_o, const float* lse, const float* delta,
                      void* q_out, void* do_out, float* lse_out, float* delta_out, Order order, cudaStream_t st);
-int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
+int launch_shared_combine(const lvx_shape& s, int prefixes, bool by_head, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
                           const float* ml_own, int ns_own, void* o, float* lse, cudaStream_t st);
 int launch_shared_dq(const lvx_shape& s, int prefixes, const float* acc_pre, int pre_slab_rows, const float* acc_own, void* dq,
                      cudaStream_t st);

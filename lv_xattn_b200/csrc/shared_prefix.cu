@@ -8,7 +8,8 @@
 // What is here are the small kernels around them, all bound by memory and small next to the prefix:
 //   pack      rows of q (dO, lse, delta) from [B, Hq, Sq] to [P, Hkv, B / P, Hq / Hkv, Sq]: one copy of the queries, against a
 //             prefix that is 100 to 100,000 times as long. Not done where the two orders are the same (one request per
-//             prefix, or one KV head).
+//             prefix, or one KV head), nor in the forward of single tokens in 16 bits, where the requests are the tokens of
+//             a view of q (eight tokens behind 6,404 keys 32 -> 29 us a call, 32 behind 102,464 128 -> 126 on the GPU).
 //   combine   partials of the prefix (packed rows) and of the own keys (rows of a request) -> O and lse
 //   dq        sum of the two fp32 accumulators, rounded once
 #include "combine.cuh"
@@ -17,10 +18,11 @@
 
 namespace lvx {
 
-// A row of [B, Hq, Sq] in the packed order [P, Hkv, per, g, Sq], per = B / P. Rows are counted in 32 bits (checked on the
+// A row of [B, Hq, Sq] in the packed order [P, Hkv, per, g, Sq], per = B / P, or with `by_head` (Sq = 1) [P, Hkv, g, per]. Rows are counted in 32 bits (checked on the
 // host): 64-bit divisions are most of what these kernels would execute.
 struct PackOrder {
   int hkv, g, sq, per;
+  bool by_head;
   __device__ __forceinline__ void split(int row, int& slab, int& in_slab) const {      // (KV head of a request, row in it)
     const int rows = g * sq;
     slab = row / rows;
@@ -30,11 +32,13 @@ struct PackOrder {
   __device__ __forceinline__ void packed(int slab, int in_slab, int& pslab, int& prow) const {
     const int b = slab / hkv, kvh = slab - b * hkv, p = b / per;
     pslab = p * hkv + kvh;
-    prow = (b - p * per) * g * sq + in_slab;
+    prow = by_head ? in_slab * per + b - p * per : (b - p * per) * g * sq + in_slab;
   }
   __device__ __forceinline__ int packed_rows() const { return per * g * sq; }
 };
-static PackOrder pack_order(const lvx_shape& s, int prefixes) { return PackOrder{s.Hkv, s.Hq / s.Hkv, s.Sq, s.B / prefixes}; }
+static PackOrder pack_order(const lvx_shape& s, int prefixes, bool by_head = false) {
+  return PackOrder{s.Hkv, s.Hq / s.Hkv, s.Sq, s.B / prefixes, by_head};
+}
 
 // ROW16: 16-byte pieces of a row (16: 16-bit types, 32: fp32), one a thread; a thread takes that piece of four rows, which are
 // in flight together (42,624 rows of bf16: 10 -> 6 us against one row a thread and 64-bit arithmetic).
@@ -173,14 +177,14 @@ int launch_pack_rows(const lvx_shape& s, int prefixes, const lvx_view& q, const 
   return e == cudaSuccess ? LVX_OK : cuda_fail(e, "pack_rows launch");
 }
 
-int launch_shared_combine(const lvx_shape& s, int prefixes, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
+int launch_shared_combine(const lvx_shape& s, int prefixes, bool by_head, const float* o_pre, const float* ml_pre, int ns_pre, const float* o_own,
                           const float* ml_own, int ns_own, void* o, float* lse, cudaStream_t st) {
   const int rows = s.B * s.Hq * s.Sq;
   // as in launch_fwd_combine: eight warps a row while the rows alone leave SMs empty and one warp's walk is long
   const bool wide = rows <= 148 * 8 && ns_pre + ns_own > 8;
   auto go = [&](auto one, auto eight) {
     return launch_kernel(ORDER_OVERLAP, wide ? eight : one, dim3(wide ? rows : (rows - 1) / 8 + 1), 256, 0, st, o_pre, ml_pre, ns_pre, o_own, ml_own,
-                         ns_own, pack_order(s, prefixes), o, lse, rows, device_status_ptr());
+                         ns_own, pack_order(s, prefixes, by_head), o, lse, rows, device_status_ptr());
   };
   const cudaError_t e = s.dtype == LVX_BF16   ? go(shared_combine_kernel<0, 1>, shared_combine_kernel<0, 8>)
                         : s.dtype == LVX_FP16 ? go(shared_combine_kernel<1, 1>, shared_combine_kernel<1, 8>)

@@ -721,7 +721,7 @@ _shared_calls: dict = {}
 
 
 def _shared_setup(q, pk, k):
-    """(shape as the library takes it, prefixes, length, forward scratch, backward scratch, launches around the block kernels)"""
+    """(shape as the library takes it, prefixes, length, forward scratch, backward scratch, launches of the forward, of the backward)"""
     key = (q.shape, pk.shape, None if k is None else k.shape[2], q.dtype)
     call = _shared_calls.get(key)
     if call is None:
@@ -733,7 +733,9 @@ def _shared_setup(q, pk, k):
         _lib.check(_lib.load().lvx_shared_workspace(shp, P, N, ctypes.byref(f), ctypes.byref(b)), "lvx_shared_workspace")
         if len(_shared_calls) >= 4096:
             _shared_calls.clear()
-        call = _shared_calls[key] = shp, P, N, f.value, b.value, (P < B and Hkv > 1) + (Skv > 0)
+        pack = P < B and Hkv > 1
+        call = _shared_calls[key] = (shp, P, N, f.value, b.value, 2 + (Skv > 0) + (pack and (Sq > 1 or q.dtype == torch.float32)),
+                                     3 + (Skv > 0) + pack)
     return call
 
 
@@ -746,7 +748,7 @@ def _text_views(*ts):
 def shared_forward(q, pk, pv, k, v, sm_scale: float, prefix_valid_len, kv_valid_len):
     """(o [B, Hq, Sq, 128], lse fp32 [B*Hq, Sq]) of attention over shared prefixes and own keys (lvx_shared_forward); k and v may
     be None. The caller has checked the tensors."""
-    shp, P, N, nbytes, _, more = _shared_setup(q, pk, k)
+    shp, P, N, nbytes, _, launches, _ = _shared_setup(q, pk, k)
     keep, (qv, pkv, pvv, kv, vv) = _text_views(q, pk, pv, k, v)
     B, Hq, Sq, _ = q.shape
     o = _dense_like(q)
@@ -755,13 +757,13 @@ def shared_forward(q, pk, pv, k, v, sm_scale: float, prefix_valid_len, kv_valid_
     _lib.check(_lib.load().lvx_shared_forward(shp, P, N, qv, pkv, pvv, _data(prefix_valid_len), kv, vv, _data(kv_valid_len),
                                               sm_scale, ws.data_ptr(), nbytes, o.data_ptr(), lse.data_ptr(), _lib.stream_int()),
                "lvx_shared_forward")
-    _count(2 + more)
+    _count(launches)
     return o, lse
 
 
 def shared_backward(do, q, pk, pv, k, v, o, lse, sm_scale: float, prefix_valid_len, kv_valid_len):
     """(dq, dpk, dpv, dk, dv) of shared_forward."""
-    shp, P, N, _, nbytes, more = _shared_setup(q, pk, k)
+    shp, P, N, _, nbytes, _, launches = _shared_setup(q, pk, k)
     keep, (qv, pkv, pvv, kv, vv) = _text_views(q, pk, pv, k, v)
     do = _dense(do)
     grads = [None if t is None else _dense_like(t) for t in (q, pk, pv, k, v)]
@@ -769,5 +771,5 @@ def shared_backward(do, q, pk, pv, k, v, o, lse, sm_scale: float, prefix_valid_l
     _lib.check(_lib.load().lvx_shared_backward(shp, P, N, do.data_ptr(), qv, pkv, pvv, _data(prefix_valid_len), kv, vv,
                                                _data(kv_valid_len), o.data_ptr(), lse.data_ptr(), sm_scale, ws.data_ptr(), nbytes,
                                                *(_data(t) for t in grads), _lib.stream_int()), "lvx_shared_backward")
-    _count(3 + more)
+    _count(launches)
     return grads

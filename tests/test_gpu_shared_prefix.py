@@ -194,3 +194,18 @@ def test_word_already_set(cuda_device):
             lib.lvx_p2p_set_timeout(120.0)
             _lib.device_status()
         assert torch.equal(lvx.shared_prefix_attention(*leaves), good)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,P,heads,N", [(6, 2, (8, 2), 300), (40, 1, (32, 8), 700), (64, 2, (16, 2), 1000), (5, 1, (12, 4), 129)])
+def test_single_tokens_where_they_are(cuda_device, B, P, heads, N, dtype):
+    """Queries of single tokens in layouts that are read without being packed, few rows and many: as in the dense layout."""
+    q, pk, pv, k, v, _ = inputs(cuda_device, B, P, *heads, 1, N, 50, dtype, B)
+    dense = lvx.shared_prefix_attention(q, pk, pv, k, v, return_lse=True)
+    wide = torch.full((B, heads[0], 3, 128), float("nan"), device=cuda_device, dtype=dtype)
+    wide[:, :, 1:2] = q
+    by_token = q.transpose(1, 2).contiguous().transpose(1, 2)
+    for other in (wide[:, :, 1:2], by_token):
+        o, lse = lvx.shared_prefix_attention(other, pk, pv, k, v, return_lse=True)
+        assert torch.equal(o, dense[0]) and torch.equal(lse, dense[1])
+    run_and_check(q, pk, pv, k, v, torch.randn_like(q), backward=False)
