@@ -860,7 +860,8 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
   if (s->Skv > 0) {
     o_own = take(c.own_plan.o_part_bytes);
     ml_own = take(c.own_plan.ml_part_bytes);
-    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr, nullptr, sp, pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
+    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr,
+                             nullptr, sp, pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
       return rc;
   }
   if ((rc = window_forward(&c.fwd, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre,
@@ -922,7 +923,8 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
   const lvx_view dov = dense_view(d_o, s->Hq, s->Sq);
   rc = f32 ? launch_bwd_block_general(c.pre, pq.data, pdo.data, pl, pd, pk->data, pv->data, prefix_valid_len, nullptr, sm_scale, acc,
                                       dpk, dpv, 2, st, &c.pre_win)
-           : launch_window_bwd(c.pre, c.pre_win, pq, pdo, *pk, *pv, pl, pd, prefix_valid_len, sm_scale, acc, nullptr, dpk, dpv, sp, ORDER_OVERLAP, st);
+           : launch_window_bwd(c.pre, c.pre_win, pq, pdo, *pk, *pv, pl, pd, prefix_valid_len, sm_scale, acc, nullptr, dpk, dpv, sp,
+                               ORDER_OVERLAP, st);
   if (!rc && s->Skv > 0)
     rc = f32 ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, acc_own, dk,
                                         dv, 2, st, &c.own_win)

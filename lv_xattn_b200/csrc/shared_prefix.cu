@@ -18,8 +18,8 @@
 
 namespace lvx {
 
-// A row of [B, Hq, Sq] in the packed order [P, Hkv, per, g, Sq], per = B / P, or with `by_head` (Sq = 1) [P, Hkv, g, per]. Rows are counted in 32 bits (checked on the
-// host): 64-bit divisions are most of what these kernels would execute.
+// A row of [B, Hq, Sq] in the packed order [P, Hkv, per, g, Sq], per = B / P, or with `by_head` (Sq = 1) [P, Hkv, g, per]. Rows are
+// counted in 32 bits (checked on the host): 64-bit divisions are most of what these kernels would execute.
 struct PackOrder {
   int hkv, g, sq, per;
   bool by_head;
