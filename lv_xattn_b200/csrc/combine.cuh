@@ -42,7 +42,10 @@ struct RowAcc {
 };
 __device__ __forceinline__ void row_merge(RowAcc& a, const RowAcc& b) {
   const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return;
+  if (m == -INFINITY) {
+    a.l += b.l;      // zeros, or the NaN of a side whose scores all are (row_four)
+    return;
+  }
   const float wa = exp2f(a.m - m), wb = exp2f(b.m - m);      // an empty side (max -inf) gets weight 0
   a.m = m;
   a.l = a.l * wa + b.l * wb;
@@ -52,9 +55,10 @@ __device__ __forceinline__ void row_merge(RowAcc& a, const RowAcc& b) {
   a.v.w = a.v.w * wa + b.v.w * wb;
 }
 
-// Four splits of a row from s0 on (those below nsplit), added to `a`.
+// Four splits of a row from s0 on (those below nsplit), added to `a`. The maxima ignore NaN, so that a split whose scores all are
+// NaN has the maximum of an empty one, -inf, and a sum of NaN; with `keep_nan` the row is NaN then, without it the split counts as empty.
 __device__ __forceinline__ void row_four(RowAcc& a, const float* __restrict__ o_part, const float* __restrict__ ml_part, size_t slab,
-                                         int nsplit, int rows_per_slab, int r, int s0, int lane) {
+                                         int nsplit, int rows_per_slab, int r, int s0, int lane, bool keep_nan) {
   float2 ml[4];
   float4 v[4];
 #pragma unroll
@@ -63,7 +67,12 @@ __device__ __forceinline__ void row_four(RowAcc& a, const float* __restrict__ o_
     const size_t prow = (slab * nsplit + s) * rows_per_slab + r;
     ml[u] = *reinterpret_cast<const float2*>(ml_part + prow * 2);
     v[u] = reinterpret_cast<const float4*>(o_part + prow * 128)[lane];
-    if (s0 + u >= nsplit) ml[u].x = -INFINITY;
+    if (s0 + u >= nsplit) ml[u] = make_float2(-INFINITY, 0.f);
+  }
+  if (keep_nan) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (ml[u].x == -INFINITY) a.l += ml[u].y;
   }
   const float m = fmaxf(fmaxf(a.m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
   if (m == -INFINITY) return;

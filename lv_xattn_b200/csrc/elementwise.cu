@@ -37,7 +37,7 @@ fwd_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ m
   a.m = -INFINITY;
   a.l = 0.f;
   a.v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = part * 4; s0 < nsplit; s0 += WPR * 4) row_four(a, o_part, ml_part, size_t(slab), nsplit, rows_per_slab, r, s0, lane);
+  for (int s0 = part * 4; s0 < nsplit; s0 += WPR * 4) row_four(a, o_part, ml_part, size_t(slab), nsplit, rows_per_slab, r, s0, lane, low.sq > 0);
   if constexpr (WPR > 1) {
     __shared__ float4 s_v[WPR][32];
     __shared__ float2 s_ml[WPR];
@@ -66,7 +66,7 @@ fwd_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ m
     const float inv = 1.f / lsum;
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
     lse_loc = (mmax + log2f(lsum)) * kLn2;
-  } else if (low.sq > 0 && lsum != 0.f) {      // a text call: NaN stays
+  } else if (low.sq > 0 && lsum != 0.f) {      // a text call (row_four): NaN stays
     acc = make_float4(lsum, lsum, lsum, lsum);
     lse_loc = lsum;
   } else {

@@ -106,8 +106,8 @@ shared_combine_kernel(const float* __restrict__ o_pre, const float* __restrict__
   // four partials at a time in flight (eight: 53 -> 73 us for 42,624 rows of seven and one, with half the warps an SM)
   const int groups = (ns_pre + 3) >> 2, own_groups = (ns_own + 3) >> 2;
   for (int i = part; i < groups + own_groups; i += WPR) {
-    if (i < groups) row_four(a, o_pre, ml_pre, pslab, ns_pre, order.packed_rows(), prow, i * 4, lane);
-    else row_four(a, o_own, ml_own, slab, ns_own, order.g * order.sq, in_slab, (i - groups) * 4, lane);
+    if (i < groups) row_four(a, o_pre, ml_pre, pslab, ns_pre, order.packed_rows(), prow, i * 4, lane, true);
+    else row_four(a, o_own, ml_own, slab, ns_own, order.g * order.sq, in_slab, (i - groups) * 4, lane, true);
   }
   if constexpr (WPR > 1) {
     __shared__ float4 s_v[WPR][32];
