@@ -860,13 +860,25 @@ int lvx_shared_forward(const lvx_shape* s, int prefixes, int prefix_len, const l
   if (s->Skv > 0) {
     o_own = take(c.own_plan.o_part_bytes);
     ml_own = take(c.own_plan.ml_part_bytes);
-    if ((rc = window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr,
-                             nullptr, sp, pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
-      return rc;
   }
-  if ((rc = window_forward(&c.fwd, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre,
-                           nullptr, nullptr, nullptr, sp, s->Skv > 0 ? ORDER_BESIDE : pack ? ORDER_OVERLAP : ORDER_AFTER, st)))
-    return rc;
+  auto own_keys = [&](Order order) {
+    return s->Skv == 0 ? LVX_OK
+                       : window_forward(s, &c.own_win, c.own_plan, c.own_few, q, k, v, kv_valid_len, sm_scale, o_own, ml_own, nullptr, nullptr,
+                                        nullptr, sp, order, st);
+  };
+  auto prefix = [&](Order order) {
+    return window_forward(&c.fwd, &c.pre_win, c.pre_plan, c.pre_few, &pq, pk, pv, prefix_valid_len, sm_scale, o_pre, ml_pre, nullptr,
+                          nullptr, nullptr, sp, order, st);
+  };
+  // Packed rows are read by the kernel that waits for the packing. The own keys' kernel reads the caller's tensors alone, and without
+  // packing so does the prefix' one: the second of them may stand beside the first. (The own keys first, which fill SMs faster, would
+  // take 53 us instead of 57 for four tokens of 32 requests behind 6,404 shared and 512 own keys, 77 tokens of eight are even; but then
+  // the packed rows' reader would not have waited for them.)
+  if (pack) {
+    if ((rc = prefix(ORDER_OVERLAP)) || (rc = own_keys(ORDER_BESIDE))) return rc;
+  } else {
+    if ((rc = own_keys(ORDER_AFTER)) || (rc = prefix(s->Skv > 0 ? ORDER_BESIDE : ORDER_AFTER))) return rc;
+  }
   return launch_shared_combine(*s, prefixes, c.in_place, o_pre, ml_pre, c.pre_plan.nsplit, o_own, ml_own, o_own ? c.own_plan.nsplit : 0, o, lse, st);
 }
 
@@ -928,7 +940,7 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
   if (!rc && s->Skv > 0)
     rc = f32 ? launch_bwd_block_general(*s, q->data, d_o, lse, delta, k->data, v->data, kv_valid_len, nullptr, sm_scale, acc_own, dk,
                                         dv, 2, st, &c.own_win)
-             : launch_window_bwd(*s, c.own_win, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, acc_own, nullptr, dk, dv, sp, ORDER_BESIDE, st);
+             : launch_window_bwd(*s, c.own_win, *q, dov, *k, *v, lse, delta, kv_valid_len, sm_scale, acc_own, nullptr, dk, dv, sp, ORDER_OVERLAP, st);
   if (rc) return rc;
   const QTiles pt = make_q_tiles(c.pre.Hq / c.pre.Hkv, 1);
   const int pre_slab_rows = f32 ? c.pre.Hq / c.pre.Hkv : pt.chunks * pt.heads;

@@ -374,10 +374,11 @@ __device__ __forceinline__ void publish_status(const int* status) {
 }
 // Kernels of one call that follow one another (enum Order): the next one is brought onto the SMs while this one still runs,
 // when all CTAs of this one have called grid_dep_launch or left, and waits in grid_dep_wait until this one is complete and
-// visible. Every kernel waits before it ends, so that completion is passed on along the call, and calls grid_dep_launch
-// after its wait, so that a kernel that follows one whose results it does not need finds all before that one complete:
-// it puts its wait off to its end (GridDep), and fills the SMs that the other one's last CTAs leave idle. Pointers that a
-// kernel reads through the non-coherent path go through grid_dep_read, so that no read of them can be moved before the wait.
+// visible. Every kernel waits before it ends, so that completion is passed on along the call. What a kernel of the call wrote is
+// read after a wait only: a kernel that puts its wait off to its end (GridDep), to fill the SMs that the last CTAs of the one
+// before leave idle, reads the caller's tensors alone. (They are complete: the call's first kernel starts in the stream's order,
+// and grid_dep_launch comes after a kernel's own wait.) Pointers that a kernel reads through the non-coherent path go through
+// grid_dep_read, so that no read of them can be moved before the wait.
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 struct GridDep {      // at the top of a kernel; `late`: launched with ORDER_BESIDE

@@ -76,7 +76,6 @@ struct SinkParts {
 struct WinBwdParams {
   int sq, skv, hkv, g, slabs, nitems;
   SinkParts sp;
-  bool beside;                         // ORDER_BESIDE
   float* parts;                        // [slab][sink tile][part][dK, dV][128][128]
   QTiles qt;
   WindowMask mask;
@@ -99,7 +98,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   float* s_stat = reinterpret_cast<float*>(smem + WB_OFF_STAT);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  GridDep dep(p.beside);
+  grid_dep_wait();      // delta and the cleared accumulator, and what packs the rows of a shared prefix
+  grid_dep_launch();
   const int heads = p.qt.heads, tile_rows = heads * p.qt.tokens;
   struct Item {
     int slab, kv0, valid, start;
@@ -683,7 +683,6 @@ int launch_window_bwd(const lvx_shape& s, const lvx_window& w, const lvx_view& q
   p.slabs = s.B * s.Hkv;
   p.sp = sink_parts(s, w);
   p.parts = parts;
-  p.beside = order == ORDER_BESIDE;
   p.nitems = ((s.Skv + 127) / 128 + p.sp.tiles * (p.sp.parts - 1)) * p.slabs;
   p.qt = qt;
   p.mask = make_window_mask(w);
