@@ -363,14 +363,16 @@ typedef struct lvx_window {
   int32_t window;        /* keys that a query sees, its own position included; 0 = all behind it */
   int32_t sinks;         /* leading keys that stay visible */
   int32_t query_start;   /* first_b for every batch entry; -1: first_b = n_b - Sq */
+  int32_t low_rows;      /* rows of o_low for each head (below); 0 = LVX_LOW_ROWS */
 } lvx_window;
 /* Scratch of lvx_window_forward and lvx_window_backward for these sizes. */
 int lvx_window_workspace(const lvx_shape* s, const lvx_window* w, size_t* fwd_bytes, size_t* bwd_bytes);
 /* o dense [B, Hq, Sq, 128] in shape.dtype, lse fp32 [B*Hq, Sq] (a row without keys: zeros and -inf). q, k, v may have any
  * strides for 16-bit types, and are dense for fp32. Keys from n_b on are never looked at, whatever they hold.
- * o_low: [B*Hq, LVX_LOW_ROWS, 128] in o's type, or NULL (always for fp32): what rounding O to 16 bits dropped, of the rows at
- * positions below LVX_LOW_ROWS, by position; others are left as they were. With it the backward's gradients are more accurate
- * where rows see few keys. */
+ * o_low: [B*Hq, low_rows, 128] in o's type, or NULL (always for fp32): what rounding O to 16 bits dropped, of the rows at
+ * positions below LVX_LOW_ROWS; others are left as they were. With it the backward's gradients are more accurate where rows
+ * see few keys. A head's rows lie by position, or where low_rows is below LVX_LOW_ROWS from the entry's first position on (position
+ * p at p - max(0, first_b), if that is below low_rows): min(Sq, LVX_LOW_ROWS) rows hold all that a call keeps. */
 #define LVX_LOW_ROWS 256
 int lvx_window_forward(const lvx_shape* s, const lvx_window* w, const lvx_view* q, const lvx_view* k, const lvx_view* v,
                        const int32_t* kv_valid_len, float sm_scale, void* workspace, size_t workspace_bytes, void* o, void* o_low,

@@ -60,7 +60,7 @@ class LvxHeadNorm(ctypes.Structure):
 
 
 class LvxWindow(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int32) for n in ("window", "sinks", "query_start")]
+    _fields_ = [(n, ctypes.c_int32) for n in ("window", "sinks", "query_start", "low_rows")]
 
 
 class LvxBlockWait(ctypes.Structure):

@@ -634,6 +634,7 @@ static int check_window(const lvx_shape* s, const lvx_window* w, const char* who
   if (s->q_blocks > 1) return fail(LVX_ERR_SHAPE, "%s: one query block only", who);
   if (w->window < 0 || w->sinks < 0 || w->query_start < -1)
     return fail(LVX_ERR_SHAPE, "%s: window %d, sinks %d, query_start %d: negative", who, w->window, w->sinks, w->query_start);
+  if (w->low_rows < 0 || w->low_rows > LVX_LOW_ROWS) return fail(LVX_ERR_SHAPE, "%s: low_rows %d outside 0..%d", who, w->low_rows, LVX_LOW_ROWS);
   if (s->Sq >= kWindowMaxLen || s->Skv >= kWindowMaxLen || w->query_start >= kWindowMaxLen)
     return fail(LVX_ERR_SHAPE, "%s: lengths and positions must be below %d", who, kWindowMaxLen);
   // the grid's second axis
@@ -768,7 +769,7 @@ struct SharedCall {
   size_t rows;              // B * Hq * Sq
 };
 static int shared_call(SharedCall* c, const lvx_shape* s, int prefixes, int prefix_len, const char* who) {
-  c->own_win = lvx_window{0, 0, -1};
+  c->own_win = lvx_window{0, 0, -1, 0};
   int rc = check_window(s, &c->own_win, who);
   if (rc) return rc;
   if (prefixes < 1 || s->B % prefixes) return fail(LVX_ERR_SHAPE, "%s: %d requests are not a multiple of %d prefixes", who, s->B, prefixes);
@@ -781,7 +782,7 @@ static int shared_call(SharedCall* c, const lvx_shape* s, int prefixes, int pref
   c->pre.Hq = int32_t(rows * s->Hkv);
   c->pre.Sq = 1;
   c->pre.Skv = prefix_len;
-  c->pre_win = lvx_window{0, 0, prefix_len};      // every row stands behind all keys
+  c->pre_win = lvx_window{0, 0, prefix_len, 0};      // every row stands behind all keys
   if ((rc = check_window(&c->pre, &c->pre_win, who))) return rc;
   c->packed = s->B != prefixes && s->Hkv > 1;
   c->rows = size_t(s->B) * s->Hq * s->Sq;

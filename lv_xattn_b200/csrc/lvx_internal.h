@@ -73,21 +73,30 @@ int launch_fwd_rows(const lvx_shape& s, const FwdPlan& p, const void* q, const v
 // position, in O's type. The backward makes delta from both parts there: such rows see few keys, and in dS the error of a rounded
 // O is then as large as the rounding of dS itself (texts of 16 tokens, bf16: gradients off by 2.80e-3 -> 2.41e-3, of 300
 // 2.49e-3 -> 2.38e-3). Rows behind that many positions hardly change it, and the parts of all rows cost 4 to 6 % of a training pass.
+// With fewer rows a head than kLowRows, [B * Hq][rows][128], they lie from the entry's first position on: a batch of 16-token texts
+// keeps as much as its O that way, and sixteen times as much by position.
 constexpr int kLowRows = LVX_LOW_ROWS;
 struct LowRows {
   uint16_t* data;                // nullptr: not kept
   const int32_t* kv_valid_len;
   int start, skv, sq, heads;     // start: query_start; heads: Hq
+  int rows;                      // of a head in `data`
+  // where the row at position `pos` lies in its head's, if the entry's first query is at `first`; -1: not kept
+  static __device__ __forceinline__ int place(int pos, int first, int rows) {
+    const int at = rows < kLowRows ? pos - max(0, first) : pos;
+    return pos >= 0 && pos < kLowRows && at < rows ? at : -1;
+  }
   // the part of row `tok` of (batch entry, head) `bh`, or nullptr
   __device__ __forceinline__ uint16_t* row(int bh, int tok) const {
     if (data == nullptr) return nullptr;
     const int valid = kv_valid_len ? min(skv, max(0, kv_valid_len[bh / heads])) : skv;
-    const int pos = (start >= 0 ? start : valid - sq) + tok;
-    return pos >= 0 && pos < kLowRows ? data + (size_t(bh) * kLowRows + pos) * 128 : nullptr;
+    const int first = start >= 0 ? start : valid - sq, at = place(first + tok, first, rows);
+    return at >= 0 ? data + (size_t(bh) * rows + at) * 128 : nullptr;
   }
 };
+inline int low_rows_of(const lvx_window& w) { return w.low_rows > 0 ? w.low_rows : kLowRows; }
 inline LowRows low_rows(const lvx_shape& s, const lvx_window& w, void* o_low, const int32_t* kv_valid_len) {
-  return {static_cast<uint16_t*>(o_low), kv_valid_len, w.query_start, s.Skv, s.Sq, s.Hq};
+  return {static_cast<uint16_t*>(o_low), kv_valid_len, w.query_start, s.Skv, s.Sq, s.Hq, low_rows_of(w)};
 }
 // How a kernel stands to the one before it in the stream: it starts when that one is complete; or comes onto the SMs while that
 // one, of the same call, still runs, and waits for it itself, at its start or, needing none of its results, at its end

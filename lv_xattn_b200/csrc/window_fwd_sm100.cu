@@ -81,7 +81,8 @@ struct WinFwdParams {
   int nsplit;
   bool beside;          // ORDER_BESIDE
   void* o;              // [B, Hq, Sq, 128] in the input type, with lse; nullptr: partials
-  uint16_t* o_low;      // LOW
+  uint16_t* o_low;      // LOW: with low_rows rows a head
+  int low_rows;
   float* lse;
   float *o_part, *ml_part;
   const uint16_t *q, *k, *v;      // for window_plain_row
@@ -455,8 +456,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int i = 0; i < 16; ++i) sum2 = add2(sum2, f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
         };
         auto low_row = [&] {
-          const int pos = I.start + tok;
-          return LOW && exists && pos >= 0 && pos < kLowRows ? p.o_low + ((size_t(I.slab) * p.g + head) * kLowRows + pos) * 128 : nullptr;
+          const int at = LOW && exists ? LowRows::place(I.start + tok, I.start, p.low_rows) : -1;
+          return at >= 0 ? p.o_low + ((size_t(I.slab) * p.g + head) * p.low_rows + at) * 128 : nullptr;
         };
         if (direct) {
           const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
@@ -864,6 +865,7 @@ int launch_window_fwd(const lvx_shape& s, const lvx_window& w, const FwdPlan& pl
   p.beside = order == ORDER_BESIDE;
   p.o = o;
   p.o_low = static_cast<uint16_t*>(o_low);
+  p.low_rows = low_rows_of(w);
   p.lse = lse;
   p.o_part = o_part;
   p.ml_part = ml_part;

@@ -660,12 +660,12 @@ def _text_view(t):
 _window_calls: dict = {}      # descriptions and scratch sizes, which are functions of the sizes alone
 
 
-def _window_setup(q, k, window, sinks, query_start):
+def _window_setup(q, k, window, sinks, query_start, low_rows=0):
     """(shape, window, forward scratch, backward scratch) of a call, the first two as the library takes them."""
-    key = (q.shape, k.shape, q.dtype, window, sinks, query_start)
+    key = (q.shape, k.shape, q.dtype, window, sinks, query_start, low_rows)
     call = _window_calls.get(key)
     if call is None:
-        shp, win = ctypes.byref(shape_of(q, k)), ctypes.byref(_lib.LvxWindow(window, sinks, query_start))
+        shp, win = ctypes.byref(shape_of(q, k)), ctypes.byref(_lib.LvxWindow(window, sinks, query_start, low_rows))
         f, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
         _lib.check(_lib.load().lvx_window_workspace(shp, win, ctypes.byref(f), ctypes.byref(b)), "lvx_window_workspace")
         if len(_window_calls) >= 4096:
@@ -680,18 +680,31 @@ def _window_setup(q, k, window, sinks, query_start):
 _LOW_TOKENS = 2048
 
 
-def window_forward(q, k, v, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len, training: bool = False):
+def window_low_rows(q, k, query_start: int, kv_valid_len) -> int:
+    """How many rows a head may have whose dropped part is kept: those of its queries that can be at early positions."""
+    if q.dtype == torch.float32 or q.shape[2] > _LOW_TOKENS:
+        return 0
+    sq, first = q.shape[2], query_start
+    if first < 0:
+        if kv_valid_len is not None:      # the lengths decide
+            return min(sq, _lib.LOW_ROWS)
+        first = k.shape[2] - sq
+    return max(0, min(sq + min(0, first), _lib.LOW_ROWS - max(0, first)))
+
+
+def window_forward(q, k, v, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len, training: bool = False,
+                   low_rows: int = _lib.LOW_ROWS):
     """(o [B, Hq, Sq, 128], lse fp32 [B*Hq, Sq]) of causal attention (lvx_window says which keys a query sees), and with
-    `training` what o's rounding dropped of early rows, for the backward (None where there are none). The caller has checked
-    the tensors."""
-    shp, win, nbytes, _ = _window_setup(q, k, window, sinks, query_start)
+    `training` what o's rounding dropped of early rows, for the backward (None where there are none): `low_rows` of them a head,
+    window_low_rows or more. The caller has checked the tensors."""
+    low_rows = low_rows if training and window_low_rows(q, k, query_start, kv_valid_len) else 0
+    shp, win, nbytes, _ = _window_setup(q, k, window, sinks, query_start, low_rows)
     qv, kv, vv = _text_view(q), _text_view(k), _text_view(v)
     B, Hq, Sq, _ = q.shape
     o = _dense_like(q)
     lse = q.new_empty((B * Hq, Sq), dtype=torch.float32)
     ws = lse.new_empty(nbytes // 4) if nbytes else None
-    early = training and q.dtype != torch.float32 and Sq <= _LOW_TOKENS and query_start < _lib.LOW_ROWS      # (-1: the lengths decide)
-    low = q.new_empty((B * Hq, _lib.LOW_ROWS, 128)) if early else None
+    low = q.new_empty((B * Hq, low_rows, 128)) if low_rows else None
     _lib.check(_lib.load().lvx_window_forward(shp, win, _ref(qv), _ref(kv), _ref(vv), _data(kv_valid_len), sm_scale, _data(ws),
                                               nbytes, o.data_ptr(), _data(low), lse.data_ptr(), _lib.stream_int()), "lvx_window_forward")
     _count(2 if nbytes else 1)
@@ -705,7 +718,7 @@ def _dense(t):
 
 def window_backward(do, q, k, v, o, low, lse, sm_scale: float, window: int, sinks: int, query_start: int, kv_valid_len):
     """(dq, dk, dv) of window_forward; `low`: the third that it returned, or None."""
-    shp, win, _, nbytes = _window_setup(q, k, window, sinks, query_start)
+    shp, win, _, nbytes = _window_setup(q, k, window, sinks, query_start, 0 if low is None else low.shape[1])
     qv, kv, vv = _text_view(q), _text_view(k), _text_view(v)
     do = _dense(do)
     dq, dk, dv = _dense_like(q), _dense_like(k), _dense_like(v)

@@ -76,7 +76,8 @@ class WindowAttentionFunc(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, sm_scale, window, sinks, query_start, kv_valid_len):
-        o, lse, low = ops.window_forward(q, k, v, sm_scale, window, sinks, query_start, kv_valid_len, True)
+        o, lse, low = ops.window_forward(q, k, v, sm_scale, window, sinks, query_start, kv_valid_len, True,
+                                         ops.window_low_rows(q, k, query_start, kv_valid_len))
         ctx.save_for_backward(q, k, v, o, low, lse, kv_valid_len)
         ctx.args = sm_scale, window, sinks, query_start
         ctx.mark_non_differentiable(lse)
