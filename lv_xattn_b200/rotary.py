@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -29,6 +30,12 @@ def watch_status(t):
     peer_memory.StatusWatch)."""
     from .peer_memory import status_watch
     status_watch.watch(t.device.index)
+
+
+def refuse_forward_mode(who, *tensors):
+    """The kernels make no tangents, and a tensor that carries one does not require a gradient: it would be lost without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who}: forward-mode derivatives are not supported")
 
 
 def _check(q, k, q_weight, k_weight, cos, sin, eps):
@@ -117,7 +124,8 @@ def head_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1
     bf16, fp16 or fp32. q_weight and k_weight [128] scale the normalised heads (None: that tensor is not normalised). cos and
     sin [S, 128] or [1 or B, S, 128] are the rotary tables as Hugging Face models hand them to their layers, both halves of
     the 128 columns filled (None: no rotation). Computed in fp32 and rounded once. Gradients flow into q, k and the weights;
-    the weights' are summed in a fixed order."""
+    the weights' are summed in a fixed order. No second and no forward-mode derivatives."""
+    refuse_forward_mode("head_norm_rope", q, k, q_weight, k_weight, cos, sin)
     _check(q, k, q_weight, k_weight, cos, sin, eps)
     q_weight, k_weight, cos, sin = (_rows(t) for t in (q_weight, k_weight, cos, sin))
     like = q if q is not None else k

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .rotary import on_device, watch_status
+from .rotary import on_device, refuse_forward_mode, watch_status
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MOST = 1 << 28          # lengths and positions are below this
@@ -107,8 +107,9 @@ def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=
     hold: a cache may be longer than what has been written. A query that sees nothing gets zeros, and -inf in the
     log-sum-exp. In the forward a key that a query does not see has no effect on it, whatever it holds; in the backward the
     valid keys have to be finite.
-    sm_scale scales the scores (None: 1 / sqrt(128)). Gradients flow into q, k and v."""
+    sm_scale scales the scores (None: 1 / sqrt(128)). Gradients flow into q, k and v; no second and no forward-mode derivatives."""
     who = "window_attention"
+    refuse_forward_mode(who, q, k, v)
     sm_scale = _scale(who, sm_scale)
     sinks = _whole(who, "sinks", sinks)
     if window is not None:
@@ -172,8 +173,10 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k=None, v=None, sm_scale=None
     last query sits on the last of the n_b valid own keys. One softmax over both. bf16, fp16 or fp32, any strides.
     prefix_valid_len (P integers) and kv_valid_len (B integers), a list or a tensor on the host or the device: how many keys
     are valid; keys behind them are never looked at, whatever they hold. A query that sees nothing gets zeros, and -inf in
-    the log-sum-exp. Gradients flow into q and all keys and values; those of a prefix are summed over its requests."""
+    the log-sum-exp. Gradients flow into q and all keys and values; those of a prefix are summed over its requests. No second and no
+    forward-mode derivatives."""
     who = "shared_prefix_attention"
+    refuse_forward_mode(who, q, k_prefix, v_prefix, k, v)
     sm_scale = _scale(who, sm_scale)
     if (k is None) != (v is None):
         raise ValueError(f"{who}: k and v go together")
