@@ -38,6 +38,12 @@ def refuse_forward_mode(who, *tensors):
         raise NotImplementedError(f"{who}: forward-mode derivatives are not supported")
 
 
+def refuse_gradient(who, name, t):
+    """For arguments that no gradient flows into."""
+    if torch.is_grad_enabled() and torch.is_tensor(t) and t.requires_grad:
+        raise ValueError(f"{who}: no gradient flows into {name}: detach it")
+
+
 def _check(q, k, q_weight, k_weight, cos, sin, eps):
     like = q if q is not None else k
     if like is None:
@@ -62,6 +68,8 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
     if (cos is None) != (sin is None):
         raise ValueError("head_norm_rope: cos and sin go together")
     if cos is not None:
+        refuse_gradient("head_norm_rope", "cos", cos)
+        refuse_gradient("head_norm_rope", "sin", sin)
         shape, kind = cos.shape, cos.dtype
         if sin.shape != shape or not (shape == (B, S, 128) or shape == (S, 128) or shape == (1, S, 128)):
             raise ValueError(f"head_norm_rope: cos and sin must be [{S}, 128] or [1 or {B}, {S}, 128], got {tuple(cos.shape)} and {tuple(sin.shape)}")
@@ -124,7 +132,7 @@ def head_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1
     bf16, fp16 or fp32. q_weight and k_weight [128] scale the normalised heads (None: that tensor is not normalised). cos and
     sin [S, 128] or [1 or B, S, 128] are the rotary tables as Hugging Face models hand them to their layers, both halves of
     the 128 columns filled (None: no rotation). Computed in fp32 and rounded once. Gradients flow into q, k and the weights;
-    the weights' are summed in a fixed order. No second and no forward-mode derivatives."""
+    the weights' are summed in a fixed order; none flow into cos and sin, which may not ask for one. No second and no forward-mode derivatives."""
     refuse_forward_mode("head_norm_rope", q, k, q_weight, k_weight, cos, sin)
     _check(q, k, q_weight, k_weight, cos, sin, eps)
     q_weight, k_weight, cos, sin = (_rows(t) for t in (q_weight, k_weight, cos, sin))

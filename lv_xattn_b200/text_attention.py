@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .rotary import on_device, refuse_forward_mode, watch_status
+from .rotary import on_device, refuse_forward_mode, refuse_gradient, watch_status
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MOST = 1 << 28          # lengths and positions are below this
@@ -59,6 +59,7 @@ def _check_devices(who, q, *kv):
 def _scale(who, sm_scale):
     if sm_scale is None:
         return 128 ** -0.5
+    refuse_gradient(who, "sm_scale", sm_scale)
     if not (sm_scale > 0 and math.isfinite(sm_scale)):
         raise ValueError(f"{who}: sm_scale must be positive and finite")
     return float(sm_scale)
