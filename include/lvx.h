@@ -402,6 +402,9 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
  * and writes D (fp32 [128,N]) to `d_out`. a/b are device buffers in the arrangement the mode
  * documents (see csrc/selftest.cu). No reference counterpart. */
 int lvx_selftest_mma(int mode, const void* a, const void* b, float* d_out, void* stream);
+/* Self-test, on the host: the key tiles of 1 << tile_shift keys that the windowed kernels walk for queries at positions p0..p1 with
+ * `valid` valid keys, in their order. The first `capacity` of them go to `tiles`, and their number to `count`. */
+int lvx_selftest_key_tiles(const lvx_window* w, int valid, int p0, int p1, int tile_shift, int* tiles, int capacity, int* count);
 
 #ifdef __cplusplus
 }

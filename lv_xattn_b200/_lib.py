@@ -27,7 +27,7 @@ SYMBOLS = [
     "lvx_p2p_signal", "lvx_p2p_gather", "lvx_p2p_fwd_merge", "lvx_p2p_sum_cast", "lvx_p2p_push", "lvx_p2p_wait",
     "lvx_p2p_push_dma",
     "lvx_head_norm_rope", "lvx_head_norm_rope_bwd", "lvx_window_workspace", "lvx_window_forward", "lvx_window_backward",
-    "lvx_shared_workspace", "lvx_shared_forward", "lvx_shared_backward",
+    "lvx_shared_workspace", "lvx_shared_forward", "lvx_shared_backward", "lvx_selftest_key_tiles",
 ]
 MAX_PEERS = 16      # LVX_MAX_PEERS
 P2P_SLOTS = 8       # LVX_P2P_SLOTS
@@ -133,6 +133,7 @@ def load():
     lib.lvx_window_backward.argtypes = [sp, winp, vp, viewp, viewp, viewp, vp, vp, vp, vp, ctypes.c_float, vp, ctypes.c_size_t, vp, vp,
                                         vp, vp]
     i32, sz = ctypes.c_int, ctypes.c_size_t
+    lib.lvx_selftest_key_tiles.argtypes = [winp, i32, i32, i32, i32, ctypes.POINTER(i32), i32, ctypes.POINTER(i32)]
     lib.lvx_shared_workspace.argtypes = [sp, i32, i32, szp, szp]
     lib.lvx_shared_forward.argtypes = [sp, i32, i32, viewp, viewp, viewp, vp, viewp, viewp, vp, ctypes.c_float, vp, sz, vp, vp, vp]
     lib.lvx_shared_backward.argtypes = [sp, i32, i32, vp, viewp, viewp, viewp, vp, viewp, viewp, vp, vp, vp, ctypes.c_float, vp, sz,

@@ -948,6 +948,17 @@ int lvx_shared_backward(const lvx_shape* s, int prefixes, int prefix_len, const 
   return launch_shared_dq(*s, prefixes, acc, pre_slab_rows, acc_own, dq, st);
 }
 
+int lvx_selftest_key_tiles(const lvx_window* w, int valid, int p0, int p1, int tile_shift, int* tiles, int capacity, int* count) {
+  const char* who = "lvx_selftest_key_tiles";
+  if (!w || !count || (!tiles && capacity > 0)) return fail(LVX_ERR_NULL, "%s: w, tiles or count is NULL", who);
+  if (valid < 0 || valid >= kWindowMaxLen || p0 > p1 || p0 <= -kWindowMaxLen || p1 >= 2 * kWindowMaxLen || tile_shift < 0 || tile_shift > 20)
+    return fail(LVX_ERR_SHAPE, "%s: a length, position or tile size out of range", who);
+  const KeyTiles kt = key_tiles(make_window_mask(*w), valid, p0, p1, tile_shift);
+  for (int j = 0; j < kt.n && j < capacity; ++j) tiles[j] = kt.tile(j);
+  *count = kt.n;
+  return LVX_OK;
+}
+
 int lvx_selftest_mma(int mode, const void* a, const void* b, float* d_out, void* stream) {
   const char* who = "lvx_selftest_mma";
   int rc = check_arch();
