@@ -29,6 +29,8 @@
 // lse; a CTA that walks all of them writes its own. That needs no scratch and no second kernel. us a call, and on the GPU
 // (a captured one): eight tokens behind 512 keys (one CTA a slab) 22 / 7.1 -> 18 / 6.8, behind 4,096 (two) 29.3 / 25.6 -> 27.9 /
 // 25.0; one token behind 1,024 (eight) 22 / 7.0 -> 18 / 6.5, behind 8,192 (eight instead of seventeen) 22.6 / 9.3 -> 18 / 12.
+// With keys that no cache holds, one token behind 4,096 of them as seventeen CTAs and a merge / as a cluster of eight: 23.2 / 9.5 and
+// 18.7 / 9.9 us, behind 8,192 23.0 / 12.1 and 19.1 / 13.1, behind 16,384 23.5 / 17.3 and 21.4 / 19.6 (where the plan has the merge).
 #include "lvx_internal.h"
 #include "sm100_prims.cuh"
 #include "window.cuh"

@@ -54,6 +54,10 @@ static_assert(WF_SMEM <= 232448, "shared memory budget");
 //    8 entries    15.5 -> 18.0    28.8 -> 29.5    44.8 -> 40.3    128 -> 107
 //   32 entries    28.6 -> 39.5      74 ->   78     140 ->  121    482 -> 370
 constexpr int kPairTiles = 32;
+// CTAs of the few-row kernel, one an SM, that run at once as clusters of n: what cudaOccupancyMaxActiveClusters says on this GPU's
+// groups of SMs, one of which has fewer than 16. (As 16 clusters of eight, of which 15 fit, two tokens behind 4,096 keys on 8 KV
+// heads took 19.0 us, as clusters of six 12.8, behind 16,384 41.6 and 27.2.)
+constexpr int kClusterCtas[kRowCluster + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
 
 enum {
   WFB_Q_FULL = 0,
@@ -789,13 +793,13 @@ FwdPlan plan_window(const lvx_shape& s, const lvx_window& w, bool* few, bool mer
   const long most = std::min<long>(tiles > 0 ? tiles : 1, *few ? 148 : 64);
   // Splits that fill whole rounds of 148 SMs, eight rounds at most (the fixed cost then outweighs what a partly filled last round
   // wastes): 3 tiles' worth of fixed cost per item, and 4 for a second kernel where one would do without. Few rows do without it
-  // as a cluster, which lies within one of eight groups of about 18 SMs (32 tokens behind 8,192 keys as 256 clusters of four: 172 us
-  // instead of 152 as 256 CTAs).
+  // as a cluster, which lies within one of the eight groups of SMs, of which fewer than all are then in use (kClusterCtas: 32 tokens
+  // behind 8,192 keys as 256 clusters of four take 172 us instead of 152 as 256 CTAs).
   long best_cost = std::numeric_limits<long>::max();
   p.nsplit = 1;
   for (long ns = 1; ns <= most && (ns == 1 || base * ns <= 148 * 8); ++ns) {
     const bool cluster = *few && !merged && ns > 1 && ns <= kRowCluster;
-    const long at_once = cluster ? 8 * (18 / ns) * ns : 148;
+    const long at_once = cluster ? kClusterCtas[ns] : 148;
     const long rounds = (base * ns + at_once - 1) / at_once, per = (tiles + ns - 1) / ns;
     const long cost = rounds * (per + 3) + (ns == 1 || cluster || (*few && merged) ? 0 : 4);
     if (cost < best_cost) {
