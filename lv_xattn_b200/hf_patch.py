@@ -28,7 +28,7 @@ from .async_communication import get_sequence_parallel_group, get_sequence_paral
 from .attn import LVXAttnRecomputeFunc, RingAttnRecomputeFunc
 from .projection import kv_project
 from .rotary import head_norm_rope
-from .text_attention import window_attention
+from .text_attention import whole_number, window_attention
 
 ATTENTION_MODES = ("lv_xattn", "ring", "ring_self")      # the reference's modes (test_llama3.py:107)
 
@@ -142,10 +142,14 @@ def patch_self_attention_forward(attention_mode="lv_xattn", window=None, sinks=0
 
     With a `window` (and `sinks`) every token sees the window of tokens that ends with it, and the first `sinks` ones. The
     layer then runs on this library's kernels: `head_norm_rope` rotates queries and keys on their way into the kernels'
-    layout, and `window_attention` reads only the keys that are seen. CUDA tensors with a head dimension of 128."""
+    layout, and `window_attention` reads only the keys that are seen. CUDA tensors with a head dimension of 128. A window as
+    long as the text, or longer, is the plain causal mask on those kernels. As without a window, `attention_mask` is not
+    looked at: texts of a batch are padded on the right, where no token sees the padding."""
     _check_mode(attention_mode)
     if window is None and sinks:
         raise ValueError("sinks stay visible beside a window: give the window")
+    if window is not None:
+        window, sinks = whole_number("the self-attention hook", "window", window), whole_number("the self-attention hook", "sinks", sinks)
     if window is not None and (window < 1 or sinks < 0):
         raise ValueError(f"window must be at least 1 and sinks not negative, got {window} and {sinks}")
 

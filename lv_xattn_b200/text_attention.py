@@ -65,7 +65,8 @@ def _scale(who, sm_scale):
     return float(sm_scale)
 
 
-def _whole(who, name, n):
+def whole_number(who, name, n):
+    """n, an integer of any kind, as an int."""
     try:
         return operator.index(n)
     except TypeError:
@@ -112,11 +113,11 @@ def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=
     who = "window_attention"
     refuse_forward_mode(who, q, k, v)
     sm_scale = _scale(who, sm_scale)
-    sinks = _whole(who, "sinks", sinks)
+    sinks = whole_number(who, "sinks", sinks)
     if window is not None:
-        window = _whole(who, "window", window)
+        window = whole_number(who, "window", window)
     if query_start is not None:
-        query_start = _whole(who, "query_start", query_start)
+        query_start = whole_number(who, "query_start", query_start)
     if window is not None and window < 1:
         raise ValueError(f"{who}: window must be at least 1 (a query's own position), got {window}")
     if sinks < 0:
