@@ -637,7 +637,7 @@ static int check_window(const lvx_shape* s, const lvx_window* w, const char* who
   if (w->low_rows < 0 || w->low_rows > LVX_LOW_ROWS) return fail(LVX_ERR_SHAPE, "%s: low_rows %d outside 0..%d", who, w->low_rows, LVX_LOW_ROWS);
   if (s->Sq >= kWindowMaxLen || s->Skv >= kWindowMaxLen || w->query_start >= kWindowMaxLen)
     return fail(LVX_ERR_SHAPE, "%s: lengths and positions must be below %d", who, kWindowMaxLen);
-  // the grid's second axis
+  // the contract of the entry points: the kernels' item lists would take more
   if (s->dtype != LVX_FP32 && make_q_tiles(s->Hq / s->Hkv, s->Sq).count > 2 * 65535)
     return fail(LVX_ERR_LIMIT, "%s: %d query rows per KV head are more than 2 x 65,535 tiles", who, s->Hq / s->Hkv * s->Sq);
   return LVX_OK;

@@ -6,7 +6,9 @@
 // (window.cuh: the heads of a group side by side, so that few tiles are seen in part) and leaves all others alone. The
 // frame, the TMEM plan (dK, dV, X: S^T -> P^T, Y: dP^T -> dQ^T, 128 columns each), the issue order and the roles are those
 // of the backward block, for its measured reasons (bwd_sm100.cu): sixteen compute warps, eight drain warps for the
-// reduce-adds of dQ^T (64 KB a tile, the bound of the whole), a TMA producer, an issuer. What differs:
+// reduce-adds of dQ^T (64 KB a tile, the bound of a tile: 4,900 of its 5,600 cycles), a TMA producer, an issuer. What bounds a whole
+// text is its longest CTA, since a key tile is walked by one: 72 query tiles where an even share is 60 for 4,096 tokens with a window of
+// 1,024, 64 where it is 29 for 2,048 causal ones (32 + 8 heads). What differs:
 //   * items go out heaviest first (the first key tiles are seen by the most queries: all of them where they are sinks or
 //     there is no window), forwards and backwards in turn, so that a CTA's share evens out;
 //   * an item knows its own number of query tiles, possibly none;

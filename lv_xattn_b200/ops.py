@@ -675,9 +675,11 @@ def _window_setup(q, k, window, sinks, query_start, low_rows=0):
     return call
 
 
-# Longer texts do without the dropped part of O's early rows: their gradients' error is that of the other rows (4,096 tokens with
-# a window of 1,024, bf16: 2.46e-3 -> 2.38e-3), and the forward that keeps it is slower (79 -> 86 us there; 2 x 2,048 tokens 46 ->
-# 48 us, shorter texts wait for the host).
+# Longer texts do without the dropped part of O's early rows: what it changes in their gradients is small, and the forward that keeps
+# it is slower. Captured forward without -> with it, us, and dQ's error against 64 bits (bf16, 32 + 8 heads): 8 x 512 tokens 40 -> 49
+# (an eager pass waits for the host), 2.52e-3 -> 2.41e-3; 1 x 1,024 25 -> 25, 2.47 -> 2.39; 1 x 2,048 41 -> 43, 4 x 2,048 138 -> 146,
+# 2.46 -> 2.39; 1 x 3,000 79 -> 81, 2.47 -> 2.39; 1 x 4,096 215 -> 219, 2.46 -> 2.39, and with a window of 1,024 74 -> 78, 2.45 -> 2.38;
+# with 16 + 16 heads 2 x 2,048 45 -> 47, 2 x 4,096 223 -> 224. There is no break in these: the line is drawn where texts count as long.
 _LOW_TOKENS = 2048
 
 
