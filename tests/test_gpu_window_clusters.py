@@ -10,18 +10,19 @@ pytestmark = pytest.mark.gpu
 
 
 def grid(call, path):
-    """Grid of the few-row kernel of one call."""
+    """Grid of the few-row kernel of a call."""
     from torch.profiler import ProfilerActivity, profile
     call()
     torch.cuda.synchronize()
     with profile(activities=[ProfilerActivity.CPU, ProfilerActivity.CUDA]) as p:
-        call()
+        for _ in range(5):      # (a profile may lack its first kernels)
+            call()
         torch.cuda.synchronize()
     p.export_chrome_trace(str(path))
     found = [e["args"]["grid"] for e in json.load(open(path))["traceEvents"] if "fwd_rows" in e.get("name", "") and "grid" in e.get("args", {})]
     if not found:
         pytest.skip("no kernel activity recorded")
-    return found[0]
+    return found[-1]
 
 
 @pytest.mark.parametrize("Skv", [1024, 4096, 16384])
