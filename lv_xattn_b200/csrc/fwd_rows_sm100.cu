@@ -294,6 +294,7 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     }
   }
   const float c = p.scale_log2;
+  constexpr float SLACK = WIN ? SoftmaxRef<IS_BF16>::slack : 8.f, UNDER = WIN ? SoftmaxRef<IS_BF16>::under : 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   float o[16][4];
 #pragma unroll
@@ -352,7 +353,7 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (c0 + t * 8 + cq + (e & 1) >= left) sc[t][e] = -INFINITY;
       }
       // online softmax in base 2; a row is spread over four lanes. The running max is a reference point only: it is
-      // raised when it would grow by more than 2^8, so that P stays below 256 and O is rarely rescaled.
+      // raised when it would grow by more than 2^8, so that P stays below 256 and O is rarely rescaled (WIN: SoftmaxRef).
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int t = 0; t < CH / 8; ++t) {
@@ -365,9 +366,9 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       for (int i = 0; i < 2; ++i) {
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * c;
-        if (mx[i] > m[i] + 8.f) {
-          alpha[i] = ex2f(m[i] - mx[i]);
-          m[i] = mx[i];
+        if (mx[i] > m[i] + SLACK) {
+          alpha[i] = ex2f(m[i] - (mx[i] - UNDER));
+          m[i] = mx[i] - UNDER;
           l[i] *= alpha[i];
           grow = true;
         }

@@ -24,6 +24,17 @@ inline WindowMask make_window_mask(const lvx_window& w) {
   return m;
 }
 
+// The softmax' reference, in base 2. P is made relative to a reference that is raised, to `under` below a row's maximum, when the
+// maximum has outgrown it by `slack`. In bf16, which has fp32's range, P stays below 2^8. In fp16 it uses the type's range instead: it
+// lies below 2^15, and from 2^12 down to 2^-14, 2^-26 of the maximum or less, it keeps all of its bits; with the maximum as the
+// reference a probability of 2^-20 of it would keep five, and one of 2^-25 none, although the row's sum counts it (a sink of a small
+// value that takes most of a row's weight). The backward's P is at most 1 and is rounded 2^14 larger.
+template <bool IS_BF16>
+struct SoftmaxRef {
+  static constexpr float slack = IS_BF16 ? 8.f : 15.f, under = IS_BF16 ? 0.f : 12.f;
+  static constexpr float grad_bits = IS_BF16 ? 0.f : 14.f, grad_gain = IS_BF16 ? 1.f : 16384.f;
+};
+
 // The key tiles that queries at positions p0..p1 see: [0, ns) for the sinks, then w0 >= ns onwards; n in all.
 struct KeyTiles {
   int ns, w0, n;

@@ -21,6 +21,8 @@
 //     value; tiles seen whole cost none;
 //   * rows of K and V behind the last valid key are cleared in shared memory: they may hold anything, and zero times
 //     that would reach dQ. (A key inside must be finite: in a backward there is no other answer than NaN.)
+//   * in fp16 P is made 2^14 times as large (SoftmaxRef): at most 1 as it is, behind 100,000 keys most of it is subnormal there, and
+//     dV erred by 1.0e-3 instead of 3e-4;
 //   * P is rounded to 16 bits for its product with dO, but dS is made from the fp32 P (dQ and dK then err by 2.4e-3 in bf16,
 //     1.7e-3 of which is their own rounding; with P taken back from its 16 bits 3.0e-3). That P has to outlive the wait for
 //     dP^T, 16 registers more in the compute warps. They come from the producer's and the issuer's warpgroup: 896 threads
@@ -183,6 +185,12 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tX = tmem_base + WB_X + lane_sel, tY = tmem_base + WB_Y + lane_sel;
     const float c = p.scale_log2;
+    using Ref = SoftmaxRef<IS_BF16>;
+    // dS = P (dP - delta): in fp16 P is grad_gain times as large as it is, and the statistics' delta as much smaller
+    auto ds = [](uint32_t pv, uint32_t dp, float dl) {
+      const float x = __uint_as_float(dp);
+      return __uint_as_float(pv) * (IS_BF16 ? x - dl : fmaf(x, 1.f / Ref::grad_gain, -dl));
+    };
     bool alive = !poisoned;
     int it = 0, jj0 = 0;
     for (int round = 0, w; alive && (w = index_of(round)) < p.nitems; ++round) {
@@ -204,11 +212,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const int col = tid & 127, tok = tile_tok(I, j) + col / heads, head = tile_chunk(j) * heads + col % heads;
         const bool exists = col < tile_rows && tok < p.sq && head < p.g;
         const size_t at = (size_t(I.slab) * p.g + head) * p.sq + tok;
-        if (tid >= 128) return exists ? p.delta[at] : 0.f;
+        if (tid >= 128) return exists ? p.delta[at] * (1.f / Ref::grad_gain) : 0.f;
         float v = INFINITY;       // +inf => P = 0: a query that does not exist, or that sees nothing
         if (exists) {
           v = p.lse[at] * 1.4426950408889634f;
-          if (v == -INFINITY) v = INFINITY;
+          v = v == -INFINITY ? INFINITY : v - Ref::grad_bits;
         }
         return v;
       };
@@ -309,10 +317,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float4 dl = sd[h * 4 + i];
-            const float d0 = __uint_as_float(s[h * 16 + 4 * i]) * (__uint_as_float(dp[4 * i]) - dl.x);
-            const float d1 = __uint_as_float(s[h * 16 + 4 * i + 1]) * (__uint_as_float(dp[4 * i + 1]) - dl.y);
-            const float d2 = __uint_as_float(s[h * 16 + 4 * i + 2]) * (__uint_as_float(dp[4 * i + 2]) - dl.z);
-            const float d3 = __uint_as_float(s[h * 16 + 4 * i + 3]) * (__uint_as_float(dp[4 * i + 3]) - dl.w);
+            const float d0 = ds(s[h * 16 + 4 * i], dp[4 * i], dl.x), d1 = ds(s[h * 16 + 4 * i + 1], dp[4 * i + 1], dl.y);
+            const float d2 = ds(s[h * 16 + 4 * i + 2], dp[4 * i + 2], dl.z), d3 = ds(s[h * 16 + 4 * i + 3], dp[4 * i + 3], dl.w);
             dsk[h * 8 + 2 * i] = IS_BF16 ? pack_bf16x2(d0, d1) : pack_f16x2(d0, d1);
             dsk[h * 8 + 2 * i + 1] = IS_BF16 ? pack_bf16x2(d2, d3) : pack_f16x2(d2, d3);
           }
@@ -350,7 +356,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           uint32_t a[32];
           tmem_ld32(tmem_base + (which ? WB_DV : WB_DK) + lane_sel + cg * 32, a);
           tc_wait_ld();
-          const float mul = which ? 1.f : p.scale;
+          const float mul = which ? 1.f / Ref::grad_gain : p.scale;
           if (I.part >= 0) {
             float4* dst = reinterpret_cast<float4*>(p.parts + ((size_t(I.part) * 2 + which) * 128 + r) * 128 + cg * 32);
 #pragma unroll

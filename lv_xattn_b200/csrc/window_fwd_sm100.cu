@@ -256,6 +256,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t tS = tmem_base + wg * 128 + lane_sel;
     const uint32_t tO = tmem_base + 256 + wg * 128 + lane_sel;
     const float c = p.scale_log2;
+    using Ref = SoftmaxRef<IS_BF16>;
     // this warpgroup's key tiles: all of an item's, or every other one
     constexpr int STEP = PAIR ? 2 : 1;
     const int first = PAIR ? wg : 0;
@@ -304,7 +305,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx[i & 3] = max3(mx[i & 3], __uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1]));
           const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
-          if (!__any_sync(0xffffffffu, top > m + 8.f)) {
+          if (!__any_sync(0xffffffffu, top > m + Ref::slack)) {
             const float moff = m == -INFINITY ? 0.f : m;
             uint64_t sum_a = f32x2(0.f, 0.f), sum_b = f32x2(0.f, 0.f);
             const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-moff, -moff);
@@ -366,12 +367,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
               for (int i = 0; i < 16; ++i) mx[i & 3] = max3(mx[i & 3], __uint_as_float(s[q][2 * i]), __uint_as_float(s[q][2 * i + 1]));
             }
-          const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
-          const bool grow = m_new > m + 8.f;       // raised only when it would grow by more than 2^8: P stays below 256
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+          const bool grow = top > m + Ref::slack;
           float alpha = 1.f;
           if (grow) {
-            alpha = ex2f(m - m_new);
-            m = m_new;
+            alpha = ex2f(m - (top - Ref::under));
+            m = top - Ref::under;
             l *= alpha;
           }
           if (t > 0 && __any_sync(0xffffffffu, grow)) {
