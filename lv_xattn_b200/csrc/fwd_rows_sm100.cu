@@ -294,8 +294,8 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     }
   }
   const float c = p.scale_log2;
-  constexpr float SLACK = WIN ? SoftmaxRef<IS_BF16>::slack : 8.f, UNDER = WIN ? SoftmaxRef<IS_BF16>::under : 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  using Ref = SoftmaxRef<IS_BF16 || !WIN>;
+  float m[2] = {-INFINITY, -INFINITY}, high[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   float o[16][4];
 #pragma unroll
   for (int t = 0; t < 16; ++t)
@@ -360,20 +360,21 @@ fwd_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         mx[0] = fmaxf(mx[0], fmaxf(sc[t][0], sc[t][1]));
         mx[1] = fmaxf(mx[1], fmaxf(sc[t][2], sc[t][3]));
       }
-      bool grow = false;
-      float alpha[2] = {1.f, 1.f};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * c;
-        if (mx[i] > m[i] + SLACK) {
-          alpha[i] = ex2f(m[i] - (mx[i] - UNDER));
-          m[i] = mx[i] - UNDER;
-          l[i] *= alpha[i];
-          grow = true;
-        }
       }
-      if (__any_sync(0xffffffffu, grow)) {
+      if (__any_sync(0xffffffffu, Ref::off(mx[0], m[0]) || Ref::off(mx[1], m[1]))) {
+        float alpha[2] = {1.f, 1.f};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (Ref::moves(mx[i], m[i], high[i])) {
+            alpha[i] = ex2f(m[i] - (mx[i] - Ref::under));
+            m[i] = mx[i] - Ref::under;
+            high[i] = fmaxf(high[i], m[i]);
+            l[i] *= alpha[i];
+          }
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
           o[t][0] *= alpha[0];

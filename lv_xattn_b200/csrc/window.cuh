@@ -24,15 +24,24 @@ inline WindowMask make_window_mask(const lvx_window& w) {
   return m;
 }
 
-// The softmax' reference, in base 2. P is made relative to a reference that is raised, to `under` below a row's maximum, when the
-// maximum has outgrown it by `slack`. In bf16, which has fp32's range, P stays below 2^8. In fp16 it uses the type's range instead: it
-// lies below 2^15, and from 2^12 down to 2^-14, 2^-26 of the maximum or less, it keeps all of its bits; with the maximum as the
-// reference a probability of 2^-20 of it would keep five, and one of 2^-25 none, although the row's sum counts it (a sink of a small
-// value that takes most of a row's weight). The backward's P is at most 1 and is rounded 2^14 larger.
+// The softmax' reference m, in base 2: P of a tile is 2^(score - m), and O and the sum, in fp32, are rescaled when m moves. In bf16,
+// which has fp32's range, m is raised to the maximum when that has outgrown it by 2^8. In fp16 P has to stay below 2^16, and what is
+// below 2^-14 loses bits (2^-25: all of them), although the row's sum counts it: beside a sink of small value that outweighs the other
+// keys by 2^18 O was off by 10 % in places. There m moves to 2^7 under the maximum of the tile at hand when that is above m by 2^15 or
+// below it by 2^2, as long as it stays within 2^60 of the highest it was: what lies further down adds nothing. (m only ever raised, to 2^12 under the maximum,
+// cost a window with sinks 23 %: the rows see few keys of their first tile, and outgrow it in the next.)
+// The backward's P is at most 1 and is rounded 2^14 larger in fp16.
 template <bool IS_BF16>
 struct SoftmaxRef {
-  static constexpr float slack = IS_BF16 ? 8.f : 15.f, under = IS_BF16 ? 0.f : 12.f;
+  static constexpr float under = IS_BF16 ? 0.f : 7.f;
   static constexpr float grad_bits = IS_BF16 ? 0.f : 14.f, grad_gain = IS_BF16 ? 1.f : 16384.f;
+#ifdef __CUDACC__
+  // whether a tile of maximum `top` may move m, and whether it does; `high`: the highest m (-inf, as `top` and m may be: no move)
+  static __device__ __forceinline__ bool off(float top, float m) { return IS_BF16 ? top > m + 8.f : fabsf(top - m - 6.5f) > 8.5f; }
+  static __device__ __forceinline__ bool moves(float top, float m, float high) {
+    return IS_BF16 ? top > m + 8.f : top > m + 15.f || (top < m - 2.f && top - under > high - 60.f);
+  }
+#endif
 };
 
 // The key tiles that queries at positions p0..p1 see: [0, ns) for the sinks, then w0 >= ns onwards; n in all.

@@ -281,7 +281,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // keys that every row of the warp sees: [0, all_sinks) and [all_lo, all_hi]
       const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
       const int all_sinks = min(p.mask.sinks, all_hi + 1);
-      float m = exists ? -INFINITY : 0.f, l = 0.f;
+      float m = exists ? -INFINITY : 0.f, high = m, l = 0.f;
       int t = 0;                       // tiles of this warpgroup in the item
       for (int j = first; j < I.n; j += STEP, ++t) {
         const int key0 = I.kt.tile(I.j0 + j) * 128;
@@ -305,7 +305,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx[i & 3] = max3(mx[i & 3], __uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1]));
           const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
-          if (!__any_sync(0xffffffffu, top > m + Ref::slack)) {
+          if (!__any_sync(0xffffffffu, Ref::off(top, m))) {
             const float moff = m == -INFINITY ? 0.f : m;
             uint64_t sum_a = f32x2(0.f, 0.f), sum_b = f32x2(0.f, 0.f);
             const uint64_t c2 = f32x2(c, c), nm2 = f32x2(-moff, -moff);
@@ -368,14 +368,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               for (int i = 0; i < 16; ++i) mx[i & 3] = max3(mx[i & 3], __uint_as_float(s[q][2 * i]), __uint_as_float(s[q][2 * i + 1]));
             }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-          const bool grow = top > m + Ref::slack;
+          const bool move = Ref::moves(top, m, high);
           float alpha = 1.f;
-          if (grow) {
+          if (move) {
             alpha = ex2f(m - (top - Ref::under));
             m = top - Ref::under;
+            high = fmaxf(high, m);
             l *= alpha;
           }
-          if (t > 0 && __any_sync(0xffffffffu, grow)) {
+          if (t > 0 && __any_sync(0xffffffffu, move)) {
 #pragma unroll
             for (int q = 0; q < 8; ++q) {      // (32 columns at a time do not fit beside the scores)
               uint32_t o[16];
