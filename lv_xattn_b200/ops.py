@@ -675,17 +675,15 @@ def _window_setup(q, k, window, sinks, query_start, low_rows=0):
     return call
 
 
-# Longer texts do without the dropped part of O's early rows: what it changes in their gradients is small, and the forward that keeps
-# it is slower. Captured forward without -> with it, us, and dQ's error against 64 bits (bf16, 32 + 8 heads): 8 x 512 tokens 40 -> 49
-# (an eager pass waits for the host), 2.52e-3 -> 2.41e-3; 1 x 1,024 25 -> 25, 2.47 -> 2.39; 1 x 2,048 41 -> 43, 4 x 2,048 138 -> 146,
-# 2.46 -> 2.39; 1 x 3,000 79 -> 81, 2.47 -> 2.39; 1 x 4,096 215 -> 219, 2.46 -> 2.39, and with a window of 1,024 74 -> 78, 2.45 -> 2.38;
-# with 16 + 16 heads 2 x 2,048 45 -> 47, 2 x 4,096 223 -> 224. There is no break in these: the line is drawn where texts count as long.
-_LOW_TOKENS = 2048
-
-
 def window_low_rows(q, k, query_start: int, kv_valid_len) -> int:
-    """How many rows a head may have whose dropped part is kept: those of its queries that can be at early positions."""
-    if q.dtype == torch.float32 or q.shape[2] > _LOW_TOKENS:
+    """How many rows a head may have whose dropped part is kept: those of its queries that can be at early positions.
+
+    Of long texts too: captured forward without -> with it, us, and dQ's error against 64 bits (bf16, 32 + 8 heads): 8 x 512 tokens
+    40 -> 49 (an eager pass waits for the host), 2.52e-3 -> 2.41e-3; 1 x 1,024 25 -> 25, 2.47 -> 2.39; 1 x 2,048 41 -> 43, 4 x 2,048
+    138 -> 146, 2.46 -> 2.39; 1 x 3,000 79 -> 81, 2.47 -> 2.39; 1 x 4,096 215 -> 219, 2.46 -> 2.39, and with a window of 1,024 74 -> 78,
+    2.45 -> 2.38. The passes that they belong to take five times as long. Without it some texts of 2,500 to 4,096 tokens had gradients
+    that were off by more than one and a half roundings (2.51e-3), with it by 2.41e-3 at most."""
+    if q.dtype == torch.float32:
         return 0
     sq, first = q.shape[2], query_start
     if first < 0:

@@ -24,7 +24,7 @@ def test_no_more_rows_than_are_early():
 def test_short_texts_keep_no_more_than_their_output():
     assert rows(16, 16) == 16 and rows(16, 16, 0) == 16 and rows(1, 1) == 1
     assert rows(1000, 9192) == 0 and rows(1, 8192) == 0      # a chunk and a token behind a long cache
-    assert rows(16, 16, dtype=torch.float32) == 0 and rows(4096, 4096) == 0
+    assert rows(16, 16, dtype=torch.float32) == 0 and rows(4096, 4096) == _lib.LOW_ROWS
 
 
 def test_abi_refusals():
