@@ -577,7 +577,7 @@ def _head_norm(q, k, q_weight, k_weight, cos, sin, eps):
                          None if k is None or k_weight is None else k_weight.data_ptr(),
                          None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
                          # (the stride of a dimension of one may be anything, and is never used)
-                         *(0 if cos is None or cos.shape[i] == 1 else cos.stride(i) for i in (0, 1)))
+                         0 if cos is None or cos.shape[0] == 1 else cos.stride(0), 0 if cos is None or cos.shape[1] == 1 else cos.stride(1))
     return c, _token_view(q), _token_view(k)
 
 

@@ -41,7 +41,7 @@ def refuse_forward_mode(who, *tensors):
 def refuse_gradient(who, name, t):
     """For arguments that no gradient flows into."""
     if torch.is_grad_enabled() and torch.is_tensor(t) and t.requires_grad:
-        raise ValueError(f"{who}: no gradient flows into {name}: detach it")
+        raise ValueError(f"{who}: no gradient flows into {name}: detach")
 
 
 def _check(q, k, q_weight, k_weight, cos, sin, eps):
@@ -68,8 +68,8 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
     if (cos is None) != (sin is None):
         raise ValueError("head_norm_rope: cos and sin go together")
     if cos is not None:
-        refuse_gradient("head_norm_rope", "cos", cos)
-        refuse_gradient("head_norm_rope", "sin", sin)
+        if cos.requires_grad or sin.requires_grad:
+            refuse_gradient("head_norm_rope", "cos and sin", cos if cos.requires_grad else sin)
         shape, kind = cos.shape, cos.dtype
         if sin.shape != shape or not (shape == (B, S, 128) or shape == (S, 128) or shape == (1, S, 128)):
             raise ValueError(f"head_norm_rope: cos and sin must be [{S}, 128] or [1 or {B}, {S}, 128], got {tuple(cos.shape)} and {tuple(sin.shape)}")

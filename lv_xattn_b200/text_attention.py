@@ -59,7 +59,8 @@ def _check_devices(who, q, *kv):
 def _scale(who, sm_scale):
     if sm_scale is None:
         return 128 ** -0.5
-    refuse_gradient(who, "sm_scale", sm_scale)
+    if type(sm_scale) is not float:
+        refuse_gradient(who, "sm_scale", sm_scale)
     if not (sm_scale > 0 and math.isfinite(sm_scale)):
         raise ValueError(f"{who}: sm_scale must be positive and finite")
     return float(sm_scale)
