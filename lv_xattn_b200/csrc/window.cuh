@@ -28,8 +28,8 @@ inline WindowMask make_window_mask(const lvx_window& w) {
 // which has fp32's range, m is raised to the maximum when that has outgrown it by 2^8. In fp16 P has to stay below 2^16, and what is
 // below 2^-14 loses bits (2^-25: all of them), although the row's sum counts it: beside a sink of small value that outweighs the other
 // keys by 2^18 O was off by 10 % in places. There m moves to 2^7 under the maximum of the tile at hand when that is above m by 2^15 or
-// below it by 2^2, as long as it stays within 2^60 of the highest it was: what lies further down adds nothing. (m only ever raised, to 2^12 under the maximum,
-// cost a window with sinks 23 %: the rows see few keys of their first tile, and outgrow it in the next.)
+// below it by 2^2, as long as it stays within 2^60 of the highest it was: what lies further down adds nothing. (m only ever raised, to
+// 2^12 under the maximum, cost a window with sinks 23 %: the rows see few keys of their first tile, and outgrow it in the next.)
 // The backward's P is at most 1 and is rounded 2^14 larger in fp16.
 template <bool IS_BF16>
 struct SoftmaxRef {

@@ -682,7 +682,7 @@ def window_low_rows(q, k, query_start: int, kv_valid_len) -> int:
     40 -> 49 (an eager pass waits for the host), 2.52e-3 -> 2.41e-3; 1 x 1,024 25 -> 25, 2.47 -> 2.39; 1 x 2,048 41 -> 43, 4 x 2,048
     138 -> 146, 2.46 -> 2.39; 1 x 3,000 79 -> 81, 2.47 -> 2.39; 1 x 4,096 215 -> 219, 2.46 -> 2.39, and with a window of 1,024 74 -> 78,
     2.45 -> 2.38. The passes that they belong to take five times as long. Without it some texts of 2,500 to 4,096 tokens had gradients
-    that were off by more than one and a half roundings (2.51e-3), with it by 2.41e-3 at most."""
+    that were off by more than one and a half roundings (2.51e-3), with it by 2.44e-3 at most."""
     if q.dtype == torch.float32:
         return 0
     sq, first = q.shape[2], query_start

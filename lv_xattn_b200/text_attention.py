@@ -108,8 +108,9 @@ def window_attention(q, k, v, sm_scale=None, window=None, sinks=0, kv_valid_len=
     window or j < sinks. window None: all keys behind it. kv_valid_len: n_b, one integer per entry (a list, or a tensor on
     the host or the device; values are taken into 0..Skv), None: Skv. Keys from n_b on are never looked at, whatever they
     hold: a cache may be longer than what has been written. A query that sees nothing gets zeros, and -inf in the
-    log-sum-exp. In the forward a key that a query does not see has no effect on it, whatever it holds, and a NaN that it does see is
-    NaN in both results; in the backward q, the valid keys and the gradient of o have to be finite (NaN reaches more of the gradients).
+    log-sum-exp. In the forward a key that a query does not see has no effect on it, whatever it holds; a NaN
+    in the query or in a key that it sees is NaN in both results, and one in a value in o. In the backward q, the valid keys and the
+    gradient of o have to be finite (NaN reaches more of the gradients).
     sm_scale scales the scores (None: 1 / sqrt(128)). Gradients flow into q, k and v; no second and no forward-mode derivatives."""
     who = "window_attention"
     refuse_forward_mode(who, q, k, v)
